@@ -1,0 +1,413 @@
+"""The operators of a 4-bit transformer block, as cases to measure: quantisation to microscaled 4-bit
+floating point (MXFP4) and back, the product of two such operands, the norms around a block fused with its
+gate and residual, and the run of them that a served block makes.
+
+MXFP4: a row is cut into blocks of 32 values; a block has one scale X = 2^(floor(log2 max|v|) - 2), held as
+the byte log2(X) + 127, and its values are held as v / X rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6
+(ties to the even code, larger ones to 6), with a sign: code = sign * 8 + index.  An operand of [rows, k] is
+  codes:  uint8 [rows, 16 * nb], nb = ceil(k / 32), the even element of a pair in the low four bits;
+  scales: uint8 tiles of 128 rows x 4 blocks, 512 bytes each, tile (R, T) at (R * ceil(nb / 4) + T) * 512,
+          row r, block b of a tile at (r % 32) * 16 + (r / 32) * 4 + b.
+
+`run` computes each operator in elementary torch operations in 32 bits, or with `own` by this repository's
+entry points; `exact` computes the definition in 64 bits.
+"""
+import math
+
+import torch
+
+own = False
+
+_TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+_SIZE = {"f32": 4, "f16": 2, "bf16": 2}
+_backend = None
+
+
+# ---------------------------------------------------------------------------
+# cases
+# ---------------------------------------------------------------------------
+
+def listed():
+    return [
+        # activations of a long prompt, quantised before a product and read back
+        {"name": "quantize prompt", "op": "quantize", "rows": 8192, "k": 4096, "type": "f16", "gap": 0},
+        # one token's activations
+        {"name": "quantize token", "op": "quantize", "rows": 1, "k": 4096, "type": "bf16", "gap": 0},
+        # a slice of a wider f32 tensor, its width no multiple of a block
+        {"name": "quantize ragged slice", "op": "quantize", "rows": 1000, "k": 1010, "type": "f32", "gap": 15},
+        # a square projection over a batch of prompts
+        {"name": "gemm 4096", "op": "gemm", "m": 4096, "n": 4096, "k": 4096, "type": "f16", "bias": False, "act": "none"},
+        # the down projection of a feed-forward layer over a short prompt
+        {"name": "gemm 256 down", "op": "gemm", "m": 256, "n": 4096, "k": 11008, "type": "bf16", "bias": True, "act": "none"},
+        # the up projection for a single token
+        {"name": "gemm token up", "op": "gemm", "m": 1, "n": 11008, "k": 4096, "type": "bf16", "bias": False, "act": "silu"},
+        # a few tokens into a classifier: every size ragged
+        {"name": "gemm ragged", "op": "gemm", "m": 37, "n": 1000, "k": 2056, "type": "f16", "bias": True, "act": "relu"},
+        # norms on both sides of a residual, over a long prompt
+        {"name": "norm prompt", "op": "norm", "rows": 8192, "c": 4096, "type": "bf16", "res": "bf16", "post": "rms",
+         "pre": "rms", "gate": "channel", "group": 0, "affine": False},
+        # residual add and the next norm for a single token
+        {"name": "norm token", "op": "norm", "rows": 1, "c": 4096, "type": "f16", "res": "f16", "post": "none", "pre": "rms",
+         "gate": "none", "group": 0, "affine": False},
+        # layer norms with a gate row for each image of a batch, an odd width
+        {"name": "norm per image", "op": "norm", "rows": 1000, "c": 1010, "type": "f32", "res": "f32", "post": "layer",
+         "pre": "layer", "gate": "group", "group": 250, "affine": True},
+        # a feed-forward block with its norms and residuals: a short prompt, a single token
+        {"name": "block prompt", "op": "block", "m": 256, "c": 4096, "f": 11008, "type": "bf16"},
+        {"name": "block token", "op": "block", "m": 1, "c": 4096, "f": 11008, "type": "bf16"},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["quantize", "gemm", "norm", "block"])
+    if op == "quantize":
+        k = _log(rng, 32, 11008)
+        rows = min(_log(rng, 1, 8192), 8192 * 4096 // k)
+        t = rng.choice(["f32", "f16", "bf16"])
+        return {"op": op, "rows": rows if t != "f32" else max(1, rows // 2), "k": k, "type": t,
+                "gap": rng.choice([0, 0, 8, 33])}
+    if op == "gemm":
+        return {"op": op, "m": _log(rng, 1, 4096), "n": _log(rng, 32, 4096), "k": _log(rng, 32, 4096),
+                "type": rng.choice(["f16", "bf16"]), "bias": rng.random() < 0.5, "act": rng.choice(["none", "relu", "silu"])}
+    if op == "norm":
+        c = _log(rng, 32, 11008)
+        t = rng.choice(["f32", "f16", "bf16"])
+        rows = max(1, min(_log(rng, 1, 8192), 8192 * 4096 // c) // (2 if t == "f32" else 1))
+        gate = rng.choice(["none", "channel", "group", "row"])
+        return {"op": op, "rows": rows, "c": c, "type": t, "res": t, "post": rng.choice(["none", "rms", "layer"]),
+                "pre": rng.choice(["rms", "layer"]), "gate": gate,
+                "group": {"none": 0, "channel": 0, "group": max(1, rows // 3), "row": 1}[gate], "affine": rng.random() < 0.5}
+    return {"op": op, "m": _log(rng, 1, 256), "c": _log(rng, 64, 4096), "f": _log(rng, 128, 11008),
+            "type": rng.choice(["f16", "bf16"])}
+
+
+def _operand_bytes(rows, k):
+    return rows * (k / 2 + k / 32)
+
+
+def work(case):
+    c = case
+    if c["op"] == "quantize":  # values in, codes and scales out, values out
+        n = c["rows"] * c["k"]
+        return {"bytes": 2 * n * _SIZE[c["type"]] + _operand_bytes(c["rows"], c["k"]), "flops": 4 * n}
+    if c["op"] == "gemm":
+        m, n, k = c["m"], c["n"], c["k"]
+        return {"bytes": _operand_bytes(m, k) + _operand_bytes(n, k) + m * n * 2 + 4 * n * c["bias"], "flops": 2.0 * m * n * k}
+    if c["op"] == "norm":  # block output and residual in, residual and next input out
+        n, es = c["rows"] * c["c"], _SIZE[c["type"]]
+        gate = {"none": 0, "channel": 1}.get(c["gate"], c["rows"] / max(1, c["group"])) * c["c"] * es
+        return {"bytes": 2 * n * es + 2 * n * _SIZE[c["res"]] + gate + 8 * c["c"], "flops": 12 * n}
+    m, ch, f = c["m"], c["c"], c["f"]
+    return {"bytes": 4 * m * ch * 2 + 2 * _operand_bytes(f, ch) + 20 * ch, "flops": 4.0 * m * ch * f}
+
+
+# ---------------------------------------------------------------------------
+# MXFP4 in torch
+# ---------------------------------------------------------------------------
+
+def _blocks(k):
+    return (k + 31) // 32
+
+
+def _pow2(e):
+    """2^e for whole e, exactly (pow and exp2 need not be), as f32."""
+    return ((e + 1023) << 52).view(torch.float64).float()
+
+
+def _tile(s):
+    """Scales [rows, nb] in tiles of 128 rows x 4 blocks; places outside [rows, nb] hold 0."""
+    rows, nb = s.shape
+    R, T = (rows + 127) // 128, (nb + 3) // 4
+    full = torch.zeros(R * 128, T * 4, dtype=torch.uint8, device=s.device)
+    full[:rows, :nb] = s
+    return full.view(R, 4, 32, T, 4).permute(0, 3, 2, 1, 4).contiguous().view(-1)
+
+
+def _untile(t, rows, k):
+    nb = _blocks(k)
+    R, T = (rows + 127) // 128, (nb + 3) // 4
+    return t.view(R, T, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(R * 128, T * 4)[:rows, :nb]
+
+
+def _values(codes, scales, rows, k):
+    """The values that an operand stands for: f32 [rows, k]."""
+    mags = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float32, device=codes.device)
+    v = mags[torch.stack((codes & 15, codes >> 4), -1).view(rows, -1).int()]
+    return (v.view(rows, -1, 32) * _pow2(_untile(scales, rows, k).long() - 127).unsqueeze(-1)).view(rows, -1)[:, :k]
+
+
+def _quantized(x):
+    """x f32 [rows, k] rounded to MXFP4: (values / X with their signs [rows, nb, 32], scale bytes [rows, nb])."""
+    rows, k = x.shape
+    nb = _blocks(k)
+    v = torch.zeros(rows, nb * 32, device=x.device)
+    v[:, :k] = x
+    v = v.view(rows, nb, 32)
+    amax = v.abs().amax(-1)
+    e = torch.frexp(amax)[1].long() - 3  # amax = f * 2^(e + 3), f in [0.5, 1): floor(log2 amax) - 2 = e
+    e = torch.where(amax > 0, e, -127).clamp(min=-127)
+    t = v * _pow2(-e).unsqueeze(-1)
+    a = t.abs()
+    step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
+    return torch.copysign(torch.clamp(torch.round(a / step) * step, max=6.0), t), e + 127
+
+
+def _rounded(x):
+    """x f32 [rows, k] -> the values its MXFP4 form stands for."""
+    q, s = _quantized(x)
+    return (q * _pow2(s - 127).unsqueeze(-1)).reshape(x.shape[0], -1)[:, :x.shape[1]]
+
+
+def _operand(x):
+    """x f32 [rows, k] -> (codes, tiled scales)."""
+    q, s = _quantized(x)
+    a = q.abs()
+    index = torch.where(a < 2, a * 2, torch.where(a < 4, a + 2, a / 2 + 4)).to(torch.uint8)
+    code = (index + 8 * (q < 0).to(torch.uint8)).view(x.shape[0], -1, 2)
+    return (code[..., 0] | (code[..., 1] << 4)).contiguous(), _tile(s.to(torch.uint8))
+
+
+# ---------------------------------------------------------------------------
+# states
+# ---------------------------------------------------------------------------
+
+def _acts(g, rows, c):
+    """Activations: normal, with channels of different size."""
+    return torch.randn(rows, c, generator=g, device="cuda") * torch.exp(0.7 * torch.randn(c, generator=g, device="cuda"))
+
+
+def _weight(g, n, k):
+    return _operand(torch.randn(n, k, generator=g, device="cuda") / math.sqrt(k))
+
+
+def _gain(g, c):
+    return 1.0 + 0.2 * torch.randn(c, generator=g, device="cuda")
+
+
+def prepare(case, seed):
+    c = case
+    g = torch.Generator(device="cuda").manual_seed(int(seed))
+    dev = "cuda"
+    s = {"case": c}
+    if c["op"] == "quantize":
+        rows, k, t = c["rows"], c["k"], _TYPES[c["type"]]
+        wide = _acts(g, rows, k + c["gap"]).to(t)
+        s["x"] = wide[:, :k]
+        s["q"] = torch.empty(rows, _blocks(k) * 16, dtype=torch.uint8, device=dev)
+        s["s"] = torch.empty(_tile_bytes(rows, k), dtype=torch.uint8, device=dev)
+        s["y"] = torch.empty(rows, k, dtype=t, device=dev)
+    elif c["op"] == "gemm":
+        m, n, k = c["m"], c["n"], c["k"]
+        s["aq"], s["as"] = _operand(_acts(g, m, k))
+        s["bq"], s["bs"] = _weight(g, n, k)
+        s["bias"] = 0.3 * torch.randn(n, generator=g, device=dev) if c["bias"] else None
+        s["y"] = torch.empty(m, n, dtype=_TYPES[c["type"]], device=dev)
+    elif c["op"] == "norm":
+        rows, ch, t = c["rows"], c["c"], _TYPES[c["type"]]
+        s["x"] = _acts(g, rows, ch).to(t)
+        s["r"] = (2 * _acts(g, rows, ch)).to(_TYPES[c["res"]])
+        groups = {"none": 0, "channel": 1, "row": rows}.get(c["gate"], -(-rows // max(1, c["group"])))
+        s["gate"] = (0.5 + 0.5 * torch.randn(groups, ch, generator=g, device=dev)).to(t) if groups else None
+        s["w0"] = _gain(g, ch) if c["post"] != "none" else None
+        s["b0"] = 0.1 * torch.randn(ch, generator=g, device=dev) if c["affine"] and c["post"] != "none" else None
+        s["w1"] = _gain(g, ch)
+        s["b1"] = 0.1 * torch.randn(ch, generator=g, device=dev) if c["affine"] else None
+        s["out"], s["y"] = torch.empty_like(s["r"]), torch.empty_like(s["x"])
+    else:
+        m, ch, f, t = c["m"], c["c"], c["f"], _TYPES[c["type"]]
+        s["x"], s["r"] = _acts(g, m, ch).to(t), (2 * _acts(g, m, ch)).to(t)
+        s["gate0"] = (0.5 + 0.5 * torch.randn(1, ch, generator=g, device=dev)).to(t)
+        s["gate1"] = (0.5 + 0.5 * torch.randn(1, ch, generator=g, device=dev)).to(t)
+        s["w0"], s["w1"], s["w2"], s["w3"] = _gain(g, ch), _gain(g, ch), _gain(g, ch), _gain(g, ch)
+        s["uq"], s["us"] = _weight(g, f, ch)
+        s["dq"], s["ds"] = _weight(g, ch, f)
+        s["out"], s["y"] = torch.empty_like(s["r"]), torch.empty_like(s["x"])
+    if own:  # a program of the framework holds its data in the backend's buffers: the same memory, wrapped once
+        _wrap(s)
+    return s
+
+
+def _tile_bytes(rows, k):
+    return ((rows + 127) // 128) * ((_blocks(k) + 3) // 4) * 512
+
+
+def _wrap(s):
+    global _backend
+    import dragonwing_edge_rs_b200 as dw
+    from dragonwing_edge_rs_b200 import ops
+    if _backend is None:
+        _backend = dw.CudaBackend(torch.cuda.current_device())
+    be, c = _backend, s["case"]
+    s["b"] = b = {n: be.wrap(t.data_ptr(), ((t.shape[0] - 1) * t.stride(0) + t.shape[-1] if t.dim() == 2 else t.numel()) * t.element_size())
+                  for n, t in s.items() if isinstance(t, torch.Tensor)}
+    kinds = {"none": ops.NORM_NONE, "rms": ops.NORM_RMS, "layer": ops.NORM_LAYER}
+    types = {"f32": ops.F32, "f16": ops.F16, "bf16": ops.BF16}
+    s["acts"] = {"none": ops.EPI_NONE, "relu": ops.EPI_RELU, "silu": ops.EPI_SILU}
+    s["t"] = t = types[c["type"]]
+    if c["op"] == "norm":
+        s["desc"] = ops.NormDesc(c["rows"], c["c"], t, types[c["res"]], t, kinds[c["pre"]], kinds[c["post"]], 1e-5,
+                                 gate_rows=c["group"], res_scale=0.7)
+    elif c["op"] == "block":
+        m, ch, f = c["m"], c["c"], c["f"]
+        s["desc"] = ops.NormDesc(m, ch, t, t, t, ops.NORM_RMS, ops.NORM_RMS, 1e-5)
+        # the block's intermediate tensors, allocated once
+        b["mid"] = be.alloc(m * ch * 2)
+        b["nq"], b["ns"] = be.alloc(ops.mxfp4_code_bytes(m, ch)), be.alloc(ops.mxfp4_scale_bytes(m, ch))
+        b["hq"], b["hs"] = be.alloc(ops.mxfp4_code_bytes(m, f)), be.alloc(ops.mxfp4_scale_bytes(m, f))
+        b["z"] = be.alloc(m * ch * 2)
+
+
+# ---------------------------------------------------------------------------
+# one pass
+# ---------------------------------------------------------------------------
+
+def run(state):
+    return _run_own(state) if own else _run_plain(state)
+
+
+def _run_own(s):
+    from dragonwing_edge_rs_b200 import ops
+    be, b, c = _backend, s["b"], s["case"]
+    if c["op"] == "quantize":
+        ops.quantize_mxfp4(be, b["x"], s["t"], c["rows"], c["k"], b["q"], b["s"], c["k"] + c["gap"])
+        ops.dequantize_mxfp4(be, b["q"], b["s"], c["rows"], c["k"], b["y"], s["t"])
+        return s["y"]
+    if c["op"] == "gemm":
+        ops.gemm_mxfp4(be, b["aq"], b["as"], b["bq"], b["bs"], b.get("bias"), b["y"], s["t"], c["m"], c["n"], c["k"],
+                       s["acts"][c["act"]])
+        return s["y"]
+    if c["op"] == "norm":
+        ops.norm_residual(be, s["desc"], b["x"], b.get("w0"), b.get("b0"), b.get("gate"), b["r"], b["out"], b["w1"],
+                          b.get("b1"), b["y"])
+        return s["out"], s["y"]
+    m, ch, f = c["m"], c["c"], c["f"]
+    ops.norm_residual_to_mxfp4(be, s["desc"], b["x"], b["w0"], None, b["gate0"], b["r"], b["mid"], b["w1"], None, b["nq"], b["ns"])
+    ops.gemm_to_mxfp4(be, b["nq"], b["ns"], b["uq"], b["us"], None, b["hq"], b["hs"], m, f, ch, ops.EPI_SILU)
+    ops.gemm_mxfp4(be, b["hq"], b["hs"], b["dq"], b["ds"], None, b["z"], s["t"], m, ch, f, ops.EPI_NONE)
+    ops.norm_residual(be, s["desc"], b["z"], b["w2"], None, b["gate1"], b["mid"], b["out"], b["w3"], None, b["y"])
+    return s["out"], s["y"]
+
+
+def _norm(x, kind, w, b):
+    if kind == "none":
+        return x
+    if kind == "layer":
+        x = x - x.mean(-1, keepdim=True)
+    n = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-5)
+    n = n * w if w is not None else n
+    return n + b if b is not None else n
+
+
+def _residual(x, r, kind, w, b, gate, group, scale):
+    n = _norm(x.float(), kind, w, b)
+    if gate is not None:
+        rows = torch.arange(x.shape[0], device=x.device)
+        n = n * gate.float()[rows // group if group else rows * 0]
+    return (r.float() + scale * n).to(r.dtype)
+
+
+def _act(y, act):
+    return torch.clamp(y, min=0) if act == "relu" else y / (1 + torch.exp(-y)) if act == "silu" else y
+
+
+def _run_plain(s):
+    c = s["case"]
+    if c["op"] == "quantize":
+        return _rounded(s["x"].float()).to(s["x"].dtype)
+    if c["op"] == "gemm":
+        m, n, k = c["m"], c["n"], c["k"]
+        y = _values(s["aq"], s["as"], m, k) @ _values(s["bq"], s["bs"], n, k).T
+        y = y + s["bias"] if s["bias"] is not None else y
+        return _act(y, c["act"]).to(s["y"].dtype)
+    if c["op"] == "norm":
+        out = _residual(s["x"], s["r"], c["post"], s["w0"], s["b0"], s["gate"], c["group"], 0.7)
+        return out, _norm(out.float(), c["pre"], s["w1"], s["b1"]).to(s["x"].dtype)
+    m, ch, f = c["m"], c["c"], c["f"]
+    mid = _residual(s["x"], s["r"], "rms", s["w0"], None, s["gate0"], 0, 1.0)
+    h = _rounded(_norm(mid.float(), "rms", s["w1"], None)) @ _values(s["uq"], s["us"], f, ch).T
+    z = (_rounded(_act(h, "silu")) @ _values(s["dq"], s["ds"], ch, f).T).to(s["x"].dtype)
+    out = _residual(z, mid, "rms", s["w2"], None, s["gate1"], 0, 1.0)
+    return out, _norm(out.float(), "rms", s["w3"], None).to(s["x"].dtype)
+
+
+# ---------------------------------------------------------------------------
+# the definitions in 64 bits
+# ---------------------------------------------------------------------------
+
+def _mx64(x):
+    """The MXFP4 rounding of x, by its definition: the nearest of the eight magnitudes, found by their midpoints."""
+    rows, k = x.shape
+    x = torch.nn.functional.pad(x.double(), (0, -k % 32)).unflatten(1, (-1, 32))
+    top = x.abs().amax(-1, keepdim=True)
+    # the largest of the powers of two that 4 X = 2^floor(log2 max|v|) can be
+    powers = torch.tensor([2.0 ** i for i in range(-125, 128)], dtype=torch.float64, device=x.device)
+    X = powers[(torch.searchsorted(powers, top, right=True) - 1).clamp(min=0)] / 4
+    u = x.abs() / X
+    # a tie goes to the even code: up from an odd one, down from an even one
+    up = torch.tensor([0.75, 1.75, 3.5], dtype=torch.float64, device=x.device)
+    down = torch.tensor([0.25, 1.25, 2.5, 5.0], dtype=torch.float64, device=x.device)
+    index = (u.unsqueeze(-1) >= up).sum(-1) + (u.unsqueeze(-1) > down).sum(-1)
+    grid = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64, device=x.device)
+    return (grid[index] * torch.sign(x) * X).flatten(1)[:, :k]
+
+
+def _decode64(codes, tiles, rows, k):
+    row, col = torch.arange(rows, device=codes.device)[:, None], torch.arange(k, device=codes.device)[None]
+    code = (codes[row, col // 2] >> (4 * (col % 2)).to(torch.uint8)) & 15
+    idx = (code & 7).long()
+    mag = torch.where(idx < 2, idx * 0.5, (1 << (idx // 2).clamp(min=1) - 1).double() * (1 + 0.5 * (idx % 2)))
+    block = col // 32
+    at = ((row // 128) * ((_blocks(k) + 3) // 4) + block // 4) * 512 + (row % 32) * 16 + (row % 128) // 32 * 4 + block % 4
+    powers = torch.tensor([2.0 ** (i - 127) for i in range(255)] + [math.nan], dtype=torch.float64, device=codes.device)
+    return mag * (1 - 2 * (code >> 3).double()) * powers[tiles[at].long()]
+
+
+def _norm64(x, kind, w, b):
+    x = x.double()
+    if kind == "none":
+        return x
+    mean = x.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(x[:, :1])
+    var = ((x - mean) ** 2).mean(-1, keepdim=True)
+    n = (x - mean) / torch.sqrt(var + 1e-5)
+    return n * (1.0 if w is None else w.double()) + (0.0 if b is None else b.double())
+
+
+def _gate64(gate, rows, group):
+    if gate is None:
+        return 1.0
+    return gate.double().repeat_interleave(group, 0)[:rows] if group else gate.double()
+
+
+def _act64(y, act):
+    return y * (y > 0) if act == "relu" else y * torch.sigmoid(y) if act == "silu" else y
+
+
+def exact(case, seed):
+    global own
+    was, own = own, False
+    try:
+        s = prepare(case, seed)
+    finally:
+        own = was
+    c = case
+    if c["op"] == "quantize":
+        step = max(1, (1 << 24) // c["k"])
+        return torch.cat([_mx64(s["x"][i:i + step]) for i in range(0, c["rows"], step)])
+    if c["op"] == "gemm":
+        m, n, k = c["m"], c["n"], c["k"]
+        y = _decode64(s["aq"], s["as"], m, k) @ _decode64(s["bq"], s["bs"], n, k).T
+        return _act64(y + (0.0 if s["bias"] is None else s["bias"].double()), c["act"])
+    if c["op"] == "norm":
+        out = s["r"].double() + 0.7 * _gate64(s["gate"], c["rows"], c["group"]) * _norm64(s["x"], c["post"], s["w0"], s["b0"])
+        return out, _norm64(out.to(s["r"].dtype), c["pre"], s["w1"], s["b1"])
+    m, ch, f = c["m"], c["c"], c["f"]
+    t = s["x"].dtype
+    mid = (s["r"].double() + s["gate0"].double() * _norm64(s["x"], "rms", s["w0"], None)).to(t)
+    h = _act64(_mx64(_norm64(mid, "rms", s["w1"], None)) @ _decode64(s["uq"], s["us"], f, ch).T, "silu")
+    z = (_mx64(h) @ _decode64(s["dq"], s["ds"], ch, f).T).to(t)
+    out = mid.double() + s["gate1"].double() * _norm64(z, "rms", s["w2"], None)
+    return out, _norm64(out.to(t), "rms", s["w3"], None)
