@@ -61,6 +61,17 @@ class DwView(ctypes.Structure):
     _fields_ = [("buf", ctypes.c_void_p), ("offset", ctypes.c_size_t), ("pitch", ctypes.c_int32)]
 
 
+# dw_dtype, dw_norm_kind
+F32, F16, BF16 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+
+
+class DwNormDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_size_t) for n in ("rows", "c", "x_pitch", "res_pitch", "y_pitch", "gate_rows")] + \
+        [(n, ctypes.c_int32) for n in ("x_dtype", "res_dtype", "y_dtype", "pre", "post")] + \
+        [("eps", ctypes.c_float), ("res_scale", ctypes.c_float)]
+
+
 # Every exported function with its argument types (restype is dw_status unless listed).
 vp, sz, i32, u32, f32 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint32, ctypes.c_float
 PDESC = ctypes.POINTER(DwConvDesc)
@@ -145,6 +156,18 @@ SIGNATURES = {
     "dw_prepare_yolo_detect": ([vp, ctypes.POINTER(DwYoloDetectDesc), PVP], i32),
     "dw_yolo_detect_i8": ([vp, ctypes.POINTER(DwYoloDetectDesc), vp, PVP, PVP, vp], i32),
     "dw_postprocess_yolo_workspace": ([sz, sz], sz),
+    # MXFP4 operands, their product, residual norms
+    "dw_mxfp4_code_bytes": ([sz, sz], sz),
+    "dw_mxfp4_scale_bytes": ([sz, sz], sz),
+    "dw_quantize_mxfp4": ([vp, vp, i32, sz, sz, sz, vp, vp], i32),
+    "dw_dequantize_mxfp4": ([vp, vp, vp, sz, sz, vp, i32], i32),
+    "dw_pack_scales_mxfp4": ([vp, vp, sz, sz, vp], i32),
+    "dw_gemm_mxfp4": ([vp] * 7 + [i32, sz, sz, sz, i32], i32),
+    "dw_gemm_to_mxfp4": ([vp] * 8 + [sz, sz, sz, i32], i32),
+    "dw_norm": ([vp, ctypes.POINTER(DwNormDesc)] + [vp] * 4, i32),
+    "dw_norm_to_mxfp4": ([vp, ctypes.POINTER(DwNormDesc)] + [vp] * 5, i32),
+    "dw_norm_residual": ([vp, ctypes.POINTER(DwNormDesc)] + [vp] * 9, i32),
+    "dw_norm_residual_to_mxfp4": ([vp, ctypes.POINTER(DwNormDesc)] + [vp] * 10, i32),
     "dw_postprocess_yolo": ([vp, vp, sz, sz, sz, u32, u32, f32, f32, ctypes.c_int32, vp, vp, vp], i32),
 }
 

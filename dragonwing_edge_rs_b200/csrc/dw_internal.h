@@ -154,4 +154,34 @@ dw_status launch_cast_f16_to_f32(dw_backend *be, const uint16_t *x, float *y, si
 dw_status launch_unfold_w_f32_to_f16(dw_backend *be, const float *x, uint16_t *y, int n, int h, int w, int c, int kw,
                                     int sw, int pl, int wo, int c_dst);
 
+// mxfp4.cu (microscaled 4-bit floating point: quantisation, back, scale layout)
+dw_status launch_quantize_mxfp4(dw_backend *be, const void *x, int dtype, size_t rows, size_t k, size_t pitch, uint8_t *q,
+                                uint8_t *s);
+dw_status launch_dequantize_mxfp4(dw_backend *be, const uint8_t *q, const uint8_t *s, size_t rows, size_t k, void *y,
+                                  int dtype);
+dw_status launch_pack_scales_mxfp4(dw_backend *be, const uint8_t *in, size_t rows, size_t k, uint8_t *s);
+
+// mxfp4_gemm.cu (tcgen05 product of two MXFP4 operands); y_s: the result as MXFP4
+struct MxGemmArgs {
+    const uint8_t *a_q, *a_s, *b_q, *b_s;
+    const float *bias;  // may be null
+    void *y;
+    uint8_t *y_s;       // null: y holds y_dtype
+    int y_dtype, act;
+    size_t m, n, k;
+};
+dw_status launch_gemm_mxfp4(dw_backend *be, const MxGemmArgs &a);
+
+// norm.cu (norms around a residual); null pointers: absent
+struct NormArgs {
+    const void *x;
+    const float *w_post, *b_post;
+    const void *gate, *res;
+    void *out;
+    const float *w_pre, *b_pre;
+    void *y;         // y_dtype
+    uint8_t *q, *s;  // or MXFP4
+};
+dw_status launch_norm(dw_backend *be, const dw_norm_desc &d, const NormArgs &a);
+
 }  // namespace dw

@@ -1,0 +1,393 @@
+// mxfp4_gemm.cu -- the product of two MXFP4 operands on the tcgen05 tensor cores
+// (kind::mxf4, block scales in tensor memory), with bias, activation and the
+// rounding or MXFP4 quantisation of the result fused into the epilogue:
+//   y[m, n] = act(sum_k A[m, k] * B[n, k] + bias[n])
+// Products and sums are the tensor core's (f32 accumulators); bias and activation
+// are f32.
+//
+// One persistent CTA per SM, warp-specialised:
+//   warp 0    producer: per 256-wide K block one TMA box of codes of each operand
+//             (128 bytes a row, 128-byte swizzle) and the bulk copies of their
+//             scale tiles, into a ring of stages;
+//   warp 1    allocates tensor memory and issues, per stage, tcgen05.cp of the
+//             scale tiles into that stage's scale columns and four
+//             tcgen05.mma (128 x BN x 64);
+//   warps 2.. epilogue: accumulators -> registers (a thread holds a row, so 32
+//             columns in one thread are one MXFP4 block of the result).
+//
+// Every mbarrier wait is bounded; on expiry the CTA records the failure, waits
+// (bounded) for its own copies and products in flight, frees its tensor memory
+// and exits.
+
+#include <algorithm>
+
+#include "dw_device.cuh"
+#include "dw_mxfp4.cuh"
+#include "dw_ptx.cuh"
+#include "dw_tcgen05.cuh"
+
+namespace dw {
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kBKBytes = 128;  // a K block: 256 codes
+constexpr int kEpiWarps = 4;
+constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
+constexpr size_t kSmemLimit = 227 * 1024;
+
+struct GemmParams {
+    const uint8_t *a_s, *b_s;
+    const float *bias;
+    void *y;
+    uint8_t *y_s;
+    size_t m, n;
+    size_t tiles_k;   // scale tiles (128 codes) along K
+    size_t out_nb, out_tiles;  // MXFP4 result: blocks and scale tiles along n
+    int k_blocks;     // 256-wide K blocks
+    int tiles_m, tiles_n, tiles;
+    int b_row_tiles;  // 128-row scale tiles of B
+    int stages, act;
+    bool vec;         // rows of y start on 16-byte boundaries
+    uint64_t wait_cap_ns;
+    int32_t *err;
+};
+
+// Bounded wait for a phase; false once the CTA is aborting or the cap expired.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const GemmParams &p, volatile int *abort_flag,
+                                           int site) {
+#pragma unroll 1
+    for (int i = 0; i < 64; i++)
+        if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+    for (;;) {
+        if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+        if (*abort_flag) return false;
+        if (globaltimer_ns() - t0 > p.wait_cap_ns) {
+            *abort_flag = 1;
+            record_error(p.err, DW_DEV_WAIT_EXPIRED, site, (int)parity);
+            return false;
+        }
+    }
+}
+
+// Waits for a phase that the CTA's own work in flight completes, whatever happened before.
+__device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, const GemmParams &p) {
+    const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+    while (!mbar_try_wait_sleep(bar, parity, 20000u))
+        if (globaltimer_ns() - t0 > p.wait_cap_ns) return;
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// 512 bytes (32 rows of 16) -> 4 columns of all four lane quarters of tensor memory.
+__device__ __forceinline__ void tc_cp_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// One 128 x N x 64 product with block scales (two 32-wide blocks per row).
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+// silu(v) = v / (1 + e^-v): ex2.approx through __expf (2 ulp plus |v| * 2^-24
+// relative) and a correctly rounded division.
+__device__ __forceinline__ float activate(float v, int act) {
+    if (act == DW_EPI_RELU) return fmaxf(v, 0.0f);
+    if (act == DW_EPI_SILU) return __fdiv_rn(v, 1.0f + __expf(-v));
+    return v;
+}
+
+// Instruction descriptor of kind::mxf4: A, B e2m1 (1 at bits 7-9 and 10-12), N >> 3
+// at bits 17-22, scales ue8m0 (bit 23), M >> 4 at bits 24-28; the scale byte pair
+// that a 64-wide step reads: bits 29-30 (A) and 4-5 (B).
+constexpr uint32_t mx_idesc(int m, int n, int pair) {
+    return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) |
+           ((uint32_t)(2 * pair) << 29) | ((uint32_t)(2 * pair) << 4);
+}
+
+// What the epilogue stores: 0 f32, 1 f16, 2 bf16, 3 MXFP4.
+template <int kOut>
+__device__ __forceinline__ void put32(float (&v)[32], size_t row, size_t col, const GemmParams &p, uint32_t &scale) {
+    if constexpr (kOut == 3) {
+#pragma unroll
+        for (int i = 0; i < 32; i++)
+            if (col + i >= p.n) v[i] = 0.0f;
+        uint4 codes;
+        scale = mx_quantize32(v, codes);
+        if (row < p.m && col < p.n) *reinterpret_cast<uint4 *>((uint8_t *)p.y + (row * p.out_nb + col / 32) * 16) = codes;
+    } else {
+        using T = std::conditional_t<kOut == 0, float, std::conditional_t<kOut == 1, __half, __nv_bfloat16>>;
+        if (row >= p.m) return;
+        T *dst = (T *)p.y + row * p.n + col;
+        if (p.vec && col + 32 <= p.n) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                Raw<T, 8> r;
+                float t[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) t[i] = v[8 * g + i];
+                r.set(t);
+                r.store(dst + 8 * g);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+                if (col + i < p.n) dst[i] = from_f32<T>(v[i]);
+        }
+    }
+}
+
+template <int BN, int kOut>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    k_mxfp4_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                 const __grid_constant__ GemmParams p) {
+    constexpr uint32_t kA = kBM * kBKBytes, kB = BN * kBKBytes, kSA = 1024, kSB = (BN / 128) * 1024;
+    constexpr uint32_t kStage = kA + kB + kSA + kSB;
+    constexpr uint32_t kScaleCols = 8 + BN / 16;  // tensor-memory columns of a stage's scales
+    constexpr int kMaxStages = 8;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+    __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tfull_bar[2], tempty_bar[2], drain_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int *abort_flag = &abort_word;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; s++) {
+            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        for (int a = 0; a < 2; a++) {
+            mbar_init(smem_u32(&tfull_bar[a]), 1);
+            mbar_init(smem_u32(&tempty_bar[a]), kEpiWarps);
+        }
+        mbar_init(smem_u32(&drain_bar), 1);
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const uint32_t sf_cols = tmem + 2 * BN;  // scales after the two accumulators
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+                const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
+                for (int kb = 0; kb < p.k_blocks; kb++) {
+                    if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p, abort_flag, 21)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t bar = smem_u32(&full_bar[s]), base = smem + s * kStage;
+                    const uint32_t sbytes = (uint32_t)min((size_t)2, p.tiles_k - 2 * (size_t)kb) * 512;
+                    const int nsb = min(BN / 128, p.b_row_tiles - tn * (BN / 128));
+                    mbar_expect_tx(bar, kA + kB + sbytes * (1 + nsb));
+                    tma_load_2d(base, &tmap_a, bar, kb * kBKBytes, tm * kBM);
+                    tma_load_2d(base + kA, &tmap_b, bar, kb * kBKBytes, tn * BN);
+                    bulk_load(base + kA + kB, p.a_s + ((size_t)tm * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
+                    for (int j = 0; j < nsb; j++)
+                        bulk_load(base + kA + kB + kSA + j * 1024,
+                                  p.b_s + (((size_t)tn * (BN / 128) + j) * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
+                    issued++;
+                    if (++s == p.stages) s = 0, ph ^= 1;
+                }
+            }
+            // the last copies into each stage have landed before the CTA ends
+            for (int i = 0; i < min(issued, p.stages); i++) {
+                if (--s < 0) s = p.stages - 1, ph ^= 1;
+                drain_phase(smem_u32(&full_bar[s]), ph, p);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int s = 0, acc = 0;
+            uint32_t ph = 0, aph = 0;
+            bool ok = true;
+            const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
+            for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+                if (!wait_phase(smem_u32(&tempty_bar[acc]), aph ^ 1u, p, abort_flag, 22)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + acc * BN;
+                for (int kb = 0; kb < p.k_blocks; kb++) {
+                    if (!wait_phase(smem_u32(&full_bar[s]), ph, p, abort_flag, 23)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t base = smem + s * kStage;
+                    const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 8;
+                    const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
+                    for (int c = 0; c < chunks; c++) {
+                        tc_cp_scales(sfa + c * 4, smem_desc_noswz(base + kA + kB + c * 512, 16, 128));
+#pragma unroll
+                        for (int j = 0; j < BN / 128; j++)
+                            tc_cp_scales(sfb + c * (BN / 32) + j * 4,
+                                         smem_desc_noswz(base + kA + kB + kSA + j * 1024 + c * 512, 16, 128));
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t off = (uint32_t)(c * 2 + h) * 32;
+                            tc_mma_mxf4(d, smem_desc(base + off, hi), smem_desc(base + kA + off, hi), mx_idesc(kBM, BN, h),
+                                        sfa + c * 4, sfb + c * (BN / 32), (kb | c | h) ? 1u : 0u);
+                        }
+                    }
+                    tc_commit(smem_u32(&empty_bar[s]));
+                    if (++s == p.stages) s = 0, ph ^= 1;
+                }
+                if (!ok) break;
+                tc_commit(smem_u32(&tfull_bar[acc]));
+                acc ^= 1;
+                if (!acc) aph ^= 1;
+            }
+            tc_commit(smem_u32(&drain_bar));
+            drain_phase(smem_u32(&drain_bar), 0, p);
+        }
+    } else {
+        const int quarter = warp & 3;  // tensor-memory lanes this warp may read
+        int acc = 0;
+        uint32_t aph = 0;
+        for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+            const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
+            if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&tfull_bar[acc]), aph, p, abort_flag, 24))) break;
+            tc_fence_after();
+            const size_t row = (size_t)tm * kBM + quarter * 32 + lane;
+            const uint32_t base = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+            for (int t = 0; t < BN / 128; t++) {
+                uint32_t scales = 0;
+#pragma unroll 1
+                for (int g = 0; g < 4; g++) {
+                    const int c0 = t * 128 + g * 32;
+                    const size_t col = (size_t)tn * BN + c0;
+                    uint32_t r[32];
+                    tc_ld32(base + c0, r);
+                    tc_wait_ld();
+                    if (t == BN / 128 - 1 && g == 3) {  // accumulators read: the next tile may overwrite them
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
+                    }
+                    if (col >= p.n) continue;
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        v[i] = __uint_as_float(r[i]);
+                        if (p.bias && col + i < p.n) v[i] += __ldg(p.bias + col + i);
+                        v[i] = activate(v[i], p.act);
+                    }
+                    uint32_t sb = 0;
+                    put32<kOut>(v, row, col, p, sb);
+                    scales |= sb << (8 * g);
+                }
+                if constexpr (kOut == 3) {
+                    const size_t st = (size_t)tn * (BN / 128) + t;
+                    if (row < p.m && st < p.out_tiles)
+                        *reinterpret_cast<uint32_t *>(p.y_s + mx_scale_at(row, st * 4, p.out_tiles)) = scales;
+                }
+            }
+            acc ^= 1;
+            if (!acc) aph ^= 1;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Codes as a 2-D byte tensor [rows][bytes of a row]; a box is 128 bytes of `box_rows` rows.
+bool code_map(dw_backend *be, CUtensorMap *map, const uint8_t *q, size_t rows, size_t k, int box_rows) {
+    cuuint64_t dims[2] = {(cuuint64_t)mx_blocks(k) * 16, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)mx_blocks(k) * 16};
+    cuuint32_t box[2] = {(cuuint32_t)kBKBytes, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return be->encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(q), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, int kOut>
+dw_status launch(dw_backend *be, const MxGemmArgs &a) {
+    constexpr size_t kStage = kBM * kBKBytes + BN * kBKBytes + 1024 + (BN / 128) * 1024;
+    GemmParams p{};
+    p.a_s = a.a_s, p.b_s = a.b_s, p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
+    p.m = a.m, p.n = a.n;
+    p.tiles_k = mx_tiles(a.k);
+    p.out_nb = mx_blocks(a.n), p.out_tiles = mx_tiles(a.n);
+    p.k_blocks = (int)((a.k + 255) / 256);
+    const size_t tm = (a.m + kBM - 1) / kBM, tn = (a.n + BN - 1) / BN;
+    if (tm * tn > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu x %zu is too large", a.m, a.n);
+    p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.tiles = (int)(tm * tn);
+    p.b_row_tiles = (int)((a.n + 127) / 128);
+    p.act = a.act;
+    const size_t es = kOut == 0 ? 4 : 2;
+    p.vec = ((uintptr_t)a.y & 15) == 0 && a.n * es % 16 == 0;
+    p.wait_cap_ns = be->wait_cap_ns, p.err = be->dev_err;
+    p.stages = (int)((kSmemLimit - 4096) / kStage);
+    // at least 116 KiB: one CTA per SM owns the tensor memory
+    const size_t smem = std::max<size_t>(1024 + p.stages * kStage, 116 * 1024);
+    CUtensorMap ta, tb;
+    if (!be->encode_tiled || !code_map(be, &ta, a.a_q, a.m, a.k, kBM) || !code_map(be, &tb, a.b_q, a.n, a.k, BN))
+        return dw_fail(be, DW_ERR_DEVICE, "gemm_mxfp4: tensor map rejected");
+    auto kernel = k_mxfp4_gemm<BN, kOut>;
+    static bool attr_set[16] = {};
+    if (be->device < 16 && !attr_set[be->device]) {
+        dw_status st = dw_cuda_check(
+            be, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemLimit - 2048)),
+            "gemm_mxfp4 attributes");
+        if (st != DW_OK) return st;
+        attr_set[be->device] = true;
+    }
+    kernel<<<std::min(p.tiles, be->sm_count), kGemmThreads, smem, be->stream>>>(ta, tb, p);
+    return dw_after_launch(be, "gemm_mxfp4");
+}
+
+}  // namespace
+
+dw_status launch_gemm_mxfp4(dw_backend *be, const MxGemmArgs &a) {
+    if (a.y_s) return launch<128, 3>(be, a);
+    switch (a.y_dtype) {
+        case DW_F32: return launch<128, 0>(be, a);
+        case DW_F16: return launch<128, 1>(be, a);
+        default: return launch<128, 2>(be, a);
+    }
+}
+
+}  // namespace dw

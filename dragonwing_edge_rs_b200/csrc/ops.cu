@@ -899,4 +899,218 @@ DW_API dw_status dw_cast_f16_to_f32(dw_backend *be, const dw_buf *x_f16, dw_buf 
     return dw::launch_cast_f16_to_f32(be, (const uint16_t *)x_f16->ptr, (float *)y_f32->ptr, x_f16->len / 2);
 }
 
+// ---------------------------------------------------------------------------
+// MXFP4 operands, their product, residual norms
+// ---------------------------------------------------------------------------
+
+namespace {
+
+size_t mx_nb(size_t k) { return k / 32 + (k % 32 != 0); }
+
+// a * b * c does not pass 2^62.
+bool fits62(size_t a, size_t b, size_t c) {
+    const long double v = (long double)a * (long double)b * (long double)c;
+    return v < 4.6e18L;
+}
+
+dw_status check_dtype(dw_backend *be, int dtype, const char *op, const char *name) {
+    if (dtype < DW_F32 || dtype > DW_BF16) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: unknown %s %d", op, name, dtype);
+    return DW_OK;
+}
+
+size_t esize(int dtype) { return dtype == DW_F32 ? 4 : 2; }
+
+dw_status check_align(dw_backend *be, const dw_buf *b, size_t a, const char *op, const char *name) {
+    if ((uintptr_t)b->ptr % a) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %s must be %zu-byte aligned", op, name, a);
+    return DW_OK;
+}
+
+// A present tensor of exactly `n` elements of `es` bytes.
+dw_status check_vec(dw_backend *be, const dw_buf *b, size_t n, size_t es, const char *op, const char *name) {
+    DW_TRY(need(be, b, op, name));
+    DW_TRY(check_len(be, b, n * es, op, name));
+    return check_align(be, b, es, op, name);
+}
+
+// A present [rows, c] tensor with rows `pitch` elements apart (0: c, exact length).
+dw_status check_rows(dw_backend *be, const dw_buf *b, size_t rows, size_t c, size_t pitch, size_t es, const char *op,
+                     const char *name) {
+    DW_TRY(need(be, b, op, name));
+    if (pitch && pitch < c) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %s pitch %zu is below the row's %zu", op, name, pitch, c);
+    if (!fits62(rows, pitch ? pitch : c, es)) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %s is too large", op, name);
+    const size_t len = pitch ? ((rows - 1) * pitch + c) * es : rows * c * es;
+    if (pitch && pitch != c ? b->len < len : b->len != len)
+        return dw_fail(be, DW_ERR_SIZE_MISMATCH, "%s: %s mismatch: expected %zu, got %zu", op, name, len, b->len);
+    return check_align(be, b, es, op, name);
+}
+
+dw_status check_operand(dw_backend *be, const dw_buf *q, const dw_buf *s, size_t rows, size_t k, const char *op,
+                        const char *name) {
+    if (!q || !s) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %s is null", op, name);
+    DW_TRY(check_len(be, q, dw_mxfp4_code_bytes(rows, k), op, name));
+    DW_TRY(check_len(be, s, dw_mxfp4_scale_bytes(rows, k), op, "scales"));
+    DW_TRY(check_align(be, q, 16, op, name));
+    return check_align(be, s, 16, op, "scales");
+}
+
+dw_status check_dims(dw_backend *be, size_t a, size_t b, const char *op) {
+    if (!a || !b) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: zero dimension", op);
+    if (a > 0x7fffffff || b > 0x7fffffff) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: dimension exceeds int32", op);
+    return DW_OK;
+}
+
+dw_status gemm_mx(dw_backend *be, const dw_buf *a_q, const dw_buf *a_s, const dw_buf *b_q, const dw_buf *b_s,
+                  const dw_buf *bias, dw_buf *y, dw_buf *y_s, int y_dtype, size_t m, size_t n, size_t k, int act,
+                  const char *op) {
+    if (!be) return DW_ERR_INVALID_ARG;
+    DW_TRY(check_dims(be, m, n, op));
+    DW_TRY(check_dims(be, k, 1, op));
+    if (act != DW_EPI_NONE && act != DW_EPI_RELU && act != DW_EPI_SILU)
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: activation %d is not NONE, RELU or SILU", op, act);
+    DW_TRY(check_operand(be, a_q, a_s, m, k, op, "A"));
+    DW_TRY(check_operand(be, b_q, b_s, n, k, op, "B"));
+    if (bias) DW_TRY(check_vec(be, bias, n, 4, op, "bias"));
+    if (y_s) {
+        DW_TRY(check_operand(be, y, y_s, m, n, op, "Y"));
+    } else {
+        DW_TRY(check_dtype(be, y_dtype, op, "y_dtype"));
+        DW_TRY(check_rows(be, y, m, n, 0, esize(y_dtype), op, "Y"));
+    }
+    dw::MxGemmArgs a{};
+    a.a_q = (const uint8_t *)a_q->ptr, a.a_s = (const uint8_t *)a_s->ptr;
+    a.b_q = (const uint8_t *)b_q->ptr, a.b_s = (const uint8_t *)b_s->ptr;
+    a.bias = bias ? (const float *)bias->ptr : nullptr;
+    a.y = y->ptr, a.y_s = y_s ? (uint8_t *)y_s->ptr : nullptr;
+    a.y_dtype = y_dtype, a.act = act, a.m = m, a.n = n, a.k = k;
+    cudaSetDevice(be->device);
+    return dw::launch_gemm_mxfp4(be, a);
+}
+
+// The checks that the four norm entry points share; `residual`: the fused form.
+dw_status norm_mx(dw_backend *be, const dw_norm_desc *d, const dw_buf *x, const dw_buf *w_post, const dw_buf *b_post,
+                  const dw_buf *gate, const dw_buf *res, dw_buf *out, const dw_buf *w_pre, const dw_buf *b_pre, dw_buf *y,
+                  dw_buf *q, dw_buf *s, bool residual, bool quantized, const char *op) {
+    if (!be) return DW_ERR_INVALID_ARG;
+    if (!d) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: descriptor is null", op);
+    DW_TRY(check_dims(be, d->rows, d->c, op));
+    DW_TRY(check_dtype(be, d->x_dtype, op, "x_dtype"));
+    if (d->pre < DW_NORM_NONE || d->pre > DW_NORM_LAYER || d->post < DW_NORM_NONE || d->post > DW_NORM_LAYER)
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: unknown norm kind", op);
+    if (!(d->eps >= 0.0f)) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: eps must be >= 0", op);
+    DW_TRY(check_rows(be, x, d->rows, d->c, d->x_pitch, esize(d->x_dtype), op, "x"));
+    const dw_buf *ws[4] = {w_post, b_post, w_pre, b_pre};
+    for (const dw_buf *w : ws)
+        if (w) DW_TRY(check_vec(be, w, d->c, 4, op, "norm weight"));
+    if (residual) {
+        DW_TRY(check_dtype(be, d->res_dtype, op, "res_dtype"));
+        if (d->res_dtype != d->x_dtype && d->res_dtype != DW_F32)
+            return dw_fail(be, DW_ERR_UNSUPPORTED, "%s: res_dtype must be x_dtype or F32", op);
+        if (!(d->res_scale == d->res_scale)) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: res_scale is NaN", op);
+        DW_TRY(check_rows(be, res, d->rows, d->c, d->res_pitch, esize(d->res_dtype), op, "residual"));
+        DW_TRY(check_rows(be, out, d->rows, d->c, d->res_pitch, esize(d->res_dtype), op, "out"));
+        if (gate) {
+            const size_t rows = d->gate_rows ? (d->rows - 1) / d->gate_rows + 1 : 1;
+            DW_TRY(check_rows(be, gate, rows, d->c, 0, esize(d->x_dtype), op, "gate"));
+        }
+    }
+    if (quantized) {
+        DW_TRY(check_operand(be, q, s, d->rows, d->c, op, "q"));
+    } else if (y || !residual) {
+        DW_TRY(check_dtype(be, d->y_dtype, op, "y_dtype"));
+        DW_TRY(check_rows(be, y, d->rows, d->c, d->y_pitch, esize(d->y_dtype), op, "y"));
+    }
+    dw::NormArgs a{};
+    auto f = [](const dw_buf *b) { return b ? (const float *)b->ptr : nullptr; };
+    a.x = x->ptr;
+    a.w_post = f(w_post), a.b_post = f(b_post), a.w_pre = f(w_pre), a.b_pre = f(b_pre);
+    if (residual) a.gate = gate ? gate->ptr : nullptr, a.res = res->ptr, a.out = out->ptr;
+    if (quantized)
+        a.q = (uint8_t *)q->ptr, a.s = (uint8_t *)s->ptr;
+    else
+        a.y = y ? y->ptr : nullptr;
+    cudaSetDevice(be->device);
+    return dw::launch_norm(be, *d, a);
+}
+
+}  // namespace
+
+DW_API size_t dw_mxfp4_code_bytes(size_t rows, size_t k) { return rows * mx_nb(k) * 16; }
+DW_API size_t dw_mxfp4_scale_bytes(size_t rows, size_t k) {
+    return ((rows + 127) / 128) * ((mx_nb(k) + 3) / 4) * 512;
+}
+
+DW_API dw_status dw_quantize_mxfp4(dw_backend *be, const dw_buf *x, int dtype, size_t rows, size_t k, size_t x_pitch,
+                                   dw_buf *q, dw_buf *s) {
+    const char *op = "quantize_mxfp4";
+    if (!be) return DW_ERR_INVALID_ARG;
+    DW_TRY(check_dims(be, rows, k, op));
+    DW_TRY(check_dtype(be, dtype, op, "dtype"));
+    DW_TRY(check_rows(be, x, rows, k, x_pitch, esize(dtype), op, "x"));
+    DW_TRY(check_operand(be, q, s, rows, k, op, "q"));
+    cudaSetDevice(be->device);
+    return dw::launch_quantize_mxfp4(be, x->ptr, dtype, rows, k, x_pitch ? x_pitch : k, (uint8_t *)q->ptr, (uint8_t *)s->ptr);
+}
+
+DW_API dw_status dw_dequantize_mxfp4(dw_backend *be, const dw_buf *q, const dw_buf *s, size_t rows, size_t k, dw_buf *y,
+                                     int dtype) {
+    const char *op = "dequantize_mxfp4";
+    if (!be) return DW_ERR_INVALID_ARG;
+    DW_TRY(check_dims(be, rows, k, op));
+    DW_TRY(check_dtype(be, dtype, op, "dtype"));
+    DW_TRY(check_operand(be, q, s, rows, k, op, "q"));
+    DW_TRY(check_rows(be, y, rows, k, 0, esize(dtype), op, "y"));
+    cudaSetDevice(be->device);
+    return dw::launch_dequantize_mxfp4(be, (const uint8_t *)q->ptr, (const uint8_t *)s->ptr, rows, k, y->ptr, dtype);
+}
+
+DW_API dw_status dw_pack_scales_mxfp4(dw_backend *be, const dw_buf *scales, size_t rows, size_t k, dw_buf *s) {
+    const char *op = "pack_scales_mxfp4";
+    if (!be) return DW_ERR_INVALID_ARG;
+    DW_TRY(check_dims(be, rows, k, op));
+    DW_TRY(check_vec(be, scales, rows * mx_nb(k), 1, op, "row-major scales"));
+    DW_TRY(need(be, s, op, "scales"));
+    DW_TRY(check_len(be, s, dw_mxfp4_scale_bytes(rows, k), op, "scales"));
+    DW_TRY(check_align(be, s, 16, op, "scales"));
+    cudaSetDevice(be->device);
+    return dw::launch_pack_scales_mxfp4(be, (const uint8_t *)scales->ptr, rows, k, (uint8_t *)s->ptr);
+}
+
+DW_API dw_status dw_gemm_mxfp4(dw_backend *be, const dw_buf *a_q, const dw_buf *a_s, const dw_buf *b_q, const dw_buf *b_s,
+                               const dw_buf *bias, dw_buf *y, int y_dtype, size_t m, size_t n, size_t k, int act) {
+    return gemm_mx(be, a_q, a_s, b_q, b_s, bias, y, nullptr, y_dtype, m, n, k, act, "gemm_mxfp4");
+}
+
+DW_API dw_status dw_gemm_to_mxfp4(dw_backend *be, const dw_buf *a_q, const dw_buf *a_s, const dw_buf *b_q,
+                                  const dw_buf *b_s, const dw_buf *bias, dw_buf *y_q, dw_buf *y_s, size_t m, size_t n,
+                                  size_t k, int act) {
+    const char *op = "gemm_to_mxfp4";
+    if (!be) return DW_ERR_INVALID_ARG;
+    DW_TRY(need(be, y_s, op, "Y scales"));
+    return gemm_mx(be, a_q, a_s, b_q, b_s, bias, y_q, y_s, DW_F32, m, n, k, act, op);
+}
+
+DW_API dw_status dw_norm(dw_backend *be, const dw_norm_desc *d, const dw_buf *x, const dw_buf *w, const dw_buf *b,
+                         dw_buf *y) {
+    return norm_mx(be, d, x, nullptr, nullptr, nullptr, nullptr, nullptr, w, b, y, nullptr, nullptr, false, false, "norm");
+}
+
+DW_API dw_status dw_norm_to_mxfp4(dw_backend *be, const dw_norm_desc *d, const dw_buf *x, const dw_buf *w,
+                                  const dw_buf *b, dw_buf *q, dw_buf *s) {
+    return norm_mx(be, d, x, nullptr, nullptr, nullptr, nullptr, nullptr, w, b, nullptr, q, s, false, true, "norm_to_mxfp4");
+}
+
+DW_API dw_status dw_norm_residual(dw_backend *be, const dw_norm_desc *d, const dw_buf *x, const dw_buf *w_post,
+                                  const dw_buf *b_post, const dw_buf *gate, const dw_buf *residual, dw_buf *out,
+                                  const dw_buf *w_pre, const dw_buf *b_pre, dw_buf *y) {
+    return norm_mx(be, d, x, w_post, b_post, gate, residual, out, w_pre, b_pre, y, nullptr, nullptr, true, false,
+                   "norm_residual");
+}
+
+DW_API dw_status dw_norm_residual_to_mxfp4(dw_backend *be, const dw_norm_desc *d, const dw_buf *x, const dw_buf *w_post,
+                                           const dw_buf *b_post, const dw_buf *gate, const dw_buf *residual, dw_buf *out,
+                                           const dw_buf *w_pre, const dw_buf *b_pre, dw_buf *q, dw_buf *s) {
+    return norm_mx(be, d, x, w_post, b_post, gate, residual, out, w_pre, b_pre, nullptr, q, s, true, true,
+                   "norm_residual_to_mxfp4");
+}
+
 }  // extern "C"

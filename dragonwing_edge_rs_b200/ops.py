@@ -324,6 +324,104 @@ def im2col_u8_to_i8(backend, x, y, n, h, w, c, k_h, k_w, s_h, s_w, p_t, p_l, h_o
 
 
 # ---------------------------------------------------------------------------
+# 4-bit transformer blocks: MXFP4 operands, their product, residual norms
+# (contracts in include/dw_cuda.h)
+# ---------------------------------------------------------------------------
+
+F32, F16, BF16 = L.F32, L.F16, L.BF16
+NORM_NONE, NORM_RMS, NORM_LAYER = L.NORM_NONE, L.NORM_RMS, L.NORM_LAYER
+
+
+def mxfp4_code_bytes(rows: int, k: int) -> int:
+    """Bytes of the code buffer of an MXFP4 operand [rows, k]."""
+    return int(L.load().dw_mxfp4_code_bytes(rows, k))
+
+
+def mxfp4_scale_bytes(rows: int, k: int) -> int:
+    """Bytes of the scale buffer of an MXFP4 operand [rows, k]."""
+    return int(L.load().dw_mxfp4_scale_bytes(rows, k))
+
+
+def quantize_mxfp4(backend: CudaBackend, x: CudaBuffer, dtype: int, rows: int, k: int, q: CudaBuffer, s: CudaBuffer,
+                   x_pitch: int = 0):
+    """x [rows, k] of `dtype` (rows x_pitch elements apart) -> MXFP4 codes q and scales s."""
+    backend._check(L.load().dw_quantize_mxfp4(backend.handle, _h(x), dtype, rows, k, x_pitch, _h(q), _h(s)))
+
+
+def dequantize_mxfp4(backend: CudaBackend, q: CudaBuffer, s: CudaBuffer, rows: int, k: int, y: CudaBuffer, dtype: int):
+    """The values [rows, k] of an MXFP4 operand, as `dtype`."""
+    backend._check(L.load().dw_dequantize_mxfp4(backend.handle, _h(q), _h(s), rows, k, _h(y), dtype))
+
+
+def pack_scales_mxfp4(backend: CudaBackend, scales: CudaBuffer, rows: int, k: int, s: CudaBuffer):
+    """Row-major scale bytes [rows, ceil(k / 32)] -> an operand's scale buffer."""
+    backend._check(L.load().dw_pack_scales_mxfp4(backend.handle, _h(scales), rows, k, _h(s)))
+
+
+def gemm_mxfp4(backend: CudaBackend, a_q, a_s, b_q, b_s, bias, y, y_dtype: int, m: int, n: int, k: int,
+               act: int = EPI_NONE):
+    """y[m, n] = act(sum_k A[m, k] * B[n, k] + bias[n]) of two MXFP4 operands."""
+    backend._check(L.load().dw_gemm_mxfp4(backend.handle, _h(a_q), _h(a_s), _h(b_q), _h(b_s), _h(bias), _h(y), y_dtype,
+                                          m, n, k, act))
+
+
+def gemm_to_mxfp4(backend: CudaBackend, a_q, a_s, b_q, b_s, bias, y_q, y_s, m: int, n: int, k: int,
+                  act: int = EPI_NONE):
+    """gemm_mxfp4 with its f32 result quantised to an MXFP4 operand [m, n]."""
+    backend._check(L.load().dw_gemm_to_mxfp4(backend.handle, _h(a_q), _h(a_s), _h(b_q), _h(b_s), _h(bias), _h(y_q),
+                                             _h(y_s), m, n, k, act))
+
+
+@dataclass
+class NormDesc:
+    """Rows of c values, their types, the norm of the next block's input (pre) and
+    of the block's output (post), and how the residual is joined."""
+
+    rows: int
+    c: int
+    x_dtype: int
+    res_dtype: int
+    y_dtype: int
+    pre: int = NORM_RMS
+    post: int = NORM_NONE
+    eps: float = 1e-5
+    gate_rows: int = 0
+    res_scale: float = 1.0
+    x_pitch: int = 0
+    res_pitch: int = 0
+    y_pitch: int = 0
+
+    def to_c(self) -> L.DwNormDesc:
+        return L.DwNormDesc(self.rows, self.c, self.x_pitch, self.res_pitch, self.y_pitch, self.gate_rows, self.x_dtype,
+                            self.res_dtype, self.y_dtype, self.pre, self.post, self.eps, self.res_scale)
+
+
+def norm(backend: CudaBackend, desc: NormDesc, x, w, b, y):
+    """y = pre(x) with weight w and bias b (f32 [c] or None)."""
+    backend._check(L.load().dw_norm(backend.handle, ctypes.byref(desc.to_c()), _h(x), _h(w), _h(b), _h(y)))
+
+
+def norm_to_mxfp4(backend: CudaBackend, desc: NormDesc, x, w, b, q, s):
+    """norm with its f32 result quantised to an MXFP4 operand."""
+    backend._check(L.load().dw_norm_to_mxfp4(backend.handle, ctypes.byref(desc.to_c()), _h(x), _h(w), _h(b), _h(q), _h(s)))
+
+
+def norm_residual(backend: CudaBackend, desc: NormDesc, x, w_post, b_post, gate, residual, out, w_pre=None, b_pre=None,
+                  y=None):
+    """out = residual + res_scale * gate * post(x); y = pre(out) (None: `out` alone)."""
+    backend._check(L.load().dw_norm_residual(backend.handle, ctypes.byref(desc.to_c()), _h(x), _h(w_post), _h(b_post),
+                                             _h(gate), _h(residual), _h(out), _h(w_pre), _h(b_pre), _h(y)))
+
+
+def norm_residual_to_mxfp4(backend: CudaBackend, desc: NormDesc, x, w_post, b_post, gate, residual, out, w_pre, b_pre,
+                           q, s):
+    """norm_residual with y quantised to an MXFP4 operand."""
+    backend._check(L.load().dw_norm_residual_to_mxfp4(backend.handle, ctypes.byref(desc.to_c()), _h(x), _h(w_post),
+                                                      _h(b_post), _h(gate), _h(residual), _h(out), _h(w_pre), _h(b_pre),
+                                                      _h(q), _h(s)))
+
+
+# ---------------------------------------------------------------------------
 # YOLOv8 Detect tail and detection post-processing
 # (crates/dragonwing-onnx/src/postprocess.rs)
 # ---------------------------------------------------------------------------

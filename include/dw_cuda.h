@@ -495,6 +495,94 @@ DW_API dw_status dw_unfold_w_f32_to_f16(dw_backend *be, const dw_buf *x_f32, dw_
 /* f16 -> f32 with F16::to_f32. */
 DW_API dw_status dw_cast_f16_to_f32(dw_backend *be, const dw_buf *x_f16, dw_buf *y_f32);
 
+/* ---------------------------------------------------------------------- */
+/* 4-bit transformer blocks: MXFP4 operands, their product, residual norms  */
+/* ---------------------------------------------------------------------- */
+/* Additions: the reference has neither a 4-bit format nor norms (it folds batch
+ * norms into convs).  All work is asynchronous on the backend's stream; nothing
+ * here allocates, so every call may be captured.  Conversions to and from f16 and
+ * bf16 are IEEE round-to-nearest-even (subnormal halves keep their value, unlike
+ * in the F16 ops above).  A dimension of 0 is DW_ERR_INVALID_ARG.
+ *
+ * MXFP4 (OCP microscaling, e2m1 elements, e8m0 scales): a row of k values is cut
+ * into nb = ceil(k / 32) blocks of 32 (the last may be short).  A block's scale is
+ * X = 2^(floor(log2 max|v|) - 2), at least 2^-127, held as the byte log2(X) + 127; a value
+ * is held as a sign and the index of the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 to
+ * |v| / X (a tie goes to the even index, more than 6 to 6).  A block with a NaN or
+ * an infinity has the scale byte 255 (NaN) and codes 0: its values are all NaN.
+ * An operand of `rows` rows is two buffers, both 16-byte aligned:
+ *   codes   dw_mxfp4_code_bytes(rows, k) = rows * 16 nb bytes: row-major, two codes a byte,
+ *           the even element in the low four bits; elements past k are 0;
+ *   scales  dw_mxfp4_scale_bytes(rows, k) = ceil(rows / 128) * ceil(nb / 4) * 512 bytes:
+ *           tiles of 128 rows x 4 blocks, those of a group of rows one after the other;
+ *           row r, block b is byte (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4 of tile
+ *           (r / 128, b / 4).  Places past the last block hold 0; places past the last row
+ *           are neither written nor used. */
+enum dw_dtype { DW_F32 = 0, DW_F16 = 1, DW_BF16 = 2 };
+
+DW_API size_t dw_mxfp4_code_bytes(size_t rows, size_t k);
+DW_API size_t dw_mxfp4_scale_bytes(size_t rows, size_t k);
+
+/* x [rows, k] of `dtype`, rows x_pitch elements apart (0: k), rounded to MXFP4. */
+DW_API dw_status dw_quantize_mxfp4(dw_backend *be, const dw_buf *x, int dtype, size_t rows, size_t k, size_t x_pitch,
+                                   dw_buf *q, dw_buf *s);
+/* The values an operand stands for, y [rows, k] of `dtype` (rounded to it; f32 and
+ * bf16 hold them exactly). */
+DW_API dw_status dw_dequantize_mxfp4(dw_backend *be, const dw_buf *q, const dw_buf *s, size_t rows, size_t k, dw_buf *y,
+                                     int dtype);
+/* Row-major scale bytes [rows, nb] (the form of stored checkpoints, whose codes need
+ * no change) -> the operand's scale buffer. */
+DW_API dw_status dw_pack_scales_mxfp4(dw_backend *be, const dw_buf *scales, size_t rows, size_t k, dw_buf *s);
+
+/* y[m, n] = act(sum_k A[m, k] * B[n, k] + bias[n]): A an operand of m rows, B (a
+ * weight, [out, in]) one of n rows, bias f32 [n] or NULL, act DW_EPI_NONE,
+ * DW_EPI_RELU or DW_EPI_SILU in f32, y [m, n] of y_dtype, rounded once.  Sums are
+ * f32, in an order that depends on m, n and k alone.  y overlaps no operand. */
+DW_API dw_status dw_gemm_mxfp4(dw_backend *be, const dw_buf *a_q, const dw_buf *a_s, const dw_buf *b_q, const dw_buf *b_s,
+                               const dw_buf *bias, dw_buf *y, int y_dtype, size_t m, size_t n, size_t k, int act);
+/* The same with the result, unrounded, as an MXFP4 operand of m rows of n values:
+ * what dw_quantize_mxfp4 makes of dw_gemm_mxfp4's f32 result. */
+DW_API dw_status dw_gemm_to_mxfp4(dw_backend *be, const dw_buf *a_q, const dw_buf *a_s, const dw_buf *b_q,
+                                  const dw_buf *b_s, const dw_buf *bias, dw_buf *y_q, dw_buf *y_s, size_t m, size_t n,
+                                  size_t k, int act);
+
+/* Norms, in f32: rms(v) = v / sqrt(mean(v^2) + eps) * w + b; layer(v) the same on
+ * v - mean(v); none(v) = v.  w and b are f32 [c], or NULL (1 and 0).  The sum of
+ * squares is an f32: values whose squares overflow it (beyond about 1e18) give 0 or NaN. */
+enum dw_norm_kind { DW_NORM_NONE = 0, DW_NORM_RMS = 1, DW_NORM_LAYER = 2 };
+
+/* Rows of c values, *_pitch elements apart (0: c; the residual and `out` share
+ * res_pitch).  x and the gate have x_dtype, the residual and `out` res_dtype (x_dtype
+ * or DW_F32), y y_dtype.  A tensor with a pitch of its own has at least
+ * (rows - 1) * pitch + c elements, one without exactly rows * c. */
+typedef struct dw_norm_desc {
+    size_t rows, c;
+    size_t x_pitch, res_pitch, y_pitch;
+    size_t gate_rows; /* rows that share a gate row: row r has gate row r / gate_rows; 0: one for all rows */
+    int32_t x_dtype, res_dtype, y_dtype;
+    int32_t pre, post; /* dw_norm_kind */
+    float eps;         /* >= 0 */
+    float res_scale;
+} dw_norm_desc;
+
+/* y = pre(x).  y may be x itself (same type and pitch). */
+DW_API dw_status dw_norm(dw_backend *be, const dw_norm_desc *d, const dw_buf *x, const dw_buf *w, const dw_buf *b,
+                         dw_buf *y);
+/* The same with the result, unrounded, as an MXFP4 operand [rows, c]. */
+DW_API dw_status dw_norm_to_mxfp4(dw_backend *be, const dw_norm_desc *d, const dw_buf *x, const dw_buf *w,
+                                  const dw_buf *b, dw_buf *q, dw_buf *s);
+/* The end of a residual block and the start of the next in one pass:
+ *   out = residual + res_scale * gate * post(x), rounded to res_dtype;  y = pre(out).
+ * x: the block's output; gate [ceil(rows / gate_rows), c] (or [c]), NULL: 1;
+ * y NULL: `out` alone.  `out` may be the residual itself; no other tensors overlap. */
+DW_API dw_status dw_norm_residual(dw_backend *be, const dw_norm_desc *d, const dw_buf *x, const dw_buf *w_post,
+                                  const dw_buf *b_post, const dw_buf *gate, const dw_buf *residual, dw_buf *out,
+                                  const dw_buf *w_pre, const dw_buf *b_pre, dw_buf *y);
+/* The same with y, unrounded, as an MXFP4 operand [rows, c]. */
+DW_API dw_status dw_norm_residual_to_mxfp4(dw_backend *be, const dw_norm_desc *d, const dw_buf *x, const dw_buf *w_post,
+                                           const dw_buf *b_post, const dw_buf *gate, const dw_buf *residual, dw_buf *out,
+                                           const dw_buf *w_pre, const dw_buf *b_pre, dw_buf *q, dw_buf *s);
+
 #ifdef __cplusplus
 }
 #endif
