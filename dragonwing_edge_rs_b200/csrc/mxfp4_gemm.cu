@@ -53,8 +53,8 @@ struct GemmParams {
 };
 
 // Bounded wait for a phase; false once the CTA is aborting or the cap expired.
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const GemmParams &p, volatile int *abort_flag,
-                                           int site) {
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, uint64_t cap_ns, int32_t *err,
+                                           volatile int *abort_flag, int site) {
 #pragma unroll 1
     for (int i = 0; i < 64; i++)
         if (mbar_try_wait(bar, parity)) return true;
@@ -63,20 +63,20 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const 
     for (;;) {
         if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
         if (*abort_flag) return false;
-        if (globaltimer_ns() - t0 > p.wait_cap_ns) {
+        if (globaltimer_ns() - t0 > cap_ns) {
             *abort_flag = 1;
-            record_error(p.err, DW_DEV_WAIT_EXPIRED, site, (int)parity);
+            record_error(err, DW_DEV_WAIT_EXPIRED, site, (int)parity);
             return false;
         }
     }
 }
 
 // Waits for a phase that the CTA's own work in flight completes, whatever happened before.
-__device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, const GemmParams &p) {
+__device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, uint64_t cap_ns) {
     const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
     while (!mbar_try_wait_sleep(bar, parity, 20000u))
-        if (globaltimer_ns() - t0 > p.wait_cap_ns) return;
+        if (globaltimer_ns() - t0 > cap_ns) return;
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
@@ -113,11 +113,15 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         : "memory");
 }
 
-// silu(v) = v / (1 + e^-v): ex2.approx through __expf (2 ulp plus |v| * 2^-24
-// relative) and a correctly rounded division.
+// silu(v) = v / (1 + e^-v) by ex2.approx and rcp.approx: a relative error of a few
+// 2^-24 plus |v| * 2^-24 (the exponent's rounding).  e^-v = inf gives v * 0 = -0.
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == DW_EPI_RELU) return fmaxf(v, 0.0f);
-    if (act == DW_EPI_SILU) return __fdiv_rn(v, 1.0f + __expf(-v));
+    if (act == DW_EPI_SILU) {
+        float r;
+        asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-v)));
+        return v * r;
+    }
     return v;
 }
 
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
                 const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
                 for (int kb = 0; kb < p.k_blocks; kb++) {
-                    if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p, abort_flag, 21)) {
+                    if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 21)) {
                         ok = false;
                         break;
                     }
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             // the last copies into each stage have landed before the CTA ends
             for (int i = 0; i < min(issued, p.stages); i++) {
                 if (--s < 0) s = p.stages - 1, ph ^= 1;
-                drain_phase(smem_u32(&full_bar[s]), ph, p);
+                drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
             }
         }
     } else if (warp == 1) {
@@ -241,11 +245,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             bool ok = true;
             const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
             for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-                if (!wait_phase(smem_u32(&tempty_bar[acc]), aph ^ 1u, p, abort_flag, 22)) break;
+                if (!wait_phase(smem_u32(&tempty_bar[acc]), aph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 22)) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * BN;
                 for (int kb = 0; kb < p.k_blocks; kb++) {
-                    if (!wait_phase(smem_u32(&full_bar[s]), ph, p, abort_flag, 23)) {
+                    if (!wait_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 23)) {
                         ok = false;
                         break;
                     }
@@ -275,7 +279,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 if (!acc) aph ^= 1;
             }
             tc_commit(smem_u32(&drain_bar));
-            drain_phase(smem_u32(&drain_bar), 0, p);
+            drain_phase(smem_u32(&drain_bar), 0, p.wait_cap_ns);
         }
     } else {
         const int quarter = warp & 3;  // tensor-memory lanes this warp may read
@@ -283,7 +287,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         uint32_t aph = 0;
         for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
             const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
-            if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&tfull_bar[acc]), aph, p, abort_flag, 24))) break;
+            if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&tfull_bar[acc]), aph, p.wait_cap_ns, p.err, abort_flag, 24))) break;
             tc_fence_after();
             const size_t row = (size_t)tm * kBM + quarter * 32 + lane;
             const uint32_t base = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
@@ -330,6 +334,225 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
+}
+
+// ---- few rows ------------------------------------------------------------------
+// The weights take the tensor core's 128-row side and the m rows of A its column
+// side (bn = 16, 32, 64 or 128 of them), so a tile's result is 128 outputs x bn
+// rows.  K is split over the CTAs of a cluster, which leave their partial tiles in
+// shared memory, and each of them adds up every S-th row of A in the order of the
+// ranks: no workspace, no atomics, the same bits each time.
+struct SkinnyParams {
+    const uint8_t *w_s, *a_s;
+    const float *bias;
+    void *y;
+    uint8_t *y_s;
+    size_t m, n;
+    size_t tiles_k;
+    size_t out_nb, out_tiles;
+    int k_blocks, bn, stages, act, out;  // out: DW_F32 .. DW_BF16, 3: MXFP4
+    uint32_t stage_bytes, idesc[2], tmem_cols;
+    uint64_t wait_cap_ns;
+    int32_t *err;
+};
+
+constexpr int kSkinnyThreads = 256;
+constexpr int kSkinnyStages = 8;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+__global__ void __launch_bounds__(kSkinnyThreads)
+    k_mxfp4_skinny(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
+                   const __grid_constant__ SkinnyParams p) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+    float *part = reinterpret_cast<float *>(smem_raw + (smem - smem_u32(smem_raw)));  // [bn][128], over the ring
+    __shared__ uint64_t full_bar[kSkinnyStages], sf_bar[kSkinnyStages], empty_bar[kSkinnyStages], done_bar, drain_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int *abort_flag = &abort_word;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank(), S = cluster_size();
+    const size_t n0 = (size_t)blockIdx.y * 128, m0 = (size_t)blockIdx.z * p.bn;
+    const int kb0 = (int)((long long)p.k_blocks * rank / S), kb1 = (int)((long long)p.k_blocks * (rank + 1) / S);
+    const uint32_t w_bytes = kBM * kBKBytes, a_bytes = (uint32_t)p.bn * kBKBytes;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; s++) {
+            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&sf_bar[s]), 1);
+            mbar_init(smem_u32(&empty_bar[s]), 1);
+        }
+        mbar_init(smem_u32(&done_bar), 1);
+        mbar_init(smem_u32(&drain_bar), 1);
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
+                     "r"(p.tmem_cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const uint32_t sf_cols = tmem + (uint32_t)p.bn;  // 16 columns a stage after the accumulators
+    const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
+
+    if (warp == 0 && lane == 0) {
+        int s = 0, issued = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; kb++) {
+            if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 31)) break;
+            const uint32_t bar = smem_u32(&full_bar[s]), base = smem + s * p.stage_bytes;
+            const uint32_t sbytes = (uint32_t)min((size_t)2, p.tiles_k - 2 * (size_t)kb) * 512;
+            mbar_expect_tx(bar, w_bytes + a_bytes + 2 * sbytes);
+            tma_load_2d(base, &tmap_w, bar, kb * kBKBytes, (int)n0);
+            bulk_load(base + w_bytes, p.w_s + ((size_t)blockIdx.y * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
+            tma_load_2d(base + w_bytes + 1024, &tmap_a, bar, kb * kBKBytes, (int)m0);
+            bulk_load(base + w_bytes + 1024 + a_bytes, p.a_s + ((m0 >> 7) * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
+            issued++;
+            if (++s == p.stages) s = 0, ph ^= 1;
+        }
+        for (int i = 0; i < min(issued, p.stages); i++) {
+            if (--s < 0) s = p.stages - 1, ph ^= 1;
+            drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
+        }
+    } else if (warp == 2 && lane == 0) {
+        // scales of each stage into tensor memory, ahead of the products
+        int s = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; kb++) {
+            if (!wait_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 32)) break;
+            tc_fence_after();
+            const uint32_t base = smem + s * p.stage_bytes + w_bytes;
+            const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
+            for (int c = 0; c < chunks; c++) {
+                tc_cp_scales(sf_cols + s * 16 + c * 4, smem_desc_noswz(base + c * 512, 16, 128));
+                tc_cp_scales(sf_cols + s * 16 + 8 + c * 4, smem_desc_noswz(base + 1024 + a_bytes + c * 512, 16, 128));
+            }
+            tc_commit(smem_u32(&sf_bar[s]));
+            if (++s == p.stages) s = 0, ph ^= 1;
+        }
+        tc_commit(smem_u32(&drain_bar));
+        drain_phase(smem_u32(&drain_bar), 0, p.wait_cap_ns);
+    } else if (warp == 1 && lane == 0) {
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; kb++) {
+            if (!wait_phase(smem_u32(&sf_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 33)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t base = smem + s * p.stage_bytes;
+            const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
+            for (int c = 0; c < chunks; c++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t off = (uint32_t)(c * 2 + h) * 32;
+                    tc_mma_mxf4(tmem, smem_desc(base + off, hi), smem_desc(base + w_bytes + 1024 + off, hi), p.idesc[h],
+                                sf_cols + s * 16 + c * 4, sf_cols + s * 16 + 8 + c * 4, (kb > kb0 || c || h) ? 1u : 0u);
+                }
+            tc_commit(smem_u32(&empty_bar[s]));
+            if (++s == p.stages) s = 0, ph ^= 1;
+        }
+        tc_commit(smem_u32(&done_bar));
+        if (!ok) drain_phase(smem_u32(&done_bar), 0, p.wait_cap_ns);
+    }
+    __syncwarp();
+    if (warp >= 4) {
+        // accumulators -> part[row of A][output]
+        const int quarter = warp & 3;
+        if (__all_sync(0xffffffffu, wait_phase(smem_u32(&done_bar), 0, p.wait_cap_ns, p.err, abort_flag, 34))) {
+            tc_fence_after();
+            const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
+            const int cols = (int)min((size_t)p.bn, p.m - m0);
+            for (int c0 = 0; c0 < cols; c0 += 16) {
+                int32_t r[16];
+                tc_ld16(base + c0, r);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (c0 + i < cols) part[(c0 + i) * 128 + quarter * 32 + lane] = __int_as_float(r[i]);
+            }
+        }
+    }
+    tc_fence_before();
+    if (S > 1)
+        cluster_sync();
+    else
+        __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+    }
+    if (*abort_flag == 0) {
+        const int t = threadIdx.x & 127;  // output of the tile
+        const size_t col = n0 + t;
+        const bool live = col < p.n;
+        const float bias = live && p.bias ? __ldg(p.bias + col) : 0.0f;
+        const int rows = (int)min((size_t)p.bn, p.m - m0);
+        for (int j = (int)rank + (int)S * (threadIdx.x >> 7); j < rows; j += 2 * (int)S) {
+            const uint32_t addr = smem_u32(part + j * 128 + t);
+            float v = 0.0f;
+            if (S > 1) {
+                float u[8];
+#pragma unroll
+                for (uint32_t r = 0; r < 8; r++) u[r] = r < S ? ld_peer(addr, r) : 0.0f;
+#pragma unroll
+                for (uint32_t r = 0; r < 8; r++)
+                    if (r < S) v += u[r];
+            } else {
+                v = part[j * 128 + t];
+            }
+            v = activate(v + bias, p.act);
+            const size_t row = m0 + j;
+            if (p.out == 3) {
+                if (!live) v = 0.0f;
+                uint32_t amax = __float_as_uint(v) & 0x7FFFFFFFu;
+#pragma unroll
+                for (int o = 16; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                const uint32_t sb = mx_scale_byte(amax);
+                const float q = v * mx_inv_scale(sb), next = __shfl_down_sync(0xffffffffu, q, 1);
+                const size_t block = col / 32;
+                if ((lane & 1) == 0 && block < p.out_nb)
+                    ((uint8_t *)p.y)[(row * p.out_nb * 32 + col) / 2] = sb == 0xFFu ? 0 : (uint8_t)mx_codes2(q, next);
+                if (lane == 0 && block < p.out_tiles * 4) p.y_s[mx_scale_at(row, block, p.out_tiles)] = (uint8_t)sb;
+            } else if (live) {
+                if (p.out == DW_F32)
+                    ((float *)p.y)[row * p.n + col] = v;
+                else if (p.out == DW_F16)
+                    ((__half *)p.y)[row * p.n + col] = __float2half_rn(v);
+                else
+                    ((__nv_bfloat16 *)p.y)[row * p.n + col] = __float2bfloat16_rn(v);
+            }
+        }
+    }
+    if (S > 1) cluster_sync();  // no CTA leaves while its partials may be read
 }
 
 // Codes as a 2-D byte tensor [rows][bytes of a row]; a box is 128 bytes of `box_rows` rows.
@@ -379,9 +602,60 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a) {
     return dw_after_launch(be, "gemm_mxfp4");
 }
 
+// CTAs of a cluster that share a tile's K: as many as fill the GPU once, each with
+// at least one K block.
+dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
+    SkinnyParams p{};
+    p.w_s = a.b_s, p.a_s = a.a_s, p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
+    p.m = a.m, p.n = a.n;
+    p.tiles_k = mx_tiles(a.k);
+    p.out_nb = mx_blocks(a.n), p.out_tiles = mx_tiles(a.n);
+    p.k_blocks = (int)((a.k + 255) / 256);
+    p.bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
+    p.act = a.act, p.out = a.y_s ? 3 : a.y_dtype;
+    p.stage_bytes = kBM * kBKBytes + 1024 + p.bn * kBKBytes + 1024;
+    for (int h = 0; h < 2; h++) p.idesc[h] = mx_idesc(128, p.bn, h);
+    // two CTAs an SM up to 64 rows (each at most 256 columns of tensor memory), one above
+    const int per_sm = p.bn <= 64 ? 2 : 1;
+    const size_t budget = (kSmemLimit - 8192) / per_sm - 2048;
+    p.stages = (int)std::min<size_t>(kSkinnyStages, budget / p.stage_bytes);
+    p.tmem_cols = 256;
+    p.wait_cap_ns = be->wait_cap_ns, p.err = be->dev_err;
+    const size_t tn = (a.n + 127) / 128, tm = (a.m + p.bn - 1) / p.bn;
+    if (tn > 65535 || tm > 65535) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu x %zu is too large", a.m, a.n);
+    unsigned S = 1;
+    while (S < 8 && 2 * S * tn * tm <= (size_t)be->sm_count * per_sm && 2 * (int)S <= p.k_blocks) S *= 2;
+    const size_t smem = 1024 + std::max<size_t>(p.stages * p.stage_bytes, (size_t)p.bn * 512);
+    CUtensorMap tw, ta;
+    if (!be->encode_tiled || !code_map(be, &tw, a.b_q, a.n, a.k, kBM) || !code_map(be, &ta, a.a_q, a.m, a.k, p.bn))
+        return dw_fail(be, DW_ERR_DEVICE, "gemm_mxfp4: tensor map rejected");
+    static bool attr_set[16] = {};
+    if (be->device < 16 && !attr_set[be->device]) {
+        dw_status st = dw_cuda_check(be,
+                                     cudaFuncSetAttribute(k_mxfp4_skinny, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                          (int)(kSmemLimit - 2048)),
+                                     "gemm_mxfp4 attributes");
+        if (st != DW_OK) return st;
+        attr_set[be->device] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S, (unsigned)tn, (unsigned)tm);
+    cfg.blockDim = dim3(kSkinnyThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = be->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    dw_status st = dw_cuda_check(be, cudaLaunchKernelEx(&cfg, k_mxfp4_skinny, tw, ta, p), "gemm_mxfp4 launch");
+    return st != DW_OK ? st : dw_after_launch(be, "gemm_mxfp4");
+}
+
 }  // namespace
 
 dw_status launch_gemm_mxfp4(dw_backend *be, const MxGemmArgs &a) {
+    if (a.m <= 256) return launch_skinny(be, a);
     if (a.y_s) return launch<128, 3>(be, a);
     switch (a.y_dtype) {
         case DW_F32: return launch<128, 0>(be, a);
