@@ -12,6 +12,8 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <cstring>
+#include <type_traits>
 
 #include "dw_cuda.h"
 
@@ -32,11 +34,22 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-__device__ __forceinline__ uint32_t pack2(__half a, __half b) {
-    return (uint32_t)__half_as_ushort(a) | ((uint32_t)__half_as_ushort(b) << 16);
+// Two f32 rounded to T, the first in the low half: one cvt.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    uint32_t u;
+    memcpy(&u, &h, 4);
+    return u;
 }
-__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) {
-    return (uint32_t)__bfloat16_as_ushort(a) | ((uint32_t)__bfloat16_as_ushort(b) << 16);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    uint32_t u;
+    memcpy(&u, &h, 4);
+    return u;
 }
 
 // V consecutive elements as raw words, loaded with the widest access that V
@@ -85,6 +98,8 @@ struct Raw {
         if constexpr (sizeof(T) == 4) {
             return __uint_as_float(w[i]);
         } else {
+            if constexpr (std::is_same_v<T, __nv_bfloat16>)  // a bf16 is the upper half of its f32
+                return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
             const unsigned short h = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
             T t;
             memcpy(&t, &h, 2);
@@ -102,7 +117,7 @@ struct Raw {
             w[0] = h;
         } else {
 #pragma unroll
-            for (int i = 0; i < V / 2; i++) w[i] = pack2(from_f32<T>(v[2 * i]), from_f32<T>(v[2 * i + 1]));
+            for (int i = 0; i < V / 2; i++) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
         }
     }
 };

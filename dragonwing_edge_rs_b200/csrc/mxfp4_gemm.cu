@@ -20,6 +20,7 @@
 // and exits.
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "dw_device.cuh"
 #include "dw_mxfp4.cuh"
@@ -31,8 +32,6 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kBKBytes = 128;  // a K block: 256 codes
-constexpr int kEpiWarps = 4;
-constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
 constexpr size_t kSmemLimit = 227 * 1024;
 
 struct GemmParams {
@@ -45,23 +44,38 @@ struct GemmParams {
     size_t out_nb, out_tiles;  // MXFP4 result: blocks and scale tiles along n
     int k_blocks;     // 256-wide K blocks
     int tiles_m, tiles_n, tiles;
-    int b_row_tiles;  // 128-row scale tiles of B
+    int a_row_tiles, b_row_tiles;  // 128-row scale tiles
     int stages, act;
-    bool vec;         // rows of y start on 16-byte boundaries
+    bool vec, bias_vec;  // rows of y, the bias start on 16-byte boundaries
     uint64_t wait_cap_ns;
     int32_t *err;
 };
 
+// try_wait that acquires what another CTA of the cluster released by its arrival.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // Bounded wait for a phase; false once the CTA is aborting or the cap expired.
+// kCluster: arrivals come from another CTA.
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, uint64_t cap_ns, int32_t *err,
                                            volatile int *abort_flag, int site) {
 #pragma unroll 1
     for (int i = 0; i < 64; i++)
-        if (mbar_try_wait(bar, parity)) return true;
+        if (kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
     for (;;) {
-        if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+        if (kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait_sleep(bar, parity, 20000u)) return true;
         if (*abort_flag) return false;
         if (globaltimer_ns() - t0 > cap_ns) {
             *abort_flag = 1;
@@ -77,12 +91,6 @@ __device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, uint6
 #pragma unroll 1
     while (!mbar_try_wait_sleep(bar, parity, 20000u))
         if (globaltimer_ns() - t0 > cap_ns) return;
-}
-
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-                 "r"(bytes), "r"(bar)
-                 : "memory");
 }
 
 // 512 bytes (32 rows of 16) -> 4 columns of all four lane quarters of tensor memory.
@@ -133,16 +141,42 @@ constexpr uint32_t mx_idesc(int m, int n, int pair) {
            ((uint32_t)(2 * pair) << 29) | ((uint32_t)(2 * pair) << 4);
 }
 
+// Bias and activation of 32 columns of a row.
+__device__ __forceinline__ void finish32(float (&v)[32], size_t col, const GemmParams &p) {
+    if (p.bias) {
+        if (col + 32 <= p.n && p.bias_vec) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float4 b = __ldg(reinterpret_cast<const float4 *>(p.bias + col) + i);
+                v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+                if (col + i < p.n) v[i] += __ldg(p.bias + col + i);
+        }
+    }
+    if (p.act == DW_EPI_RELU) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[i] = activate(v[i], DW_EPI_RELU);
+    } else if (p.act == DW_EPI_SILU) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[i] = activate(v[i], DW_EPI_SILU);
+    }
+}
+
 // What the epilogue stores: 0 f32, 1 f16, 2 bf16, 3 MXFP4.
 template <int kOut>
 __device__ __forceinline__ void put32(float (&v)[32], size_t row, size_t col, const GemmParams &p, uint32_t &scale) {
     if constexpr (kOut == 3) {
+        if (col + 32 > p.n) {
 #pragma unroll
-        for (int i = 0; i < 32; i++)
-            if (col + i >= p.n) v[i] = 0.0f;
+            for (int i = 0; i < 32; i++)
+                if (col + i >= p.n) v[i] = 0.0f;
+        }
         uint4 codes;
         scale = mx_quantize32(v, codes);
-        if (row < p.m && col < p.n) *reinterpret_cast<uint4 *>((uint8_t *)p.y + (row * p.out_nb + col / 32) * 16) = codes;
+        if (row < p.m && col / 32 < p.out_nb) *reinterpret_cast<uint4 *>((uint8_t *)p.y + (row * p.out_nb + col / 32) * 16) = codes;
     } else {
         using T = std::conditional_t<kOut == 0, float, std::conditional_t<kOut == 1, __half, __nv_bfloat16>>;
         if (row >= p.m) return;
@@ -165,54 +199,119 @@ __device__ __forceinline__ void put32(float (&v)[32], size_t row, size_t col, co
     }
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ---- many rows -----------------------------------------------------------------
+// A pair of CTAs (cta_group::2) computes a 256 x BN tile: each holds 128 rows of A,
+// half of B's rows, the scales of its rows of A and those of all BN rows of B, so a
+// K block costs each SM's L2 port (128 + BN / 2) * 128 bytes of codes for
+// 256 * BN * 256 products of the pair.  The leader issues for both; the peer's
+// copies reach it by a remote arrival.  The epilogue takes its accumulators into
+// registers at once and gives the tensor memory back before it converts and stores.
+constexpr int kEpiWarps = 16;
+constexpr int kGemmThreads = 128 + 32 * kEpiWarps;
+constexpr int kMaxStages = 8;
+
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Commits of the pair: to the leader's barrier, or to the same barrier of both CTAs.
+__device__ __forceinline__ void tc_commit2(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_commit2_both(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_cp_scales2(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tc_mma_mxf4_2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                              uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
 template <int BN, int kOut>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     k_mxfp4_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                  const __grid_constant__ GemmParams p) {
-    constexpr uint32_t kA = kBM * kBKBytes, kB = BN * kBKBytes, kSA = 1024, kSB = (BN / 128) * 1024;
+    constexpr uint32_t kA = kBM * kBKBytes, kB = BN / 2 * kBKBytes, kSA = 1024, kSB = (BN / 128) * 1024;
     constexpr uint32_t kStage = kA + kB + kSA + kSB;
     constexpr uint32_t kScaleCols = 8 + BN / 16;  // tensor-memory columns of a stage's scales
-    constexpr int kMaxStages = 8;
+    constexpr int kAcc = 256 / BN;                // accumulator buffers
+    constexpr int kCols = BN / 4;                 // columns of an epilogue warp
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-    __shared__ uint64_t full_bar[kMaxStages], empty_bar[kMaxStages], tfull_bar[2], tempty_bar[2], drain_bar;
+    __shared__ uint64_t full_bar[kMaxStages], peer_bar[kMaxStages], sf_bar[kMaxStages], empty_bar[kMaxStages];
+    __shared__ uint64_t tfull_bar[kAcc], tempty_bar[kAcc], drain_bar[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; s++) {
             mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&peer_bar[s]), 1);
+            mbar_init(smem_u32(&sf_bar[s]), 1);
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
-        for (int a = 0; a < 2; a++) {
+        for (int a = 0; a < kAcc; a++) {
             mbar_init(smem_u32(&tfull_bar[a]), 1);
-            mbar_init(smem_u32(&tempty_bar[a]), kEpiWarps);
+            mbar_init(smem_u32(&tempty_bar[a]), 2 * kEpiWarps);
         }
-        mbar_init(smem_u32(&drain_bar), 1);
+        mbar_init(smem_u32(&drain_bar[0]), 1);
+        mbar_init(smem_u32(&drain_bar[1]), 1);
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u)
                      : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
-    __syncthreads();
+    cluster_sync();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const uint32_t sf_cols = tmem + 2 * BN;  // scales after the two accumulators
+    const uint32_t sf_cols = tmem + 256;  // scales after the accumulators
 
     if (warp == 0) {
         if (lane == 0) {
             int s = 0, issued = 0;
             uint32_t ph = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-                const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
+            for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
+                const int tm = (tile % p.tiles_m) * 2 + (int)rank, tn = tile / p.tiles_m;  // 128-row tile of A, BN-row tile of B
+                // a 128-row tile of A past the end has no scales (its rows are zeros, and not stored)
+                const bool sa = tm < p.a_row_tiles;
+                const int nsb = min(BN / 128, p.b_row_tiles - tn * (BN / 128));
                 for (int kb = 0; kb < p.k_blocks; kb++) {
                     if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 21)) {
                         ok = false;
@@ -220,11 +319,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     }
                     const uint32_t bar = smem_u32(&full_bar[s]), base = smem + s * kStage;
                     const uint32_t sbytes = (uint32_t)min((size_t)2, p.tiles_k - 2 * (size_t)kb) * 512;
-                    const int nsb = min(BN / 128, p.b_row_tiles - tn * (BN / 128));
-                    mbar_expect_tx(bar, kA + kB + sbytes * (1 + nsb));
+                    mbar_expect_tx(bar, kA + kB + sbytes * (sa + nsb));
                     tma_load_2d(base, &tmap_a, bar, kb * kBKBytes, tm * kBM);
-                    tma_load_2d(base + kA, &tmap_b, bar, kb * kBKBytes, tn * BN);
-                    bulk_load(base + kA + kB, p.a_s + ((size_t)tm * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
+                    tma_load_2d(base + kA, &tmap_b, bar, kb * kBKBytes, tn * BN + (int)rank * (BN / 2));
+                    if (sa) bulk_load(base + kA + kB, p.a_s + ((size_t)tm * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
                     for (int j = 0; j < nsb; j++)
                         bulk_load(base + kA + kB + kSA + j * 1024,
                                   p.b_s + (((size_t)tn * (BN / 128) + j) * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
@@ -238,18 +336,54 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
             }
         }
-    } else if (warp == 1) {
+    } else if (warp == 2) {
+        // the leader: each stage's scales into both CTAs' tensor memory, ahead of the
+        // products; the peer: tells the leader that its stage has landed
         if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
+                for (int kb = 0; kb < p.k_blocks; kb++) {
+                    if (!wait_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 22) ||
+                        (rank == 0 && !wait_phase<true>(smem_u32(&peer_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 23))) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) {
+                        tc_fence_after();
+                        const uint32_t base = smem + s * kStage + kA + kB;
+                        const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 8;
+                        const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
+                        for (int c = 0; c < chunks; c++) {
+                            tc_cp_scales2(sfa + c * 4, smem_desc_noswz(base + c * 512, 16, 128));
+#pragma unroll
+                            for (int j = 0; j < BN / 128; j++)
+                                tc_cp_scales2(sfb + c * (BN / 32) + j * 4, smem_desc_noswz(base + kSA + j * 1024 + c * 512, 16, 128));
+                        }
+                        tc_commit2(smem_u32(&sf_bar[s]));
+                    } else {
+                        mbar_arrive_cluster(peer_addr(smem_u32(&peer_bar[s]), 0));
+                    }
+                    if (++s == p.stages) s = 0, ph ^= 1;
+                }
+            }
+            if (rank == 0) {
+                tc_commit2(smem_u32(&drain_bar[1]));
+                drain_phase(smem_u32(&drain_bar[1]), 0, p.wait_cap_ns);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
             int s = 0, acc = 0;
             uint32_t ph = 0, aph = 0;
             bool ok = true;
             const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
-            for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
-                if (!wait_phase(smem_u32(&tempty_bar[acc]), aph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 22)) break;
-                tc_fence_after();
+            for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
+                if (!wait_phase<true>(smem_u32(&tempty_bar[acc]), aph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 24)) break;
                 const uint32_t d = tmem + acc * BN;
                 for (int kb = 0; kb < p.k_blocks; kb++) {
-                    if (!wait_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 23)) {
+                    if (!wait_phase(smem_u32(&sf_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 25)) {
                         ok = false;
                         break;
                     }
@@ -257,82 +391,76 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     const uint32_t base = smem + s * kStage;
                     const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 8;
                     const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
-                    for (int c = 0; c < chunks; c++) {
-                        tc_cp_scales(sfa + c * 4, smem_desc_noswz(base + kA + kB + c * 512, 16, 128));
-#pragma unroll
-                        for (int j = 0; j < BN / 128; j++)
-                            tc_cp_scales(sfb + c * (BN / 32) + j * 4,
-                                         smem_desc_noswz(base + kA + kB + kSA + j * 1024 + c * 512, 16, 128));
+                    for (int c = 0; c < chunks; c++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             const uint32_t off = (uint32_t)(c * 2 + h) * 32;
-                            tc_mma_mxf4(d, smem_desc(base + off, hi), smem_desc(base + kA + off, hi), mx_idesc(kBM, BN, h),
-                                        sfa + c * 4, sfb + c * (BN / 32), (kb | c | h) ? 1u : 0u);
+                            tc_mma_mxf4_2(d, smem_desc(base + off, hi), smem_desc(base + kA + off, hi), mx_idesc(2 * kBM, BN, h),
+                                          sfa + c * 4, sfb + c * (BN / 32), (kb | c | h) ? 1u : 0u);
                         }
-                    }
-                    tc_commit(smem_u32(&empty_bar[s]));
+                    tc_commit2_both(smem_u32(&empty_bar[s]));
                     if (++s == p.stages) s = 0, ph ^= 1;
                 }
                 if (!ok) break;
-                tc_commit(smem_u32(&tfull_bar[acc]));
-                acc ^= 1;
-                if (!acc) aph ^= 1;
+                tc_commit2_both(smem_u32(&tfull_bar[acc]));
+                if (++acc == kAcc) acc = 0, aph ^= 1;
             }
-            tc_commit(smem_u32(&drain_bar));
-            drain_phase(smem_u32(&drain_bar), 0, p.wait_cap_ns);
+            tc_commit2(smem_u32(&drain_bar[0]));
+            drain_phase(smem_u32(&drain_bar[0]), 0, p.wait_cap_ns);
         }
-    } else {
+    } else if (warp >= 4) {
         const int quarter = warp & 3;  // tensor-memory lanes this warp may read
+        const int part = (warp - 4) >> 2;
         int acc = 0;
         uint32_t aph = 0;
-        for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+        for (int tile = pair; tile < p.tiles; tile += pairs) {
             const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
-            if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&tfull_bar[acc]), aph, p.wait_cap_ns, p.err, abort_flag, 24))) break;
+            if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&tfull_bar[acc]), aph, p.wait_cap_ns, p.err, abort_flag, 26))) break;
             tc_fence_after();
-            const size_t row = (size_t)tm * kBM + quarter * 32 + lane;
-            const uint32_t base = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
-#pragma unroll 1
-            for (int t = 0; t < BN / 128; t++) {
-                uint32_t scales = 0;
-#pragma unroll 1
-                for (int g = 0; g < 4; g++) {
-                    const int c0 = t * 128 + g * 32;
-                    const size_t col = (size_t)tn * BN + c0;
-                    uint32_t r[32];
-                    tc_ld32(base + c0, r);
-                    tc_wait_ld();
-                    if (t == BN / 128 - 1 && g == 3) {  // accumulators read: the next tile may overwrite them
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
-                    }
-                    if (col >= p.n) continue;
-                    float v[32];
+            const size_t row = ((size_t)tm * 2 + rank) * kBM + quarter * 32 + lane;
+            const size_t col0 = (size_t)tn * BN + part * kCols;
+            const uint32_t base = tmem + acc * BN + part * kCols + ((uint32_t)(quarter * 32) << 16);
+            uint32_t r[kCols / 32][32];
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        v[i] = __uint_as_float(r[i]);
-                        if (p.bias && col + i < p.n) v[i] += __ldg(p.bias + col + i);
-                        v[i] = activate(v[i], p.act);
-                    }
-                    uint32_t sb = 0;
-                    put32<kOut>(v, row, col, p, sb);
-                    scales |= sb << (8 * g);
-                }
-                if constexpr (kOut == 3) {
-                    const size_t st = (size_t)tn * (BN / 128) + t;
-                    if (row < p.m && st < p.out_tiles)
-                        *reinterpret_cast<uint32_t *>(p.y_s + mx_scale_at(row, st * 4, p.out_tiles)) = scales;
+            for (int g = 0; g < kCols / 32; g++) tc_ld32(base + g * 32, r[g]);
+            tc_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(peer_addr(smem_u32(&tempty_bar[acc]), 0));
+            if (++acc == kAcc) acc = 0, aph ^= 1;
+            if (col0 >= p.n) continue;
+            uint32_t scales = 0;
+#pragma unroll
+            for (int g = 0; g < kCols / 32; g++) {
+                const size_t col = col0 + g * 32;
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[g][i]);
+                finish32(v, col, p);
+                uint32_t sb = 0;
+                put32<kOut>(v, row, col, p, sb);
+                scales |= sb << (8 * g);
+            }
+            if constexpr (kOut == 3) {
+                // kCols / 32 blocks' scales: two bytes (BN = 256) or one of a tile's four
+                const size_t block = col0 / 32;
+                if (row < p.m) {
+                    uint8_t *s = p.y_s + mx_scale_at(row, block, p.out_tiles);
+                    if constexpr (kCols == 64)
+                        *reinterpret_cast<uint16_t *>(s) = (uint16_t)scales;
+                    else
+                        *s = (uint8_t)scales;
+                    if (block + kCols / 32 >= p.out_nb)  // the places of the tile past the last block
+                        for (size_t b = block + kCols / 32; b < p.out_tiles * 4; b++) p.y_s[mx_scale_at(row, b, p.out_tiles)] = 0;
                 }
             }
-            acc ^= 1;
-            if (!acc) aph ^= 1;
         }
     }
     tc_fence_before();
-    __syncthreads();
+    cluster_sync();  // all products and copies of the pair are done
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 
@@ -359,19 +487,6 @@ struct SkinnyParams {
 constexpr int kSkinnyThreads = 256;
 constexpr int kSkinnyStages = 8;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
     uint32_t a;
     float v;
@@ -568,26 +683,27 @@ bool code_map(dw_backend *be, CUtensorMap *map, const uint8_t *q, size_t rows, s
 
 template <int BN, int kOut>
 dw_status launch(dw_backend *be, const MxGemmArgs &a) {
-    constexpr size_t kStage = kBM * kBKBytes + BN * kBKBytes + 1024 + (BN / 128) * 1024;
+    constexpr size_t kStage = kBM * kBKBytes + BN / 2 * kBKBytes + 1024 + (BN / 128) * 1024;
     GemmParams p{};
     p.a_s = a.a_s, p.b_s = a.b_s, p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
     p.m = a.m, p.n = a.n;
     p.tiles_k = mx_tiles(a.k);
     p.out_nb = mx_blocks(a.n), p.out_tiles = mx_tiles(a.n);
     p.k_blocks = (int)((a.k + 255) / 256);
-    const size_t tm = (a.m + kBM - 1) / kBM, tn = (a.n + BN - 1) / BN;
+    const size_t tm = (a.m + 2 * kBM - 1) / (2 * kBM), tn = (a.n + BN - 1) / BN;
     if (tm * tn > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu x %zu is too large", a.m, a.n);
-    p.tiles_m = (int)tm, p.tiles_n = (int)tn, p.tiles = (int)(tm * tn);
-    p.b_row_tiles = (int)((a.n + 127) / 128);
+    p.tiles_m = (int)tm, p.tiles = (int)(tm * tn);
+    p.a_row_tiles = (int)((a.m + 127) / 128), p.b_row_tiles = (int)((a.n + 127) / 128);
     p.act = a.act;
     const size_t es = kOut == 0 ? 4 : 2;
     p.vec = ((uintptr_t)a.y & 15) == 0 && a.n * es % 16 == 0;
+    p.bias_vec = ((uintptr_t)a.bias & 15) == 0;
     p.wait_cap_ns = be->wait_cap_ns, p.err = be->dev_err;
-    p.stages = (int)((kSmemLimit - 4096) / kStage);
+    p.stages = (int)std::min<size_t>(kMaxStages, (kSmemLimit - 4096) / kStage);
     // at least 116 KiB: one CTA per SM owns the tensor memory
     const size_t smem = std::max<size_t>(1024 + p.stages * kStage, 116 * 1024);
     CUtensorMap ta, tb;
-    if (!be->encode_tiled || !code_map(be, &ta, a.a_q, a.m, a.k, kBM) || !code_map(be, &tb, a.b_q, a.n, a.k, BN))
+    if (!be->encode_tiled || !code_map(be, &ta, a.a_q, a.m, a.k, kBM) || !code_map(be, &tb, a.b_q, a.n, a.k, BN / 2))
         return dw_fail(be, DW_ERR_DEVICE, "gemm_mxfp4: tensor map rejected");
     auto kernel = k_mxfp4_gemm<BN, kOut>;
     static bool attr_set[16] = {};
@@ -598,7 +714,7 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a) {
         if (st != DW_OK) return st;
         attr_set[be->device] = true;
     }
-    kernel<<<std::min(p.tiles, be->sm_count), kGemmThreads, smem, be->stream>>>(ta, tb, p);
+    kernel<<<2 * std::min(p.tiles, be->sm_count / 2), kGemmThreads, smem, be->stream>>>(ta, tb, p);
     return dw_after_launch(be, "gemm_mxfp4");
 }
 
@@ -656,11 +772,19 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
 
 dw_status launch_gemm_mxfp4(dw_backend *be, const MxGemmArgs &a) {
     if (a.m <= 256) return launch_skinny(be, a);
-    if (a.y_s) return launch<128, 3>(be, a);
-    switch (a.y_dtype) {
+    const int out = a.y_s ? 3 : a.y_dtype;
+    static const int bn = getenv("DW_MXBN") ? atoi(getenv("DW_MXBN")) : 256;
+    if (bn == 128) switch (out) {
         case DW_F32: return launch<128, 0>(be, a);
         case DW_F16: return launch<128, 1>(be, a);
-        default: return launch<128, 2>(be, a);
+        case DW_BF16: return launch<128, 2>(be, a);
+        default: return launch<128, 3>(be, a);
+    }
+    switch (out) {
+        case DW_F32: return launch<256, 0>(be, a);
+        case DW_F16: return launch<256, 1>(be, a);
+        case DW_BF16: return launch<256, 2>(be, a);
+        default: return launch<256, 3>(be, a);
     }
 }
 

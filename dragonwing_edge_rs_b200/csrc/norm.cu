@@ -14,12 +14,14 @@
 
 #include "dw_device.cuh"
 #include "dw_mxfp4.cuh"
+#include "dw_ptx.cuh"
 
 namespace dw {
 namespace {
 
 constexpr int kMaxT = 512;  // threads of a row
 constexpr int kMaxE = 32;   // elements of a thread
+constexpr size_t kSmemBudget = 216 * 1024;  // of an SM's shared memory for rows to come
 
 struct Params {
     const void *x, *gate, *res;
@@ -32,18 +34,30 @@ struct Params {
     bool has_res;
 };
 
-// Sum over the threads of a row.  `slot` alternates over four buffers, so a
-// buffer is written again only after three more barriers.
-__device__ __forceinline__ float row_sum(float v, float (*red)[32], int &slot) {
+// Sum over the T threads of a row (a power of two; rows of T <= 32 lie in one warp,
+// longer ones take whole warps, and all threads of the block call together).
+// `slot` alternates over four buffers, so a buffer is written again only after
+// three more barriers.
+__device__ __forceinline__ float row_sum(float v, int T, float (*red)[16], int &slot) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (blockDim.x == 32) return v;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    for (int o = 16; o; o >>= 1)
+        if (o < T) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (T <= 32) return v;
+    const int thread = threadIdx.y * blockDim.x + threadIdx.x, lane = thread & 31, warp = thread >> 5;
+    const int warps = T >> 5, first = warp & ~(warps - 1);
     if (lane == 0) red[slot][warp] = v;
     __syncthreads();
-    v = lane < warps ? red[slot][lane] : 0.0f;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const float *part = &red[slot][first];  // every thread adds the warps' sums, in the same order
+    v = part[0] + part[1];
+    if (T >= 128) v += part[2] + part[3];
+    if (T >= 256) {
+        const float4 q = *reinterpret_cast<const float4 *>(part + 4);
+        v += (q.x + q.y) + (q.z + q.w);
+    }
+    if (T >= 512) {
+        const float4 q = *reinterpret_cast<const float4 *>(part + 8), r = *reinterpret_cast<const float4 *>(part + 12);
+        v += ((q.x + q.y) + (q.z + q.w)) + ((r.x + r.y) + (r.z + r.w));
+    }
     slot = (slot + 1) & 3;
     return v;
 }
@@ -57,18 +71,18 @@ __device__ __forceinline__ void load_f32(const float *p, float (&v)[V]) {
 }
 
 // v[j][i] -> its norm, in place.  Elements past the row are 0 and stay out of the
-// statistics (`live`: element group j lies in the row).
-template <int V, int N>
-__device__ __forceinline__ void normalise(float (&v)[N][V], const bool (&live)[N], int kind, const float *w, const float *b,
-                                          const Params &p, float (*red)[32], int &slot) {
-    const int T = blockDim.x, tid = threadIdx.x;
+// statistics (`live`: element group j lies in the row).  weight(j, wv) and bias(j,
+// bv) give a group's weights and return whether there are any.
+template <int V, int N, typename W, typename B>
+__device__ __forceinline__ void normalise(float (&v)[N][V], const bool (&live)[N], int kind, int T, const Params &p,
+                                          float (*red)[16], int &slot, W weight, B bias) {
     if (kind == DW_NORM_LAYER) {
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < N; j++)
 #pragma unroll
             for (int i = 0; i < V; i++) sum += v[j][i];
-        const float mean = row_sum(sum, red, slot) * p.inv_c;
+        const float mean = row_sum(sum, T, red, slot) * p.inv_c;
 #pragma unroll
         for (int j = 0; j < N; j++)
 #pragma unroll
@@ -79,26 +93,27 @@ __device__ __forceinline__ void normalise(float (&v)[N][V], const bool (&live)[N
     for (int j = 0; j < N; j++)
 #pragma unroll
         for (int i = 0; i < V; i++) sq = fmaf(v[j][i], v[j][i], sq);
-    const float rstd = __frsqrt_rn(fmaf(row_sum(sq, red, slot), p.inv_c, p.eps));
+    const float rstd = __frsqrt_rn(fmaf(row_sum(sq, T, red, slot), p.inv_c, p.eps));
 #pragma unroll
     for (int j = 0; j < N; j++) {
         if (!live[j]) continue;
-        const size_t at = ((size_t)j * T + tid) * V;
-        float wv[V], bv[V];
-        if (w) load_f32<V>(w + at, wv);
-        if (b) load_f32<V>(b + at, bv);
+        float t[V];
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            v[j][i] *= rstd;
-            if (w) v[j][i] *= wv[i];
-            if (b) v[j][i] += bv[i];
+        for (int i = 0; i < V; i++) v[j][i] *= rstd;
+        if (weight(j, t)) {
+#pragma unroll
+            for (int i = 0; i < V; i++) v[j][i] *= t[i];
+        }
+        if (bias(j, t)) {
+#pragma unroll
+            for (int i = 0; i < V; i++) v[j][i] += t[i];
         }
     }
 }
 
 // One group of V values as MXFP4: 32 / V neighbouring threads hold a block.
 template <int V>
-__device__ __forceinline__ void put_mxfp4(const float (&v)[V], size_t at, size_t row, const Params &p) {
+__device__ __forceinline__ void put_mxfp4(const float (&v)[V], size_t at, size_t row, bool there, const Params &p) {
     uint32_t amax = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
@@ -112,14 +127,18 @@ __device__ __forceinline__ void put_mxfp4(const float (&v)[V], size_t at, size_t
         float t[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) t[i] = v[i] * inv;
-        if (block < p.nb) *reinterpret_cast<uint32_t *>(dst) = sb == 0xFFu ? 0u : mx_codes8(t);
+        if (there && block < p.nb) *reinterpret_cast<uint32_t *>(dst) = sb == 0xFFu ? 0u : mx_codes8(t);
     } else if constexpr (V == 2) {
-        if (block < p.nb) *dst = sb == 0xFFu ? (uint8_t)0 : (uint8_t)mx_codes2(v[0] * inv, v[1] * inv);
+        if (there && block < p.nb) *dst = sb == 0xFFu ? (uint8_t)0 : (uint8_t)mx_codes2(v[0] * inv, v[1] * inv);
     } else {
         const float next = __shfl_down_sync(0xffffffffu, v[0], 1);
-        if ((threadIdx.x & 1) == 0 && block < p.nb) *dst = sb == 0xFFu ? (uint8_t)0 : (uint8_t)mx_codes2(v[0] * inv, next * inv);
+        if ((threadIdx.x & 1) == 0 && there && block < p.nb) *dst = sb == 0xFFu ? (uint8_t)0 : (uint8_t)mx_codes2(v[0] * inv, next * inv);
     }
-    if ((at & 31) == 0 && block < p.tiles * 4) p.s[mx_scale_at(row, block, p.tiles)] = (uint8_t)sb;
+    if ((at & 31) == 0 && there && block < p.nb) {
+        p.s[mx_scale_at(row, block, p.tiles)] = (uint8_t)sb;
+        if (block + 1 == p.nb)  // the places of the tile past the last block
+            for (size_t b = p.nb; b < p.tiles * 4; b++) p.s[mx_scale_at(row, b, p.tiles)] = 0;
+    }
 }
 
 template <typename T, int V>
@@ -132,10 +151,16 @@ __device__ __forceinline__ void put(void *y, size_t at, const float (&v)[V]) {
 // blockDim = (threads of a row, rows); element group j of thread t starts at
 // column (j * threads + t) * V.
 template <typename X, typename R, int V, int N>
-__global__ void __launch_bounds__(kMaxT) k_norm(const __grid_constant__ Params p) {
-    __shared__ float red[4][32];
+__global__ void __launch_bounds__(kMaxT, V * N <= 8 ? 2 : 1) k_norm(const __grid_constant__ Params p) {
+    __shared__ __align__(16) float red[4][16];
     int slot = 0;
     const int T = blockDim.x, tid = threadIdx.x;
+    auto from = [&](const float *w) {
+        return [w, T, tid](int j, float (&t)[V]) {
+            if (w) load_f32<V>(w + ((size_t)j * T + tid) * V, t);
+            return w != nullptr;
+        };
+    };
     for (size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y; row < p.rows; row += (size_t)gridDim.x * blockDim.y) {
         Raw<X, V> xr[N], gr[N];
         Raw<R, V> rr[N];
@@ -160,7 +185,7 @@ __global__ void __launch_bounds__(kMaxT) k_norm(const __grid_constant__ Params p
 #pragma unroll
             for (int i = 0; i < V; i++) v[j][i] = xr[j].get(i);
         if (p.has_res) {
-            if (p.post != DW_NORM_NONE) normalise<V, N>(v, live, p.post, p.w0, p.b0, p, red, slot);
+            if (p.post != DW_NORM_NONE) normalise<V, N>(v, live, p.post, T, p, red, slot, from(p.w0), from(p.b0));
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 if (!live[j]) continue;
@@ -178,12 +203,12 @@ __global__ void __launch_bounds__(kMaxT) k_norm(const __grid_constant__ Params p
             }
         }
         if (p.y_dtype == -1) continue;
-        if (p.pre != DW_NORM_NONE) normalise<V, N>(v, live, p.pre, p.w1, p.b1, p, red, slot);
+        if (p.pre != DW_NORM_NONE) normalise<V, N>(v, live, p.pre, T, p, red, slot, from(p.w1), from(p.b1));
 #pragma unroll
         for (int j = 0; j < N; j++) {
             const size_t at = ((size_t)j * T + tid) * V;
             if (p.y_dtype == -2) {
-                put_mxfp4<V>(v[j], at, row, p);
+                put_mxfp4<V>(v[j], at, row, true, p);
                 continue;
             }
             if (!live[j]) continue;
@@ -198,14 +223,245 @@ __global__ void __launch_bounds__(kMaxT) k_norm(const __grid_constant__ Params p
     }
 }
 
+// Many rows: persistent thread blocks fed by bulk copies.  A step is G = threads / T
+// rows; a ring of stages holds the x and residual rows of the steps to come, so the
+// loads in flight do not depend on how many rows the registers hold, and the
+// weights and a shared gate row of a thread's columns stay in registers.
+constexpr int kStreamStages = 8;
+
+template <typename X, typename R, int N, int kThreads, bool kFull>
+__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
+    k_norm_stream(const __grid_constant__ Params p, const int T, const int stages, uint64_t wait_cap_ns, int32_t *err) {
+    constexpr int V = 8;
+    constexpr bool kKeep = N <= 2;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ __align__(16) float red[4][16];
+    __shared__ uint64_t full_bar[kStreamStages];
+    __shared__ int abort_word;
+    int slot = 0;
+    const int G = kThreads / T, g = threadIdx.x / T, tid = threadIdx.x & (T - 1);
+    const size_t steps = (p.rows + G - 1) / G;
+    const uint32_t x_bytes = (uint32_t)(p.c * sizeof(X)), r_bytes = p.has_res ? (uint32_t)(p.c * sizeof(R)) : 0u;
+    const uint32_t stage_bytes = G * (x_bytes + r_bytes);
+    const uint32_t base = smem_u32(ring);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; s++) mbar_init(smem_u32(&full_bar[s]), 1);
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncthreads();
+    auto fetch = [&](size_t step, int s) {
+        const size_t row0 = step * G;
+        const uint32_t rows = (uint32_t)min((size_t)G, p.rows - row0), bar = smem_u32(&full_bar[s]);
+        const uint32_t dx = base + s * stage_bytes, dr = dx + G * x_bytes;
+        mbar_expect_tx(bar, rows * (x_bytes + r_bytes));
+        auto copy = [&](uint32_t dst, const uint8_t *src, size_t pitch, uint32_t bytes) {
+            if (pitch == bytes) {
+                bulk_load(dst, src + row0 * pitch, rows * bytes, bar);
+            } else {
+                for (uint32_t r = 0; r < rows; r++) bulk_load(dst + r * bytes, src + (row0 + r) * pitch, bytes, bar);
+            }
+        };
+        copy(dx, (const uint8_t *)p.x, p.x_pitch * sizeof(X), x_bytes);
+        if (p.has_res) copy(dr, (const uint8_t *)p.res, p.res_pitch * sizeof(R), r_bytes);
+    };
+    if (threadIdx.x == 0) {
+        size_t step = blockIdx.x;
+        for (int s = 0; s < stages && step < steps; s++, step += gridDim.x) fetch(step, s);
+    }
+    // c0: what the normalised x of a column is multiplied by (weight, residual scale and,
+    // where all rows share it, the gate); w1: the weight of the next norm
+    float c0[kKeep ? N : 1][V], w1[kKeep ? N : 1][V];
+    bool live[N];
+    const bool row_gate = p.gate && p.gate_rows;
+    auto column = [&](int j) { return ((size_t)j * T + tid) * V; };
+    auto coefficients = [&](int j, float (&t)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; i++) t[i] = p.res_scale;
+        if (p.gate && !row_gate) {
+            Raw<X, V> g;
+            g.load((const X *)p.gate + column(j));
+#pragma unroll
+            for (int i = 0; i < V; i++) t[i] *= g.get(i);
+        }
+        if (p.w0 && p.post != DW_NORM_NONE) {
+            float w[V];
+            load_f32<V>(p.w0 + column(j), w);
+#pragma unroll
+            for (int i = 0; i < V; i++) t[i] *= w[i];
+        }
+    };
+    auto weights = [&](int j, float (&t)[V]) {
+        if (p.w1) {
+            load_f32<V>(p.w1 + column(j), t);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) t[i] = 1.0f;
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        live[j] = kFull || column(j) < p.c;
+        if constexpr (kKeep) {
+            if (live[j] && p.has_res) coefficients(j, c0[j]);
+            if (live[j]) weights(j, w1[j]);
+        }
+    }
+    // (mean, 1 / root) of v over the row; elements past the row are 0
+    auto statistics = [&](float (&v)[N][V], int kind) {
+        if (kind == DW_NORM_LAYER) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < N; j++)
+#pragma unroll
+                for (int i = 0; i < V; i++) sum += v[j][i];
+            const float mean = row_sum(sum, T, red, slot) * p.inv_c;
+#pragma unroll
+            for (int j = 0; j < N; j++)
+#pragma unroll
+                for (int i = 0; i < V; i++) v[j][i] = live[j] ? v[j][i] - mean : 0.0f;
+        }
+        float sq = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; j++)
+#pragma unroll
+            for (int i = 0; i < V; i++) sq = fmaf(v[j][i], v[j][i], sq);
+        return __frsqrt_rn(fmaf(row_sum(sq, T, red, slot), p.inv_c, p.eps));
+    };
+    int s = 0;
+    uint32_t ph = 0;
+    size_t step = blockIdx.x;
+    for (; step < steps; step += gridDim.x) {
+        if (!mbar_try_wait(smem_u32(&full_bar[s]), ph)) {
+            const uint64_t t0 = globaltimer_ns();
+            while (!mbar_try_wait_sleep(smem_u32(&full_bar[s]), ph, 20000u))
+                if (globaltimer_ns() - t0 > wait_cap_ns) {
+                    abort_word = 1;
+                    record_error(err, DW_DEV_WAIT_EXPIRED, 41, (int)ph);
+                    break;
+                }
+        }
+        // rows of the last step past the end hold what the stage held: they stay in
+        // their own threads and nothing of them is stored
+        Raw<X, V> xr[N];
+        Raw<R, V> rr[N];
+        const X *xs = reinterpret_cast<const X *>(ring + s * stage_bytes + g * x_bytes);
+        const R *rs = reinterpret_cast<const R *>(ring + s * stage_bytes + G * x_bytes + g * r_bytes);
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            if (!kFull) xr[j].zero(), rr[j].zero();
+            if (live[j]) {
+                xr[j].load(xs + column(j));
+                if (p.has_res) rr[j].load(rs + column(j));
+            }
+        }
+        __syncthreads();  // the stage has been read
+        if (abort_word) break;
+        if (threadIdx.x == 0 && step + (size_t)stages * gridDim.x < steps) fetch(step + (size_t)stages * gridDim.x, s);
+        if (++s == stages) s = 0, ph ^= 1;
+
+        const size_t row = step * G + g;
+        const bool there = row < p.rows;
+        float v[N][V];
+#pragma unroll
+        for (int j = 0; j < N; j++)
+#pragma unroll
+            for (int i = 0; i < V; i++) v[j][i] = xr[j].get(i);
+        if (p.has_res) {
+            const float rstd = p.post != DW_NORM_NONE ? statistics(v, p.post) : 1.0f;
+            const X *gate = (const X *)p.gate + (row_gate && there ? row / p.gate_rows : 0) * p.c;
+            R *out = (R *)p.out + row * p.res_pitch;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                if (!live[j]) continue;
+                float o[V], t[V];
+                if constexpr (kKeep) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) t[i] = c0[j][i];
+                } else {
+                    coefficients(j, t);
+                }
+                Raw<X, V> gr;
+                if (row_gate) gr.load(gate + column(j));
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    if (row_gate) t[i] *= gr.get(i);
+                    o[i] = fmaf(v[j][i] * rstd, t[i], rr[j].get(i));
+                }
+                if (p.b0 && p.post != DW_NORM_NONE) {  // + res_scale * gate * b
+                    float b[V];
+                    load_f32<V>(p.b0 + column(j), b);
+                    if (p.gate && !row_gate) gr.load((const X *)p.gate + column(j));
+#pragma unroll
+                    for (int i = 0; i < V; i++) o[i] = fmaf(b[i], p.gate ? p.res_scale * gr.get(i) : p.res_scale, o[i]);
+                }
+                Raw<R, V> r;
+                r.set(o);
+                if (there) r.store(out + column(j));
+#pragma unroll
+                for (int i = 0; i < V; i++) v[j][i] = r.get(i);
+            }
+        }
+        if (p.y_dtype == -1) continue;
+        if (p.pre != DW_NORM_NONE) {
+            const float rstd = statistics(v, p.pre);
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                if (!live[j]) continue;
+                float t[V];
+                if constexpr (kKeep) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) t[i] = w1[j][i];
+                } else {
+                    weights(j, t);
+                }
+#pragma unroll
+                for (int i = 0; i < V; i++) v[j][i] = v[j][i] * rstd * t[i];
+                if (p.b1) {
+                    load_f32<V>(p.b1 + column(j), t);
+#pragma unroll
+                    for (int i = 0; i < V; i++) v[j][i] += t[i];
+                }
+            }
+        }
+        if (p.y_dtype == -2) {
+#pragma unroll
+            for (int j = 0; j < N; j++) put_mxfp4<V>(v[j], column(j), row, there, p);
+        } else if (there) {
+            auto store = [&](auto *y) {
+                y += row * p.y_pitch;
+#pragma unroll
+                for (int j = 0; j < N; j++)
+                    if (live[j]) put<std::remove_pointer_t<decltype(y)>, V>(y, column(j), v[j]);
+            };
+            if (p.y_dtype == DW_F32)
+                store((float *)p.y);
+            else if (p.y_dtype == DW_F16)
+                store((__half *)p.y);
+            else
+                store((__nv_bfloat16 *)p.y);
+        }
+    }
+    // after an expired wait: the copies still in flight land before the block ends
+    if (threadIdx.x == 0 && step < steps) {
+        for (int i = 0; i < stages && step < steps; i++, step += gridDim.x) {
+            const uint64_t t0 = globaltimer_ns();
+            while (!mbar_try_wait_sleep(smem_u32(&full_bar[s]), ph, 20000u) && globaltimer_ns() - t0 < wait_cap_ns) {
+            }
+            if (++s == stages) s = 0, ph ^= 1;
+        }
+    }
+}
+
 // Rows too long for registers: one thread block a row, elements read again for
 // each reduction (from L2) and `out` read back by the thread that wrote it.
 template <typename X, typename R>
 __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Params p) {
-    __shared__ float red[4][32];
+    __shared__ __align__(16) float red[4][16];
     int slot = 0;
     const size_t row = blockIdx.x;
-    const size_t T = blockDim.x, end = p.tiles * 128;
+    const size_t T = blockDim.x, end = p.nb * 32;
     const X *x = (const X *)p.x + row * p.x_pitch;
     const R *res = (const R *)p.res + row * p.res_pitch;
     const X *gate = (const X *)p.gate + (p.gate_rows ? row / p.gate_rows : 0) * p.c;
@@ -216,14 +472,14 @@ __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Par
         if (kind == DW_NORM_LAYER) {
             float sum = 0.0f;
             for (size_t i = threadIdx.x; i < p.c; i += T) sum += at(i);
-            mean = row_sum(sum, red, slot) * p.inv_c;
+            mean = row_sum(sum, (int)T, red, slot) * p.inv_c;
         }
         float sq = 0.0f;
         for (size_t i = threadIdx.x; i < p.c; i += T) {
             const float d = at(i) - mean;
             sq = fmaf(d, d, sq);
         }
-        rstd = __frsqrt_rn(fmaf(row_sum(sq, red, slot), p.inv_c, p.eps));
+        rstd = __frsqrt_rn(fmaf(row_sum(sq, (int)T, red, slot), p.inv_c, p.eps));
     };
     auto scaled = [&](float v, size_t i, float mean, float rstd, const float *w, const float *b) {
         v = (v - mean) * rstd;
@@ -254,7 +510,7 @@ __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Par
             if (p.pre != DW_NORM_NONE) v[0] = scaled(v[0], i, mean, rstd, p.w1, p.b1);
         }
         if (p.y_dtype == -2) {
-            put_mxfp4<1>(v, i, row, p);
+            put_mxfp4<1>(v, i, row, true, p);
         } else if (i < p.c) {
             const size_t to = row * p.y_pitch + i;
             if (p.y_dtype == DW_F32)
@@ -265,6 +521,36 @@ __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Par
                 put<__nv_bfloat16, 1>(p.y, to, v);
         }
     }
+}
+
+template <typename X, typename R, int N, int kThreads, bool kFull>
+dw_status stream_as(dw_backend *be, const Params &p, int T) {
+    auto kernel = k_norm_stream<X, R, N, kThreads, kFull>;
+    const size_t G = kThreads / T, stage = G * p.c * (sizeof(X) + (p.has_res ? sizeof(R) : 0));
+    const int per_sm = kThreads == 256 ? 2 : 1;
+    const int stages = (int)std::min<size_t>(kStreamStages, (kSmemBudget / per_sm) / stage);
+    static bool attr_set[16] = {};
+    if (be->device < 16 && !attr_set[be->device]) {
+        dw_status st = dw_cuda_check(
+            be, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBudget), "norm attributes");
+        if (st != DW_OK) return st;
+        attr_set[be->device] = true;
+    }
+    const size_t steps = (p.rows + G - 1) / G;
+    const unsigned grid = (unsigned)std::min<size_t>(steps, (size_t)be->sm_count * per_sm);
+    kernel<<<grid, kThreads, stages * stage, be->stream>>>(p, T, stages, be->wait_cap_ns, be->dev_err);
+    return dw_after_launch(be, "norm");
+}
+
+template <typename X, typename R>
+dw_status stream(dw_backend *be, const Params &p) {
+    int T = 8;
+    while ((size_t)T * (T < 32 ? 8 : 16) < p.c && T < 256) T *= 2;
+    if ((size_t)T * 8 >= p.c) return stream_as<X, R, 1, 256, false>(be, p, T);
+    if ((size_t)T * 16 == p.c) return stream_as<X, R, 2, 256, true>(be, p, T);
+    if ((size_t)T * 16 >= p.c) return stream_as<X, R, 2, 256, false>(be, p, T);
+    if ((size_t)512 * 16 >= p.c) return stream_as<X, R, 2, 512, false>(be, p, 512);
+    return stream_as<X, R, 4, 512, false>(be, p, 512);
 }
 
 template <typename X, typename R>
@@ -286,6 +572,7 @@ dw_status run(dw_backend *be, const Params &p) {
         k_norm_long<X, R><<<(unsigned)p.rows, kMaxT, 0, be->stream>>>(p);
         return dw_after_launch(be, "norm (long rows)");
     }
+    if (fits(8) && p.c <= (size_t)kMaxT * kMaxE && p.rows >= (size_t)be->sm_count * 2) return stream<X, R>(be, p);
     // E: elements of a thread; T: threads of a row (a power of two from 32 to 512)
     int E = 8, T = 32;
     while ((size_t)T * E < p.c && T < kMaxT) T *= 2;

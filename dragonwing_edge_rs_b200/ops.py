@@ -372,51 +372,38 @@ def gemm_to_mxfp4(backend: CudaBackend, a_q, a_s, b_q, b_s, bias, y_q, y_s, m: i
                                              _h(y_s), m, n, k, act))
 
 
-@dataclass
-class NormDesc:
+class NormDesc(L.DwNormDesc):
     """Rows of c values, their types, the norm of the next block's input (pre) and
-    of the block's output (post), and how the residual is joined."""
+    of the block's output (post), and how the residual is joined (dw_norm_desc)."""
 
-    rows: int
-    c: int
-    x_dtype: int
-    res_dtype: int
-    y_dtype: int
-    pre: int = NORM_RMS
-    post: int = NORM_NONE
-    eps: float = 1e-5
-    gate_rows: int = 0
-    res_scale: float = 1.0
-    x_pitch: int = 0
-    res_pitch: int = 0
-    y_pitch: int = 0
-
-    def to_c(self) -> L.DwNormDesc:
-        return L.DwNormDesc(self.rows, self.c, self.x_pitch, self.res_pitch, self.y_pitch, self.gate_rows, self.x_dtype,
-                            self.res_dtype, self.y_dtype, self.pre, self.post, self.eps, self.res_scale)
+    def __init__(self, rows: int, c: int, x_dtype: int, res_dtype: int, y_dtype: int, pre: int = NORM_RMS,
+                 post: int = NORM_NONE, eps: float = 1e-5, gate_rows: int = 0, res_scale: float = 1.0, x_pitch: int = 0,
+                 res_pitch: int = 0, y_pitch: int = 0):
+        super().__init__(rows, c, x_pitch, res_pitch, y_pitch, gate_rows, x_dtype, res_dtype, y_dtype, pre, post, eps,
+                         res_scale)
 
 
 def norm(backend: CudaBackend, desc: NormDesc, x, w, b, y):
     """y = pre(x) with weight w and bias b (f32 [c] or None)."""
-    backend._check(L.load().dw_norm(backend.handle, ctypes.byref(desc.to_c()), _h(x), _h(w), _h(b), _h(y)))
+    backend._check(L.load().dw_norm(backend.handle, ctypes.byref(desc), _h(x), _h(w), _h(b), _h(y)))
 
 
 def norm_to_mxfp4(backend: CudaBackend, desc: NormDesc, x, w, b, q, s):
     """norm with its f32 result quantised to an MXFP4 operand."""
-    backend._check(L.load().dw_norm_to_mxfp4(backend.handle, ctypes.byref(desc.to_c()), _h(x), _h(w), _h(b), _h(q), _h(s)))
+    backend._check(L.load().dw_norm_to_mxfp4(backend.handle, ctypes.byref(desc), _h(x), _h(w), _h(b), _h(q), _h(s)))
 
 
 def norm_residual(backend: CudaBackend, desc: NormDesc, x, w_post, b_post, gate, residual, out, w_pre=None, b_pre=None,
                   y=None):
     """out = residual + res_scale * gate * post(x); y = pre(out) (None: `out` alone)."""
-    backend._check(L.load().dw_norm_residual(backend.handle, ctypes.byref(desc.to_c()), _h(x), _h(w_post), _h(b_post),
+    backend._check(L.load().dw_norm_residual(backend.handle, ctypes.byref(desc), _h(x), _h(w_post), _h(b_post),
                                              _h(gate), _h(residual), _h(out), _h(w_pre), _h(b_pre), _h(y)))
 
 
 def norm_residual_to_mxfp4(backend: CudaBackend, desc: NormDesc, x, w_post, b_post, gate, residual, out, w_pre, b_pre,
                            q, s):
     """norm_residual with y quantised to an MXFP4 operand."""
-    backend._check(L.load().dw_norm_residual_to_mxfp4(backend.handle, ctypes.byref(desc.to_c()), _h(x), _h(w_post),
+    backend._check(L.load().dw_norm_residual_to_mxfp4(backend.handle, ctypes.byref(desc), _h(x), _h(w_post),
                                                       _h(b_post), _h(gate), _h(residual), _h(out), _h(w_pre), _h(b_pre),
                                                       _h(q), _h(s)))
 

@@ -56,7 +56,9 @@ def pitched(v, dtype, pitch):
 
 
 CASES = [(1, 1), (1, 4096), (3, 7), (9, 32), (257, 64), (40, 101), (5, 1010), (6, 1024), (33, 576), (2, 5000), (3, 8192), (2, 11008),
-         (2, 16383), (2, 16384), (3, 20001), (2, 40000)]
+         (2, 16383), (2, 16384), (3, 20001), (2, 40000),
+         # many rows
+         (333, 8), (300, 64), (1001, 104), (400, 1024), (297, 4096), (300, 8192), (299, 11008), (298, 16384)]
 
 
 @pytest.mark.parametrize("dtype,ydtype", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f32", "bf16")])
@@ -78,7 +80,10 @@ def test_norm(be, dtype, ydtype, kind, rows, c):
 @pytest.mark.parametrize("dtype,res", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f32")])
 @pytest.mark.parametrize("rows,c,post,pre,gate_rows", [(1, 4096, NONE, RMS, None), (7, 1010, RMS, RMS, 0), (10, 333, LAYER, LAYER, 4),
                                                        (70, 96, RMS, LAYER, 1), (3, 20001, LAYER, RMS, 2), (2, 16384, RMS, RMS, 0),
-                                                       (5, 64, RMS, NONE, None), (300, 512, NONE, LAYER, 100)])
+                                                       (5, 64, RMS, NONE, None), (300, 512, NONE, LAYER, 100),
+                                                       (310, 4096, RMS, RMS, 0), (301, 2048, LAYER, LAYER, 100),
+                                                       (305, 104, RMS, RMS, 1), (300, 5120, LAYER, RMS, 7),
+                                                       (299, 11008, RMS, RMS, None), (1030, 72, RMS, NONE, 0)])
 def test_norm_residual(be, dtype, res, rows, c, post, pre, gate_rows):
     """`out` against float64, and y against the norm of the stored `out`."""
     rng = np.random.default_rng(rows * 7 + c)
@@ -88,18 +93,23 @@ def test_norm_residual(be, dtype, res, rows, c, post, pre, gate_rows):
     gr, g = R.to_type(rng.normal(0.5, 0.5, (groups, c)), dtype) if groups else (None, None)
     w0, w1 = rng.normal(1, 0.3, c).astype(np.float32), rng.normal(1, 0.3, c).astype(np.float32)
     b1 = rng.normal(0, 0.3, c).astype(np.float32)
+    b0 = rng.normal(0, 0.3, c).astype(np.float32) if post == LAYER else None
     scale = 0.75
     d = ops.NormDesc(rows, c, R.DTYPES[dtype], R.DTYPES[res], R.DTYPES[dtype], pre, post, 1e-6, gate_rows or 0, scale)
     es, rs = (4 if dtype == "f32" else 2), (4 if res == "f32" else 2)
     out, y = be.alloc(rows * c * rs), be.alloc(rows * c * es)
     bx, bw0, bw1, bb1 = be.upload_array(xr), be.upload_array(w0), be.upload_array(w1), be.upload_array(b1)
     bg = be.upload_array(gr) if groups else None
-    ops.norm_residual(be, d, bx, bw0, None, bg, be.upload_array(rr), out, bw1, bb1, y)
+    bb0 = be.upload_array(b0) if b0 is not None else None
+    ops.norm_residual(be, d, bx, bw0, bb0, bg, be.upload_array(rr), out, bw1, bb1, y)
     raw_out = be.download_array(out, R.np_type(res))
     got = R.from_type(raw_out, res).reshape(rows, c)
     gv = g[np.arange(rows) // gate_rows if gate_rows else np.zeros(rows, int)] if groups else 1.0
-    n = R.norm(x, post, w0, None, 1e-6) * gv
-    tol = scale * (np.abs(gv) * norm_tol(x, post, w0, None, 1e-6) + 2.0 ** -24 * np.abs(n))
+    n = R.norm(x, post, w0, b0, 1e-6) * gv
+    # the products by the gate and the scale, and the sum with the bias' part, round once each
+    tol = scale * (np.abs(gv) * norm_tol(x, post, w0, b0, 1e-6) + 3 * 2.0 ** -24 * np.abs(n))
+    if b0 is not None:
+        tol = tol + 4 * 2.0 ** -24 * (np.abs(scale * gv * b0) + np.abs(r))
     near(got, r + scale * n, tol * 1.01, res)
     got_y = R.from_type(be.download_array(y, R.np_type(dtype)), dtype).reshape(rows, c)
     wy, by = (w1, b1) if pre != NONE else (None, None)
@@ -107,7 +117,7 @@ def test_norm_residual(be, dtype, res, rows, c, post, pre, gate_rows):
 
     # in place, and without y: the same bits
     inplace = be.upload_array(rr)
-    ops.norm_residual(be, d, bx, bw0, None, bg, inplace, inplace)
+    ops.norm_residual(be, d, bx, bw0, bb0, bg, inplace, inplace)
     np.testing.assert_array_equal(be.download_array(inplace, R.np_type(res)), raw_out)
     # the fused quantisation: what the quantiser makes of the f32 norm of `out`
     df = ops.NormDesc(rows, c, R.DTYPES[res], R.DTYPES[res], ops.F32, pre, eps=1e-6)
@@ -117,7 +127,7 @@ def test_norm_residual(be, dtype, res, rows, c, post, pre, gate_rows):
     q2, s2 = (be.upload_array(np.full(f(rows, c), 0xAB, np.uint8)) for f in (ops.mxfp4_code_bytes, ops.mxfp4_scale_bytes))
     ops.quantize_mxfp4(be, yf, ops.F32, rows, c, q, s)
     out2 = be.alloc(rows * c * rs)
-    ops.norm_residual_to_mxfp4(be, d, bx, bw0, None, bg, be.upload_array(rr), out2, bw1, bb1, q2, s2)
+    ops.norm_residual_to_mxfp4(be, d, bx, bw0, bb0, bg, be.upload_array(rr), out2, bw1, bb1, q2, s2)
     np.testing.assert_array_equal(be.download_array(out2, R.np_type(res)), raw_out)
     np.testing.assert_array_equal(be.download_array(q2, np.uint8), be.download_array(q, np.uint8))
     np.testing.assert_array_equal(be.download_array(s2, np.uint8), be.download_array(s, np.uint8))
