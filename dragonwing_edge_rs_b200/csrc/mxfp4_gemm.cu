@@ -35,7 +35,6 @@ constexpr int kBKBytes = 128;  // a K block: 256 codes
 constexpr size_t kSmemLimit = 227 * 1024;
 
 struct GemmParams {
-    const uint8_t *a_s, *b_s;
     const float *bias;
     void *y;
     uint8_t *y_s;
@@ -43,39 +42,23 @@ struct GemmParams {
     size_t tiles_k;   // scale tiles (128 codes) along K
     size_t out_nb, out_tiles;  // MXFP4 result: blocks and scale tiles along n
     int k_blocks;     // 256-wide K blocks
-    int tiles_m, tiles_n, tiles;
-    int a_row_tiles, b_row_tiles;  // 128-row scale tiles
+    int tiles_m, tiles;
     int stages, act;
     bool vec, bias_vec;  // rows of y, the bias start on 16-byte boundaries
     uint64_t wait_cap_ns;
     int32_t *err;
 };
 
-// try_wait that acquires what another CTA of the cluster released by its arrival.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 // Bounded wait for a phase; false once the CTA is aborting or the cap expired.
-// kCluster: arrivals come from another CTA.
-template <bool kCluster = false>
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, uint64_t cap_ns, int32_t *err,
                                            volatile int *abort_flag, int site) {
 #pragma unroll 1
     for (int i = 0; i < 64; i++)
-        if (kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+        if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
     for (;;) {
-        if (kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+        if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
         if (*abort_flag) return false;
         if (globaltimer_ns() - t0 > cap_ns) {
             *abort_flag = 1;
@@ -230,7 +213,22 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
     return a;
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// Copies into this CTA that complete on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+        "[%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+        "[%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
 }
 // Commits of the pair: to the leader's barrier, or to the same barrier of both CTAs.
 __device__ __forceinline__ void tc_commit2(uint32_t bar) {
@@ -257,6 +255,7 @@ __device__ __forceinline__ void tc_mma_mxf4_2(uint32_t d, uint64_t a, uint64_t b
 template <int BN, int kOut>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     k_mxfp4_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                 const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb,
                  const __grid_constant__ GemmParams p) {
     constexpr uint32_t kA = kBM * kBKBytes, kB = BN / 2 * kBKBytes, kSA = 1024, kSB = (BN / 128) * 1024;
     constexpr uint32_t kStage = kA + kB + kSA + kSB;
@@ -265,7 +264,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     constexpr int kCols = BN / 4;                 // columns of an epilogue warp
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-    __shared__ uint64_t full_bar[kMaxStages], peer_bar[kMaxStages], sf_bar[kMaxStages], empty_bar[kMaxStages];
+    __shared__ uint64_t full_bar[kMaxStages], sf_bar[kMaxStages], empty_bar[kMaxStages];
     __shared__ uint64_t tfull_bar[kAcc], tempty_bar[kAcc], drain_bar[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
@@ -277,7 +276,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; s++) {
             mbar_init(smem_u32(&full_bar[s]), 1);
-            mbar_init(smem_u32(&peer_bar[s]), 1);
             mbar_init(smem_u32(&sf_bar[s]), 1);
             mbar_init(smem_u32(&empty_bar[s]), 1);
         }
@@ -309,69 +307,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             bool ok = true;
             for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
                 const int tm = (tile % p.tiles_m) * 2 + (int)rank, tn = tile / p.tiles_m;  // 128-row tile of A, BN-row tile of B
-                // a 128-row tile of A past the end has no scales (its rows are zeros, and not stored)
-                const bool sa = tm < p.a_row_tiles;
-                const int nsb = min(BN / 128, p.b_row_tiles - tn * (BN / 128));
                 for (int kb = 0; kb < p.k_blocks; kb++) {
                     if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 21)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t bar = smem_u32(&full_bar[s]), base = smem + s * kStage;
-                    const uint32_t sbytes = (uint32_t)min((size_t)2, p.tiles_k - 2 * (size_t)kb) * 512;
-                    mbar_expect_tx(bar, kA + kB + sbytes * (sa + nsb));
-                    tma_load_2d(base, &tmap_a, bar, kb * kBKBytes, tm * kBM);
-                    tma_load_2d(base + kA, &tmap_b, bar, kb * kBKBytes, tn * BN + (int)rank * (BN / 2));
-                    if (sa) bulk_load(base + kA + kB, p.a_s + ((size_t)tm * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
-                    for (int j = 0; j < nsb; j++)
-                        bulk_load(base + kA + kB + kSA + j * 1024,
-                                  p.b_s + (((size_t)tn * (BN / 128) + j) * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
+                    // both CTAs' copies complete on the leader's barrier
+                    const uint32_t bar = peer_addr(smem_u32(&full_bar[s]), 0), base = smem + s * kStage;
+                    if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[s]), 2 * kStage);
+                    tma_load_2d_pair(base, &tmap_a, bar, kb * kBKBytes, tm * kBM);
+                    tma_load_2d_pair(base + kA, &tmap_b, bar, kb * kBKBytes, tn * BN + (int)rank * (BN / 2));
+                    tma_load_3d_pair(base + kA + kB, &tmap_sa, bar, 0, 2 * kb, tm);
+                    tma_load_3d_pair(base + kA + kB + kSA, &tmap_sb, bar, 0, 2 * kb, tn * (BN / 128));
                     issued++;
                     if (++s == p.stages) s = 0, ph ^= 1;
                 }
             }
-            // the last copies into each stage have landed before the CTA ends
-            for (int i = 0; i < min(issued, p.stages); i++) {
+            // the last copies into each stage have landed before the pair ends
+            for (int i = 0; rank == 0 && i < min(issued, p.stages); i++) {
                 if (--s < 0) s = p.stages - 1, ph ^= 1;
                 drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
             }
         }
     } else if (warp == 2) {
-        // the leader: each stage's scales into both CTAs' tensor memory, ahead of the
-        // products; the peer: tells the leader that its stage has landed
-        if (lane == 0) {
+        // each stage's scales into both CTAs' tensor memory, ahead of the products
+        if (lane == 0 && rank == 0) {
             int s = 0;
             uint32_t ph = 0;
             bool ok = true;
             for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
                 for (int kb = 0; kb < p.k_blocks; kb++) {
-                    if (!wait_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 22) ||
-                        (rank == 0 && !wait_phase<true>(smem_u32(&peer_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 23))) {
+                    if (!wait_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 22)) {
                         ok = false;
                         break;
                     }
-                    if (rank == 0) {
-                        tc_fence_after();
-                        const uint32_t base = smem + s * kStage + kA + kB;
-                        const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 8;
-                        const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
-                        for (int c = 0; c < chunks; c++) {
-                            tc_cp_scales2(sfa + c * 4, smem_desc_noswz(base + c * 512, 16, 128));
+                    const uint32_t base = smem + s * kStage + kA + kB;
+                    const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 8;
+                    const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
+                    for (int c = 0; c < chunks; c++) {
+                        tc_cp_scales2(sfa + c * 4, smem_desc_noswz(base + c * 512, 16, 128));
 #pragma unroll
-                            for (int j = 0; j < BN / 128; j++)
-                                tc_cp_scales2(sfb + c * (BN / 32) + j * 4, smem_desc_noswz(base + kSA + j * 1024 + c * 512, 16, 128));
-                        }
-                        tc_commit2(smem_u32(&sf_bar[s]));
-                    } else {
-                        mbar_arrive_cluster(peer_addr(smem_u32(&peer_bar[s]), 0));
+                        for (int j = 0; j < BN / 128; j++)
+                            tc_cp_scales2(sfb + c * (BN / 32) + j * 4, smem_desc_noswz(base + kSA + j * 1024 + c * 512, 16, 128));
                     }
+                    tc_commit2(smem_u32(&sf_bar[s]));
                     if (++s == p.stages) s = 0, ph ^= 1;
                 }
             }
-            if (rank == 0) {
-                tc_commit2(smem_u32(&drain_bar[1]));
-                drain_phase(smem_u32(&drain_bar[1]), 0, p.wait_cap_ns);
-            }
+            tc_commit2(smem_u32(&drain_bar[1]));
+            drain_phase(smem_u32(&drain_bar[1]), 0, p.wait_cap_ns);
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
@@ -380,7 +364,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             bool ok = true;
             const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
             for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
-                if (!wait_phase<true>(smem_u32(&tempty_bar[acc]), aph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 24)) break;
+                if (!wait_phase(smem_u32(&tempty_bar[acc]), aph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 24)) break;
                 const uint32_t d = tmem + acc * BN;
                 for (int kb = 0; kb < p.k_blocks; kb++) {
                     if (!wait_phase(smem_u32(&sf_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 25)) {
@@ -456,6 +440,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             }
         }
     }
+    __syncwarp();
     tc_fence_before();
     cluster_sync();  // all products and copies of the pair are done
     if (warp == 1) {
@@ -681,11 +666,23 @@ bool code_map(dw_backend *be, CUtensorMap *map, const uint8_t *q, size_t rows, s
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Scales as a 3-D tensor [row tiles][tiles along K][512 bytes]; a box is two tiles
+// along K of `row_tiles` row tiles.
+bool scale_map(dw_backend *be, CUtensorMap *map, const uint8_t *s, size_t rows, size_t k, int row_tiles) {
+    cuuint64_t dims[3] = {128, (cuuint64_t)mx_tiles(k), (cuuint64_t)((rows + 127) / 128)};
+    cuuint64_t strides[2] = {512, (cuuint64_t)mx_tiles(k) * 512};
+    cuuint32_t box[3] = {128, 2, (cuuint32_t)row_tiles};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return be->encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t *>(s), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int BN, int kOut>
 dw_status launch(dw_backend *be, const MxGemmArgs &a) {
     constexpr size_t kStage = kBM * kBKBytes + BN / 2 * kBKBytes + 1024 + (BN / 128) * 1024;
     GemmParams p{};
-    p.a_s = a.a_s, p.b_s = a.b_s, p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
+    p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
     p.m = a.m, p.n = a.n;
     p.tiles_k = mx_tiles(a.k);
     p.out_nb = mx_blocks(a.n), p.out_tiles = mx_tiles(a.n);
@@ -693,7 +690,6 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a) {
     const size_t tm = (a.m + 2 * kBM - 1) / (2 * kBM), tn = (a.n + BN - 1) / BN;
     if (tm * tn > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu x %zu is too large", a.m, a.n);
     p.tiles_m = (int)tm, p.tiles = (int)(tm * tn);
-    p.a_row_tiles = (int)((a.m + 127) / 128), p.b_row_tiles = (int)((a.n + 127) / 128);
     p.act = a.act;
     const size_t es = kOut == 0 ? 4 : 2;
     p.vec = ((uintptr_t)a.y & 15) == 0 && a.n * es % 16 == 0;
@@ -702,8 +698,9 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a) {
     p.stages = (int)std::min<size_t>(kMaxStages, (kSmemLimit - 4096) / kStage);
     // at least 116 KiB: one CTA per SM owns the tensor memory
     const size_t smem = std::max<size_t>(1024 + p.stages * kStage, 116 * 1024);
-    CUtensorMap ta, tb;
-    if (!be->encode_tiled || !code_map(be, &ta, a.a_q, a.m, a.k, kBM) || !code_map(be, &tb, a.b_q, a.n, a.k, BN / 2))
+    CUtensorMap ta, tb, tsa, tsb;
+    if (!be->encode_tiled || !code_map(be, &ta, a.a_q, a.m, a.k, kBM) || !code_map(be, &tb, a.b_q, a.n, a.k, BN / 2) ||
+        !scale_map(be, &tsa, a.a_s, a.m, a.k, 1) || !scale_map(be, &tsb, a.b_s, a.n, a.k, BN / 128))
         return dw_fail(be, DW_ERR_DEVICE, "gemm_mxfp4: tensor map rejected");
     auto kernel = k_mxfp4_gemm<BN, kOut>;
     static bool attr_set[16] = {};
@@ -714,7 +711,7 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a) {
         if (st != DW_OK) return st;
         attr_set[be->device] = true;
     }
-    kernel<<<2 * std::min(p.tiles, be->sm_count / 2), kGemmThreads, smem, be->stream>>>(ta, tb, p);
+    kernel<<<2 * std::min(p.tiles, be->sm_count / 2), kGemmThreads, smem, be->stream>>>(ta, tb, tsa, tsb, p);
     return dw_after_launch(be, "gemm_mxfp4");
 }
 
