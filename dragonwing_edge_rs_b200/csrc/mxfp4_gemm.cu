@@ -41,7 +41,7 @@ struct GemmParams {
     size_t m, n;
     size_t tiles_k;   // scale tiles (128 codes) along K
     size_t out_nb, out_tiles;  // MXFP4 result: blocks and scale tiles along n
-    int k_blocks;     // 256-wide K blocks
+    int k_blocks;     // 512-wide K blocks
     int tiles_m, tiles;
     int stages, act;
     bool vec, bias_vec;  // rows of y, the bias start on 16-byte boundaries
@@ -257,9 +257,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     k_mxfp4_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                  const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb,
                  const __grid_constant__ GemmParams p) {
-    constexpr uint32_t kA = kBM * kBKBytes, kB = BN / 2 * kBKBytes, kSA = 1024, kSB = (BN / 128) * 1024;
-    constexpr uint32_t kStage = kA + kB + kSA + kSB;
-    constexpr uint32_t kScaleCols = 8 + BN / 16;  // tensor-memory columns of a stage's scales
+    // a stage: 512 codes of a row in two swizzled boxes of 128 bytes, four scale tiles
+    constexpr uint32_t kA = kBM * kBKBytes, kB = BN / 2 * kBKBytes, kSA = 2048, kSB = (BN / 128) * 2048;
+    constexpr uint32_t kStage = 2 * (kA + kB) + kSA + kSB;
+    constexpr uint32_t kScaleCols = 16 + BN / 8;  // tensor-memory columns of a stage's scales
     constexpr int kAcc = 256 / BN;                // accumulator buffers
     constexpr int kCols = BN / 4;                 // columns of an epilogue warp
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -314,11 +315,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     }
                     // both CTAs' copies complete on the leader's barrier
                     const uint32_t bar = peer_addr(smem_u32(&full_bar[s]), 0), base = smem + s * kStage;
+                    const uint32_t sf = base + 2 * (kA + kB);
                     if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[s]), 2 * kStage);
-                    tma_load_2d_pair(base, &tmap_a, bar, kb * kBKBytes, tm * kBM);
-                    tma_load_2d_pair(base + kA, &tmap_b, bar, kb * kBKBytes, tn * BN + (int)rank * (BN / 2));
-                    tma_load_3d_pair(base + kA + kB, &tmap_sa, bar, 0, 2 * kb, tm);
-                    tma_load_3d_pair(base + kA + kB + kSA, &tmap_sb, bar, 0, 2 * kb, tn * (BN / 128));
+                    const int b_row = tn * BN + (int)rank * (BN / 2);
+                    tma_load_2d_pair(base, &tmap_a, bar, 2 * kb * kBKBytes, tm * kBM);
+                    tma_load_2d_pair(base + 2 * kA, &tmap_b, bar, 2 * kb * kBKBytes, b_row);
+                    tma_load_3d_pair(sf, &tmap_sa, bar, 0, 4 * kb, tm);
+                    tma_load_3d_pair(sf + kSA, &tmap_sb, bar, 0, 4 * kb, tn * (BN / 128));
+                    tma_load_2d_pair(base + kA, &tmap_a, bar, (2 * kb + 1) * kBKBytes, tm * kBM);
+                    tma_load_2d_pair(base + 2 * kA + kB, &tmap_b, bar, (2 * kb + 1) * kBKBytes, b_row);
                     issued++;
                     if (++s == p.stages) s = 0, ph ^= 1;
                 }
@@ -330,7 +335,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             }
         }
     } else if (warp == 2) {
-        // each stage's scales into both CTAs' tensor memory, ahead of the products
+        // each stage's scales into both CTAs' tensor memory, ahead of the products (a
+        // thread of its own: copies that the issuing thread puts between its products
+        // hold these up, 0.58 instead of 0.40 us per 256 x 256 x 256)
         if (lane == 0 && rank == 0) {
             int s = 0;
             uint32_t ph = 0;
@@ -341,14 +348,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                         ok = false;
                         break;
                     }
-                    const uint32_t base = smem + s * kStage + kA + kB;
-                    const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 8;
-                    const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
+                    const uint32_t sf = smem + s * kStage + 2 * (kA + kB);
+                    const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 16;
+                    const int chunks = (int)min((size_t)4, p.tiles_k - 4 * (size_t)kb);
                     for (int c = 0; c < chunks; c++) {
-                        tc_cp_scales2(sfa + c * 4, smem_desc_noswz(base + c * 512, 16, 128));
+                        tc_cp_scales2(sfa + c * 4, smem_desc_noswz(sf + c * 512, 16, 128));
 #pragma unroll
                         for (int j = 0; j < BN / 128; j++)
-                            tc_cp_scales2(sfb + c * (BN / 32) + j * 4, smem_desc_noswz(base + kSA + j * 1024 + c * 512, 16, 128));
+                            tc_cp_scales2(sfb + c * (BN / 32) + j * 4, smem_desc_noswz(sf + kSA + j * 2048 + c * 512, 16, 128));
                     }
                     tc_commit2(smem_u32(&sf_bar[s]));
                     if (++s == p.stages) s = 0, ph ^= 1;
@@ -358,28 +365,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             drain_phase(smem_u32(&drain_bar[1]), 0, p.wait_cap_ns);
         }
     } else if (warp == 1) {
+        // a commit costs the tensor pipe about 0.1 us, so a stage is 512 wide: eight products
         if (lane == 0 && rank == 0) {
+            const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
             int s = 0, acc = 0;
             uint32_t ph = 0, aph = 0;
             bool ok = true;
-            const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
             for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
-                if (!wait_phase(smem_u32(&tempty_bar[acc]), aph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 24)) break;
+                if (!wait_phase(smem_u32(&tempty_bar[acc]), aph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 23)) break;
                 const uint32_t d = tmem + acc * BN;
                 for (int kb = 0; kb < p.k_blocks; kb++) {
-                    if (!wait_phase(smem_u32(&sf_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 25)) {
+                    if (!wait_phase(smem_u32(&sf_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 24)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t base = smem + s * kStage;
-                    const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 8;
-                    const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
+                    const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 16;
+                    const int chunks = (int)min((size_t)4, p.tiles_k - 4 * (size_t)kb);
                     for (int c = 0; c < chunks; c++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            const uint32_t off = (uint32_t)(c * 2 + h) * 32;
-                            tc_mma_mxf4_2(d, smem_desc(base + off, hi), smem_desc(base + kA + off, hi), mx_idesc(2 * kBM, BN, h),
+                            const uint32_t off = (uint32_t)((c & 1) * 2 + h) * 32;
+                            tc_mma_mxf4_2(d, smem_desc(base + (c >> 1) * kA + off, hi),
+                                          smem_desc(base + 2 * kA + (c >> 1) * kB + off, hi), mx_idesc(2 * kBM, BN, h),
                                           sfa + c * 4, sfb + c * (BN / 32), (kb | c | h) ? 1u : 0u);
                         }
                     tc_commit2_both(smem_u32(&empty_bar[s]));
@@ -666,12 +675,12 @@ bool code_map(dw_backend *be, CUtensorMap *map, const uint8_t *q, size_t rows, s
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Scales as a 3-D tensor [row tiles][tiles along K][512 bytes]; a box is two tiles
+// Scales as a 3-D tensor [row tiles][tiles along K][512 bytes]; a box is four tiles
 // along K of `row_tiles` row tiles.
 bool scale_map(dw_backend *be, CUtensorMap *map, const uint8_t *s, size_t rows, size_t k, int row_tiles) {
     cuuint64_t dims[3] = {128, (cuuint64_t)mx_tiles(k), (cuuint64_t)((rows + 127) / 128)};
     cuuint64_t strides[2] = {512, (cuuint64_t)mx_tiles(k) * 512};
-    cuuint32_t box[3] = {128, 2, (cuuint32_t)row_tiles};
+    cuuint32_t box[3] = {128, 4, (cuuint32_t)row_tiles};
     cuuint32_t estr[3] = {1, 1, 1};
     return be->encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t *>(s), dims, strides, box, estr,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -680,13 +689,13 @@ bool scale_map(dw_backend *be, CUtensorMap *map, const uint8_t *s, size_t rows, 
 
 template <int BN, int kOut>
 dw_status launch(dw_backend *be, const MxGemmArgs &a) {
-    constexpr size_t kStage = kBM * kBKBytes + BN / 2 * kBKBytes + 1024 + (BN / 128) * 1024;
+    constexpr size_t kStage = 2 * (kBM + BN / 2) * kBKBytes + 2048 + (BN / 128) * 2048;
     GemmParams p{};
     p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
     p.m = a.m, p.n = a.n;
     p.tiles_k = mx_tiles(a.k);
     p.out_nb = mx_blocks(a.n), p.out_tiles = mx_tiles(a.n);
-    p.k_blocks = (int)((a.k + 255) / 256);
+    p.k_blocks = (int)((a.k + 511) / 512);
     const size_t tm = (a.m + 2 * kBM - 1) / (2 * kBM), tn = (a.n + BN - 1) / BN;
     if (tm * tn > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu x %zu is too large", a.m, a.n);
     p.tiles_m = (int)tm, p.tiles = (int)(tm * tn);
