@@ -5,6 +5,7 @@
 #include <algorithm>
 
 #include "dw_device.cuh"
+#include "dw_launch.h"
 #include "dw_mxfp4.cuh"
 
 namespace dw {
@@ -33,6 +34,8 @@ __global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *__restrict
     const size_t unit = ((size_t)blockIdx.y << p.lux) + u;
     const size_t col = unit * 128 + lane16 * 8;
     const size_t row0 = (size_t)blockIdx.x * rows_blk * kRows + ry;
+    pdl_wait();
+    pdl_trigger();
     Raw<T, 8> raw[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
@@ -86,6 +89,8 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__
     const size_t unit = ((size_t)blockIdx.y << p.lux) + u;
     const size_t col = unit * 128 + lane16 * 8;
     const size_t row0 = (size_t)blockIdx.x * rows_blk * kRows + ry;
+    pdl_wait();
+    pdl_trigger();
     uint32_t codes[kRows], sb[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
@@ -121,6 +126,8 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__
 // get byte 0 (rows past the last are left as they are).  One thread per (row, tile).
 __global__ void __launch_bounds__(kThreads) k_pack_scales(const uint8_t *__restrict__ in, uint8_t *__restrict__ s,
                                                           size_t rows, size_t nb, size_t tiles) {
+    pdl_wait();
+    pdl_trigger();
     const size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x;
     if (i >= rows * tiles) return;
     const size_t row = i / tiles, t = i - row * tiles;
@@ -153,8 +160,7 @@ dw_status quantize(dw_backend *be, const void *x, size_t rows, size_t k, size_t 
     const bool vec = ((uintptr_t)x & 15) == 0 && pitch * sizeof(T) % 16 == 0;
     if (!make_shape(rows, k, pitch, vec, &p, &grid))
         return dw_fail(be, DW_ERR_UNSUPPORTED, "quantize_mxfp4: %zu x %zu is too large", rows, k);
-    k_quantize_mxfp4<T, kRowsPer><<<grid, kThreads, 0, be->stream>>>((const T *)x, q, s, p);
-    return dw_after_launch(be, "quantize_mxfp4");
+    return launch_dependent(be, "quantize_mxfp4", k_quantize_mxfp4<T, kRowsPer>, grid, kThreads, 0, 0, (const T *)x, q, s, p);
 }
 
 template <typename T>
@@ -164,8 +170,7 @@ dw_status dequantize(dw_backend *be, const uint8_t *q, const uint8_t *s, size_t 
     const bool vec = ((uintptr_t)y & 15) == 0 && k * sizeof(T) % 16 == 0;
     if (!make_shape(rows, k, k, vec, &p, &grid))
         return dw_fail(be, DW_ERR_UNSUPPORTED, "dequantize_mxfp4: %zu x %zu is too large", rows, k);
-    k_dequantize_mxfp4<T, kRowsPer><<<grid, kThreads, 0, be->stream>>>(q, s, (T *)y, p);
-    return dw_after_launch(be, "dequantize_mxfp4");
+    return launch_dependent(be, "dequantize_mxfp4", k_dequantize_mxfp4<T, kRowsPer>, grid, kThreads, 0, 0, q, s, (T *)y, p);
 }
 
 }  // namespace
@@ -191,8 +196,7 @@ dw_status launch_dequantize_mxfp4(dw_backend *be, const uint8_t *q, const uint8_
 dw_status launch_pack_scales_mxfp4(dw_backend *be, const uint8_t *in, size_t rows, size_t k, uint8_t *s) {
     const size_t nb = mx_blocks(k), tiles = mx_tiles(k), blocks = (rows * tiles + kThreads - 1) / kThreads;
     if (blocks > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "pack_scales_mxfp4: %zu x %zu is too large", rows, k);
-    k_pack_scales<<<(unsigned)blocks, kThreads, 0, be->stream>>>(in, s, rows, nb, tiles);
-    return dw_after_launch(be, "pack_scales_mxfp4");
+    return launch_dependent(be, "pack_scales_mxfp4", k_pack_scales, (unsigned)blocks, kThreads, 0, 0, in, s, rows, nb, tiles);
 }
 
 }  // namespace dw

@@ -20,9 +20,9 @@
 // and exits.
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "dw_device.cuh"
+#include "dw_launch.h"
 #include "dw_mxfp4.cuh"
 #include "dw_ptx.cuh"
 #include "dw_tcgen05.cuh"
@@ -49,12 +49,15 @@ struct GemmParams {
     int32_t *err;
 };
 
-// Bounded wait for a phase; false once the CTA is aborting or the cap expired.
+// Bounded wait for a phase; false once the CTA is aborting or the cap expired.  The
+// single threads that feed the tensor core poll (a thread that try_wait suspended
+// resumes late, and a stage's round trip bounds the rate); whole warps suspend soon.
+template <int kPolls = 1024>
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, uint64_t cap_ns, int32_t *err,
                                            volatile int *abort_flag, int site) {
 #pragma unroll 1
-    for (int i = 0; i < 64; i++)
-        if (mbar_try_wait(bar, parity)) return true;
+    for (int i = 0; i < kPolls; i++)
+        if (mbar_test_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
     for (;;) {
@@ -298,6 +301,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     tc_fence_before();
     cluster_sync();
     tc_fence_after();
+    pdl_trigger();
+    pdl_wait();
     const uint32_t tmem = tmem_slot;
     const uint32_t sf_cols = tmem + 256;  // scales after the accumulators
 
@@ -408,7 +413,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
         uint32_t aph = 0;
         for (int tile = pair; tile < p.tiles; tile += pairs) {
             const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
-            if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&tfull_bar[acc]), aph, p.wait_cap_ns, p.err, abort_flag, 26))) break;
+            if (!__all_sync(0xffffffffu, wait_phase<8>(smem_u32(&tfull_bar[acc]), aph, p.wait_cap_ns, p.err, abort_flag, 26))) break;
             tc_fence_after();
             const size_t row = ((size_t)tm * 2 + rank) * kBM + quarter * 32 + lane;
             const size_t col0 = (size_t)tn * BN + part * kCols;
@@ -526,6 +531,8 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_trigger();
+    pdl_wait();
     const uint32_t tmem = tmem_slot;
     const uint32_t sf_cols = tmem + (uint32_t)p.bn;  // 16 columns a stage after the accumulators
     const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -596,7 +603,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     if (warp >= 4) {
         // accumulators -> part[row of A][output]
         const int quarter = warp & 3;
-        if (__all_sync(0xffffffffu, wait_phase(smem_u32(&done_bar), 0, p.wait_cap_ns, p.err, abort_flag, 34))) {
+        if (__all_sync(0xffffffffu, wait_phase<8>(smem_u32(&done_bar), 0, p.wait_cap_ns, p.err, abort_flag, 34))) {
             tc_fence_after();
             const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
             const int cols = (int)min((size_t)p.bn, p.m - m0);
@@ -720,8 +727,8 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a) {
         if (st != DW_OK) return st;
         attr_set[be->device] = true;
     }
-    kernel<<<2 * std::min(p.tiles, be->sm_count / 2), kGemmThreads, smem, be->stream>>>(ta, tb, tsa, tsb, p);
-    return dw_after_launch(be, "gemm_mxfp4");
+    return launch_dependent(be, "gemm_mxfp4", kernel, 2 * std::min(p.tiles, be->sm_count / 2), kGemmThreads, smem, 0, ta, tb, tsa,
+                            tsb, p);
 }
 
 // CTAs of a cluster that share a tile's K: as many as fill the GPU once, each with
@@ -760,18 +767,7 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
         if (st != DW_OK) return st;
         attr_set[be->device] = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(S, (unsigned)tn, (unsigned)tm);
-    cfg.blockDim = dim3(kSkinnyThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = be->stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = S, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    dw_status st = dw_cuda_check(be, cudaLaunchKernelEx(&cfg, k_mxfp4_skinny, tw, ta, p), "gemm_mxfp4 launch");
-    return st != DW_OK ? st : dw_after_launch(be, "gemm_mxfp4");
+    return launch_dependent(be, "gemm_mxfp4", k_mxfp4_skinny, dim3(S, (unsigned)tn, (unsigned)tm), kSkinnyThreads, smem, S, tw, ta, p);
 }
 
 }  // namespace

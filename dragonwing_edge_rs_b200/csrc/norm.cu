@@ -13,6 +13,7 @@
 #include <algorithm>
 
 #include "dw_device.cuh"
+#include "dw_launch.h"
 #include "dw_mxfp4.cuh"
 #include "dw_ptx.cuh"
 
@@ -161,6 +162,8 @@ __global__ void __launch_bounds__(kMaxT, V * N <= 8 ? 2 : 1) k_norm(const __grid
             return w != nullptr;
         };
     };
+    pdl_wait();
+    pdl_trigger();
     for (size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y; row < p.rows; row += (size_t)gridDim.x * blockDim.y) {
         Raw<X, V> xr[N], gr[N];
         Raw<R, V> rr[N];
@@ -266,6 +269,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
         copy(dx, (const uint8_t *)p.x, p.x_pitch * sizeof(X), x_bytes);
         if (p.has_res) copy(dr, (const uint8_t *)p.res, p.res_pitch * sizeof(R), r_bytes);
     };
+    pdl_wait();
+    pdl_trigger();
     if (threadIdx.x == 0) {
         size_t step = blockIdx.x;
         for (int s = 0; s < stages && step < steps; s++, step += gridDim.x) fetch(step, s);
@@ -466,6 +471,8 @@ __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Par
     const R *res = (const R *)p.res + row * p.res_pitch;
     const X *gate = (const X *)p.gate + (p.gate_rows ? row / p.gate_rows : 0) * p.c;
     R *out = (R *)p.out + row * p.res_pitch;
+    pdl_wait();
+    pdl_trigger();
     auto stats = [&](auto at, int kind, float &mean, float &rstd) {
         mean = 0.0f, rstd = 1.0f;
         if (kind == DW_NORM_NONE) return;
@@ -538,8 +545,7 @@ dw_status stream_as(dw_backend *be, const Params &p, int T) {
     }
     const size_t steps = (p.rows + G - 1) / G;
     const unsigned grid = (unsigned)std::min<size_t>(steps, (size_t)be->sm_count * per_sm);
-    kernel<<<grid, kThreads, stages * stage, be->stream>>>(p, T, stages, be->wait_cap_ns, be->dev_err);
-    return dw_after_launch(be, "norm");
+    return launch_dependent(be, "norm", kernel, grid, kThreads, stages * stage, 0, p, T, stages, be->wait_cap_ns, be->dev_err);
 }
 
 template <typename X, typename R>
@@ -569,8 +575,7 @@ dw_status run(dw_backend *be, const Params &p) {
     };
     if (p.rows > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "norm: more than 2^31 - 1 rows");
     if (p.c > (size_t)kMaxT * kMaxE) {
-        k_norm_long<X, R><<<(unsigned)p.rows, kMaxT, 0, be->stream>>>(p);
-        return dw_after_launch(be, "norm (long rows)");
+        return launch_dependent(be, "norm (long rows)", k_norm_long<X, R>, (unsigned)p.rows, kMaxT, 0, 0, p);
     }
     if (fits(8) && p.c <= (size_t)kMaxT * kMaxE && p.rows >= (size_t)be->sm_count * 2) return stream<X, R>(be, p);
     // E: elements of a thread; T: threads of a row (a power of two from 32 to 512)
@@ -581,8 +586,7 @@ dw_status run(dw_backend *be, const Params &p) {
     const size_t blocks = (p.rows + rows_blk - 1) / rows_blk;
     const dim3 block(T, rows_blk);
     auto go = [&](auto kernel) {
-        kernel<<<(unsigned)blocks, block, 0, be->stream>>>(p);
-        return dw_after_launch(be, "norm");
+        return launch_dependent(be, "norm", kernel, (unsigned)blocks, block, 0, 0, p);
     };
     if (fits(8)) {
         if (E == 8) return go(k_norm<X, R, 8, 1>);
