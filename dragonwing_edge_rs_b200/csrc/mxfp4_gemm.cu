@@ -20,6 +20,7 @@
 // and exits.
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "dw_device.cuh"
 #include "dw_launch.h"
@@ -39,7 +40,7 @@ struct GemmParams {
     void *y;
     uint8_t *y_s;
     size_t m, n;
-    size_t tiles_k;   // scale tiles (128 codes) along K
+    int tiles_k;      // scale tiles (128 codes) along K
     size_t out_nb, out_tiles;  // MXFP4 result: blocks and scale tiles along n
     int k_blocks;     // 512-wide K blocks
     int tiles_m, tiles;
@@ -71,6 +72,15 @@ __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, uint64
     }
 }
 
+// The same for a whole warp, with one answer.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, uint64_t cap_ns, int32_t *err, volatile int *abort_flag,
+                                          int site) {
+#pragma unroll 1
+    for (int i = 0; i < 1024; i++)
+        if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, wait_phase<8>(bar, parity, cap_ns, err, abort_flag, site));
+}
+
 // Waits for a phase that the CTA's own work in flight completes, whatever happened before.
 __device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, uint64_t cap_ns) {
     const uint64_t t0 = globaltimer_ns();
@@ -79,20 +89,48 @@ __device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, uint6
         if (globaltimer_ns() - t0 > cap_ns) return;
 }
 
-// 512 bytes (32 rows of 16) -> 4 columns of all four lane quarters of tensor memory.
-__device__ __forceinline__ void tc_cp_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+// The warps that feed the tensor core run their loops with all lanes, on warp-uniform
+// values, and predicate each issue on one elected lane: operands then come from
+// uniform registers.  (A loop inside `if (lane == 0)` issues an MMA only every ~110
+// cycles and a scale copy every ~80.)
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
 }
 
-// One 128 x N x 64 product with block scales (two 32-wide blocks per row).
-__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                            uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
+// 512 bytes (32 rows of 16) -> 4 columns of all four lane quarters of tensor memory
+// (of both CTAs of a pair).
+template <int kCtas>
+__device__ __forceinline__ void tc_cp_scales(uint32_t elected, uint32_t taddr, uint64_t desc) {
+    if constexpr (kCtas == 1)
+        asm volatile(
+            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr),
+            "l"(desc), "r"(elected)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr),
+            "l"(desc), "r"(elected)
+            : "memory");
+}
+
+// One product of 128 (256 by a pair) x N x 64 with block scales (two 32-wide blocks a row).
+template <int kCtas>
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                            uint32_t sfb, uint32_t accumulate) {
+    if constexpr (kCtas == 1)
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(elected)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(elected)
+            : "memory");
 }
 
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -199,6 +237,20 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The scale bytes of kN (1 or 2) blocks of a row, the last of a row with the zeros of
+// the tile's places past it.
+template <int kN>
+__device__ __forceinline__ void put_scales(uint32_t scales, size_t row, size_t block, const GemmParams &p) {
+    if (row >= p.m) return;
+    uint8_t *s = p.y_s + mx_scale_at(row, block, p.out_tiles);
+    if constexpr (kN == 2)
+        *reinterpret_cast<uint16_t *>(s) = (uint16_t)scales;
+    else
+        *s = (uint8_t)scales;
+    if (block + kN >= p.out_nb)
+        for (size_t b = block + kN; b < p.out_tiles * 4; b++) p.y_s[mx_scale_at(row, b, p.out_tiles)] = 0;
+}
+
 // ---- many rows -----------------------------------------------------------------
 // A pair of CTAs (cta_group::2) computes a 256 x BN tile: each holds 128 rows of A,
 // half of B's rows, the scales of its rows of A and those of all BN rows of B, so a
@@ -234,29 +286,23 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
         : "memory");
 }
 // Commits of the pair: to the leader's barrier, or to the same barrier of both CTAs.
-__device__ __forceinline__ void tc_commit2(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_commit2_both(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-                 "h"((uint16_t)3)
-                 : "memory");
-}
-__device__ __forceinline__ void tc_cp_scales2(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-__device__ __forceinline__ void tc_mma_mxf4_2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                              uint32_t accumulate) {
+__device__ __forceinline__ void tc_commit2(uint32_t elected, uint32_t bar) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(elected)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit2_both(uint32_t elected, uint32_t bar, uint16_t ctas) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+        "h"(ctas), "r"(elected)
         : "memory");
 }
 
 template <int BN, int kOut>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(kGemmThreads, 1)
     k_mxfp4_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                  const __grid_constant__ CUtensorMap tmap_sa, const __grid_constant__ CUtensorMap tmap_sb,
                  const __grid_constant__ GemmParams p) {
@@ -273,9 +319,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_rank();
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    // CTAs of the cluster: pairs that share a tile's K (one pair: all of it, and the
+    // pairs of the grid loop over the tiles)
+    const uint32_t cta = cluster_rank(), rank = cta & 1, lead = cta & ~1u, S = cluster_size() >> 1, part_k = cta >> 1;
+    const int pair = (int)(blockIdx.x / (2 * S)), pairs = (int)(gridDim.x / (2 * S));
+    const int kb0 = (int)((long long)p.k_blocks * part_k / S), kb1 = (int)((long long)p.k_blocks * (part_k + 1) / S);
+    const uint16_t both = (uint16_t)(3u << lead);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; s++) {
@@ -303,8 +353,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
     tc_fence_after();
     pdl_trigger();
     pdl_wait();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const uint32_t sf_cols = tmem + 256;  // scales after the accumulators
+    float *partial = reinterpret_cast<float *>(smem_raw + (smem - smem_u32(smem_raw)));  // [BN][128]
 
     if (warp == 0) {
         if (lane == 0) {
@@ -313,13 +364,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
             bool ok = true;
             for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
                 const int tm = (tile % p.tiles_m) * 2 + (int)rank, tn = tile / p.tiles_m;  // 128-row tile of A, BN-row tile of B
-                for (int kb = 0; kb < p.k_blocks; kb++) {
+                for (int kb = kb0; kb < kb1; kb++) {
                     if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 21)) {
                         ok = false;
                         break;
                     }
                     // both CTAs' copies complete on the leader's barrier
-                    const uint32_t bar = peer_addr(smem_u32(&full_bar[s]), 0), base = smem + s * kStage;
+                    const uint32_t bar = peer_addr(smem_u32(&full_bar[s]), lead), base = smem + s * kStage;
                     const uint32_t sf = base + 2 * (kA + kB);
                     if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[s]), 2 * kStage);
                     const int b_row = tn * BN + (int)rank * (BN / 2);
@@ -339,73 +390,76 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
             }
         }
-    } else if (warp == 2) {
+    } else if (warp == 2 && rank == 0) {
         // each stage's scales into both CTAs' tensor memory, ahead of the products (a
         // thread of its own: copies that the issuing thread puts between its products
         // hold these up, 0.58 instead of 0.40 us per 256 x 256 x 256)
-        if (lane == 0 && rank == 0) {
-            int s = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
-                for (int kb = 0; kb < p.k_blocks; kb++) {
-                    if (!wait_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 22)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t sf = smem + s * kStage + 2 * (kA + kB);
-                    const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 16;
-                    const int chunks = (int)min((size_t)4, p.tiles_k - 4 * (size_t)kb);
-                    for (int c = 0; c < chunks; c++) {
-                        tc_cp_scales2(sfa + c * 4, smem_desc_noswz(sf + c * 512, 16, 128));
-#pragma unroll
-                        for (int j = 0; j < BN / 128; j++)
-                            tc_cp_scales2(sfb + c * (BN / 32) + j * 4, smem_desc_noswz(sf + kSA + j * 2048 + c * 512, 16, 128));
-                    }
-                    tc_commit2(smem_u32(&sf_bar[s]));
-                    if (++s == p.stages) s = 0, ph ^= 1;
+        const uint32_t elected = elect_one();
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!wait_warp(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 22)) {
+                    ok = false;
+                    break;
                 }
+                const uint32_t sf = smem + s * kStage + 2 * (kA + kB);
+                const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 16;
+                const int chunks = min(4, p.tiles_k - 4 * kb);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (c >= chunks) break;
+                    tc_cp_scales<2>(elected, sfa + c * 4, smem_desc_noswz(sf + c * 512, 16, 128));
+#pragma unroll
+                    for (int j = 0; j < BN / 128; j++)
+                        tc_cp_scales<2>(elected, sfb + c * (BN / 32) + j * 4, smem_desc_noswz(sf + kSA + j * 2048 + c * 512, 16, 128));
+                }
+                tc_commit2(elected, smem_u32(&sf_bar[s]));
+                if (++s == p.stages) s = 0, ph ^= 1;
             }
-            tc_commit2(smem_u32(&drain_bar[1]));
-            drain_phase(smem_u32(&drain_bar[1]), 0, p.wait_cap_ns);
         }
-    } else if (warp == 1) {
+        tc_commit2(elected, smem_u32(&drain_bar[1]));
+        drain_phase(smem_u32(&drain_bar[1]), 0, p.wait_cap_ns);
+    } else if (warp == 1 && rank == 0) {
         // a commit costs the tensor pipe about 0.1 us, so a stage is 512 wide: eight products
-        if (lane == 0 && rank == 0) {
-            const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
-            int s = 0, acc = 0;
-            uint32_t ph = 0, aph = 0;
-            bool ok = true;
-            for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
-                if (!wait_phase(smem_u32(&tempty_bar[acc]), aph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 23)) break;
-                const uint32_t d = tmem + acc * BN;
-                for (int kb = 0; kb < p.k_blocks; kb++) {
-                    if (!wait_phase(smem_u32(&sf_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 24)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t base = smem + s * kStage;
-                    const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 16;
-                    const int chunks = (int)min((size_t)4, p.tiles_k - 4 * (size_t)kb);
-                    for (int c = 0; c < chunks; c++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const uint32_t off = (uint32_t)((c & 1) * 2 + h) * 32;
-                            tc_mma_mxf4_2(d, smem_desc(base + (c >> 1) * kA + off, hi),
-                                          smem_desc(base + 2 * kA + (c >> 1) * kB + off, hi), mx_idesc(2 * kBM, BN, h),
-                                          sfa + c * 4, sfb + c * (BN / 32), (kb | c | h) ? 1u : 0u);
-                        }
-                    tc_commit2_both(smem_u32(&empty_bar[s]));
-                    if (++s == p.stages) s = 0, ph ^= 1;
+        const uint32_t elected = elect_one();
+        const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
+        int s = 0, acc = 0;
+        uint32_t ph = 0, aph = 0;
+        bool ok = true;
+        for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
+            if (!wait_warp(smem_u32(&tempty_bar[acc]), aph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 23)) break;
+            const uint32_t d = tmem + acc * BN;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!wait_warp(smem_u32(&sf_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 24)) {
+                    ok = false;
+                    break;
                 }
-                if (!ok) break;
-                tc_commit2_both(smem_u32(&tfull_bar[acc]));
-                if (++acc == kAcc) acc = 0, aph ^= 1;
+                tc_fence_after();
+                const uint32_t base = smem + s * kStage;
+                const uint32_t sfa = sf_cols + s * kScaleCols, sfb = sfa + 16;
+                const int chunks = min(4, p.tiles_k - 4 * kb);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (c >= chunks) break;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t off = (uint32_t)((c & 1) * 2 + h) * 32;
+                        tc_mma_mxf4<2>(elected, d, smem_desc(base + (c >> 1) * kA + off, hi),
+                                       smem_desc(base + 2 * kA + (c >> 1) * kB + off, hi), mx_idesc(2 * kBM, BN, h), sfa + c * 4,
+                                       sfb + c * (BN / 32), (kb > kb0 || c || h) ? 1u : 0u);
+                    }
+                }
+                tc_commit2_both(elected, smem_u32(&empty_bar[s]), both);
+                if (++s == p.stages) s = 0, ph ^= 1;
             }
-            tc_commit2(smem_u32(&drain_bar[0]));
-            drain_phase(smem_u32(&drain_bar[0]), 0, p.wait_cap_ns);
+            if (!ok) break;
+            tc_commit2_both(elected, smem_u32(&tfull_bar[acc]), both);
+            if (++acc == kAcc) acc = 0, aph ^= 1;
         }
+        tc_commit2(elected, smem_u32(&drain_bar[0]));
+        drain_phase(smem_u32(&drain_bar[0]), 0, p.wait_cap_ns);
     } else if (warp >= 4) {
         const int quarter = warp & 3;  // tensor-memory lanes this warp may read
         const int part = (warp - 4) >> 2;
@@ -422,9 +476,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
             for (int g = 0; g < kCols / 32; g++) tc_ld32(base + g * 32, r[g]);
             tc_wait_ld();
+            if (S > 1) {  // the cluster's only tile: the partial sums, over the ring (all of it has been read)
+#pragma unroll
+                for (int g = 0; g < kCols / 32; g++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) partial[(part * kCols + g * 32 + i) * 128 + quarter * 32 + lane] = __uint_as_float(r[g][i]);
+                break;
+            }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(peer_addr(smem_u32(&tempty_bar[acc]), 0));
+            if (lane == 0) mbar_arrive_cluster(peer_addr(smem_u32(&tempty_bar[acc]), lead));
             if (++acc == kAcc) acc = 0, aph ^= 1;
             if (col0 >= p.n) continue;
             uint32_t scales = 0;
@@ -440,23 +501,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 scales |= sb << (8 * g);
             }
             if constexpr (kOut == 3) {
-                // kCols / 32 blocks' scales: two bytes (BN = 256) or one of a tile's four
-                const size_t block = col0 / 32;
-                if (row < p.m) {
-                    uint8_t *s = p.y_s + mx_scale_at(row, block, p.out_tiles);
-                    if constexpr (kCols == 64)
-                        *reinterpret_cast<uint16_t *>(s) = (uint16_t)scales;
-                    else
-                        *s = (uint8_t)scales;
-                    if (block + kCols / 32 >= p.out_nb)  // the places of the tile past the last block
-                        for (size_t b = block + kCols / 32; b < p.out_tiles * 4; b++) p.y_s[mx_scale_at(row, b, p.out_tiles)] = 0;
-                }
+                put_scales<kCols / 32>(scales, row, col0 / 32, p);
             }
         }
     }
     __syncwarp();
     tc_fence_before();
-    cluster_sync();  // all products and copies of the pair are done
+    cluster_sync();  // all products and copies are done, the partial sums lie ready
+    if (S > 1) {
+        // each pair adds up BN / S columns of the partial tiles, in the order of the pairs
+        const int w = warp - 4, quarter = w & 3, group = w >> 2;
+        if (w >= 0 && group < (int)(BN / 32 / S) && *abort_flag == 0) {
+            const int tm = pair % p.tiles_m, tn = pair / p.tiles_m;
+            const int c0 = (int)(part_k * (BN / S)) + group * 32;
+            const size_t row = ((size_t)tm * 2 + rank) * kBM + quarter * 32 + lane, col = (size_t)tn * BN + c0;
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; i++) v[i] = 0.0f;
+            for (uint32_t q = 0; q < S; q++) {
+                const uint32_t from = peer_addr(smem_u32(partial + c0 * 128 + quarter * 32 + lane), 2 * q + rank);
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    float u;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u) : "r"(from + i * 512) : "memory");
+                    v[i] += u;
+                }
+            }
+            if (col < p.n) {
+                finish32(v, col, p);
+                uint32_t sb = 0;
+                put32<kOut>(v, row, col, p, sb);
+                if constexpr (kOut == 3) put_scales<1>(sb, row, col / 32, p);
+            }
+        }
+        cluster_sync();  // no CTA leaves while its partial sums may be read
+    }
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
@@ -566,8 +645,8 @@ __global__ void __launch_bounds__(kSkinnyThreads)
             const uint32_t base = smem + s * p.stage_bytes + w_bytes;
             const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
             for (int c = 0; c < chunks; c++) {
-                tc_cp_scales(sf_cols + s * 16 + c * 4, smem_desc_noswz(base + c * 512, 16, 128));
-                tc_cp_scales(sf_cols + s * 16 + 8 + c * 4, smem_desc_noswz(base + 1024 + a_bytes + c * 512, 16, 128));
+                tc_cp_scales<1>(1u, sf_cols + s * 16 + c * 4, smem_desc_noswz(base + c * 512, 16, 128));
+                tc_cp_scales<1>(1u, sf_cols + s * 16 + 8 + c * 4, smem_desc_noswz(base + 1024 + a_bytes + c * 512, 16, 128));
             }
             tc_commit(smem_u32(&sf_bar[s]));
             if (++s == p.stages) s = 0, ph ^= 1;
@@ -590,7 +669,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const uint32_t off = (uint32_t)(c * 2 + h) * 32;
-                    tc_mma_mxf4(tmem, smem_desc(base + off, hi), smem_desc(base + w_bytes + 1024 + off, hi), p.idesc[h],
+                    tc_mma_mxf4<1>(1u, tmem, smem_desc(base + off, hi), smem_desc(base + w_bytes + 1024 + off, hi), p.idesc[h],
                                 sf_cols + s * 16 + c * 4, sf_cols + s * 16 + 8 + c * 4, (kb > kb0 || c || h) ? 1u : 0u);
                 }
             tc_commit(smem_u32(&empty_bar[s]));
@@ -695,12 +774,12 @@ bool scale_map(dw_backend *be, CUtensorMap *map, const uint8_t *s, size_t rows, 
 }
 
 template <int BN, int kOut>
-dw_status launch(dw_backend *be, const MxGemmArgs &a) {
+dw_status launch(dw_backend *be, const MxGemmArgs &a, int S) {
     constexpr size_t kStage = 2 * (kBM + BN / 2) * kBKBytes + 2048 + (BN / 128) * 2048;
     GemmParams p{};
     p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
     p.m = a.m, p.n = a.n;
-    p.tiles_k = mx_tiles(a.k);
+    p.tiles_k = (int)mx_tiles(a.k);
     p.out_nb = mx_blocks(a.n), p.out_tiles = mx_tiles(a.n);
     p.k_blocks = (int)((a.k + 511) / 512);
     const size_t tm = (a.m + 2 * kBM - 1) / (2 * kBM), tn = (a.n + BN - 1) / BN;
@@ -713,7 +792,8 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a) {
     p.wait_cap_ns = be->wait_cap_ns, p.err = be->dev_err;
     p.stages = (int)std::min<size_t>(kMaxStages, (kSmemLimit - 4096) / kStage);
     // at least 116 KiB: one CTA per SM owns the tensor memory
-    const size_t smem = std::max<size_t>(1024 + p.stages * kStage, 116 * 1024);
+    // and the partial tile of a split K lies over the ring
+    const size_t smem = std::max<size_t>(1024 + std::max<size_t>(p.stages * kStage, BN * 512), 116 * 1024);
     CUtensorMap ta, tb, tsa, tsb;
     if (!be->encode_tiled || !code_map(be, &ta, a.a_q, a.m, a.k, kBM) || !code_map(be, &tb, a.b_q, a.n, a.k, BN / 2) ||
         !scale_map(be, &tsa, a.a_s, a.m, a.k, 1) || !scale_map(be, &tsb, a.b_s, a.n, a.k, BN / 128))
@@ -727,8 +807,8 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a) {
         if (st != DW_OK) return st;
         attr_set[be->device] = true;
     }
-    return launch_dependent(be, "gemm_mxfp4", kernel, 2 * std::min(p.tiles, be->sm_count / 2), kGemmThreads, smem, 0, ta, tb, tsa,
-                            tsb, p);
+    return launch_dependent(be, "gemm_mxfp4", kernel, 2 * S * (S > 1 ? p.tiles : std::min(p.tiles, be->sm_count / 2)), kGemmThreads,
+                            smem, 2 * S, ta, tb, tsa, tsb, p);
 }
 
 // CTAs of a cluster that share a tile's K: as many as fill the GPU once, each with
@@ -773,21 +853,26 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
 }  // namespace
 
 dw_status launch_gemm_mxfp4(dw_backend *be, const MxGemmArgs &a) {
-    if (a.m <= 256) return launch_skinny(be, a);
+    const int skm = getenv("DW_MXSK") ? atoi(getenv("DW_MXSK")) : 64;
+    if (a.m <= skm) return launch_skinny(be, a);
     const int out = a.y_s ? 3 : a.y_dtype;
-    static const int bn = getenv("DW_MXBN") ? atoi(getenv("DW_MXBN")) : 256;
-    if (bn == 128) switch (out) {
-        case DW_F32: return launch<128, 0>(be, a);
-        case DW_F16: return launch<128, 1>(be, a);
-        case DW_BF16: return launch<128, 2>(be, a);
-        default: return launch<128, 3>(be, a);
+    int bn = getenv("DW_MXBN") ? atoi(getenv("DW_MXBN")) : 0, S = getenv("DW_MXS") ? atoi(getenv("DW_MXS")) : 0;
+    if (!bn || !S) {
+        double best = 1e30;
+        const long kb = (long)((a.k + 511) / 512);
+        for (int b : {256, 128})
+            for (int q : {1, 2, 4}) {
+                if (q > kb) continue;
+                const long tiles = (long)((a.m + 255) / 256) * (long)((a.n + b - 1) / b);
+                const long slots = q == 1 ? be->sm_count / 2 : q == 2 ? be->sm_count / 4 - 1 : be->sm_count / 8 - 2;
+                const double t = (double)((tiles + slots - 1) / slots) * ((kb + q - 1) / q * (b == 256 ? 0.72 : 0.64) + 1.5 + (q > 1 ? 2.0 : 0.0));
+                if (t < best) best = t, bn = b, S = q;
+            }
     }
-    switch (out) {
-        case DW_F32: return launch<256, 0>(be, a);
-        case DW_F16: return launch<256, 1>(be, a);
-        case DW_BF16: return launch<256, 2>(be, a);
-        default: return launch<256, 3>(be, a);
-    }
+    while (S > (int)((a.k + 511) / 512)) S /= 2;
+    auto go = [&](auto k0, auto k1, auto k2, auto k3) { return (out == 0 ? k0 : out == 1 ? k1 : out == 2 ? k2 : k3)(be, a, S); };
+    if (bn == 128) return go(launch<128, 0>, launch<128, 1>, launch<128, 2>, launch<128, 3>);
+    return go(launch<256, 0>, launch<256, 1>, launch<256, 2>, launch<256, 3>);
 }
 
 }  // namespace dw
