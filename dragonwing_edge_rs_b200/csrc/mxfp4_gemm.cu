@@ -285,6 +285,13 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
         "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
+__device__ __forceinline__ void tc_commit1(uint32_t elected, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(elected)
+        : "memory");
+}
 // Commits of the pair: to the leader's barrier, or to the same barrier of both CTAs.
 __device__ __forceinline__ void tc_commit2(uint32_t elected, uint32_t bar) {
     asm volatile(
@@ -549,14 +556,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 // shared memory, and each of them adds up every S-th row of A in the order of the
 // ranks: no workspace, no atomics, the same bits each time.
 struct SkinnyParams {
-    const uint8_t *w_s, *a_s;
     const float *bias;
     void *y;
     uint8_t *y_s;
     size_t m, n;
-    size_t tiles_k;
     size_t out_nb, out_tiles;
-    int k_blocks, bn, stages, act, out;  // out: DW_F32 .. DW_BF16, 3: MXFP4
+    int tiles_k, k_blocks, bn, stages, act, out;  // out: DW_F32 .. DW_BF16, 3: MXFP4
     uint32_t stage_bytes, idesc[2], tmem_cols;
     uint64_t wait_cap_ns;
     int32_t *err;
@@ -575,6 +580,7 @@ __device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
 
 __global__ void __launch_bounds__(kSkinnyThreads)
     k_mxfp4_skinny(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
+                   const __grid_constant__ CUtensorMap tmap_sw, const __grid_constant__ CUtensorMap tmap_sa,
                    const __grid_constant__ SkinnyParams p) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
@@ -583,7 +589,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), S = cluster_size();
     const size_t n0 = (size_t)blockIdx.y * 128, m0 = (size_t)blockIdx.z * p.bn;
     const int kb0 = (int)((long long)p.k_blocks * rank / S), kb1 = (int)((long long)p.k_blocks * (rank + 1) / S);
@@ -612,70 +618,77 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     tc_fence_after();
     pdl_trigger();
     pdl_wait();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const uint32_t sf_cols = tmem + (uint32_t)p.bn;  // 16 columns a stage after the accumulators
     const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
 
-    if (warp == 0 && lane == 0) {
-        int s = 0, issued = 0;
-        uint32_t ph = 0;
-        for (int kb = kb0; kb < kb1; kb++) {
-            if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 31)) break;
-            const uint32_t bar = smem_u32(&full_bar[s]), base = smem + s * p.stage_bytes;
-            const uint32_t sbytes = (uint32_t)min((size_t)2, p.tiles_k - 2 * (size_t)kb) * 512;
-            mbar_expect_tx(bar, w_bytes + a_bytes + 2 * sbytes);
-            tma_load_2d(base, &tmap_w, bar, kb * kBKBytes, (int)n0);
-            bulk_load(base + w_bytes, p.w_s + ((size_t)blockIdx.y * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
-            tma_load_2d(base + w_bytes + 1024, &tmap_a, bar, kb * kBKBytes, (int)m0);
-            bulk_load(base + w_bytes + 1024 + a_bytes, p.a_s + ((m0 >> 7) * p.tiles_k + 2 * (size_t)kb) * 512, sbytes, bar);
-            issued++;
-            if (++s == p.stages) s = 0, ph ^= 1;
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 31)) break;
+                const uint32_t bar = smem_u32(&full_bar[s]), base = smem + s * p.stage_bytes;
+                mbar_expect_tx(bar, p.stage_bytes);
+                tma_load_2d(base, &tmap_w, bar, kb * kBKBytes, (int)n0);
+                tma_load_3d(base + w_bytes, &tmap_sw, bar, 0, 2 * kb, (int)blockIdx.y);
+                tma_load_2d(base + w_bytes + 1024, &tmap_a, bar, kb * kBKBytes, (int)m0);
+                tma_load_3d(base + w_bytes + 1024 + a_bytes, &tmap_sa, bar, 0, 2 * kb, (int)(m0 >> 7));
+                issued++;
+                if (++s == p.stages) s = 0, ph ^= 1;
+            }
+            for (int i = 0; i < min(issued, p.stages); i++) {
+                if (--s < 0) s = p.stages - 1, ph ^= 1;
+                drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
+            }
         }
-        for (int i = 0; i < min(issued, p.stages); i++) {
-            if (--s < 0) s = p.stages - 1, ph ^= 1;
-            drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
-        }
-    } else if (warp == 2 && lane == 0) {
+    } else if (warp == 2) {
         // scales of each stage into tensor memory, ahead of the products
+        const uint32_t elected = elect_one();
         int s = 0;
         uint32_t ph = 0;
         for (int kb = kb0; kb < kb1; kb++) {
-            if (!wait_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 32)) break;
-            tc_fence_after();
+            if (!wait_warp(smem_u32(&full_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 32)) break;
             const uint32_t base = smem + s * p.stage_bytes + w_bytes;
-            const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
-            for (int c = 0; c < chunks; c++) {
-                tc_cp_scales<1>(1u, sf_cols + s * 16 + c * 4, smem_desc_noswz(base + c * 512, 16, 128));
-                tc_cp_scales<1>(1u, sf_cols + s * 16 + 8 + c * 4, smem_desc_noswz(base + 1024 + a_bytes + c * 512, 16, 128));
+            const int chunks = min(2, p.tiles_k - 2 * kb);
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                if (c >= chunks) break;
+                tc_cp_scales<1>(elected, sf_cols + s * 16 + c * 4, smem_desc_noswz(base + c * 512, 16, 128));
+                tc_cp_scales<1>(elected, sf_cols + s * 16 + 8 + c * 4, smem_desc_noswz(base + 1024 + a_bytes + c * 512, 16, 128));
             }
-            tc_commit(smem_u32(&sf_bar[s]));
+            tc_commit1(elected, smem_u32(&sf_bar[s]));
             if (++s == p.stages) s = 0, ph ^= 1;
         }
-        tc_commit(smem_u32(&drain_bar));
+        tc_commit1(elected, smem_u32(&drain_bar));
         drain_phase(smem_u32(&drain_bar), 0, p.wait_cap_ns);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
+        const uint32_t elected = elect_one();
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
         for (int kb = kb0; kb < kb1; kb++) {
-            if (!wait_phase(smem_u32(&sf_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 33)) {
+            if (!wait_warp(smem_u32(&sf_bar[s]), ph, p.wait_cap_ns, p.err, abort_flag, 33)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
             const uint32_t base = smem + s * p.stage_bytes;
-            const int chunks = (int)min((size_t)2, p.tiles_k - 2 * (size_t)kb);
-            for (int c = 0; c < chunks; c++)
+            const int chunks = min(2, p.tiles_k - 2 * kb);
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                if (c >= chunks) break;
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const uint32_t off = (uint32_t)(c * 2 + h) * 32;
-                    tc_mma_mxf4<1>(1u, tmem, smem_desc(base + off, hi), smem_desc(base + w_bytes + 1024 + off, hi), p.idesc[h],
-                                sf_cols + s * 16 + c * 4, sf_cols + s * 16 + 8 + c * 4, (kb > kb0 || c || h) ? 1u : 0u);
+                    tc_mma_mxf4<1>(elected, tmem, smem_desc(base + off, hi), smem_desc(base + w_bytes + 1024 + off, hi), p.idesc[h],
+                                   sf_cols + s * 16 + c * 4, sf_cols + s * 16 + 8 + c * 4, (kb > kb0 || c || h) ? 1u : 0u);
                 }
-            tc_commit(smem_u32(&empty_bar[s]));
+            }
+            tc_commit1(elected, smem_u32(&empty_bar[s]));
             if (++s == p.stages) s = 0, ph ^= 1;
         }
-        tc_commit(smem_u32(&done_bar));
+        tc_commit1(elected, smem_u32(&done_bar));
         if (!ok) drain_phase(smem_u32(&done_bar), 0, p.wait_cap_ns);
     }
     __syncwarp();
@@ -761,12 +774,12 @@ bool code_map(dw_backend *be, CUtensorMap *map, const uint8_t *q, size_t rows, s
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Scales as a 3-D tensor [row tiles][tiles along K][512 bytes]; a box is four tiles
-// along K of `row_tiles` row tiles.
-bool scale_map(dw_backend *be, CUtensorMap *map, const uint8_t *s, size_t rows, size_t k, int row_tiles) {
+// Scales as a 3-D tensor [row tiles][tiles along K][512 bytes]; a box is
+// `k_tiles` tiles along K of `row_tiles` row tiles.
+bool scale_map(dw_backend *be, CUtensorMap *map, const uint8_t *s, size_t rows, size_t k, int k_tiles, int row_tiles) {
     cuuint64_t dims[3] = {128, (cuuint64_t)mx_tiles(k), (cuuint64_t)((rows + 127) / 128)};
     cuuint64_t strides[2] = {512, (cuuint64_t)mx_tiles(k) * 512};
-    cuuint32_t box[3] = {128, 4, (cuuint32_t)row_tiles};
+    cuuint32_t box[3] = {128, (cuuint32_t)k_tiles, (cuuint32_t)row_tiles};
     cuuint32_t estr[3] = {1, 1, 1};
     return be->encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t *>(s), dims, strides, box, estr,
                             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -796,7 +809,7 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a, int S) {
     const size_t smem = std::max<size_t>(1024 + std::max<size_t>(p.stages * kStage, BN * 512), 116 * 1024);
     CUtensorMap ta, tb, tsa, tsb;
     if (!be->encode_tiled || !code_map(be, &ta, a.a_q, a.m, a.k, kBM) || !code_map(be, &tb, a.b_q, a.n, a.k, BN / 2) ||
-        !scale_map(be, &tsa, a.a_s, a.m, a.k, 1) || !scale_map(be, &tsb, a.b_s, a.n, a.k, BN / 128))
+        !scale_map(be, &tsa, a.a_s, a.m, a.k, 4, 1) || !scale_map(be, &tsb, a.b_s, a.n, a.k, 4, BN / 128))
         return dw_fail(be, DW_ERR_DEVICE, "gemm_mxfp4: tensor map rejected");
     auto kernel = k_mxfp4_gemm<BN, kOut>;
     static bool attr_set[16] = {};
@@ -815,9 +828,9 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a, int S) {
 // at least one K block.
 dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
     SkinnyParams p{};
-    p.w_s = a.b_s, p.a_s = a.a_s, p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
+    p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
     p.m = a.m, p.n = a.n;
-    p.tiles_k = mx_tiles(a.k);
+    p.tiles_k = (int)mx_tiles(a.k);
     p.out_nb = mx_blocks(a.n), p.out_tiles = mx_tiles(a.n);
     p.k_blocks = (int)((a.k + 255) / 256);
     p.bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
@@ -835,8 +848,9 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
     unsigned S = 1;
     while (S < 8 && 2 * S * tn * tm <= (size_t)be->sm_count * per_sm && 2 * (int)S <= p.k_blocks) S *= 2;
     const size_t smem = 1024 + std::max<size_t>(p.stages * p.stage_bytes, (size_t)p.bn * 512);
-    CUtensorMap tw, ta;
-    if (!be->encode_tiled || !code_map(be, &tw, a.b_q, a.n, a.k, kBM) || !code_map(be, &ta, a.a_q, a.m, a.k, p.bn))
+    CUtensorMap tw, ta, tsw, tsa;
+    if (!be->encode_tiled || !code_map(be, &tw, a.b_q, a.n, a.k, kBM) || !code_map(be, &ta, a.a_q, a.m, a.k, p.bn) ||
+        !scale_map(be, &tsw, a.b_s, a.n, a.k, 2, 1) || !scale_map(be, &tsa, a.a_s, a.m, a.k, 2, 1))
         return dw_fail(be, DW_ERR_DEVICE, "gemm_mxfp4: tensor map rejected");
     static bool attr_set[16] = {};
     if (be->device < 16 && !attr_set[be->device]) {
@@ -847,7 +861,8 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
         if (st != DW_OK) return st;
         attr_set[be->device] = true;
     }
-    return launch_dependent(be, "gemm_mxfp4", k_mxfp4_skinny, dim3(S, (unsigned)tn, (unsigned)tm), kSkinnyThreads, smem, S, tw, ta, p);
+    return launch_dependent(be, "gemm_mxfp4", k_mxfp4_skinny, dim3(S, (unsigned)tn, (unsigned)tm), kSkinnyThreads, smem, S, tw, ta,
+                            tsw, tsa, p);
 }
 
 }  // namespace
