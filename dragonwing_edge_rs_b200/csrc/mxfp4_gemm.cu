@@ -93,6 +93,9 @@ __device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, uint6
 // values, and predicate each issue on one elected lane: operands then come from
 // uniform registers.  (A loop inside `if (lane == 0)` issues an MMA only every ~110
 // cycles and a scale copy every ~80.)
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 __device__ __forceinline__ uint32_t elect_one() {
     uint32_t e;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
@@ -189,6 +192,34 @@ __device__ __forceinline__ void finish32(float (&v)[32], size_t col, const GemmP
     }
 }
 
+// 64 bytes of each of 32 consecutive rows (lane = row) -> y.  Four lanes exchange
+// 16-byte pieces first, so that a store covers 8 rows of 64 bytes instead of 32 of 16
+// (one line a row: the epilogue of a 256 x 256 tile took 4 us of stores).
+template <typename T>
+__device__ __forceinline__ void store64(uint32_t (&w)[16], size_t row, size_t col, const GemmParams &p) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int s = 1; s < 4; s <<= 1)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            if (c & s) continue;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t a = w[4 * c + i], b = w[4 * (c | s) + i];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, lane & s ? a : b, s);
+                if (lane & s)
+                    w[4 * c + i] = got;
+                else
+                    w[4 * (c | s) + i] = got;
+            }
+        }
+    const size_t row0 = row - (lane & 3);
+    T *dst = (T *)p.y + row0 * p.n + col + (lane & 3) * (16 / sizeof(T));
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (row0 + k < p.m) *reinterpret_cast<uint4 *>(dst + k * p.n) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+}
+
 // What the epilogue stores: 0 f32, 1 f16, 2 bf16, 3 MXFP4.
 template <int kOut>
 __device__ __forceinline__ void put32(float (&v)[32], size_t row, size_t col, const GemmParams &p, uint32_t &scale) {
@@ -203,19 +234,22 @@ __device__ __forceinline__ void put32(float (&v)[32], size_t row, size_t col, co
         if (row < p.m && col / 32 < p.out_nb) *reinterpret_cast<uint4 *>((uint8_t *)p.y + (row * p.out_nb + col / 32) * 16) = codes;
     } else {
         using T = std::conditional_t<kOut == 0, float, std::conditional_t<kOut == 1, __half, __nv_bfloat16>>;
-        if (row >= p.m) return;
-        T *dst = (T *)p.y + row * p.n + col;
         if (p.vec && col + 32 <= p.n) {
+            constexpr int kPer = 64 / sizeof(T);  // columns of 64 bytes
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                Raw<T, 8> r;
-                float t[8];
+            for (int h = 0; h < 32 / kPer; h++) {
+                uint32_t w[16];
+                if constexpr (kOut == 0) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) t[i] = v[8 * g + i];
-                r.set(t);
-                r.store(dst + 8 * g);
+                    for (int i = 0; i < 16; i++) w[i] = __float_as_uint(v[16 * h + i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+                }
+                store64<T>(w, row, col + h * kPer, p);
             }
-        } else {
+        } else if (row < p.m) {
+            T *dst = (T *)p.y + row * p.n + col;
 #pragma unroll
             for (int i = 0; i < 32; i++)
                 if (col + i < p.n) dst[i] = from_f32<T>(v[i]);
@@ -334,6 +368,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const int kb0 = (int)((long long)p.k_blocks * part_k / S), kb1 = (int)((long long)p.k_blocks * (part_k + 1) / S);
     const uint16_t both = (uint16_t)(3u << lead);
 
+    if (threadIdx.x == 32 * 3) {
+        prefetch_map(&tmap_a), prefetch_map(&tmap_b), prefetch_map(&tmap_sa), prefetch_map(&tmap_sb);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; s++) {
             mbar_init(smem_u32(&full_bar[s]), 1);
@@ -358,14 +395,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     tc_fence_before();
     cluster_sync();
     tc_fence_after();
-    pdl_trigger();
-    pdl_wait();
+    pdl_trigger();  // the warps that touch global memory wait below
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const uint32_t sf_cols = tmem + 256;  // scales after the accumulators
     float *partial = reinterpret_cast<float *>(smem_raw + (smem - smem_u32(smem_raw)));  // [BN][128]
 
     if (warp == 0) {
         if (lane == 0) {
+            pdl_wait();
             int s = 0, issued = 0;
             uint32_t ph = 0;
             bool ok = true;
@@ -468,6 +505,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         tc_commit2(elected, smem_u32(&drain_bar[0]));
         drain_phase(smem_u32(&drain_bar[0]), 0, p.wait_cap_ns);
     } else if (warp >= 4) {
+        pdl_wait();
         const int quarter = warp & 3;  // tensor-memory lanes this warp may read
         const int part = (warp - 4) >> 2;
         int acc = 0;
@@ -595,6 +633,9 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     const int kb0 = (int)((long long)p.k_blocks * rank / S), kb1 = (int)((long long)p.k_blocks * (rank + 1) / S);
     const uint32_t w_bytes = kBM * kBKBytes, a_bytes = (uint32_t)p.bn * kBKBytes;
 
+    if (threadIdx.x == 32 * 3) {
+        prefetch_map(&tmap_w), prefetch_map(&tmap_a), prefetch_map(&tmap_sw), prefetch_map(&tmap_sa);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; s++) {
             mbar_init(smem_u32(&full_bar[s]), 1);
@@ -616,14 +657,14 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    pdl_trigger();
-    pdl_wait();
+    pdl_trigger();  // the warps wait where they first touch global memory
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const uint32_t sf_cols = tmem + (uint32_t)p.bn;  // 16 columns a stage after the accumulators
     const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
 
     if (warp == 0) {
         if (lane == 0) {
+            pdl_wait();
             int s = 0, issued = 0;
             uint32_t ph = 0;
             for (int kb = kb0; kb < kb1; kb++) {
@@ -718,6 +759,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
     }
+    pdl_wait();
     if (*abort_flag == 0) {
         const int t = threadIdx.x & 127;  // output of the tile
         const size_t col = n0 + t;
