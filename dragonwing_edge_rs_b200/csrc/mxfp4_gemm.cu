@@ -267,6 +267,10 @@ __device__ __forceinline__ uint32_t cluster_size() {
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
 }
+// The same without ordering memory: nobody leaves (or reuses) before all are here.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -401,38 +405,39 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     float *partial = reinterpret_cast<float *>(smem_raw + (smem - smem_u32(smem_raw)));  // [BN][128]
 
     if (warp == 0) {
-        if (lane == 0) {
-            pdl_wait();
-            int s = 0, issued = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
-                const int tm = (tile % p.tiles_m) * 2 + (int)rank, tn = tile / p.tiles_m;  // 128-row tile of A, BN-row tile of B
-                for (int kb = kb0; kb < kb1; kb++) {
-                    if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 21)) {
-                        ok = false;
-                        break;
-                    }
-                    // both CTAs' copies complete on the leader's barrier
-                    const uint32_t bar = peer_addr(smem_u32(&full_bar[s]), lead), base = smem + s * kStage;
-                    const uint32_t sf = base + 2 * (kA + kB);
+        pdl_wait();
+        const uint32_t elected = elect_one();
+        int s = 0, issued = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int tile = pair; ok && tile < p.tiles; tile += pairs) {
+            const int tm = (tile % p.tiles_m) * 2 + (int)rank, tn = tile / p.tiles_m;  // 128-row tile of A, BN-row tile of B
+            const int a_row = tm * kBM, b_row = tn * BN + (int)rank * (BN / 2);
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (issued >= p.stages && !wait_warp(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 21)) {
+                    ok = false;
+                    break;
+                }
+                // both CTAs' copies complete on the leader's barrier
+                const uint32_t bar = peer_addr(smem_u32(&full_bar[s]), lead), base = smem + s * kStage;
+                const uint32_t sf = base + 2 * (kA + kB);
+                if (elected) {
                     if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[s]), 2 * kStage);
-                    const int b_row = tn * BN + (int)rank * (BN / 2);
-                    tma_load_2d_pair(base, &tmap_a, bar, 2 * kb * kBKBytes, tm * kBM);
+                    tma_load_2d_pair(base, &tmap_a, bar, 2 * kb * kBKBytes, a_row);
                     tma_load_2d_pair(base + 2 * kA, &tmap_b, bar, 2 * kb * kBKBytes, b_row);
                     tma_load_3d_pair(sf, &tmap_sa, bar, 0, 4 * kb, tm);
                     tma_load_3d_pair(sf + kSA, &tmap_sb, bar, 0, 4 * kb, tn * (BN / 128));
-                    tma_load_2d_pair(base + kA, &tmap_a, bar, (2 * kb + 1) * kBKBytes, tm * kBM);
+                    tma_load_2d_pair(base + kA, &tmap_a, bar, (2 * kb + 1) * kBKBytes, a_row);
                     tma_load_2d_pair(base + 2 * kA + kB, &tmap_b, bar, (2 * kb + 1) * kBKBytes, b_row);
-                    issued++;
-                    if (++s == p.stages) s = 0, ph ^= 1;
                 }
+                issued++;
+                if (++s == p.stages) s = 0, ph ^= 1;
             }
-            // the last copies into each stage have landed before the pair ends
-            for (int i = 0; rank == 0 && i < min(issued, p.stages); i++) {
-                if (--s < 0) s = p.stages - 1, ph ^= 1;
-                drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
-            }
+        }
+        // the last copies into each stage have landed before the pair ends
+        for (int i = 0; rank == 0 && i < min(issued, p.stages); i++) {
+            if (--s < 0) s = p.stages - 1, ph ^= 1;
+            drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
         }
     } else if (warp == 2 && rank == 0) {
         // each stage's scales into both CTAs' tensor memory, ahead of the products (a
@@ -536,24 +541,24 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             uint32_t scales = 0;
 #pragma unroll
             for (int g = 0; g < kCols / 32; g++) {
-                const size_t col = col0 + g * 32;
                 float v[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[g][i]);
+                const size_t col = col0 + g * 32;
                 finish32(v, col, p);
                 uint32_t sb = 0;
                 put32<kOut>(v, row, col, p, sb);
                 scales |= sb << (8 * g);
             }
-            if constexpr (kOut == 3) {
-                put_scales<kCols / 32>(scales, row, col0 / 32, p);
-            }
+            if constexpr (kOut == 3) put_scales<kCols / 32>(scales, row, col0 / 32, p);
         }
     }
     __syncwarp();
     tc_fence_before();
-    cluster_sync();  // all products and copies are done, the partial sums lie ready
-    if (S > 1) {
+    if (S == 1) {
+        cluster_sync_relaxed();  // all products and copies are done
+    } else {
+        cluster_sync();  // the same, and the partial sums lie ready
         // each pair adds up BN / S columns of the partial tiles, in the order of the pairs
         const int w = warp - 4, quarter = w & 3, group = w >> 2;
         if (w >= 0 && group < (int)(BN / 32 / S) && *abort_flag == 0) {
@@ -579,7 +584,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 if constexpr (kOut == 3) put_scales<1>(sb, row, col / 32, p);
             }
         }
-        cluster_sync();  // no CTA leaves while its partial sums may be read
+        cluster_sync_relaxed();  // no CTA leaves while its partial sums may be read
     }
     if (warp == 1) {
         tc_fence_after();
@@ -663,25 +668,26 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
 
     if (warp == 0) {
-        if (lane == 0) {
-            pdl_wait();
-            int s = 0, issued = 0;
-            uint32_t ph = 0;
-            for (int kb = kb0; kb < kb1; kb++) {
-                if (issued >= p.stages && !wait_phase(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 31)) break;
-                const uint32_t bar = smem_u32(&full_bar[s]), base = smem + s * p.stage_bytes;
+        pdl_wait();
+        const uint32_t elected = elect_one();
+        int s = 0, issued = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; kb++) {
+            if (issued >= p.stages && !wait_warp(smem_u32(&empty_bar[s]), ph ^ 1u, p.wait_cap_ns, p.err, abort_flag, 31)) break;
+            const uint32_t bar = smem_u32(&full_bar[s]), base = smem + s * p.stage_bytes;
+            if (elected) {
                 mbar_expect_tx(bar, p.stage_bytes);
                 tma_load_2d(base, &tmap_w, bar, kb * kBKBytes, (int)n0);
                 tma_load_3d(base + w_bytes, &tmap_sw, bar, 0, 2 * kb, (int)blockIdx.y);
                 tma_load_2d(base + w_bytes + 1024, &tmap_a, bar, kb * kBKBytes, (int)m0);
                 tma_load_3d(base + w_bytes + 1024 + a_bytes, &tmap_sa, bar, 0, 2 * kb, (int)(m0 >> 7));
-                issued++;
-                if (++s == p.stages) s = 0, ph ^= 1;
             }
-            for (int i = 0; i < min(issued, p.stages); i++) {
-                if (--s < 0) s = p.stages - 1, ph ^= 1;
-                drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
-            }
+            issued++;
+            if (++s == p.stages) s = 0, ph ^= 1;
+        }
+        for (int i = 0; i < min(issued, p.stages); i++) {
+            if (--s < 0) s = p.stages - 1, ph ^= 1;
+            drain_phase(smem_u32(&full_bar[s]), ph, p.wait_cap_ns);
         }
     } else if (warp == 2) {
         // scales of each stage into tensor memory, ahead of the products
@@ -802,7 +808,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
             }
         }
     }
-    if (S > 1) cluster_sync();  // no CTA leaves while its partials may be read
+    if (S > 1) cluster_sync_relaxed();  // no CTA leaves while its partials may be read
 }
 
 // Codes as a 2-D byte tensor [rows][bytes of a row]; a box is 128 bytes of `box_rows` rows.
