@@ -20,7 +20,6 @@
 // and exits.
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "dw_device.cuh"
 #include "dw_launch.h"
@@ -526,7 +525,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
             for (int g = 0; g < kCols / 32; g++) tc_ld32(base + g * 32, r[g]);
             tc_wait_ld();
-            if (S > 1) {  // the cluster's only tile: the partial sums, over the ring (all of it has been read)
+            if (BN == 128 && S > 1) {  // the cluster's only tile: the partial sums, over the ring (all of it has been read)
 #pragma unroll
                 for (int g = 0; g < kCols / 32; g++)
 #pragma unroll
@@ -555,7 +554,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
     __syncwarp();
     tc_fence_before();
-    if (S == 1) {
+    if (BN != 128 || S == 1) {
         cluster_sync_relaxed();  // all products and copies are done
     } else {
         cluster_sync();  // the same, and the partial sums lie ready
@@ -606,6 +605,7 @@ struct SkinnyParams {
     size_t out_nb, out_tiles;
     int tiles_k, k_blocks, bn, stages, act, out;  // out: DW_F32 .. DW_BF16, 3: MXFP4
     uint32_t stage_bytes, idesc[2], tmem_cols;
+    bool vec;  // y is aligned for stores of four outputs
     uint64_t wait_cap_ns;
     int32_t *err;
 };
@@ -613,11 +613,12 @@ struct SkinnyParams {
 constexpr int kSkinnyThreads = 256;
 constexpr int kSkinnyStages = 8;
 
-__device__ __forceinline__ float ld_peer(uint32_t addr, uint32_t rank) {
-    uint32_t a;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+__device__ __forceinline__ float4 ld_peer4(uint32_t addr, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(peer_addr(addr, rank))
+                 : "memory");
     return v;
 }
 
@@ -634,7 +635,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     volatile int *abort_flag = &abort_word;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), S = cluster_size();
-    const size_t n0 = (size_t)blockIdx.y * 128, m0 = (size_t)blockIdx.z * p.bn;
+    const size_t n0 = (size_t)blockIdx.y * 128;
     const int kb0 = (int)((long long)p.k_blocks * rank / S), kb1 = (int)((long long)p.k_blocks * (rank + 1) / S);
     const uint32_t w_bytes = kBM * kBKBytes, a_bytes = (uint32_t)p.bn * kBKBytes;
 
@@ -679,8 +680,8 @@ __global__ void __launch_bounds__(kSkinnyThreads)
                 mbar_expect_tx(bar, p.stage_bytes);
                 tma_load_2d(base, &tmap_w, bar, kb * kBKBytes, (int)n0);
                 tma_load_3d(base + w_bytes, &tmap_sw, bar, 0, 2 * kb, (int)blockIdx.y);
-                tma_load_2d(base + w_bytes + 1024, &tmap_a, bar, kb * kBKBytes, (int)m0);
-                tma_load_3d(base + w_bytes + 1024 + a_bytes, &tmap_sa, bar, 0, 2 * kb, (int)(m0 >> 7));
+                tma_load_2d(base + w_bytes + 1024, &tmap_a, bar, kb * kBKBytes, 0);
+                tma_load_3d(base + w_bytes + 1024 + a_bytes, &tmap_sa, bar, 0, 2 * kb, 0);
             }
             issued++;
             if (++s == p.stages) s = 0, ph ^= 1;
@@ -745,7 +746,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
         if (__all_sync(0xffffffffu, wait_phase<8>(smem_u32(&done_bar), 0, p.wait_cap_ns, p.err, abort_flag, 34))) {
             tc_fence_after();
             const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
-            const int cols = (int)min((size_t)p.bn, p.m - m0);
+            const int cols = (int)p.m;
             for (int c0 = 0; c0 < cols; c0 += 16) {
                 int32_t r[16];
                 tc_ld16(base + c0, r);
@@ -767,44 +768,61 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     }
     pdl_wait();
     if (*abort_flag == 0) {
-        const int t = threadIdx.x & 127;  // output of the tile
-        const size_t col = n0 + t;
-        const bool live = col < p.n;
-        const float bias = live && p.bias ? __ldg(p.bias + col) : 0.0f;
-        const int rows = (int)min((size_t)p.bn, p.m - m0);
-        for (int j = (int)rank + (int)S * (threadIdx.x >> 7); j < rows; j += 2 * (int)S) {
-            const uint32_t addr = smem_u32(part + j * 128 + t);
-            float v = 0.0f;
-            if (S > 1) {
-                float u[8];
+        // a warp takes a row of A, a lane four neighbouring outputs
+        const size_t col = n0 + 4 * lane;
+        float bias[4];
 #pragma unroll
-                for (uint32_t r = 0; r < 8; r++) u[r] = r < S ? ld_peer(addr, r) : 0.0f;
+        for (int i = 0; i < 4; i++) bias[i] = p.bias && col + i < p.n ? __ldg(p.bias + col + i) : 0.0f;
+        const int rows = (int)p.m;
+        for (int j = (int)rank + (int)S * warp; j < rows; j += (kSkinnyThreads / 32) * (int)S) {
+            const uint32_t addr = smem_u32(part + j * 128 + 4 * lane);
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float4 u[8];
 #pragma unroll
-                for (uint32_t r = 0; r < 8; r++)
-                    if (r < S) v += u[r];
-            } else {
-                v = part[j * 128 + t];
-            }
-            v = activate(v + bias, p.act);
-            const size_t row = m0 + j;
+            for (uint32_t r = 0; r < 8; r++)
+                if (r < S) u[r] = ld_peer4(addr, r);
+#pragma unroll
+            for (uint32_t r = 0; r < 8; r++)
+                if (r < S) v[0] += u[r].x, v[1] += u[r].y, v[2] += u[r].z, v[3] += u[r].w;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = activate(v[i] + bias[i], p.act);
+            const size_t row = j;
             if (p.out == 3) {
-                if (!live) v = 0.0f;
-                uint32_t amax = __float_as_uint(v) & 0x7FFFFFFFu;
+                uint32_t amax = 0;
 #pragma unroll
-                for (int o = 16; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                for (int i = 0; i < 4; i++) {
+                    if (col + i >= p.n) v[i] = 0.0f;
+                    amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+                }
+#pragma unroll
+                for (int o = 4; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                 const uint32_t sb = mx_scale_byte(amax);
-                const float q = v * mx_inv_scale(sb), next = __shfl_down_sync(0xffffffffu, q, 1);
+                const float inv = mx_inv_scale(sb);
                 const size_t block = col / 32;
-                if ((lane & 1) == 0 && block < p.out_nb)
-                    ((uint8_t *)p.y)[(row * p.out_nb * 32 + col) / 2] = sb == 0xFFu ? 0 : (uint8_t)mx_codes2(q, next);
-                if (lane == 0 && block < p.out_tiles * 4) p.y_s[mx_scale_at(row, block, p.out_tiles)] = (uint8_t)sb;
-            } else if (live) {
+                const uint32_t codes = mx_codes2(v[0] * inv, v[1] * inv) | (mx_codes2(v[2] * inv, v[3] * inv) << 8);
+                if (block < p.out_nb)
+                    *reinterpret_cast<uint16_t *>((uint8_t *)p.y + (row * p.out_nb * 32 + col) / 2) = sb == 0xFFu ? 0 : (uint16_t)codes;
+                if ((lane & 7) == 0 && block < p.out_tiles * 4) p.y_s[mx_scale_at(row, block, p.out_tiles)] = (uint8_t)sb;
+            } else {
+                auto store = [&](auto *y) {
+                    using T = std::remove_pointer_t<decltype(y)>;
+                    y += row * p.n + col;
+                    if (p.vec && col + 4 <= p.n) {
+                        Raw<T, 4> r;
+                        r.set(v);
+                        r.store(y);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (col + i < p.n) y[i] = from_f32<T>(v[i]);
+                    }
+                };
                 if (p.out == DW_F32)
-                    ((float *)p.y)[row * p.n + col] = v;
+                    store((float *)p.y);
                 else if (p.out == DW_F16)
-                    ((__half *)p.y)[row * p.n + col] = __float2half_rn(v);
+                    store((__half *)p.y);
                 else
-                    ((__nv_bfloat16 *)p.y)[row * p.n + col] = __float2bfloat16_rn(v);
+                    store((__nv_bfloat16 *)p.y);
             }
         }
     }
@@ -872,8 +890,6 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a, int S) {
                             smem, 2 * S, ta, tb, tsa, tsb, p);
 }
 
-// CTAs of a cluster that share a tile's K: as many as fill the GPU once, each with
-// at least one K block.
 dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
     SkinnyParams p{};
     p.bias = a.bias, p.y = a.y, p.y_s = a.y_s;
@@ -883,6 +899,7 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
     p.k_blocks = (int)((a.k + 255) / 256);
     p.bn = a.m <= 16 ? 16 : a.m <= 32 ? 32 : a.m <= 64 ? 64 : 128;
     p.act = a.act, p.out = a.y_s ? 3 : a.y_dtype;
+    p.vec = a.n % 4 == 0 && (uintptr_t)a.y % (a.y_dtype == DW_F32 ? 16 : 8) == 0;
     p.stage_bytes = kBM * kBKBytes + 1024 + p.bn * kBKBytes + 1024;
     for (int h = 0; h < 2; h++) p.idesc[h] = mx_idesc(128, p.bn, h);
     // two CTAs an SM up to 64 rows (each at most 256 columns of tensor memory), one above
@@ -891,10 +908,14 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
     p.stages = (int)std::min<size_t>(kSkinnyStages, budget / p.stage_bytes);
     p.tmem_cols = 256;
     p.wait_cap_ns = be->wait_cap_ns, p.err = be->dev_err;
-    const size_t tn = (a.n + 127) / 128, tm = (a.m + p.bn - 1) / p.bn;
-    if (tn > 65535 || tm > 65535) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu x %zu is too large", a.m, a.n);
+    const size_t tn = (a.n + 127) / 128;
+    if (tn > 65535) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu outputs are too many", a.n);
+    // CTAs that share a tile's K: about one an SM (4096 outputs, K 4096, one row: S = 1, 2,
+    // 4, 8 took 5.5, 4.4, 4.2, 4.6 us; 11008 outputs S = 1, 2, 4: 6.2, 6.2, 8.1), each with
+    // a K block at least; clusters of 8 CTAs that fill an SM each do not fit 16 at a time
     unsigned S = 1;
-    while (S < 8 && 2 * S * tn * tm <= (size_t)be->sm_count * per_sm && 2 * (int)S <= p.k_blocks) S *= 2;
+    const unsigned most = per_sm == 2 ? 8 : 4;
+    while (S < most && 2 * S * tn <= (size_t)be->sm_count * 4 / 3 && 2 * (int)S <= p.k_blocks) S *= 2;
     const size_t smem = 1024 + std::max<size_t>(p.stages * p.stage_bytes, (size_t)p.bn * 512);
     CUtensorMap tw, ta, tsw, tsa;
     if (!be->encode_tiled || !code_map(be, &tw, a.b_q, a.n, a.k, kBM) || !code_map(be, &ta, a.a_q, a.m, a.k, p.bn) ||
@@ -909,33 +930,37 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
         if (st != DW_OK) return st;
         attr_set[be->device] = true;
     }
-    return launch_dependent(be, "gemm_mxfp4", k_mxfp4_skinny, dim3(S, (unsigned)tn, (unsigned)tm), kSkinnyThreads, smem, S, tw, ta,
+    return launch_dependent(be, "gemm_mxfp4", k_mxfp4_skinny, dim3(S, (unsigned)tn), kSkinnyThreads, smem, S, tw, ta,
                             tsw, tsa, p);
 }
 
 }  // namespace
 
+// Which kernel, tile and split of K (times on B200, launches in a row, us):
+//   few rows: up to 64 (m 64, n 11008, k 4096: 7.7 against 9.5), or up to 128 where the
+//     pairs would have few tiles of a long K (m 128, k 4096: n 1000 5.8 against 7.0, n 4096
+//     6.9 against 6.5; k 11008, n 4096: 8.9 against 10.3);
+//   256 x 256 tiles once they fill the pairs four times over (8192^3 192 against 218),
+//     256 x 128 below, whose accumulators are double-buffered and whose last round is
+//     shorter (4096^3 29.4 against 32; 256 x 11008 x 4096 9.9 against 10.7);
+//   two pairs for each tile's K when both fit at once and K is long (256 x 4096 x 11008
+//     10.4 against 11.0; with k 4096 7.8 against 6.6).
 dw_status launch_gemm_mxfp4(dw_backend *be, const MxGemmArgs &a) {
-    const int skm = getenv("DW_MXSK") ? atoi(getenv("DW_MXSK")) : 64;
-    if (a.m <= skm) return launch_skinny(be, a);
-    const int out = a.y_s ? 3 : a.y_dtype;
-    int bn = getenv("DW_MXBN") ? atoi(getenv("DW_MXBN")) : 0, S = getenv("DW_MXS") ? atoi(getenv("DW_MXS")) : 0;
-    if (!bn || !S) {
-        double best = 1e30;
-        const long kb = (long)((a.k + 511) / 512);
-        for (int b : {256, 128})
-            for (int q : {1, 2, 4}) {
-                if (q > kb) continue;
-                const long tiles = (long)((a.m + 255) / 256) * (long)((a.n + b - 1) / b);
-                const long slots = q == 1 ? be->sm_count / 2 : q == 2 ? be->sm_count / 4 - 1 : be->sm_count / 8 - 2;
-                const double t = (double)((tiles + slots - 1) / slots) * ((kb + q - 1) / q * (b == 256 ? 0.72 : 0.64) + 1.5 + (q > 1 ? 2.0 : 0.0));
-                if (t < best) best = t, bn = b, S = q;
-            }
+    const size_t pairs = (size_t)be->sm_count / 2, rows = (a.m + 255) / 256, k_blocks = (a.k + 511) / 512;
+    if (a.m <= 64 || (a.m <= 128 && a.n <= 4096 && a.k > 4096) || (a.m <= 128 && a.n <= 1024 && a.k >= 2048))
+        return launch_skinny(be, a);
+    const bool wide = rows * ((a.n + 255) / 256) >= 4 * pairs;
+    const int S = !wide && rows * ((a.n + 127) / 128) <= pairs / 2 - 1 && k_blocks >= 16 ? 2 : 1;
+    switch ((wide ? 4 : 0) + (a.y_s ? 3 : a.y_dtype)) {
+        case 0: return launch<128, 0>(be, a, S);
+        case 1: return launch<128, 1>(be, a, S);
+        case 2: return launch<128, 2>(be, a, S);
+        case 3: return launch<128, 3>(be, a, S);
+        case 4: return launch<256, 0>(be, a, S);
+        case 5: return launch<256, 1>(be, a, S);
+        case 6: return launch<256, 2>(be, a, S);
+        default: return launch<256, 3>(be, a, S);
     }
-    while (S > (int)((a.k + 511) / 512)) S /= 2;
-    auto go = [&](auto k0, auto k1, auto k2, auto k3) { return (out == 0 ? k0 : out == 1 ? k1 : out == 2 ? k2 : k3)(be, a, S); };
-    if (bn == 128) return go(launch<128, 0>, launch<128, 1>, launch<128, 2>, launch<128, 3>);
-    return go(launch<256, 0>, launch<256, 1>, launch<256, 2>, launch<256, 3>);
 }
 
 }  // namespace dw

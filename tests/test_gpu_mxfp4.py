@@ -138,7 +138,7 @@ def run_gemm(be, a, b, m, n, k, dtype="f32", bias=None, act=0):
 
 SIZES = [(1, 1, 1), (1, 128, 32), (128, 128, 128), (128, 128, 64), (2, 3, 31), (129, 257, 257), (64, 96, 576), (16, 100, 40),
          (300, 130, 1000), (1, 4096, 4096), (7, 1000, 2056), (33, 640, 4128), (256, 384, 11008), (513, 1025, 96),
-         (1100, 2100, 300)]
+         (1100, 2100, 300), (100, 130, 64), (100, 1000, 2056), (128, 4096, 4128), (200, 300, 8200), (5100, 3890, 160)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -156,7 +156,9 @@ def test_gemm_exact(be, m, n, k):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("m,n,k,act,bias", [(1, 1000, 4096, 3, False), (37, 1000, 2056, 1, True), (130, 257, 999, 3, True),
-                                            (256, 512, 11008, 0, True), (5, 33, 70, 0, False)])
+                                            (256, 512, 11008, 0, True), (5, 33, 70, 0, False),
+                                            (5100, 3890, 96, 3, True), (5100, 3904, 96, 1, True), (64, 1003, 4200, 0, True),
+                                            (100, 1004, 4200, 3, True), (300, 2052, 520, 3, True)])
 def test_gemm_scales_bias_act(be, dtype, m, n, k, act, bias):
     """Scales over 2^+-6.  Products are exact; f32 sums in groups of at least 16 products: (k / 16 + 2)
     additions, each off by at most one step (2^-23, truncation included) of a partial sum, which sum |ab|
@@ -178,7 +180,8 @@ def test_gemm_scales_bias_act(be, dtype, m, n, k, act, bias):
 
 
 @pytest.mark.parametrize("m,n,k,act", [(1, 32, 32, 0), (1, 1000, 4096, 3), (5, 97, 300, 0), (37, 1000, 2056, 1), (130, 257, 999, 3),
-                                       (300, 640, 512, 3)])
+                                       (300, 640, 512, 3), (5100, 3890, 96, 0), (256, 500, 11008, 3), (100, 1000, 2056, 0),
+                                       (64, 1003, 96, 3)])
 def test_gemm_to_mxfp4_is_quantized_gemm(be, m, n, k, act):
     rng = np.random.default_rng(m * n + k)
     a = operand(be, *random_operand(rng, m, k, 121, 133), k)
