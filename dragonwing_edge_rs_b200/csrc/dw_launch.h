@@ -1,9 +1,10 @@
 // dw_launch.h -- launches as a programmatic dependent of the previous kernel on the
 // backend's stream.  The kernel's blocks may start while that kernel finishes; they
 // touch no global memory before pdl_wait(), which returns once it has completed and
-// its writes are visible.  Each kernel calls pdl_trigger() in every block, after any
-// tcgen05.alloc (a dependent block that took tensor memory first would wait for a
-// kernel that waits for it).
+// its writes are visible.  Each block then calls pdl_trigger(): not before pdl_wait()
+// (kernels waiting in a row would fill the SMs: quantise and dequantise of 1000 x 1010
+// f32 took 18 instead of 9 us), and after any tcgen05.alloc (a dependent block that
+// took tensor memory first would wait for a kernel that waits for it).
 #pragma once
 
 #include <cstdlib>

@@ -34,8 +34,8 @@ __global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *__restrict
     const size_t unit = ((size_t)blockIdx.y << p.lux) + u;
     const size_t col = unit * 128 + lane16 * 8;
     const size_t row0 = (size_t)blockIdx.x * rows_blk * kRows + ry;
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     Raw<T, 8> raw[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__
     const size_t unit = ((size_t)blockIdx.y << p.lux) + u;
     const size_t col = unit * 128 + lane16 * 8;
     const size_t row0 = (size_t)blockIdx.x * rows_blk * kRows + ry;
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     uint32_t codes[kRows], sb[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; i++) {
@@ -126,8 +126,8 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__
 // get byte 0 (rows past the last are left as they are).  One thread per (row, tile).
 __global__ void __launch_bounds__(kThreads) k_pack_scales(const uint8_t *__restrict__ in, uint8_t *__restrict__ s,
                                                           size_t rows, size_t nb, size_t tiles) {
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     const size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x;
     if (i >= rows * tiles) return;
     const size_t row = i / tiles, t = i - row * tiles;

@@ -398,13 +398,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     tc_fence_before();
     cluster_sync();
     tc_fence_after();
-    pdl_trigger();  // the warps that touch global memory wait below
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const uint32_t sf_cols = tmem + 256;  // scales after the accumulators
     float *partial = reinterpret_cast<float *>(smem_raw + (smem - smem_u32(smem_raw)));  // [BN][128]
 
     if (warp == 0) {
-        pdl_wait();
+        pdl_wait();  // (the other warps wait where they first touch global memory)
+        pdl_trigger();
         const uint32_t elected = elect_one();
         int s = 0, issued = 0;
         uint32_t ph = 0;
@@ -663,13 +663,13 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    pdl_trigger();  // the warps wait where they first touch global memory
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const uint32_t sf_cols = tmem + (uint32_t)p.bn;  // 16 columns a stage after the accumulators
     const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
 
     if (warp == 0) {
-        pdl_wait();
+        pdl_wait();  // (the other warps wait where they first touch global memory)
+        pdl_trigger();
         const uint32_t elected = elect_one();
         int s = 0, issued = 0;
         uint32_t ph = 0;

@@ -162,8 +162,8 @@ __global__ void __launch_bounds__(kMaxT, V * N <= 8 ? 2 : 1) k_norm(const __grid
             return w != nullptr;
         };
     };
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     for (size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y; row < p.rows; row += (size_t)gridDim.x * blockDim.y) {
         Raw<X, V> xr[N], gr[N];
         Raw<R, V> rr[N];
@@ -269,8 +269,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
         copy(dx, (const uint8_t *)p.x, p.x_pitch * sizeof(X), x_bytes);
         if (p.has_res) copy(dr, (const uint8_t *)p.res, p.res_pitch * sizeof(R), r_bytes);
     };
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     if (threadIdx.x == 0) {
         size_t step = blockIdx.x;
         for (int s = 0; s < stages && step < steps; s++, step += gridDim.x) fetch(step, s);
@@ -471,8 +471,8 @@ __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Par
     const R *res = (const R *)p.res + row * p.res_pitch;
     const X *gate = (const X *)p.gate + (p.gate_rows ? row / p.gate_rows : 0) * p.c;
     R *out = (R *)p.out + row * p.res_pitch;
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();
     auto stats = [&](auto at, int kind, float &mean, float &rstd) {
         mean = 0.0f, rstd = 1.0f;
         if (kind == DW_NORM_NONE) return;
