@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
     float c0[kKeep ? N : 1][V], w1[kKeep ? N : 1][V];
     bool live[N];
     const bool row_gate = p.gate && p.gate_rows;
-    auto column = [&](int j) { return ((size_t)j * T + tid) * V; };
+    auto column = [&](int j) { return (uint32_t)(j * T + tid) * V; };
     auto coefficients = [&](int j, float (&t)[V]) {
 #pragma unroll
         for (int i = 0; i < V; i++) t[i] = p.res_scale;
@@ -375,37 +375,53 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
             for (int i = 0; i < V; i++) v[j][i] = xr[j].get(i);
         if (p.has_res) {
             const float rstd = p.post != DW_NORM_NONE ? statistics(v, p.post) : 1.0f;
-            const X *gate = (const X *)p.gate + (row_gate && there ? row / p.gate_rows : 0) * p.c;
             R *out = (R *)p.out + row * p.res_pitch;
+            // the gate of the row or the bias: branches around whole loops (inside, each
+            // element would carry their predicated instructions)
+            auto join = [&](auto coefficient, auto bias) {
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                if (!live[j]) continue;
-                float o[V], t[V];
-                if constexpr (kKeep) {
+                for (int j = 0; j < N; j++) {
+                    if (!live[j]) continue;
+                    float o[V], t[V];
+                    if constexpr (kKeep) {
 #pragma unroll
-                    for (int i = 0; i < V; i++) t[i] = c0[j][i];
-                } else {
-                    coefficients(j, t);
+                        for (int i = 0; i < V; i++) t[i] = c0[j][i];
+                    } else {
+                        coefficients(j, t);
+                    }
+                    coefficient(j, t);
+#pragma unroll
+                    for (int i = 0; i < V; i++) o[i] = fmaf(v[j][i] * rstd, t[i], rr[j].get(i));
+                    bias(j, o);
+                    Raw<R, V> r;
+                    r.set(o);
+                    if (there) r.store(out + column(j));
+#pragma unroll
+                    for (int i = 0; i < V; i++) v[j][i] = r.get(i);
                 }
-                Raw<X, V> gr;
-                if (row_gate) gr.load(gate + column(j));
+            };
+            auto nothing = [](int, float (&)[V]) {};
+            if (!row_gate && !(p.b0 && p.post != DW_NORM_NONE)) {
+                join(nothing, nothing);
+            } else {
+                const X *gate = (const X *)p.gate + (row_gate && there ? row / p.gate_rows : 0) * p.c;
+                join(
+                    [&](int j, float (&t)[V]) {
+                        if (!row_gate) return;
+                        Raw<X, V> g;
+                        g.load(gate + column(j));
 #pragma unroll
-                for (int i = 0; i < V; i++) {
-                    if (row_gate) t[i] *= gr.get(i);
-                    o[i] = fmaf(v[j][i] * rstd, t[i], rr[j].get(i));
-                }
-                if (p.b0 && p.post != DW_NORM_NONE) {  // + res_scale * gate * b
-                    float b[V];
-                    load_f32<V>(p.b0 + column(j), b);
-                    if (p.gate && !row_gate) gr.load((const X *)p.gate + column(j));
+                        for (int i = 0; i < V; i++) t[i] *= g.get(i);
+                    },
+                    [&](int j, float (&o)[V]) {  // + res_scale * gate * b
+                        if (!p.b0 || p.post == DW_NORM_NONE) return;
+                        float b[V];
+                        load_f32<V>(p.b0 + column(j), b);
+                        Raw<X, V> g;
+                        if (p.gate) g.load(gate + column(j));
 #pragma unroll
-                    for (int i = 0; i < V; i++) o[i] = fmaf(b[i], p.gate ? p.res_scale * gr.get(i) : p.res_scale, o[i]);
-                }
-                Raw<R, V> r;
-                r.set(o);
-                if (there) r.store(out + column(j));
-#pragma unroll
-                for (int i = 0; i < V; i++) v[j][i] = r.get(i);
+                        for (int i = 0; i < V; i++) o[i] = fmaf(b[i], p.gate ? p.res_scale * g.get(i) : p.res_scale, o[i]);
+                    });
             }
         }
         if (p.y_dtype == -1) continue;
@@ -423,7 +439,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
                 }
 #pragma unroll
                 for (int i = 0; i < V; i++) v[j][i] = v[j][i] * rstd * t[i];
-                if (p.b1) {
+            }
+            if (p.b1) {
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    if (!live[j]) continue;
+                    float t[V];
                     load_f32<V>(p.b1 + column(j), t);
 #pragma unroll
                     for (int i = 0; i < V; i++) v[j][i] += t[i];
