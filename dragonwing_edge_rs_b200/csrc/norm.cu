@@ -233,10 +233,9 @@ __global__ void __launch_bounds__(kMaxT, V * N <= 8 ? 2 : 1) k_norm(const __grid
 constexpr int kStreamStages = 8;
 
 template <typename X, typename R, int N, int kThreads, bool kFull>
-__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 3 : 1)
     k_norm_stream(const __grid_constant__ Params p, const int T, const int stages, uint64_t wait_cap_ns, int32_t *err) {
     constexpr int V = 8;
-    constexpr bool kKeep = N <= 2;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(16) float red[4][16];
     __shared__ uint64_t full_bar[kStreamStages];
@@ -277,42 +276,47 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
     }
     // c0: what the normalised x of a column is multiplied by (weight, residual scale and,
     // where all rows share it, the gate); w1: the weight of the next norm
-    float c0[kKeep ? N : 1][V], w1[kKeep ? N : 1][V];
+    // (both in shared memory, 16 bytes of a thread beside its neighbour's: registers go to
+    // a third block on the SM instead)
+    float4 *c0 = reinterpret_cast<float4 *>(ring + (size_t)stages * stage_bytes), *w1 = c0 + 2 * N * T;
     bool live[N];
     const bool row_gate = p.gate && p.gate_rows;
     auto column = [&](int j) { return (uint32_t)(j * T + tid) * V; };
-    auto coefficients = [&](int j, float (&t)[V]) {
-#pragma unroll
-        for (int i = 0; i < V; i++) t[i] = p.res_scale;
-        if (p.gate && !row_gate) {
-            Raw<X, V> g;
-            g.load((const X *)p.gate + column(j));
-#pragma unroll
-            for (int i = 0; i < V; i++) t[i] *= g.get(i);
-        }
-        if (p.w0 && p.post != DW_NORM_NONE) {
-            float w[V];
-            load_f32<V>(p.w0 + column(j), w);
-#pragma unroll
-            for (int i = 0; i < V; i++) t[i] *= w[i];
-        }
+    auto kept = [&](const float4 *from, int j, float (&t)[V]) {
+        const float4 a = from[2 * j * T + tid], b = from[(2 * j + 1) * T + tid];
+        t[0] = a.x, t[1] = a.y, t[2] = a.z, t[3] = a.w, t[4] = b.x, t[5] = b.y, t[6] = b.z, t[7] = b.w;
     };
-    auto weights = [&](int j, float (&t)[V]) {
-        if (p.w1) {
-            load_f32<V>(p.w1 + column(j), t);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; i++) t[i] = 1.0f;
-        }
+    auto keep = [&](float4 *to, int j, const float (&t)[V]) {
+        to[2 * j * T + tid] = make_float4(t[0], t[1], t[2], t[3]), to[(2 * j + 1) * T + tid] = make_float4(t[4], t[5], t[6], t[7]);
     };
 #pragma unroll
     for (int j = 0; j < N; j++) {
         live[j] = kFull || column(j) < p.c;
-        if constexpr (kKeep) {
-            if (live[j] && p.has_res) coefficients(j, c0[j]);
-            if (live[j]) weights(j, w1[j]);
+        if (!live[j] || g) continue;
+        float t[V];
+        if (p.has_res) {
+#pragma unroll
+            for (int i = 0; i < V; i++) t[i] = p.res_scale;
+            if (p.gate && !row_gate) {
+                Raw<X, V> x;
+                x.load((const X *)p.gate + column(j));
+#pragma unroll
+                for (int i = 0; i < V; i++) t[i] *= x.get(i);
+            }
+            if (p.w0 && p.post != DW_NORM_NONE) {
+                float w[V];
+                load_f32<V>(p.w0 + column(j), w);
+#pragma unroll
+                for (int i = 0; i < V; i++) t[i] *= w[i];
+            }
+            keep(c0, j, t);
         }
+#pragma unroll
+        for (int i = 0; i < V; i++) t[i] = 1.0f;
+        if (p.w1) load_f32<V>(p.w1 + column(j), t);
+        keep(w1, j, t);
     }
+    __syncthreads();
     // (mean, 1 / root) of v over the row; elements past the row are 0
     auto statistics = [&](float (&v)[N][V], int kind) {
         if (kind == DW_NORM_LAYER) {
@@ -383,12 +387,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
                 for (int j = 0; j < N; j++) {
                     if (!live[j]) continue;
                     float o[V], t[V];
-                    if constexpr (kKeep) {
-#pragma unroll
-                        for (int i = 0; i < V; i++) t[i] = c0[j][i];
-                    } else {
-                        coefficients(j, t);
-                    }
+                    kept(c0, j, t);
                     coefficient(j, t);
 #pragma unroll
                     for (int i = 0; i < V; i++) o[i] = fmaf(v[j][i] * rstd, t[i], rr[j].get(i));
@@ -431,12 +430,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1)
             for (int j = 0; j < N; j++) {
                 if (!live[j]) continue;
                 float t[V];
-                if constexpr (kKeep) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) t[i] = w1[j][i];
-                } else {
-                    weights(j, t);
-                }
+                kept(w1, j, t);
 #pragma unroll
                 for (int i = 0; i < V; i++) v[j][i] = v[j][i] * rstd * t[i];
             }
@@ -555,8 +549,10 @@ template <typename X, typename R, int N, int kThreads, bool kFull>
 dw_status stream_as(dw_backend *be, const Params &p, int T) {
     auto kernel = k_norm_stream<X, R, N, kThreads, kFull>;
     const size_t G = kThreads / T, stage = G * p.c * (sizeof(X) + (p.has_res ? sizeof(R) : 0));
-    const int per_sm = kThreads == 256 ? 2 : 1;
-    const int stages = (int)std::min<size_t>(kStreamStages, (kSmemBudget / per_sm) / stage);
+    const size_t weights = (size_t)T * N * 8 * 4 * 2;
+    // three blocks an SM where each has room for two steps
+    auto fits = [&](int blocks) { return (int)std::min<size_t>(kStreamStages, (kSmemBudget / blocks - weights) / stage); };
+    const int per_sm = kThreads > 256 ? 1 : fits(3) >= 2 ? 3 : 2, stages = fits(per_sm);
     static bool attr_set[16] = {};
     if (be->device < 16 && !attr_set[be->device]) {
         dw_status st = dw_cuda_check(
@@ -566,7 +562,7 @@ dw_status stream_as(dw_backend *be, const Params &p, int T) {
     }
     const size_t steps = (p.rows + G - 1) / G;
     const unsigned grid = (unsigned)std::min<size_t>(steps, (size_t)be->sm_count * per_sm);
-    return launch_dependent(be, "norm", kernel, grid, kThreads, stages * stage, 0, p, T, stages, be->wait_cap_ns, be->dev_err);
+    return launch_dependent(be, "norm", kernel, grid, kThreads, stages * stage + weights, 0, p, T, stages, be->wait_cap_ns, be->dev_err);
 }
 
 template <typename X, typename R>
