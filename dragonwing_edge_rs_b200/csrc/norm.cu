@@ -231,9 +231,14 @@ __global__ void __launch_bounds__(kMaxT, V * N <= 8 ? 2 : 1) k_norm(const __grid
 // loads in flight do not depend on how many rows the registers hold, and the
 // weights and a shared gate row of a thread's columns stay in registers.
 constexpr int kStreamStages = 8;
+// Blocks an SM: three where 80 registers a thread and the ring allow it.
+template <typename R, int N, int kThreads>
+constexpr int stream_blocks() {
+    return kThreads > 256 ? 1 : N > 1 && sizeof(R) == 4 ? 2 : 3;
+}
 
 template <typename X, typename R, int N, int kThreads, bool kFull>
-__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 3 : 1)
+__global__ void __launch_bounds__(kThreads, stream_blocks<R, N, kThreads>())
     k_norm_stream(const __grid_constant__ Params p, const int T, const int stages, uint64_t wait_cap_ns, int32_t *err) {
     constexpr int V = 8;
     extern __shared__ __align__(128) uint8_t ring[];
@@ -244,7 +249,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 3 : 1)
     const int G = kThreads / T, g = threadIdx.x / T, tid = threadIdx.x & (T - 1);
     const size_t steps = (p.rows + G - 1) / G;
     const uint32_t x_bytes = (uint32_t)(p.c * sizeof(X)), r_bytes = p.has_res ? (uint32_t)(p.c * sizeof(R)) : 0u;
-    const uint32_t stage_bytes = G * (x_bytes + r_bytes);
+    // a gate row of the rows themselves comes with them
+    const bool row_gate = p.gate && p.gate_rows;
+    const uint32_t g_bytes = row_gate ? x_bytes : 0u, row_bytes = x_bytes + r_bytes + g_bytes, stage_bytes = G * row_bytes;
     const uint32_t base = smem_u32(ring);
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; s++) mbar_init(smem_u32(&full_bar[s]), 1);
@@ -256,8 +263,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 3 : 1)
     auto fetch = [&](size_t step, int s) {
         const size_t row0 = step * G;
         const uint32_t rows = (uint32_t)min((size_t)G, p.rows - row0), bar = smem_u32(&full_bar[s]);
-        const uint32_t dx = base + s * stage_bytes, dr = dx + G * x_bytes;
-        mbar_expect_tx(bar, rows * (x_bytes + r_bytes));
+        const uint32_t dx = base + s * stage_bytes, dr = dx + G * x_bytes, dg = dr + G * r_bytes;
+        mbar_expect_tx(bar, rows * row_bytes);
         auto copy = [&](uint32_t dst, const uint8_t *src, size_t pitch, uint32_t bytes) {
             if (pitch == bytes) {
                 bulk_load(dst, src + row0 * pitch, rows * bytes, bar);
@@ -267,6 +274,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 3 : 1)
         };
         copy(dx, (const uint8_t *)p.x, p.x_pitch * sizeof(X), x_bytes);
         if (p.has_res) copy(dr, (const uint8_t *)p.res, p.res_pitch * sizeof(R), r_bytes);
+        if (row_gate)
+            for (uint32_t r = 0; r < rows; r++)
+                bulk_load(dg + r * x_bytes, (const X *)p.gate + (row0 + r) / p.gate_rows * p.c, x_bytes, bar);
     };
     pdl_wait();
     pdl_trigger();
@@ -280,7 +290,6 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 3 : 1)
     // a third block on the SM instead)
     float4 *c0 = reinterpret_cast<float4 *>(ring + (size_t)stages * stage_bytes), *w1 = c0 + 2 * N * T;
     bool live[N];
-    const bool row_gate = p.gate && p.gate_rows;
     auto column = [&](int j) { return (uint32_t)(j * T + tid) * V; };
     auto kept = [&](const float4 *from, int j, float (&t)[V]) {
         const float4 a = from[2 * j * T + tid], b = from[(2 * j + 1) * T + tid];
@@ -353,16 +362,18 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 3 : 1)
         }
         // rows of the last step past the end hold what the stage held: they stay in
         // their own threads and nothing of them is stored
-        Raw<X, V> xr[N];
+        Raw<X, V> xr[N], gr[N];
         Raw<R, V> rr[N];
         const X *xs = reinterpret_cast<const X *>(ring + s * stage_bytes + g * x_bytes);
         const R *rs = reinterpret_cast<const R *>(ring + s * stage_bytes + G * x_bytes + g * r_bytes);
+        const X *gs = reinterpret_cast<const X *>(ring + s * stage_bytes + G * (x_bytes + r_bytes) + g * x_bytes);
 #pragma unroll
         for (int j = 0; j < N; j++) {
             if (!kFull) xr[j].zero(), rr[j].zero();
             if (live[j]) {
                 xr[j].load(xs + column(j));
                 if (p.has_res) rr[j].load(rs + column(j));
+                if (row_gate) gr[j].load(gs + column(j));
             }
         }
         __syncthreads();  // the stage has been read
@@ -403,21 +414,18 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 3 : 1)
             if (!row_gate && !(p.b0 && p.post != DW_NORM_NONE)) {
                 join(nothing, nothing);
             } else {
-                const X *gate = (const X *)p.gate + (row_gate && there ? row / p.gate_rows : 0) * p.c;
                 join(
                     [&](int j, float (&t)[V]) {
                         if (!row_gate) return;
-                        Raw<X, V> g;
-                        g.load(gate + column(j));
 #pragma unroll
-                        for (int i = 0; i < V; i++) t[i] *= g.get(i);
+                        for (int i = 0; i < V; i++) t[i] *= gr[j].get(i);
                     },
                     [&](int j, float (&o)[V]) {  // + res_scale * gate * b
                         if (!p.b0 || p.post == DW_NORM_NONE) return;
                         float b[V];
                         load_f32<V>(p.b0 + column(j), b);
-                        Raw<X, V> g;
-                        if (p.gate) g.load(gate + column(j));
+                        Raw<X, V> g = gr[j];
+                        if (p.gate && !row_gate) g.load((const X *)p.gate + column(j));
 #pragma unroll
                         for (int i = 0; i < V; i++) o[i] = fmaf(b[i], p.gate ? p.res_scale * g.get(i) : p.res_scale, o[i]);
                     });
@@ -546,34 +554,41 @@ __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Par
 }
 
 template <typename X, typename R, int N, int kThreads, bool kFull>
-dw_status stream_as(dw_backend *be, const Params &p, int T) {
+bool stream_as(dw_backend *be, const Params &p, int T, dw_status *st) {
     auto kernel = k_norm_stream<X, R, N, kThreads, kFull>;
-    const size_t G = kThreads / T, stage = G * p.c * (sizeof(X) + (p.has_res ? sizeof(R) : 0));
+    const size_t G = kThreads / T, stage = G * p.c * (sizeof(X) * (p.gate && p.gate_rows ? 2 : 1) + (p.has_res ? sizeof(R) : 0));
     const size_t weights = (size_t)T * N * 8 * 4 * 2;
-    // three blocks an SM where each has room for two steps
-    auto fits = [&](int blocks) { return (int)std::min<size_t>(kStreamStages, (kSmemBudget / blocks - weights) / stage); };
-    const int per_sm = kThreads > 256 ? 1 : fits(3) >= 2 ? 3 : 2, stages = fits(per_sm);
+    // the most blocks an SM that have room for two steps each, or else for one
+    auto fits = [&](size_t blocks) {
+        const size_t room = kSmemBudget / blocks;
+        return room < weights + stage ? 0 : (int)std::min<size_t>(kStreamStages, (room - weights) / stage);
+    };
+    constexpr int kBlocks = stream_blocks<R, N, kThreads>();
+    const int per_sm = kBlocks == 3 && fits(3) >= 2 ? 3 : kBlocks >= 2 && fits(2) >= 1 ? 2 : 1, stages = fits(per_sm);
+    if (stages < 1) return false;
     static bool attr_set[16] = {};
     if (be->device < 16 && !attr_set[be->device]) {
-        dw_status st = dw_cuda_check(
+        *st = dw_cuda_check(
             be, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBudget), "norm attributes");
-        if (st != DW_OK) return st;
+        if (*st != DW_OK) return true;
         attr_set[be->device] = true;
     }
     const size_t steps = (p.rows + G - 1) / G;
     const unsigned grid = (unsigned)std::min<size_t>(steps, (size_t)be->sm_count * per_sm);
-    return launch_dependent(be, "norm", kernel, grid, kThreads, stages * stage + weights, 0, p, T, stages, be->wait_cap_ns, be->dev_err);
+    *st = launch_dependent(be, "norm", kernel, grid, kThreads, stages * stage + weights, 0, p, T, stages, be->wait_cap_ns, be->dev_err);
+    return true;
 }
 
+// Launches the streaming form; false where a row is too long for it.
 template <typename X, typename R>
-dw_status stream(dw_backend *be, const Params &p) {
+bool stream(dw_backend *be, const Params &p, dw_status *st) {
     int T = 8;
     while ((size_t)T * (T < 32 ? 8 : 16) < p.c && T < 256) T *= 2;
-    if ((size_t)T * 8 >= p.c) return stream_as<X, R, 1, 256, false>(be, p, T);
-    if ((size_t)T * 16 == p.c) return stream_as<X, R, 2, 256, true>(be, p, T);
-    if ((size_t)T * 16 >= p.c) return stream_as<X, R, 2, 256, false>(be, p, T);
-    if ((size_t)512 * 16 >= p.c) return stream_as<X, R, 2, 512, false>(be, p, 512);
-    return stream_as<X, R, 4, 512, false>(be, p, 512);
+    if ((size_t)T * 8 >= p.c) return stream_as<X, R, 1, 256, false>(be, p, T, st);
+    if ((size_t)T * 16 == p.c) return stream_as<X, R, 2, 256, true>(be, p, T, st);
+    if ((size_t)T * 16 >= p.c) return stream_as<X, R, 2, 256, false>(be, p, T, st);
+    if ((size_t)512 * 16 >= p.c) return stream_as<X, R, 2, 512, false>(be, p, 512, st);
+    return stream_as<X, R, 4, 512, false>(be, p, 512, st);
 }
 
 template <typename X, typename R>
@@ -594,7 +609,8 @@ dw_status run(dw_backend *be, const Params &p) {
     if (p.c > (size_t)kMaxT * kMaxE) {
         return launch_dependent(be, "norm (long rows)", k_norm_long<X, R>, (unsigned)p.rows, kMaxT, 0, 0, p);
     }
-    if (fits(8) && p.c <= (size_t)kMaxT * kMaxE && p.rows >= (size_t)be->sm_count * 2) return stream<X, R>(be, p);
+    dw_status st;
+    if (fits(8) && p.c <= (size_t)kMaxT * kMaxE && p.rows >= (size_t)be->sm_count * 2 && stream<X, R>(be, p, &st)) return st;
     // E: elements of a thread; T: threads of a row (a power of two from 32 to 512)
     int E = 8, T = 32;
     while ((size_t)T * E < p.c && T < kMaxT) T *= 2;

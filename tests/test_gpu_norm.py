@@ -83,7 +83,8 @@ def test_norm(be, dtype, ydtype, kind, rows, c):
                                                        (5, 64, RMS, NONE, None), (300, 512, NONE, LAYER, 100),
                                                        (310, 4096, RMS, RMS, 0), (301, 2048, LAYER, LAYER, 100),
                                                        (305, 104, RMS, RMS, 1), (300, 5120, LAYER, RMS, 7),
-                                                       (299, 11008, RMS, RMS, None), (1030, 72, RMS, NONE, 0)])
+                                                       (299, 11008, RMS, RMS, None), (1030, 72, RMS, NONE, 0), (298, 16384, RMS, RMS, 1),
+                                                       (298, 8192, LAYER, RMS, 0), (600, 1024, RMS, LAYER, 3)])
 def test_norm_residual(be, dtype, res, rows, c, post, pre, gate_rows):
     """`out` against float64, and y against the norm of the stored `out`."""
     rng = np.random.default_rng(rows * 7 + c)
