@@ -122,6 +122,27 @@ struct Raw {
     }
 };
 
+// 8 elements in one access: 16 bytes, or 32 aligned ones.
+template <typename T>
+__device__ __forceinline__ void load_wide(Raw<T, 8> &r, const T *p) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]),
+                       "=r"(r.w[7])
+                     : "l"(p));
+    else
+        r.load(p);
+}
+template <typename T>
+__device__ __forceinline__ void store_wide(const Raw<T, 8> &r, T *p) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]),
+                     "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7])
+                     : "memory");
+    else
+        r.store(p);
+}
+
 // ---- the format --------------------------------------------------------------
 __host__ __device__ inline size_t mx_blocks(size_t k) { return (k + 31) / 32; }      // scales of a row
 __host__ __device__ inline size_t mx_tiles(size_t k) { return (mx_blocks(k) + 3) / 4; }  // scale tiles along a row
