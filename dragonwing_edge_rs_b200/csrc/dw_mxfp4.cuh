@@ -216,6 +216,19 @@ __device__ __forceinline__ void mx_decode8(uint32_t c, float (&v)[8]) {
     }
 }
 
+// The value of the code in the low four bits.
+__device__ __forceinline__ float mx_decode1(uint32_t c) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t}"
+        : "=r"(h)
+        : "r"(c));
+    __half2 t;
+    memcpy(&t, &h, 4);
+    return __low2float(t);
+}
+
 // 32 values of one thread -> 16 code bytes and the scale byte.
 __device__ __forceinline__ uint32_t mx_quantize32(const float (&v)[32], uint4 &codes) {
     uint32_t amax = 0;
