@@ -940,16 +940,16 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
 //   few rows: up to 64 (m 64, n 11008, k 4096: 7.7 against 9.5), or up to 128 where the
 //     pairs would have few tiles of a long K (m 128, k 4096: n 1000 5.8 against 7.0, n 4096
 //     6.9 against 6.5; k 11008, n 4096: 8.9 against 10.3);
-//   256 x 256 tiles once they fill the pairs four times over (8192^3 192 against 218),
-//     256 x 128 below, whose accumulators are double-buffered and whose last round is
-//     shorter (4096^3 29.4 against 32; 256 x 11008 x 4096 9.9 against 10.7);
+//   256 x 256 tiles once they fill the pairs (other operands each time: 4096^3 30.6 against
+//     32.8, 2048 x 4096 x 4096 17.7 against 19.0), 256 x 128 below, whose accumulators are
+//     double-buffered and whose last round is shorter (256 x 11008 x 4096 12.2 against 13.4);
 //   two pairs for each tile's K when both fit at once and K is long (256 x 4096 x 11008
 //     10.4 against 11.0; with k 4096 7.8 against 6.6).
 dw_status launch_gemm_mxfp4(dw_backend *be, const MxGemmArgs &a) {
     const size_t pairs = (size_t)be->sm_count / 2, rows = (a.m + 255) / 256, k_blocks = (a.k + 511) / 512;
     if (a.m <= 64 || (a.m <= 128 && a.n <= 4096 && a.k > 4096) || (a.m <= 128 && a.n <= 1024 && a.k >= 2048))
         return launch_skinny(be, a);
-    const bool wide = rows * ((a.n + 255) / 256) >= 4 * pairs;
+    const bool wide = rows * ((a.n + 255) / 256) >= pairs;
     const int S = !wide && rows * ((a.n + 127) / 128) <= pairs / 2 - 1 && k_blocks >= 16 ? 2 : 1;
     switch ((wide ? 4 : 0) + (a.y_s ? 3 : a.y_dtype)) {
         case 0: return launch<128, 0>(be, a, S);

@@ -345,31 +345,43 @@ def mxfp4_scale_bytes(rows: int, k: int) -> int:
 def quantize_mxfp4(backend: CudaBackend, x: CudaBuffer, dtype: int, rows: int, k: int, q: CudaBuffer, s: CudaBuffer,
                    x_pitch: int = 0):
     """x [rows, k] of `dtype` (rows x_pitch elements apart) -> MXFP4 codes q and scales s."""
-    backend._check(L.load().dw_quantize_mxfp4(backend.handle, _h(x), dtype, rows, k, x_pitch, _h(q), _h(s)))
+    st = L.load().dw_quantize_mxfp4(backend.handle, x and x.handle, dtype, rows, k, x_pitch, q and q.handle,
+                                    s and s.handle)
+    if st:
+        backend._check(st)
 
 
 def dequantize_mxfp4(backend: CudaBackend, q: CudaBuffer, s: CudaBuffer, rows: int, k: int, y: CudaBuffer, dtype: int):
     """The values [rows, k] of an MXFP4 operand, as `dtype`."""
-    backend._check(L.load().dw_dequantize_mxfp4(backend.handle, _h(q), _h(s), rows, k, _h(y), dtype))
+    st = L.load().dw_dequantize_mxfp4(backend.handle, q and q.handle, s and s.handle, rows, k, y and y.handle, dtype)
+    if st:
+        backend._check(st)
 
 
 def pack_scales_mxfp4(backend: CudaBackend, scales: CudaBuffer, rows: int, k: int, s: CudaBuffer):
     """Row-major scale bytes [rows, ceil(k / 32)] -> an operand's scale buffer."""
-    backend._check(L.load().dw_pack_scales_mxfp4(backend.handle, _h(scales), rows, k, _h(s)))
+    st = L.load().dw_pack_scales_mxfp4(backend.handle, scales and scales.handle, rows, k, s and s.handle)
+    if st:
+        backend._check(st)
 
 
 def gemm_mxfp4(backend: CudaBackend, a_q, a_s, b_q, b_s, bias, y, y_dtype: int, m: int, n: int, k: int,
                act: int = EPI_NONE):
     """y[m, n] = act(sum_k A[m, k] * B[n, k] + bias[n]) of two MXFP4 operands."""
-    backend._check(L.load().dw_gemm_mxfp4(backend.handle, _h(a_q), _h(a_s), _h(b_q), _h(b_s), _h(bias), _h(y), y_dtype,
-                                          m, n, k, act))
+    st = L.load().dw_gemm_mxfp4(backend.handle, a_q and a_q.handle, a_s and a_s.handle, b_q and b_q.handle,
+                                b_s and b_s.handle, bias and bias.handle, y and y.handle, y_dtype, m, n, k, act)
+    if st:
+        backend._check(st)
 
 
 def gemm_to_mxfp4(backend: CudaBackend, a_q, a_s, b_q, b_s, bias, y_q, y_s, m: int, n: int, k: int,
                   act: int = EPI_NONE):
     """gemm_mxfp4 with its f32 result quantised to an MXFP4 operand [m, n]."""
-    backend._check(L.load().dw_gemm_to_mxfp4(backend.handle, _h(a_q), _h(a_s), _h(b_q), _h(b_s), _h(bias), _h(y_q),
-                                             _h(y_s), m, n, k, act))
+    st = L.load().dw_gemm_to_mxfp4(backend.handle, a_q and a_q.handle, a_s and a_s.handle, b_q and b_q.handle,
+                                   b_s and b_s.handle, bias and bias.handle, y_q and y_q.handle, y_s and y_s.handle,
+                                   m, n, k, act)
+    if st:
+        backend._check(st)
 
 
 class NormDesc(L.DwNormDesc):
@@ -385,27 +397,41 @@ class NormDesc(L.DwNormDesc):
 
 def norm(backend: CudaBackend, desc: NormDesc, x, w, b, y):
     """y = pre(x) with weight w and bias b (f32 [c] or None)."""
-    backend._check(L.load().dw_norm(backend.handle, ctypes.byref(desc), _h(x), _h(w), _h(b), _h(y)))
+    st = L.load().dw_norm(backend.handle, ctypes.byref(desc), x and x.handle, w and w.handle, b and b.handle,
+                          y and y.handle)
+    if st:
+        backend._check(st)
 
 
 def norm_to_mxfp4(backend: CudaBackend, desc: NormDesc, x, w, b, q, s):
     """norm with its f32 result quantised to an MXFP4 operand."""
-    backend._check(L.load().dw_norm_to_mxfp4(backend.handle, ctypes.byref(desc), _h(x), _h(w), _h(b), _h(q), _h(s)))
+    st = L.load().dw_norm_to_mxfp4(backend.handle, ctypes.byref(desc), x and x.handle, w and w.handle, b and b.handle,
+                                   q and q.handle, s and s.handle)
+    if st:
+        backend._check(st)
 
 
 def norm_residual(backend: CudaBackend, desc: NormDesc, x, w_post, b_post, gate, residual, out, w_pre=None, b_pre=None,
                   y=None):
     """out = residual + res_scale * gate * post(x); y = pre(out) (None: `out` alone)."""
-    backend._check(L.load().dw_norm_residual(backend.handle, ctypes.byref(desc), _h(x), _h(w_post), _h(b_post),
-                                             _h(gate), _h(residual), _h(out), _h(w_pre), _h(b_pre), _h(y)))
+    st = L.load().dw_norm_residual(backend.handle, ctypes.byref(desc), x and x.handle, w_post and w_post.handle,
+                                   b_post and b_post.handle, gate and gate.handle, residual and residual.handle,
+                                   out and out.handle,
+                                   w_pre and w_pre.handle, b_pre and b_pre.handle, y and y.handle)
+    if st:
+        backend._check(st)
 
 
 def norm_residual_to_mxfp4(backend: CudaBackend, desc: NormDesc, x, w_post, b_post, gate, residual, out, w_pre, b_pre,
                            q, s):
     """norm_residual with y quantised to an MXFP4 operand."""
-    backend._check(L.load().dw_norm_residual_to_mxfp4(backend.handle, ctypes.byref(desc), _h(x), _h(w_post),
-                                                      _h(b_post), _h(gate), _h(residual), _h(out), _h(w_pre), _h(b_pre),
-                                                      _h(q), _h(s)))
+    st = L.load().dw_norm_residual_to_mxfp4(backend.handle, ctypes.byref(desc), x and x.handle,
+                                            w_post and w_post.handle, b_post and b_post.handle, gate and gate.handle,
+                                            residual and residual.handle, out and out.handle, w_pre and w_pre.handle,
+                                            b_pre and b_pre.handle,
+                                            q and q.handle, s and s.handle)
+    if st:
+        backend._check(st)
 
 
 # ---------------------------------------------------------------------------
