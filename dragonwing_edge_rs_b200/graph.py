@@ -47,7 +47,9 @@ class CompiledOp:
     """builder.rs:204 CompiledOp.  op_type values used here:
     Conv2dRequantReluI8Nhwc (fused conv), AddQuantized, MaxPool, Concat, Split,
     Resize, QuantizeU8, Dequantize, YoloDetect (the Detect head's tail),
-    YoloPostprocess (postprocess_yolo), and the fp16 ops."""
+    YoloPostprocess (postprocess_yolo), the fp16 ops, and the 4-bit block's:
+    NormResidual, QuantizeMxfp4, DequantizeMxfp4 and GemmMxfp4 (an MXFP4 operand is a pair of
+    u8 tensors, codes and scales)."""
 
     name: str
     op_type: str
@@ -84,7 +86,7 @@ class Graph:
                 d = conv_desc_of(self, op)
                 ho, wo = d.out_hw()
                 total += 2 * d.n * ho * wo * d.c_out * d.k_h * d.k_w * (d.c_in if d.group == 1 else 1)
-            elif op.op_type == "GemmF16":
+            elif op.op_type in ("GemmF16", "GemmMxfp4"):
                 total += 2 * op.params["m"] * op.params["n"] * op.params["k"]
         return total
 
@@ -339,6 +341,69 @@ class F16GraphBuilder:
         g.initializers[name + "_b"] = self._f16(bias)
         g.ops.append(CompiledOp(name, "GemmF16", [x, name + "_w", name + "_b"], [y], {"m": m, "n": n_out, "k": k}))
         return y
+
+    # ---- 4-bit transformer blocks: f16 tensors [rows, c], MXFP4 operands as (codes, scales)
+    def input_f16(self, name, shape):
+        self.g.add_tensor(name, shape, "f16")
+        self.g.inputs.append(name)
+        return name
+
+    def _operand(self, name, rows, k):
+        """The two tensors of an MXFP4 operand [rows, k]."""
+        nb = -(-k // 32)
+        return (self.g.add_tensor(name + "_q", (rows, nb * 16), "u8"),
+                self.g.add_tensor(name + "_s", (-(-rows // 128) * -(-nb // 4) * 512,), "u8"))
+
+    def quantize_mxfp4(self, x, name=None):
+        name = name or self._name("quantize")
+        rows, k = self.g.tensors[x].shape
+        q, s = self._operand(name, rows, k)
+        self.g.ops.append(CompiledOp(name, "QuantizeMxfp4", [x], [q, s], {"rows": rows, "k": k}))
+        return q, s
+
+    def dequantize_mxfp4(self, a, rows, k, name=None):
+        name = name or self._name("dequantize")
+        y = self.g.add_tensor(name + "_out", (rows, k), "f16")
+        self.g.ops.append(CompiledOp(name, "DequantizeMxfp4", list(a), [y], {"rows": rows, "k": k}))
+        return y
+
+    def gemm_mxfp4(self, a, m, k, n_out, act=L.EPI_NONE, quantized=False, name=None):
+        """act(A @ W^T + bias) with a random MXFP4 weight [n_out, k]: f16, or `quantized` an operand again."""
+        g = self.g
+        name = name or self._name("gemm4")
+        w = self.rng.normal(0.0, np.sqrt(1.0 / k), (n_out, k)).astype(np.float32)
+        g.initializers[name + "_wq"], g.initializers[name + "_ws"] = Q.mxfp4_operand(w)
+        g.initializers[name + "_b"] = self.rng.normal(0.0, 0.05, n_out).astype(np.float32)
+        out = self._operand(name, m, n_out) if quantized else (g.add_tensor(name + "_out", (m, n_out), "f16"),)
+        g.ops.append(CompiledOp(name, "GemmMxfp4", list(a) + [name + "_wq", name + "_ws", name + "_b"], list(out),
+                                {"m": m, "n": n_out, "k": k, "act": act}))
+        return out if quantized else out[0]
+
+    def norm_residual(self, x, residual, post=L.NORM_NONE, pre=L.NORM_RMS, quantized=False, eps=1e-5, res_scale=1.0,
+                      name=None):
+        """out = residual + res_scale * post(x); y = pre(out), f16 or `quantized` an operand: (out, y).
+        Without a residual out is None and y = pre(x)."""
+        g = self.g
+        name = name or self._name("norm")
+        rows, c = g.tensors[x].shape
+        ws = []
+        for tag, kind in (("_wpost", post if residual else L.NORM_NONE), ("_wpre", pre)):
+            if kind != L.NORM_NONE:
+                g.initializers[name + tag] = self.rng.normal(1.0, 0.1, c).astype(np.float32)
+            ws.append(name + tag if kind != L.NORM_NONE else "")
+        out = g.add_tensor(name + "_out", (rows, c), "f16") if residual else None
+        y = self._operand(name, rows, c) if quantized else (g.add_tensor(name + "_y", (rows, c), "f16"),)
+        g.ops.append(CompiledOp(name, "NormResidual", [x, residual or ""] + ws, ([out] if out else []) + list(y),
+                                {"rows": rows, "c": c, "post": post, "pre": pre, "eps": eps, "res_scale": res_scale}))
+        return out, (y if quantized else y[0])
+
+    def mlp_mxfp4(self, x, residual, f, post=L.NORM_NONE):
+        """A feed-forward block: x (the branch before) joins the residual, is normalised and quantised, and
+        goes through up (c -> f, SiLU, quantised again) and down (f -> c): (branch, residual)."""
+        rows, c = self.g.tensors[x].shape
+        residual, a = self.norm_residual(x, residual, post, quantized=True)
+        h = self.gemm_mxfp4(a, rows, c, f, act=L.EPI_SILU, quantized=True)
+        return self.gemm_mxfp4(h, rows, f, c), residual
 
     def output_f32(self, x, name):
         g = self.g
@@ -1286,6 +1351,37 @@ class CudaGraphRuntime:
             wp = self._cached(wn + "_prep", lambda: ops.prepare_gemm_b_f16(be, consts[wn], k, n))
             bx, bb, y = bufs[x], consts[bn], bufs[op.outputs[0]]
             return lambda: ops.gemm_f16_bias(be, bx, wp, bb, y, m, n, k)
+        # ---- 4-bit transformer blocks
+        if t == "QuantizeMxfp4":
+            x, q, s = bufs[op.inputs[0]], bufs[op.outputs[0]], bufs[op.outputs[1]]
+            rows, k = op.params["rows"], op.params["k"]
+            return lambda: ops.quantize_mxfp4(be, x, ops.F16, rows, k, q, s)
+        if t == "DequantizeMxfp4":
+            q, s, y = bufs[op.inputs[0]], bufs[op.inputs[1]], bufs[op.outputs[0]]
+            rows, k = op.params["rows"], op.params["k"]
+            return lambda: ops.dequantize_mxfp4(be, q, s, rows, k, y, ops.F16)
+        if t == "GemmMxfp4":
+            m, n, k, act = (op.params[v] for v in ("m", "n", "k", "act"))
+            aq, as_ = bufs[op.inputs[0]], bufs[op.inputs[1]]
+            wq, ws, bias = (consts[v] for v in op.inputs[2:])
+            if len(op.outputs) == 2:
+                yq, ys = bufs[op.outputs[0]], bufs[op.outputs[1]]
+                return lambda: ops.gemm_to_mxfp4(be, aq, as_, wq, ws, bias, yq, ys, m, n, k, act)
+            y = bufs[op.outputs[0]]
+            return lambda: ops.gemm_mxfp4(be, aq, as_, wq, ws, bias, y, ops.F16, m, n, k, act)
+        if t == "NormResidual":
+            pr = op.params
+            desc = ops.NormDesc(pr["rows"], pr["c"], ops.F16, ops.F16, ops.F16, pr["pre"], pr["post"], pr["eps"],
+                                res_scale=pr["res_scale"])
+            x, w0, w1 = bufs[op.inputs[0]], consts.get(op.inputs[2]), consts.get(op.inputs[3])
+            if not op.inputs[1]:
+                y = [bufs[o] for o in op.outputs]
+                fn = ops.norm_to_mxfp4 if len(y) == 2 else ops.norm
+                return lambda: fn(be, desc, x, w1, None, *y)
+            r, out = bufs[op.inputs[1]], bufs[op.outputs[0]]
+            y = [bufs[o] for o in op.outputs[1:]]
+            fn = ops.norm_residual_to_mxfp4 if len(y) == 2 else ops.norm_residual
+            return lambda: fn(be, desc, x, w0, None, None, r, out, w1, None, *y)
         if t == "CastF16ToF32":
             x, y = bufs[op.inputs[0]], bufs[op.outputs[0]]
             return lambda: ops.cast_f16_to_f32(be, x, y)

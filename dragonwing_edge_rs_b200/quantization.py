@@ -57,3 +57,30 @@ def per_channel_symmetric(w_oc_first: np.ndarray):
     q = np.clip(q, np.float32(-128.0), np.float32(127.0))
     q = roundf_away(q).astype(np.int8)
     return q.reshape(w.shape), scales
+
+
+def mxfp4_operand(w: np.ndarray):
+    """w [rows, k] -> the code and scale buffers of an MXFP4 operand (format in
+    include/dw_cuda.h), on the host: for weights prepared once.  The same values
+    as dw_quantize_mxfp4 on the array as float32."""
+    w = np.asarray(w, np.float32)
+    rows, k = w.shape
+    nb = -(-k // 32)
+    v = np.zeros((rows, nb * 32), np.float32)
+    v[:, :k] = w
+    v = v.reshape(rows, nb, 32)
+    bad = ~np.isfinite(v).all(-1)
+    v = np.where(bad[..., None], np.float32(0), v)
+    amax = np.abs(v).max(-1)
+    e = np.maximum(np.where(amax > 0, np.frexp(amax)[1] - 3, -127), -127)
+    u = np.abs(v) * np.ldexp(np.float32(1), -e)[..., None]  # exact: a power of two
+    # ties go to the even index: up from an odd one (>=), down from an even one (>)
+    index = np.zeros(u.shape, np.uint8)
+    for i, mid in enumerate((0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)):
+        index += (u >= mid) if i % 2 else (u > mid)
+    code = np.where(bad[..., None], 0, index + 8 * np.signbit(v)).astype(np.uint8).reshape(rows, -1)
+    tiles = -(-nb // 4)
+    scales = np.zeros((rows + -rows % 128, tiles * 4), np.uint8)
+    scales[:rows, :nb] = np.where(bad, 255, e + 127)
+    tiled = scales.reshape(-1, 4, 32, tiles, 4).transpose(0, 3, 2, 1, 4)
+    return (code[:, 0::2] | (code[:, 1::2] << 4)).reshape(-1), np.ascontiguousarray(tiled).reshape(-1)
