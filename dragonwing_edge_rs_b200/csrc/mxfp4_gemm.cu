@@ -398,13 +398,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     tc_fence_before();
     cluster_sync();
     tc_fence_after();
+    pdl_wait();  // in every warp: the bounded waits count from here
+    pdl_trigger();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const uint32_t sf_cols = tmem + 256;  // scales after the accumulators
     float *partial = reinterpret_cast<float *>(smem_raw + (smem - smem_u32(smem_raw)));  // [BN][128]
 
     if (warp == 0) {
-        pdl_wait();  // (the other warps wait where they first touch global memory)
-        pdl_trigger();
         const uint32_t elected = elect_one();
         int s = 0, issued = 0;
         uint32_t ph = 0;
@@ -509,7 +509,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         tc_commit2(elected, smem_u32(&drain_bar[0]));
         drain_phase(smem_u32(&drain_bar[0]), 0, p.wait_cap_ns);
     } else if (warp >= 4) {
-        pdl_wait();
         const int quarter = warp & 3;  // tensor-memory lanes this warp may read
         const int part = (warp - 4) >> 2;
         int acc = 0;
@@ -663,13 +662,13 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_wait();  // in every warp: the bounded waits count from here
+    pdl_trigger();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
     const uint32_t sf_cols = tmem + (uint32_t)p.bn;  // 16 columns a stage after the accumulators
     const uint64_t hi = ((uint64_t)((8 * kBKBytes) >> 4) << 32) | (1ull << 46) | (2ull << 61);
 
     if (warp == 0) {
-        pdl_wait();  // (the other warps wait where they first touch global memory)
-        pdl_trigger();
         const uint32_t elected = elect_one();
         int s = 0, issued = 0;
         uint32_t ph = 0;
@@ -766,7 +765,6 @@ __global__ void __launch_bounds__(kSkinnyThreads)
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
     }
-    pdl_wait();
     if (*abort_flag == 0) {
         // a warp takes a row of A, a lane four neighbouring outputs
         const size_t col = n0 + 4 * lane;
@@ -862,7 +860,7 @@ dw_status launch(dw_backend *be, const MxGemmArgs &a, int S) {
     p.out_nb = mx_blocks(a.n), p.out_tiles = mx_tiles(a.n);
     p.k_blocks = (int)((a.k + 511) / 512);
     const size_t tm = (a.m + 2 * kBM - 1) / (2 * kBM), tn = (a.n + BN - 1) / BN;
-    if (tm * tn > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu x %zu is too large", a.m, a.n);
+    if (tm * tn > 0x7fff0000u) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu x %zu is too large", a.m, a.n);
     p.tiles_m = (int)tm, p.tiles = (int)(tm * tn);
     p.act = a.act;
     const size_t es = kOut == 0 ? 4 : 2;
@@ -909,7 +907,6 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
     p.tmem_cols = 256;
     p.wait_cap_ns = be->wait_cap_ns, p.err = be->dev_err;
     const size_t tn = (a.n + 127) / 128;
-    if (tn > 65535) return dw_fail(be, DW_ERR_UNSUPPORTED, "gemm_mxfp4: %zu outputs are too many", a.n);
     // CTAs that share a tile's K: about one an SM (4096 outputs, K 4096, one row: S = 1, 2,
     // 4, 8 took 5.5, 4.4, 4.2, 4.6 us; 11008 outputs S = 1, 2, 4: 6.2, 6.2, 8.1), each with
     // a K block at least; clusters of 8 CTAs that fill an SM each do not fit 16 at a time
@@ -947,7 +944,8 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
 //     10.4 against 11.0; with k 4096 7.8 against 6.6).
 dw_status launch_gemm_mxfp4(dw_backend *be, const MxGemmArgs &a) {
     const size_t pairs = (size_t)be->sm_count / 2, rows = (a.m + 255) / 256, k_blocks = (a.k + 511) / 512;
-    if (a.m <= 64 || (a.m <= 128 && a.n <= 4096 && a.k > 4096) || (a.m <= 128 && a.n <= 1024 && a.k >= 2048))
+    const bool few = a.n <= 65535ull * 128;  // outputs that the few-rows grid holds
+    if (few && (a.m <= 64 || (a.m <= 128 && a.n <= 4096 && a.k > 4096) || (a.m <= 128 && a.n <= 1024 && a.k >= 2048)))
         return launch_skinny(be, a);
     const bool wide = rows * ((a.n + 255) / 256) >= pairs;
     const int S = !wide && rows * ((a.n + 127) / 128) <= pairs / 2 - 1 && k_blocks >= 16 ? 2 : 1;
