@@ -29,7 +29,8 @@ struct Params {
     const float *w0, *b0, *w1, *b1;
     void *out, *y;
     uint8_t *q, *s;
-    size_t rows, c, x_pitch, res_pitch, y_pitch, gate_rows, nb, tiles;
+    size_t rows, c, x_pitch, res_pitch, y_pitch, nb, tiles;
+    uint32_t gate_rows;
     int pre, post, y_dtype;  // y_dtype: DW_F32..DW_BF16, -1: none, -2: MXFP4
     float eps, inv_c, res_scale;
     bool has_res;
@@ -38,7 +39,8 @@ struct Params {
 // Sum over the T threads of a row (a power of two; rows of T <= 32 lie in one warp,
 // longer ones take whole warps, and all threads of the block call together).
 // `slot` alternates over four buffers, so a buffer is written again only after
-// three more barriers.
+// three more barriers.  kBar: the threads that call, where these are not the whole block.
+template <int kBar = 0>
 __device__ __forceinline__ float row_sum(float v, int T, float (*red)[16], int &slot) {
 #pragma unroll
     for (int o = 16; o; o >>= 1)
@@ -47,7 +49,10 @@ __device__ __forceinline__ float row_sum(float v, int T, float (*red)[16], int &
     const int thread = threadIdx.y * blockDim.x + threadIdx.x, lane = thread & 31, warp = thread >> 5;
     const int warps = T >> 5, first = warp & ~(warps - 1);
     if (lane == 0) red[slot][warp] = v;
-    __syncthreads();
+    if (kBar)
+        named_barrier_sync(1, kBar);
+    else
+        __syncthreads();
     const float *part = &red[slot][first];  // every thread adds the warps' sums, in the same order
     v = part[0] + part[1];
     if (T >= 128) v += part[2] + part[3];
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(kMaxT, V * N <= 8 ? 2 : 1) k_norm(const __grid
         bool live[N];
         const X *x = (const X *)p.x + row * p.x_pitch;
         const R *res = (const R *)p.res + row * p.res_pitch;
-        const X *gate = (const X *)p.gate + (p.gate_rows ? row / p.gate_rows : 0) * p.c;
+        const X *gate = (const X *)p.gate + (size_t)(p.gate_rows ? (uint32_t)row / p.gate_rows : 0) * p.c;
 #pragma unroll
         for (int j = 0; j < N; j++) {
             const size_t at = ((size_t)j * T + tid) * V;
@@ -226,77 +231,174 @@ __global__ void __launch_bounds__(kMaxT, V * N <= 8 ? 2 : 1) k_norm(const __grid
     }
 }
 
-// Many rows: persistent thread blocks fed by bulk copies.  A step is G = threads / T
-// rows; a ring of stages holds the x and residual rows of the steps to come, so the
-// loads in flight do not depend on how many rows the registers hold, and the
-// weights and a shared gate row of a thread's columns stay in registers.
+// Many rows: persistent thread blocks fed by bulk copies, which a warp of its own
+// issues (kThreads others compute).  A step is G = kThreads / T rows; a ring of stages holds the x, residual and gate rows of the steps to come, so
+// the loads in flight do not depend on how many rows the registers hold.  Bulk copies
+// move whole 16-byte pieces: a row that starts or ends inside one is copied with its
+// surroundings (its neighbours' elements), except where that would leave the tensor.
 constexpr int kStreamStages = 8;
+
+// Bytes of a stage: per tensor G rows, one after the other as in memory (`packed`: one
+// copy), or each in a place of its own.
+struct StreamRows {
+    uint32_t bytes, stride, region;
+    __host__ __device__ StreamRows(size_t c, size_t es, int G, bool packed, bool present)
+        : bytes(present ? (uint32_t)(c * es) : 0u),
+          stride(!present ? 0u : packed ? bytes : (bytes + 31) & ~15u),
+          region(!present ? 0u : (G * stride + 31) & ~15u) {}
+};
+
+// The part of [src, src + bytes) that bulk copies bring, with what surrounds it.
+struct Span {
+    uintptr_t from, to, base;  // base: the 16-byte piece of src
+    __device__ __forceinline__ Span(const uint8_t *src, uint32_t bytes, const uint8_t *first, const uint8_t *last) {
+        const uintptr_t a = (uintptr_t)src, e = a + bytes;
+        base = a & ~(uintptr_t)15;
+        from = base < (uintptr_t)first ? base + 16 : base;
+        to = (e + 15) & ~(uintptr_t)15;
+        if (to > (uintptr_t)last) to -= 16;
+        if (to < from) to = from;
+    }
+    __device__ __forceinline__ uint32_t bytes() const { return (uint32_t)(to - from); }
+    // The bytes at the tensor's ends that it leaves out (fewer than 16 at each).
+    __device__ __forceinline__ void edges(uint8_t *dst, const uint8_t *src, uint32_t bytes) const {
+        const uintptr_t a = (uintptr_t)src, e = a + bytes;
+        for (uintptr_t q = a; q < e && q < from; q++) dst[q - base] = *(const uint8_t *)q;
+        for (uintptr_t q = to > a ? to : a; q < e; q++) dst[q - base] = *(const uint8_t *)q;
+    }
+};
+
 // Blocks an SM: three where 80 registers a thread and the ring allow it.
-template <typename R, int N, int kThreads>
+template <typename R, int V, int N, int kThreads>
 constexpr int stream_blocks() {
-    return kThreads > 256 ? 1 : N > 1 && sizeof(R) == 4 ? 2 : 3;
+    return kThreads > 256 ? 1 : V * N > 8 && (V < 8 || sizeof(R) == 4) ? 2 : 3;
 }
 
-template <typename X, typename R, int N, int kThreads, bool kFull>
-__global__ void __launch_bounds__(kThreads, stream_blocks<R, N, kThreads>())
+template <typename X, typename R, int V, int N, int kThreads, bool kFull>
+__global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads>())
     k_norm_stream(const __grid_constant__ Params p, const int T, const int stages, uint64_t wait_cap_ns, int32_t *err) {
-    constexpr int V = 8;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(16) float red[4][16];
-    __shared__ uint64_t full_bar[kStreamStages];
+    __shared__ uint64_t full_bar[kStreamStages], empty_bar[kStreamStages];
     __shared__ int abort_word;
+    volatile int *abort_flag = &abort_word;
     int slot = 0;
+    const int lane = threadIdx.x & 31;
     const int G = kThreads / T, g = threadIdx.x / T, tid = threadIdx.x & (T - 1);
     const size_t steps = (p.rows + G - 1) / G;
-    const uint32_t x_bytes = (uint32_t)(p.c * sizeof(X)), r_bytes = p.has_res ? (uint32_t)(p.c * sizeof(R)) : 0u;
     // a gate row of the rows themselves comes with them
-    const bool row_gate = p.gate && p.gate_rows;
-    const uint32_t g_bytes = row_gate ? x_bytes : 0u, row_bytes = x_bytes + r_bytes + g_bytes, stage_bytes = G * row_bytes;
+    const bool row_gate = p.gate && p.gate_rows, packed_x = p.x_pitch == p.c, packed_r = p.res_pitch == p.c;
+    const StreamRows lx(p.c, sizeof(X), G, packed_x, true), lr(p.c, sizeof(R), G, packed_r, p.has_res),
+        lg(p.c, sizeof(X), G, false, row_gate);
+    const uint32_t stage_bytes = lx.region + lr.region + lg.region;
     const uint32_t base = smem_u32(ring);
+    const uint8_t *const x0 = (const uint8_t *)p.x, *const r0 = (const uint8_t *)p.res, *const g0 = (const uint8_t *)p.gate;
+    const size_t x_pitch = p.x_pitch * sizeof(X), r_pitch = p.res_pitch * sizeof(R);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < stages; s++) mbar_init(smem_u32(&full_bar[s]), 1);
+        for (int s = 0; s < stages; s++) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), kThreads / 32);
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     __syncthreads();
-    auto fetch = [&](size_t step, int s) {
-        const size_t row0 = step * G;
-        const uint32_t rows = (uint32_t)min((size_t)G, p.rows - row0), bar = smem_u32(&full_bar[s]);
-        const uint32_t dx = base + s * stage_bytes, dr = dx + G * x_bytes, dg = dr + G * r_bytes;
-        mbar_expect_tx(bar, rows * row_bytes);
-        auto copy = [&](uint32_t dst, const uint8_t *src, size_t pitch, uint32_t bytes) {
-            if (pitch == bytes) {
-                bulk_load(dst, src + row0 * pitch, rows * bytes, bar);
-            } else {
-                for (uint32_t r = 0; r < rows; r++) bulk_load(dst + r * bytes, src + (row0 + r) * pitch, bytes, bar);
+    // Waits for a phase; after an expired wait nothing waits any more and what is left runs
+    // through on what the ring holds.
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (mbar_try_wait(smem_u32(bar), parity)) return;
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait_sleep(smem_u32(bar), parity, 20000u) && !*abort_flag)
+            if (globaltimer_ns() - t0 > wait_cap_ns) {
+                *abort_flag = 1;
+                record_error(err, DW_DEV_WAIT_EXPIRED, 41, (int)parity);
             }
-        };
-        copy(dx, (const uint8_t *)p.x, p.x_pitch * sizeof(X), x_bytes);
-        if (p.has_res) copy(dr, (const uint8_t *)p.res, p.res_pitch * sizeof(R), r_bytes);
-        if (row_gate)
-            for (uint32_t r = 0; r < rows; r++)
-                bulk_load(dg + r * x_bytes, (const X *)p.gate + (row0 + r) / p.gate_rows * p.c, x_bytes, bar);
     };
     pdl_wait();
     pdl_trigger();
-    if (threadIdx.x == 0) {
-        size_t step = blockIdx.x;
-        for (int s = 0; s < stages && step < steps; s++, step += gridDim.x) fetch(step, s);
+    if (threadIdx.x >= kThreads) {
+        int s = 0, issued = 0;
+        uint32_t ph = 0;
+        for (size_t step = blockIdx.x; step < steps && !*abort_flag; step += gridDim.x) {
+            if (issued >= stages) wait(&empty_bar[s], ph ^ 1u);
+            __syncwarp();
+            if (__any_sync(0xffffffffu, *abort_flag)) break;
+            const size_t row0 = step * G;
+            const uint32_t rows = (uint32_t)min((size_t)G, p.rows - row0), bar = smem_u32(&full_bar[s]);
+            // the copies of the step, each to one lane
+            auto copies = [&](auto each) {
+                auto tensor = [&](const StreamRows &l, const uint8_t *t, size_t pitch, bool packed, uint32_t at, int first_lane) {
+                    const uint8_t *last = t + (p.rows - 1) * pitch + l.bytes;
+                    if (packed) {
+                        if (lane == first_lane) each(t + row0 * pitch, rows * l.bytes, t, last, at);
+                    } else {
+                        for (uint32_t r = lane; r < rows; r += 32) each(t + (row0 + r) * pitch, l.bytes, t, last, at + r * l.stride);
+                    }
+                };
+                tensor(lx, x0, x_pitch, packed_x, s * stage_bytes, 0);
+                if (p.has_res) tensor(lr, r0, r_pitch, packed_r, s * stage_bytes + lx.region, 1);
+                if (row_gate) {
+                    const uint8_t *last = g0 + (size_t)((uint32_t)(p.rows - 1) / p.gate_rows + 1) * lg.bytes;
+                    for (uint32_t r = lane; r < rows; r += 32)
+                        each(g0 + (size_t)((uint32_t)(row0 + r) / p.gate_rows) * lg.bytes, lg.bytes, g0, last,
+                             s * stage_bytes + lx.region + lr.region + r * lg.stride);
+                }
+            };
+            if constexpr (V == 8) {  // whole pieces
+                if (lane == 0) mbar_expect_tx(bar, rows * (lx.bytes + lr.bytes + lg.bytes));
+                __syncwarp();
+                copies([&](const uint8_t *src, uint32_t n, const uint8_t *, const uint8_t *, uint32_t at) {
+                    bulk_load(base + at, src, n, bar);
+                });
+            } else {
+                uint32_t bytes = 0;
+                copies([&](const uint8_t *src, uint32_t n, const uint8_t *first, const uint8_t *last, uint32_t at) {
+                    const Span span(src, n, first, last);
+                    bytes += span.bytes();
+                    span.edges(ring + at, src, n);
+                });
+                bytes = __reduce_add_sync(0xffffffffu, bytes);
+                if (lane == 0) mbar_expect_tx(bar, bytes);
+                __syncwarp();
+                copies([&](const uint8_t *src, uint32_t n, const uint8_t *first, const uint8_t *last, uint32_t at) {
+                    const Span span(src, n, first, last);
+                    if (span.bytes()) bulk_load(base + at + (uint32_t)(span.from - span.base), (const void *)span.from, span.bytes(), bar);
+                });
+            }
+            issued++;
+            if (++s == stages) s = 0, ph ^= 1;
+        }
+        // the last copies into each stage have landed before the block ends
+        for (int i = 0; i < min(issued, stages); i++) {
+            if (--s < 0) s = stages - 1, ph ^= 1;
+            const uint64_t t0 = globaltimer_ns();
+            while (!mbar_try_wait_sleep(smem_u32(&full_bar[s]), ph, 20000u) && globaltimer_ns() - t0 < wait_cap_ns) {
+            }
+        }
+        return;
     }
     // c0: what the normalised x of a column is multiplied by (weight, residual scale and,
-    // where all rows share it, the gate); w1: the weight of the next norm
-    // (both in shared memory, 16 bytes of a thread beside its neighbour's: registers go to
-    // a third block on the SM instead)
-    float4 *c0 = reinterpret_cast<float4 *>(ring + (size_t)stages * stage_bytes), *w1 = c0 + 2 * N * T;
+    // where all rows share it, the gate); w1: the weight of the next norm (both in shared
+    // memory, 16 bytes of a thread beside its neighbour's: registers go to a third block
+    // on the SM instead)
+    float *c0 = reinterpret_cast<float *>(ring + (size_t)stages * stage_bytes), *w1 = c0 + N * T * V;
     bool live[N];
     auto column = [&](int j) { return (uint32_t)(j * T + tid) * V; };
-    auto kept = [&](const float4 *from, int j, float (&t)[V]) {
-        const float4 a = from[2 * j * T + tid], b = from[(2 * j + 1) * T + tid];
-        t[0] = a.x, t[1] = a.y, t[2] = a.z, t[3] = a.w, t[4] = b.x, t[5] = b.y, t[6] = b.z, t[7] = b.w;
+    auto kept = [&](const float *from, int j, float (&t)[V]) {
+        if constexpr (V == 8) {
+            const float4 *f = reinterpret_cast<const float4 *>(from);
+            const float4 a = f[2 * j * T + tid], b = f[(2 * j + 1) * T + tid];
+            t[0] = a.x, t[1] = a.y, t[2] = a.z, t[3] = a.w, t[4] = b.x, t[5] = b.y, t[6] = b.z, t[7] = b.w;
+        } else {
+            load_f32<V>(from + column(j), t);
+        }
     };
-    auto keep = [&](float4 *to, int j, const float (&t)[V]) {
-        to[2 * j * T + tid] = make_float4(t[0], t[1], t[2], t[3]), to[(2 * j + 1) * T + tid] = make_float4(t[4], t[5], t[6], t[7]);
+    auto keep = [&](float *to, int j, const float (&t)[V]) {
+        if constexpr (V == 8) {
+            float4 *f = reinterpret_cast<float4 *>(to);
+            f[2 * j * T + tid] = make_float4(t[0], t[1], t[2], t[3]), f[(2 * j + 1) * T + tid] = make_float4(t[4], t[5], t[6], t[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++) to[column(j) + i] = t[i];
+        }
     };
 #pragma unroll
     for (int j = 0; j < N; j++) {
@@ -325,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, stream_blocks<R, N, kThreads>())
         if (p.w1) load_f32<V>(p.w1 + column(j), t);
         keep(w1, j, t);
     }
-    __syncthreads();
+    named_barrier_sync(1, kThreads);
     // (mean, 1 / root) of v over the row; elements past the row are 0
     auto statistics = [&](float (&v)[N][V], int kind) {
         if (kind == DW_NORM_LAYER) {
@@ -334,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, stream_blocks<R, N, kThreads>())
             for (int j = 0; j < N; j++)
 #pragma unroll
                 for (int i = 0; i < V; i++) sum += v[j][i];
-            const float mean = row_sum(sum, T, red, slot) * p.inv_c;
+            const float mean = row_sum<kThreads>(sum, T, red, slot) * p.inv_c;
 #pragma unroll
             for (int j = 0; j < N; j++)
 #pragma unroll
@@ -345,49 +447,46 @@ __global__ void __launch_bounds__(kThreads, stream_blocks<R, N, kThreads>())
         for (int j = 0; j < N; j++)
 #pragma unroll
             for (int i = 0; i < V; i++) sq = fmaf(v[j][i], v[j][i], sq);
-        return __frsqrt_rn(fmaf(row_sum(sq, T, red, slot), p.inv_c, p.eps));
+        return __frsqrt_rn(fmaf(row_sum<kThreads>(sq, T, red, slot), p.inv_c, p.eps));
     };
     int s = 0;
     uint32_t ph = 0;
     size_t step = blockIdx.x;
     for (; step < steps; step += gridDim.x) {
-        if (!mbar_try_wait(smem_u32(&full_bar[s]), ph)) {
-            const uint64_t t0 = globaltimer_ns();
-            while (!mbar_try_wait_sleep(smem_u32(&full_bar[s]), ph, 20000u))
-                if (globaltimer_ns() - t0 > wait_cap_ns) {
-                    abort_word = 1;
-                    record_error(err, DW_DEV_WAIT_EXPIRED, 41, (int)ph);
-                    break;
-                }
-        }
+        wait(&full_bar[s], ph);
+        const size_t row = step * G + g, row0 = packed_x ? step * G : row, rrow0 = packed_r ? step * G : row;
+        const bool there = row < p.rows;
         // rows of the last step past the end hold what the stage held: they stay in
         // their own threads and nothing of them is stored
-        Raw<X, V> xr[N], gr[N];
-        Raw<R, V> rr[N];
-        const X *xs = reinterpret_cast<const X *>(ring + s * stage_bytes + g * x_bytes);
-        const R *rs = reinterpret_cast<const R *>(ring + s * stage_bytes + G * x_bytes + g * r_bytes);
-        const X *gs = reinterpret_cast<const X *>(ring + s * stage_bytes + G * (x_bytes + r_bytes) + g * x_bytes);
+        const uint8_t *stage = ring + s * stage_bytes;
+        const X *xs = reinterpret_cast<const X *>(stage + g * lx.stride + (((uintptr_t)x0 + row0 * x_pitch) & 15));
+        const R *rs = reinterpret_cast<const R *>(stage + lx.region + g * lr.stride + (((uintptr_t)r0 + rrow0 * r_pitch) & 15));
+        const X *gs = reinterpret_cast<const X *>(stage + lx.region + lr.region + g * lg.stride +
+                                                  (((uintptr_t)g0 + (size_t)(row_gate ? (uint32_t)row / p.gate_rows : 0) * lx.bytes) & 15));
+        auto release = [&]() {  // the warp has read the stage
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
+            if (++s == stages) s = 0, ph ^= 1;
+        };
+        float v[N][V];
+        // 16-byte accesses: the residual and gate rows go to registers too and the stage is
+        // free at once; shorter ones: they are read where they are used
+        Raw<R, V> rr[V == 8 ? N : 1];
+        Raw<X, V> gr[V == 8 ? N : 1];
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            if (!kFull) xr[j].zero(), rr[j].zero();
+            Raw<X, V> xr;
+            xr.zero();
+            if (V == 8 && !kFull) rr[V == 8 ? j : 0].zero();
             if (live[j]) {
-                xr[j].load(xs + column(j));
-                if (p.has_res) rr[j].load(rs + column(j));
-                if (row_gate) gr[j].load(gs + column(j));
+                xr.load(xs + column(j));
+                if (V == 8 && p.has_res) rr[V == 8 ? j : 0].load(rs + column(j));
+                if (V == 8 && row_gate) gr[V == 8 ? j : 0].load(gs + column(j));
             }
+#pragma unroll
+            for (int i = 0; i < V; i++) v[j][i] = xr.get(i);
         }
-        __syncthreads();  // the stage has been read
-        if (abort_word) break;
-        if (threadIdx.x == 0 && step + (size_t)stages * gridDim.x < steps) fetch(step + (size_t)stages * gridDim.x, s);
-        if (++s == stages) s = 0, ph ^= 1;
-
-        const size_t row = step * G + g;
-        const bool there = row < p.rows;
-        float v[N][V];
-#pragma unroll
-        for (int j = 0; j < N; j++)
-#pragma unroll
-            for (int i = 0; i < V; i++) v[j][i] = xr[j].get(i);
+        if (V == 8 || !p.has_res) release();
         if (p.has_res) {
             const float rstd = p.post != DW_NORM_NONE ? statistics(v, p.post) : 1.0f;
             R *out = (R *)p.out + row * p.res_pitch;
@@ -400,8 +499,10 @@ __global__ void __launch_bounds__(kThreads, stream_blocks<R, N, kThreads>())
                     float o[V], t[V];
                     kept(c0, j, t);
                     coefficient(j, t);
+                    Raw<R, V> res = rr[V == 8 ? j : 0];
+                    if constexpr (V < 8) res.load(rs + column(j));
 #pragma unroll
-                    for (int i = 0; i < V; i++) o[i] = fmaf(v[j][i] * rstd, t[i], rr[j].get(i));
+                    for (int i = 0; i < V; i++) o[i] = fmaf(v[j][i] * rstd, t[i], res.get(i));
                     bias(j, o);
                     Raw<R, V> r;
                     r.set(o);
@@ -417,20 +518,24 @@ __global__ void __launch_bounds__(kThreads, stream_blocks<R, N, kThreads>())
                 join(
                     [&](int j, float (&t)[V]) {
                         if (!row_gate) return;
+                        Raw<X, V> g = gr[V == 8 ? j : 0];
+                        if constexpr (V < 8) g.load(gs + column(j));
 #pragma unroll
-                        for (int i = 0; i < V; i++) t[i] *= gr[j].get(i);
+                        for (int i = 0; i < V; i++) t[i] *= g.get(i);
                     },
                     [&](int j, float (&o)[V]) {  // + res_scale * gate * b
                         if (!p.b0 || p.post == DW_NORM_NONE) return;
                         float b[V];
                         load_f32<V>(p.b0 + column(j), b);
-                        Raw<X, V> g = gr[j];
+                        Raw<X, V> g = gr[V == 8 ? j : 0];
+                        if (V < 8 && row_gate) g.load(gs + column(j));
                         if (p.gate && !row_gate) g.load((const X *)p.gate + column(j));
 #pragma unroll
                         for (int i = 0; i < V; i++) o[i] = fmaf(b[i], p.gate ? p.res_scale * g.get(i) : p.res_scale, o[i]);
                     });
             }
         }
+        if (V < 8 && p.has_res) release();
         if (p.y_dtype == -1) continue;
         if (p.pre != DW_NORM_NONE) {
             const float rstd = statistics(v, p.pre);
@@ -471,15 +576,6 @@ __global__ void __launch_bounds__(kThreads, stream_blocks<R, N, kThreads>())
                 store((__nv_bfloat16 *)p.y);
         }
     }
-    // after an expired wait: the copies still in flight land before the block ends
-    if (threadIdx.x == 0 && step < steps) {
-        for (int i = 0; i < stages && step < steps; i++, step += gridDim.x) {
-            const uint64_t t0 = globaltimer_ns();
-            while (!mbar_try_wait_sleep(smem_u32(&full_bar[s]), ph, 20000u) && globaltimer_ns() - t0 < wait_cap_ns) {
-            }
-            if (++s == stages) s = 0, ph ^= 1;
-        }
-    }
 }
 
 // Rows too long for registers: one thread block a row, elements read again for
@@ -492,7 +588,7 @@ __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Par
     const size_t T = blockDim.x, end = p.nb * 32;
     const X *x = (const X *)p.x + row * p.x_pitch;
     const R *res = (const R *)p.res + row * p.res_pitch;
-    const X *gate = (const X *)p.gate + (p.gate_rows ? row / p.gate_rows : 0) * p.c;
+    const X *gate = (const X *)p.gate + (size_t)(p.gate_rows ? (uint32_t)row / p.gate_rows : 0) * p.c;
     R *out = (R *)p.out + row * p.res_pitch;
     pdl_wait();
     pdl_trigger();
@@ -553,19 +649,25 @@ __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Par
     }
 }
 
-template <typename X, typename R, int N, int kThreads, bool kFull>
+template <typename X, typename R, int V, int N, int kThreads, bool kFull = false>
 bool stream_as(dw_backend *be, const Params &p, int T, dw_status *st) {
-    auto kernel = k_norm_stream<X, R, N, kThreads, kFull>;
-    const size_t G = kThreads / T, stage = G * p.c * (sizeof(X) * (p.gate && p.gate_rows ? 2 : 1) + (p.has_res ? sizeof(R) : 0));
-    const size_t weights = (size_t)T * N * 8 * 4 * 2;
+    auto kernel = k_norm_stream<X, R, V, N, kThreads, kFull>;
+    const int G = kThreads / T;
+    const size_t stage = StreamRows(p.c, sizeof(X), G, p.x_pitch == p.c, true).region +
+                         StreamRows(p.c, sizeof(R), G, p.res_pitch == p.c, p.has_res).region +
+                         StreamRows(p.c, sizeof(X), G, false, p.gate && p.gate_rows).region;
+    const size_t weights = (size_t)T * N * V * 4 * 2;
     // the most blocks an SM that have room for two steps each, or else for one
     auto fits = [&](size_t blocks) {
         const size_t room = kSmemBudget / blocks;
         return room < weights + stage ? 0 : (int)std::min<size_t>(kStreamStages, (room - weights) / stage);
     };
-    constexpr int kBlocks = stream_blocks<R, N, kThreads>();
+    constexpr int kBlocks = stream_blocks<R, V, N, kThreads>();
     const int per_sm = kBlocks == 3 && fits(3) >= 2 ? 3 : kBlocks >= 2 && fits(2) >= 1 ? 2 : 1, stages = fits(per_sm);
-    if (stages < 1) return false;
+    const size_t steps = (p.rows + G - 1) / (size_t)G;
+    // with fewer steps than that nothing is there to fetch ahead (1000 x 1010 f32, 250 steps:
+    // 9.0 against 6.8 us by a block a row)
+    if (stages < 1 || steps < (size_t)be->sm_count * 2) return false;
     static bool attr_set[16] = {};
     if (be->device < 16 && !attr_set[be->device]) {
         *st = dw_cuda_check(
@@ -573,22 +675,37 @@ bool stream_as(dw_backend *be, const Params &p, int T, dw_status *st) {
         if (*st != DW_OK) return true;
         attr_set[be->device] = true;
     }
-    const size_t steps = (p.rows + G - 1) / G;
     const unsigned grid = (unsigned)std::min<size_t>(steps, (size_t)be->sm_count * per_sm);
-    *st = launch_dependent(be, "norm", kernel, grid, kThreads, stages * stage + weights, 0, p, T, stages, be->wait_cap_ns, be->dev_err);
+    *st = launch_dependent(be, "norm", kernel, grid, kThreads + 32, stages * stage + weights, 0, p, T, stages, be->wait_cap_ns, be->dev_err);
     return true;
 }
 
-// Launches the streaming form; false where a row is too long for it.
+// Launches the streaming form with accesses of V elements; false where a row is too long
+// or the rows too few for it.
 template <typename X, typename R>
-bool stream(dw_backend *be, const Params &p, dw_status *st) {
-    int T = 8;
-    while ((size_t)T * (T < 32 ? 8 : 16) < p.c && T < 256) T *= 2;
-    if ((size_t)T * 8 >= p.c) return stream_as<X, R, 1, 256, false>(be, p, T, st);
-    if ((size_t)T * 16 == p.c) return stream_as<X, R, 2, 256, true>(be, p, T, st);
-    if ((size_t)T * 16 >= p.c) return stream_as<X, R, 2, 256, false>(be, p, T, st);
-    if ((size_t)512 * 16 >= p.c) return stream_as<X, R, 2, 512, false>(be, p, 512, st);
-    return stream_as<X, R, 4, 512, false>(be, p, 512, st);
+bool stream(dw_backend *be, const Params &p, int V, dw_status *st) {
+    if (V == 8) {
+        int T = 8;
+        while ((size_t)T * (T < 32 ? 8 : 16) < p.c && T < 256) T *= 2;
+        if ((size_t)T * 8 >= p.c) return stream_as<X, R, 8, 1, 256>(be, p, T, st);
+        if ((size_t)T * 16 == p.c) return stream_as<X, R, 8, 2, 256, true>(be, p, T, st);
+        if ((size_t)T * 16 >= p.c) return stream_as<X, R, 8, 2, 256>(be, p, T, st);
+        if ((size_t)512 * 16 >= p.c) return stream_as<X, R, 8, 2, 512>(be, p, 512, st);
+        return stream_as<X, R, 8, 4, 512>(be, p, 512, st);
+    }
+    // an MXFP4 block is 32 / V threads (the same split for every y: the same sums)
+    int T = 32 / V;
+    while ((size_t)T * 16 < p.c && T < 256) T *= 2;
+    if (V == 2) {
+        if (p.c <= 64) return stream_as<X, R, 2, 2, 256>(be, p, T, st);
+        if ((size_t)T * 16 >= p.c) return stream_as<X, R, 2, 8, 256>(be, p, T, st);
+        if ((size_t)512 * 16 >= p.c) return stream_as<X, R, 2, 8, 512>(be, p, 512, st);
+        return stream_as<X, R, 2, 16, 512>(be, p, 512, st);
+    }
+    if (p.c <= 128) return stream_as<X, R, 1, 4, 256>(be, p, T, st);
+    if ((size_t)T * 16 >= p.c) return stream_as<X, R, 1, 16, 256>(be, p, T, st);
+    if ((size_t)512 * 16 >= p.c) return stream_as<X, R, 1, 16, 512>(be, p, 512, st);
+    return stream_as<X, R, 1, 32, 512>(be, p, 512, st);
 }
 
 template <typename X, typename R>
@@ -610,7 +727,8 @@ dw_status run(dw_backend *be, const Params &p) {
         return launch_dependent(be, "norm (long rows)", k_norm_long<X, R>, (unsigned)p.rows, kMaxT, 0, 0, p);
     }
     dw_status st;
-    if (fits(8) && p.c <= (size_t)kMaxT * kMaxE && p.rows >= (size_t)be->sm_count * 2 && stream<X, R>(be, p, &st)) return st;
+    const int V = fits(8) ? 8 : fits(2) ? 2 : 1;
+    if (stream<X, R>(be, p, V, &st)) return st;
     // E: elements of a thread; T: threads of a row (a power of two from 32 to 512)
     int E = 8, T = 32;
     while ((size_t)T * E < p.c && T < kMaxT) T *= 2;
@@ -621,12 +739,12 @@ dw_status run(dw_backend *be, const Params &p) {
     auto go = [&](auto kernel) {
         return launch_dependent(be, "norm", kernel, (unsigned)blocks, block, 0, 0, p);
     };
-    if (fits(8)) {
+    if (V == 8) {
         if (E == 8) return go(k_norm<X, R, 8, 1>);
         if (E == 16) return go(k_norm<X, R, 8, 2>);
         return go(k_norm<X, R, 8, 4>);
     }
-    if (fits(2)) {
+    if (V == 2) {
         if (E == 8) return go(k_norm<X, R, 2, 4>);
         if (E == 16) return go(k_norm<X, R, 2, 8>);
         return go(k_norm<X, R, 2, 16>);
@@ -642,7 +760,7 @@ dw_status launch_norm(dw_backend *be, const dw_norm_desc &d, const NormArgs &a) 
     Params p{};
     p.x = a.x, p.gate = a.gate, p.res = a.res, p.out = a.out, p.y = a.y, p.q = a.q, p.s = a.s;
     p.w0 = a.w_post, p.b0 = a.b_post, p.w1 = a.w_pre, p.b1 = a.b_pre;
-    p.rows = d.rows, p.c = d.c, p.gate_rows = d.gate_rows;
+    p.rows = d.rows, p.c = d.c, p.gate_rows = (uint32_t)std::min(d.gate_rows, d.rows);
     p.x_pitch = d.x_pitch ? d.x_pitch : d.c, p.res_pitch = d.res_pitch ? d.res_pitch : d.c;
     p.y_pitch = d.y_pitch ? d.y_pitch : d.c;
     p.nb = mx_blocks(d.c), p.tiles = mx_tiles(d.c);

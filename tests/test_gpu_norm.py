@@ -58,7 +58,8 @@ def pitched(v, dtype, pitch):
 CASES = [(1, 1), (1, 4096), (3, 7), (9, 32), (257, 64), (40, 101), (5, 1010), (6, 1024), (33, 576), (2, 5000), (3, 8192), (2, 11008),
          (2, 16383), (2, 16384), (3, 20001), (2, 40000),
          # many rows
-         (333, 8), (300, 64), (1001, 104), (400, 1024), (297, 4096), (300, 8192), (299, 11008), (298, 16384)]
+         (333, 8), (300, 64), (1001, 104), (400, 1024), (297, 4096), (300, 8192), (299, 11008), (298, 16384),
+         (300, 7), (301, 129), (500, 1001), (297, 4094), (299, 8191), (297, 11009), (296, 16383)]
 
 
 @pytest.mark.parametrize("dtype,ydtype", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32"), ("f32", "bf16")])
@@ -84,7 +85,9 @@ def test_norm(be, dtype, ydtype, kind, rows, c):
                                                        (310, 4096, RMS, RMS, 0), (301, 2048, LAYER, LAYER, 100),
                                                        (305, 104, RMS, RMS, 1), (300, 5120, LAYER, RMS, 7),
                                                        (299, 11008, RMS, RMS, None), (1030, 72, RMS, NONE, 0), (298, 16384, RMS, RMS, 1),
-                                                       (298, 8192, LAYER, RMS, 0), (600, 1024, RMS, LAYER, 3)])
+                                                       (298, 8192, LAYER, RMS, 0), (600, 1024, RMS, LAYER, 3),
+                                                       (333, 33, RMS, RMS, 1), (501, 1010, LAYER, LAYER, 250), (300, 4095, RMS, RMS, 7),
+                                                       (297, 10003, NONE, RMS, 0), (700, 62, LAYER, RMS, None)])
 def test_norm_residual(be, dtype, res, rows, c, post, pre, gate_rows):
     """`out` against float64, and y against the norm of the stored `out`."""
     rng = np.random.default_rng(rows * 7 + c)
@@ -137,9 +140,10 @@ def test_norm_residual(be, dtype, res, rows, c, post, pre, gate_rows):
     np.testing.assert_array_equal(be.download_array(s2, np.uint8), be.download_array(s, np.uint8))
 
 
-def test_pitches(be):
+@pytest.mark.parametrize("rows", [9, 700])
+@pytest.mark.parametrize("c", [200, 199])
+def test_pitches(be, rows, c):
     """x, residual, out and y as slices of wider tensors: what lies between the rows is not touched."""
-    rows, c = 9, 200
     rng = np.random.default_rng(2)
     xr, x = pitched(rng.normal(0, 1, (rows, c)), "f16", 208)
     rr, r = pitched(rng.normal(0, 1, (rows, c)), "f32", 211)
@@ -154,6 +158,37 @@ def test_pitches(be):
     assert (yr[:, c:] == 0x4110).all()
     g64 = got[:, :c].astype(np.float64)
     near(R.from_type(yr, "bf16")[:, :c], R.norm(g64, RMS, None, None, 1e-5), norm_tol(g64, RMS, None, None, 1e-5), "bf16")
+
+
+@pytest.mark.parametrize("rows", [1, 5, 400])
+@pytest.mark.parametrize("start", [1, 3, 8])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_tensors_that_start_anywhere(be, rows, start, dtype):
+    """Tensors inside larger buffers, `start` elements in: the elements before and after them (NaN here, and
+    closer than a 16-byte piece) are neither used nor changed."""
+    c = 101
+    rng = np.random.default_rng(start)
+    es = 4 if dtype == "f32" else 2
+    xr, x = R.to_type(rng.normal(0, 1, rows * c), dtype)
+    rr, r = R.to_type(rng.normal(0, 1, rows * c), dtype)
+    gr, g = R.to_type(rng.normal(0, 1, rows * c), dtype)
+    nan = R.to_type(np.full(start, np.nan), dtype)[0]
+    whole = [be.upload_array(np.concatenate([nan, v, nan[:1]])) for v in (xr, rr, gr, rr, xr)]
+    bx, br, bg, bo, by = (be.wrap(b.device_ptr + start * es, rows * c * es) for b in whole)
+    d = ops.NormDesc(rows, c, R.DTYPES[dtype], R.DTYPES[dtype], R.DTYPES[dtype], RMS, RMS, 1e-5, gate_rows=1)
+    ops.norm_residual(be, d, bx, None, None, bg, br, bo, None, None, by)
+    x, r, g = (v.reshape(rows, c) for v in (x, r, g))
+    n = R.norm(x, RMS, None, None, 1e-5)
+    raw = [be.download_array(b, R.np_type(dtype)) for b in whole]
+    for b, v in zip(raw, (xr, rr, gr, None, None)):
+        np.testing.assert_array_equal(b[:start], nan)
+        np.testing.assert_array_equal(b[-1:], nan[:1])
+        if v is not None:
+            np.testing.assert_array_equal(b[start:-1], v)
+    out = R.from_type(raw[3][start:-1].copy(), dtype).reshape(rows, c)
+    near(out, r + g * n, 1.01 * np.abs(g) * (norm_tol(x, RMS, None, None, 1e-5) + 3 * 2.0 ** -24 * np.abs(n)), dtype)
+    near(R.from_type(raw[4][start:-1].copy(), dtype).reshape(rows, c), R.norm(out, RMS, None, None, 1e-5),
+         norm_tol(out, RMS, None, None, 1e-5), dtype)
 
 
 @pytest.mark.parametrize("c", [100, 20001])
