@@ -13,12 +13,14 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// 16 threads take one unit: 128 values of a row, 8 each, four blocks, four
-// scale bytes of one tile.  A thread block is `ux` units across and
-// kThreads / (16 * ux) rows down, and does kRows such groups of rows, so that
-// each thread has kRows independent loads in flight and its addresses and bounds
-// along the row are worked out once.  Both kernels are near the issue rate, not only the
-// memory's: 8192 x 4096 f16 took 19.3 us to quantise at 135 instructions for 8 values.
+// 16 threads take 128 values of a row, 8 each: four blocks.  A thread does so for four
+// rows, 32 apart, whose scales are 16 neighbouring bytes of a tile: four independent
+// loads in flight, and its addresses and bounds worked out once.  A thread block is
+// `ux` such units across and kThreads / (16 * ux) rows of a 32-row group down.  Both
+// kernels are near the issue rate, not only the memory's (8192 x 4096 f16 took 19.3 us
+// to quantise at 135 instructions for 8 values, 15.6 at 110).
+constexpr int kRows = 4;
+
 struct Shape {
     size_t rows, k, pitch;  // pitch: elements from row to row
     size_t nb, tiles;
@@ -28,13 +30,18 @@ struct Shape {
 
 struct Place {
     size_t row, col;  // of the first row's 8 values
-    uint32_t step;    // rows from one row of the thread to the next
+    size_t scale;     // byte of its block's scale; the next rows' are 4 bytes apart each
+    int rows;         // how many of the four rows there are
     bool whole;       // 8 values, loaded or stored at once
-    __device__ __forceinline__ Place(const Shape &p, int rows_per_thread) {
+    __device__ __forceinline__ explicit Place(const Shape &p) {
         const uint32_t u = (threadIdx.x >> 4) & ((1u << p.lux) - 1);
-        step = kThreads >> (4 + p.lux);
-        col = ((((size_t)blockIdx.y << p.lux) + u) << 7) + (threadIdx.x & 15) * 8;
-        row = (size_t)blockIdx.x * step * rows_per_thread + (threadIdx.x >> (4 + p.lux));
+        const int lr = 4 - p.lux;  // log2(rows of a thread block)
+        const uint32_t r32 = ((blockIdx.x & ((32u >> lr) - 1)) << lr) + (threadIdx.x >> (4 + p.lux));
+        const size_t unit = ((size_t)blockIdx.y << p.lux) + u, tile = blockIdx.x >> (5 - lr);
+        col = (unit << 7) + (threadIdx.x & 15) * 8;
+        row = tile * 128 + r32;
+        scale = (tile * p.tiles + unit) * 512 + r32 * 16 + ((threadIdx.x & 15) >> 2);
+        rows = row >= p.rows ? 0 : (int)min((p.rows - row + 31) >> 5, (size_t)kRows);
         whole = p.vec && col + 8 <= p.k;
     }
 };
@@ -57,18 +64,55 @@ __device__ __forceinline__ uint32_t amax8(const Raw<T, 8> &r) {
     }
 }
 
-template <typename T, int kRows>
+// 8 values divided by X, as f32.  The 16-bit types are scaled in their own type, two at
+// a time: a power of two changes no digit (what falls below the smallest f16 would round
+// to code 0), unless it is beyond f16 (then `inv` > 2^15 and f32 does it).
+template <typename T>
+__device__ __forceinline__ void scale8(const Raw<T, 8> &r, float inv, float (&v)[8]) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        const __nv_bfloat162 f = __float2bfloat162_rn(inv);
+        Raw<T, 8> t;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            __nv_bfloat162 h;
+            memcpy(&h, &r.w[i], 4);
+            h = __hmul2(h, f);
+            memcpy(&t.w[i], &h, 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = t.get(i);
+    } else if constexpr (sizeof(T) == 2) {
+        if (inv <= 32768.0f) {
+            const __half2 f = __float2half2_rn(inv);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                __half2 h;
+                memcpy(&h, &r.w[i], 4);
+                const float2 g = __half22float2(__hmul2(h, f));
+                v[2 * i] = g.x, v[2 * i + 1] = g.y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = r.get(i) * inv;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = r.get(i) * inv;
+    }
+}
+
+template <typename T>
 __global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *__restrict__ x, uint8_t *__restrict__ q,
                                                              uint8_t *__restrict__ s, const __grid_constant__ Shape p) {
     pdl_wait();
     pdl_trigger();
-    const Place at(p, kRows);
+    const Place at(p);
     const T *src = x + at.row * p.pitch + at.col;
     Raw<T, 8> raw[kRows];
 #pragma unroll
-    for (int i = 0; i < kRows; i++, src += at.step * p.pitch) {
+    for (int i = 0; i < kRows; i++, src += 32 * p.pitch) {
         raw[i].zero();
-        if (at.row + i * at.step >= p.rows || at.col >= p.k) continue;
+        if (i >= at.rows || at.col >= p.k) continue;
         if (at.whole) {
             load_wide(raw[i], src);
         } else {
@@ -78,44 +122,40 @@ __global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *__restrict
             raw[i].set(v);
         }
     }
-    const size_t block = at.col / 32;
     uint8_t *dst = q + (at.row * p.nb * 32 + at.col) / 2;
-    const bool codes_here = at.col < p.nb * 32, scale_here = (threadIdx.x & 3) == 0 && block < p.tiles * 4;
+    s += at.scale;
+    const bool codes_here = at.col < p.nb * 32, scale_here = (threadIdx.x & 3) == 0 && at.col < p.tiles * 128;
 #pragma unroll
-    for (int i = 0; i < kRows; i++, dst += at.step * p.nb * 16) {
+    for (int i = 0; i < kRows; i++, dst += p.nb * 512) {
         uint32_t amax = amax8(raw[i]);
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const uint32_t sb = mx_scale_byte(amax);
-        const float inv = mx_inv_scale(sb);
         float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = raw[i].get(j) * inv;
+        scale8(raw[i], mx_inv_scale(sb), v);
         const uint32_t codes = sb == 0xFFu ? 0u : mx_codes8(v);
-        const size_t row = at.row + i * at.step;
-        if (row >= p.rows) continue;
+        if (i >= at.rows) continue;
         if (codes_here) *reinterpret_cast<uint32_t *>(dst) = codes;
-        if (scale_here) s[mx_scale_at(row, block, p.tiles)] = (uint8_t)sb;  // four neighbours: one word
+        if (scale_here) s[4 * i] = (uint8_t)sb;
     }
 }
 
-template <typename T, int kRows, bool kVec>
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__restrict__ q, const uint8_t *__restrict__ s,
                                                                T *__restrict__ y, const __grid_constant__ Shape p) {
     pdl_wait();
     pdl_trigger();
-    const Place at(p, kRows);
+    const Place at(p);
     if (kVec && at.col >= p.k) return;
-    const size_t block = at.col / 32;
     const uint8_t *src = q + (at.row * p.nb * 32 + at.col) / 2;
+    s += at.scale;
     uint32_t codes[kRows], sb[kRows];
 #pragma unroll
-    for (int i = 0; i < kRows; i++, src += at.step * p.nb * 16) {
-        const size_t row = at.row + i * at.step;
+    for (int i = 0; i < kRows; i++, src += p.nb * 512) {
         codes[i] = sb[i] = 0;
-        if (row >= p.rows || at.col >= p.k) continue;
+        if (i >= at.rows || at.col >= p.k) continue;
         codes[i] = __ldg(reinterpret_cast<const uint32_t *>(src));
-        sb[i] = __ldg(s + mx_scale_at(row, block, p.tiles));
+        sb[i] = __ldg(s + 4 * i);
     }
     if constexpr (!kVec) {
         // rows that start anywhere: the 16 threads of a unit write 16 neighbours at a time
@@ -124,20 +164,20 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__
         const size_t col0 = at.col - lane16 * 8;
         T *dst = y + at.row * p.k + col0 + lane16;
 #pragma unroll
-        for (int i = 0; i < kRows; i++, dst += at.step * p.k)
+        for (int i = 0; i < kRows; i++, dst += 32 * p.k)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const uint32_t c = __shfl_sync(0xffffffffu, codes[i], 2 * j + (lane16 >> 3), 16);
                 const uint32_t b = __shfl_sync(0xffffffffu, sb[i], 2 * j, 16);
                 const float v = mx_decode1(c >> (4 * (lane16 & 7))) * mx_scale(b);
-                if (at.row + i * at.step < p.rows && col0 + 16 * j + lane16 < p.k) dst[16 * j] = from_f32<T>(v);
+                if (i < at.rows && col0 + 16 * j + lane16 < p.k) dst[16 * j] = from_f32<T>(v);
             }
         return;
     }
     T *dst = y + at.row * p.k + at.col;
 #pragma unroll
-    for (int i = 0; i < kRows; i++, dst += at.step * p.k) {
-        if (at.row + i * at.step >= p.rows) continue;
+    for (int i = 0; i < kRows; i++, dst += 32 * p.k) {
+        if (i >= at.rows) continue;
         float v[8];
         mx_decode8(codes[i], v);
         const float X = mx_scale(sb[i]);
@@ -171,16 +211,17 @@ __global__ void __launch_bounds__(kThreads) k_pack_scales(const uint8_t *__restr
     *reinterpret_cast<uint32_t *>(s + mx_scale_at(row, t * 4, tiles)) = w;
 }
 
-constexpr int kRowsPer = 4;
-
-// The grid of the streaming kernels: x over groups of rows, y over groups of units.
+// The grid of the streaming kernels: x over 128-row tiles and groups of their 32 rows, y
+// over groups of units.
 bool make_shape(size_t rows, size_t k, size_t pitch, bool vec, Shape *p, dim3 *grid) {
     p->rows = rows, p->k = k, p->pitch = pitch, p->vec = vec;
     p->nb = mx_blocks(k), p->tiles = mx_tiles(k);
     p->lux = 0;
     while (p->lux < 4 && ((size_t)1 << p->lux) < p->tiles) p->lux++;
-    const size_t rows_blk = (size_t)(kThreads >> (4 + p->lux)) * kRowsPer;
-    const size_t gx = (rows + rows_blk - 1) / rows_blk, gy = (p->tiles + ((size_t)1 << p->lux) - 1) >> p->lux;
+    const size_t per_block = kThreads >> (4 + p->lux);  // rows of a thread block, of a group's 32
+    // (one tile needs only the groups that it has rows in)
+    const size_t gx = rows <= 32 ? (rows + per_block - 1) / per_block : (rows + 127) / 128 * (32 / per_block);
+    const size_t gy = (p->tiles + ((size_t)1 << p->lux) - 1) >> p->lux;
     if (gx > 0x7fffffffu || gy > 65535u) return false;
     *grid = dim3((unsigned)gx, (unsigned)gy);
     return true;
@@ -194,7 +235,7 @@ dw_status quantize(dw_backend *be, const void *x, size_t rows, size_t k, size_t 
     const bool vec = (uintptr_t)x % kWide == 0 && pitch * sizeof(T) % kWide == 0;
     if (!make_shape(rows, k, pitch, vec, &p, &grid))
         return dw_fail(be, DW_ERR_UNSUPPORTED, "quantize_mxfp4: %zu x %zu is too large", rows, k);
-    return launch_dependent(be, "quantize_mxfp4", k_quantize_mxfp4<T, kRowsPer>, grid, kThreads, 0, 0, (const T *)x, q, s, p);
+    return launch_dependent(be, "quantize_mxfp4", k_quantize_mxfp4<T>, grid, kThreads, 0, 0, (const T *)x, q, s, p);
 }
 
 template <typename T>
@@ -205,7 +246,7 @@ dw_status dequantize(dw_backend *be, const uint8_t *q, const uint8_t *s, size_t 
     const bool vec = (uintptr_t)y % kWide == 0 && k * sizeof(T) % kWide == 0;
     if (!make_shape(rows, k, k, vec, &p, &grid))
         return dw_fail(be, DW_ERR_UNSUPPORTED, "dequantize_mxfp4: %zu x %zu is too large", rows, k);
-    return launch_dependent(be, "dequantize_mxfp4", vec ? k_dequantize_mxfp4<T, kRowsPer, true> : k_dequantize_mxfp4<T, kRowsPer, false>, grid, kThreads, 0, 0, q, s, (T *)y, p);
+    return launch_dependent(be, "dequantize_mxfp4", vec ? k_dequantize_mxfp4<T, true> : k_dequantize_mxfp4<T, false>, grid, kThreads, 0, 0, q, s, (T *)y, p);
 }
 
 }  // namespace
