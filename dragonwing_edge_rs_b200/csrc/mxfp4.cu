@@ -64,6 +64,40 @@ __device__ __forceinline__ uint32_t amax8(const Raw<T, 8> &r) {
     }
 }
 
+// 8 elements from anywhere: the widest accesses that the address allows; 16-bit elements
+// at an odd place from the five words around them, where these lie in [first, last).
+template <typename T>
+__device__ __forceinline__ void load_any(Raw<T, 8> &r, const T *src, const T *first, const T *last) {
+    const uint32_t a = (uint32_t)(uintptr_t)src & 15;
+    constexpr int kWords = Raw<T, 8>::kWords;
+    if (a == 0) {
+        r.load(src);
+    } else if ((a & 7) == 0) {
+#pragma unroll
+        for (int i = 0; i < kWords / 2; i++) {
+            const uint2 w = reinterpret_cast<const uint2 *>(src)[i];
+            r.w[2 * i] = w.x, r.w[2 * i + 1] = w.y;
+        }
+    } else if ((a & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) r.w[i] = reinterpret_cast<const uint32_t *>(src)[i];
+    } else if (sizeof(T) == 2 && src > first && src + 9 <= last) {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(src - 1);
+        uint32_t lo = w[0];
+#pragma unroll
+        for (int i = 0; i < kWords; i++) {
+            const uint32_t hi = w[i + 1];
+            r.w[i] = __funnelshift_r(lo, hi, 16);
+            lo = hi;
+        }
+    } else {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_f32(src[i]);
+        r.set(v);
+    }
+}
+
 // 8 values divided by X, as f32.  The 16-bit types are scaled in their own type, two at
 // a time: a power of two changes no digit (what falls below the smallest f16 would round
 // to code 0), unless it is beyond f16 (then `inv` > 2^15 and f32 does it).
@@ -115,6 +149,8 @@ __global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *__restrict
         if (i >= at.rows || at.col >= p.k) continue;
         if (at.whole) {
             load_wide(raw[i], src);
+        } else if (at.col + 8 <= p.k) {
+            load_any(raw[i], src, x, x + (p.rows - 1) * p.pitch + p.k);
         } else {
             float v[8];
 #pragma unroll

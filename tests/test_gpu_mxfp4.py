@@ -52,6 +52,42 @@ def test_quantize(be, dtype, rows, k, gap):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("start", [0, 1, 2, 3, 4, 8])
+@pytest.mark.parametrize("gap", [0, 1, 2, 4])
+def test_quantize_starts_anywhere(be, dtype, start, gap):
+    """A slice that begins `start` elements into its buffer, every alignment of its rows; NaN around it."""
+    rows, k = 133, 104
+    rng = np.random.default_rng(start * 10 + gap)
+    wide = np.full((rows, k + gap), np.nan)
+    wide[:, :k] = rng.normal(0, 1, (rows, k))
+    raw, val = R.to_type(wide, dtype)
+    nan = R.to_type(np.full(start + 1, np.nan), dtype)[0]
+    whole = be.upload_array(np.concatenate([nan[:start], raw.reshape(-1)[:rows * (k + gap) - gap], nan[:1]]))
+    es = 4 if dtype == "f32" else 2
+    x = be.wrap(whole.device_ptr + start * es, (rows * (k + gap) - gap) * es)
+    q = be.upload_array(np.full(ops.mxfp4_code_bytes(rows, k), 0xCD, np.uint8))
+    s = be.upload_array(np.full(ops.mxfp4_scale_bytes(rows, k), 0xAB, np.uint8))
+    ops.quantize_mxfp4(be, x, R.DTYPES[dtype], rows, k, q, s, k + gap)
+    check_quantized(be.download_array(q, np.uint8), be.download_array(s, np.uint8), val[:, :k], k)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("start", [1, 3, 4])
+def test_dequantize_starts_anywhere(be, dtype, start):
+    rows, k = 133, 104
+    rng = np.random.default_rng(start)
+    codes, scales = rng.integers(0, 16, (rows, 128)).astype(np.uint8), rng.integers(120, 134, (rows, 4)).astype(np.uint8)
+    es = 4 if dtype == "f32" else 2
+    whole = be.upload_array(np.full(rows * k + start + 5, 7, R.np_type(dtype)))
+    q, s = operand(be, codes, scales, k)
+    ops.dequantize_mxfp4(be, q, s, rows, k, be.wrap(whole.device_ptr + start * es, rows * k * es), R.DTYPES[dtype])
+    raw = be.download_array(whole, R.np_type(dtype))
+    assert (raw[:start] == 7).all() and (raw[start + rows * k:] == 7).all()
+    got = R.from_type(raw[start:start + rows * k].copy(), dtype).reshape(rows, k)
+    np.testing.assert_array_equal(got, R.to_type(R.values(codes, scales, k), dtype)[1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_quantize_ties_and_limits(be, dtype):
     """Every tie at several scales, powers of two and their neighbours, zeros of both signs, the type's
     smallest and largest values."""
