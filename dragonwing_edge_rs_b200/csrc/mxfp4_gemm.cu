@@ -32,7 +32,8 @@ namespace {
 
 constexpr int kBM = 128;
 constexpr int kBKBytes = 128;  // a K block: 256 codes
-constexpr size_t kSmemLimit = 227 * 1024;
+constexpr size_t kSmemLimit = 227 * 1024;  // of a CTA
+constexpr size_t kSmemSm = 228 * 1024;     // of an SM
 
 struct GemmParams {
     const float *bias;
@@ -900,11 +901,7 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
     p.vec = a.n % 4 == 0 && (uintptr_t)a.y % (a.y_dtype == DW_F32 ? 16 : 8) == 0;
     p.stage_bytes = kBM * kBKBytes + 1024 + p.bn * kBKBytes + 1024;
     for (int h = 0; h < 2; h++) p.idesc[h] = mx_idesc(128, p.bn, h);
-    // two CTAs an SM up to 64 rows (each at most 256 columns of tensor memory), one above
-    const int per_sm = p.bn <= 64 ? 2 : 1;
-    const size_t budget = (kSmemLimit - 8192) / per_sm - 2048;
-    p.stages = (int)std::min<size_t>(kSkinnyStages, budget / p.stage_bytes);
-    p.tmem_cols = 256;
+    const int per_sm = p.bn <= 64 ? 2 : 1;  // CTAs whose rings an SM holds
     p.wait_cap_ns = be->wait_cap_ns, p.err = be->dev_err;
     const size_t tn = (a.n + 127) / 128;
     // CTAs that share a tile's K: about one an SM (4096 outputs, K 4096, one row: S = 1, 2,
@@ -913,7 +910,20 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
     unsigned S = 1;
     const unsigned most = per_sm == 2 ? 8 : 4;
     while (S < most && 2 * S * tn <= (size_t)be->sm_count * 4 / 3 && 2 * (int)S <= p.k_blocks) S *= 2;
-    const size_t smem = 1024 + std::max<size_t>(p.stages * p.stage_bytes, (size_t)p.bn * 512);
+    // The ring: no longer than a CTA's K blocks, and of three stages where the CTAs outnumber
+    // the SMs and have few blocks each: a third of them then fits beside two others, or
+    // the next launch's (11008 outputs, K 4096, one row 6.4 -> 5.3 us)
+    const int own = (p.k_blocks + (int)S - 1) / (int)S;
+    p.stages = (int)std::min<size_t>(kSkinnyStages, ((kSmemLimit - 8192) / per_sm - 2048) / p.stage_bytes);
+    p.stages = std::min(p.stages, p.bn <= 32 && S * tn > (size_t)be->sm_count && own <= 8 ? 3 : own);
+    // Tensor memory: accumulators and 16 columns a stage.  A CTA takes no larger share of an
+    // SM's 512 columns than of its shared memory, so those that fit together, of this launch
+    // and others, find columns: none waits for another's, which might itself wait for a
+    // CTA of the waiting one's cluster.
+    p.tmem_cols = 32;
+    while ((int)p.tmem_cols < p.bn + 16 * p.stages) p.tmem_cols *= 2;
+    const size_t smem = std::max(1024 + std::max<size_t>(p.stages * p.stage_bytes, (size_t)p.bn * 512),
+                                 kSmemSm * p.tmem_cols / 512);
     CUtensorMap tw, ta, tsw, tsa;
     if (!be->encode_tiled || !code_map(be, &tw, a.b_q, a.n, a.k, kBM) || !code_map(be, &ta, a.a_q, a.m, a.k, p.bn) ||
         !scale_map(be, &tsw, a.b_s, a.n, a.k, 2, 1) || !scale_map(be, &tsa, a.a_s, a.m, a.k, 2, 1))
