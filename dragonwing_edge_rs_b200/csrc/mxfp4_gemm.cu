@@ -5,15 +5,20 @@
 // Products and sums are the tensor core's (f32 accumulators); bias and activation
 // are f32.
 //
-// One persistent CTA per SM, warp-specialised:
-//   warp 0    producer: per 256-wide K block one TMA box of codes of each operand
-//             (128 bytes a row, 128-byte swizzle) and the bulk copies of their
-//             scale tiles, into a ring of stages;
-//   warp 1    allocates tensor memory and issues, per stage, tcgen05.cp of the
-//             scale tiles into that stage's scale columns and four
-//             tcgen05.mma (128 x BN x 64);
-//   warps 2.. epilogue: accumulators -> registers (a thread holds a row, so 32
-//             columns in one thread are one MXFP4 block of the result).
+// Two kernels, one for many rows of A (pairs of CTAs, cta_group::2) and one for few (the
+// weights on the 128-row side), built alike and warp-specialised:
+//   warp 0    producer: TMA boxes of codes (128 bytes a row, 128-byte swizzle) and of
+//             scale tiles into a ring of stages;
+//   warp 2    tcgen05.cp of a stage's scale tiles into that stage's scale columns of
+//             tensor memory;
+//   warp 1    the products of a stage, tcgen05.mma.kind::mxf4 of 64 codes each;
+//   the rest  epilogue: accumulators -> bias, activation, rounding or requantisation.
+// What bounds them (B200): with many rows each SM's intake from L2 -- a stage of 512 codes
+// is 70 KB for 256 x 256 outputs (0.63 us; 0.54 us at the tensor rate) and 52 KB for
+// 256 x 128 (0.36 us) -- and beyond one round of tiles the power limit; 8192^3 runs at
+// 5.7 PFLOP/s, 4096^3 at 4.5.  With few rows the weights' bytes and about 2.3 us of
+// launch, first copies and hand-offs: 11008 x 4096 (24 MB) 5.4 us from L2, 7.6 from HBM.
+// What a step of it cost and saved stands beside each part.
 //
 // Every mbarrier wait is bounded; on expiry the CTA records the failure, waits
 // (bounded) for its own copies and products in flight, frees its tensor memory
@@ -50,14 +55,12 @@ struct GemmParams {
     int32_t *err;
 };
 
-// Bounded wait for a phase; false once the CTA is aborting or the cap expired.  The
-// single threads that feed the tensor core poll (a thread that try_wait suspended
-// resumes late, and a stage's round trip bounds the rate); whole warps suspend soon.
-template <int kPolls = 1024>
+// Bounded wait for a phase: polls first (most waits are short), then suspends; false
+// once the CTA is aborting or the cap expired.
 __device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, uint64_t cap_ns, int32_t *err,
                                            volatile int *abort_flag, int site) {
 #pragma unroll 1
-    for (int i = 0; i < kPolls; i++)
+    for (int i = 0; i < 8; i++)
         if (mbar_test_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
@@ -78,7 +81,7 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, uint64_
 #pragma unroll 1
     for (int i = 0; i < 1024; i++)
         if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, wait_phase<8>(bar, parity, cap_ns, err, abort_flag, site));
+    return __all_sync(0xffffffffu, wait_phase(bar, parity, cap_ns, err, abort_flag, site));
 }
 
 // Waits for a phase that the CTA's own work in flight completes, whatever happened before.
@@ -92,7 +95,7 @@ __device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, uint6
 // The warps that feed the tensor core run their loops with all lanes, on warp-uniform
 // values, and predicate each issue on one elected lane: operands then come from
 // uniform registers.  (A loop inside `if (lane == 0)` issues an MMA only every ~110
-// cycles and a scale copy every ~80.)
+// cycles and a scale copy every ~80: 4096^3 took 34 us so, 30.7 this way.)
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -293,9 +296,14 @@ __device__ __forceinline__ void put_scales(uint32_t scales, size_t row, size_t b
 // A pair of CTAs (cta_group::2) computes a 256 x BN tile: each holds 128 rows of A,
 // half of B's rows, the scales of its rows of A and those of all BN rows of B, so a
 // K block costs each SM's L2 port (128 + BN / 2) * 128 bytes of codes for
-// 256 * BN * 256 products of the pair.  The leader issues for both; the peer's
-// copies reach it by a remote arrival.  The epilogue takes its accumulators into
-// registers at once and gives the tensor memory back before it converts and stores.
+// 256 * BN * 256 products of the pair.  The leader issues for both, and both CTAs' copies
+// complete on its barrier (a relay by the peer, releasing and acquiring at cluster scope,
+// took 64 us for 4096^3; this 40).  The epilogue takes its accumulators into registers
+// at once and gives the tensor memory back before it converts and stores.
+//
+// Pairs of one cluster can share a tile's K (then it is the cluster's only tile): each
+// leaves its partial tile in shared memory, over the ring, and adds up its share of the
+// columns in the order of the pairs.
 constexpr int kEpiWarps = 16;
 constexpr int kGemmThreads = 128 + 32 * kEpiWarps;
 constexpr int kMaxStages = 8;
@@ -516,7 +524,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         uint32_t aph = 0;
         for (int tile = pair; tile < p.tiles; tile += pairs) {
             const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
-            if (!__all_sync(0xffffffffu, wait_phase<8>(smem_u32(&tfull_bar[acc]), aph, p.wait_cap_ns, p.err, abort_flag, 26))) break;
+            if (!__all_sync(0xffffffffu, wait_phase(smem_u32(&tfull_bar[acc]), aph, p.wait_cap_ns, p.err, abort_flag, 26))) break;
             tc_fence_after();
             const size_t row = ((size_t)tm * 2 + rank) * kBM + quarter * 32 + lane;
             const size_t col0 = (size_t)tn * BN + part * kCols;
@@ -743,7 +751,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     if (warp >= 4) {
         // accumulators -> part[row of A][output]
         const int quarter = warp & 3;
-        if (__all_sync(0xffffffffu, wait_phase<8>(smem_u32(&done_bar), 0, p.wait_cap_ns, p.err, abort_flag, 34))) {
+        if (__all_sync(0xffffffffu, wait_phase(smem_u32(&done_bar), 0, p.wait_cap_ns, p.err, abort_flag, 34))) {
             tc_fence_after();
             const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
             const int cols = (int)p.m;
