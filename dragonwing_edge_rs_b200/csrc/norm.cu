@@ -79,6 +79,49 @@ __device__ __forceinline__ void load_f32(const float *p, float (&v)[V]) {
     for (int i = 0; i < V; i++) v[i] = r.get(i);
 }
 
+// Element-wise f32 over V values, two to an instruction where V is even (the streaming
+// kernel is half issue-bound).
+template <int V>
+__device__ __forceinline__ void mul_all(float (&a)[V], const float (&b)[V]) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 r = __fmul2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+            a[i] = r.x, a[i + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) a[i] *= b[i];
+    }
+}
+template <int V>
+__device__ __forceinline__ void scale_all(float (&a)[V], float s) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 r = __fmul2_rn(make_float2(a[i], a[i + 1]), make_float2(s, s));
+            a[i] = r.x, a[i + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) a[i] *= s;
+    }
+}
+// c += a * b
+template <int V>
+__device__ __forceinline__ void fma_all(const float (&a)[V], const float (&b)[V], float (&c)[V]) {
+    if constexpr (V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 r = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), make_float2(c[i], c[i + 1]));
+            c[i] = r.x, c[i + 1] = r.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) c[i] = fmaf(a[i], b[i], c[i]);
+    }
+}
+
 // v[j][i] -> its norm, in place.  Elements past the row are 0 and stay out of the
 // statistics (`live`: element group j lies in the row).  weight(j, wv) and bias(j,
 // bv) give a group's weights and return whether there are any.
@@ -445,11 +488,13 @@ __global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads
 #pragma unroll
                 for (int i = 0; i < V; i++) v[j][i] = live[j] ? v[j][i] - mean : 0.0f;
         }
-        float sq = 0.0f;
+        float part[V], sq = 0.0f;
 #pragma unroll
-        for (int j = 0; j < N; j++)
+        for (int i = 0; i < V; i++) part[i] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < V; i++) sq = fmaf(v[j][i], v[j][i], sq);
+        for (int j = 0; j < N; j++) fma_all<V>(v[j], v[j], part);
+#pragma unroll
+        for (int i = 0; i < V; i++) sq += part[i];
         return __frsqrt_rn(fmaf(row_sum<kThreads>(sq, T, red, slot), p.inv_c, p.eps));
     };
     int s = 0;
@@ -505,7 +550,9 @@ __global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads
                     Raw<R, V> res = rr[V == 8 ? j : 0];
                     if constexpr (V < 8) res.load(rs + column(j));
 #pragma unroll
-                    for (int i = 0; i < V; i++) o[i] = fmaf(v[j][i] * rstd, t[i], res.get(i));
+                    for (int i = 0; i < V; i++) o[i] = res.get(i);
+                    scale_all<V>(v[j], rstd);
+                    fma_all<V>(v[j], t, o);
                     bias(j, o);
                     Raw<R, V> r;
                     r.set(o);
@@ -547,8 +594,8 @@ __global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads
                 if (!live[j]) continue;
                 float t[V];
                 kept(w1, j, t);
-#pragma unroll
-                for (int i = 0; i < V; i++) v[j][i] = v[j][i] * rstd * t[i];
+                scale_all<V>(v[j], rstd);
+                mul_all<V>(v[j], t);
             }
             if (p.b1) {
 #pragma unroll
