@@ -9,7 +9,7 @@
 //
 // Bandwidth-bound: x, res and gate are read once, out and y written once.  Three forms:
 // persistent blocks that stream many rows through a ring (8192 x 4096 bf16 with both
-// norms 50 us, 5.4 TB/s; half issue-bound at 470 instructions a warp and row), a block
+// norms 44.4 us, 6.0 TB/s; then the issue rate, 470 instructions a warp and row), a block
 // a row in registers for few (1 x 4096 2.3 us, latency), and a re-reading one for rows
 // over 16384.
 
@@ -25,7 +25,7 @@ namespace {
 
 constexpr int kMaxT = 512;  // threads of a row
 constexpr int kMaxE = 32;   // elements of a thread
-constexpr size_t kSmemBudget = 216 * 1024;  // of an SM's shared memory for rows to come
+constexpr size_t kSmemBudget = 216 * 1024;  // of an SM's shared memory for weights and rows to come
 
 struct Params {
     const void *x, *gate, *res;
@@ -42,18 +42,20 @@ struct Params {
 // Sum over the T threads of a row (a power of two; rows of T <= 32 lie in one warp,
 // longer ones take whole warps, and all threads of the block call together).
 // `slot` alternates over four buffers, so a buffer is written again only after
-// three more barriers.  kBar: the threads that call, where these are not the whole block.
+// three more barriers.  kBar: the threads that call and meet at barrier `bar`, where these
+// are not the whole block (`thread`: the place among them).
 template <int kBar = 0>
-__device__ __forceinline__ float row_sum(float v, int T, float (*red)[16], int &slot) {
+__device__ __forceinline__ float row_sum(float v, int T, float (*red)[16], int &slot, int thread = 0, int bar = 0) {
 #pragma unroll
     for (int o = 16; o; o >>= 1)
         if (o < T) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (T <= 32) return v;
-    const int thread = threadIdx.y * blockDim.x + threadIdx.x, lane = thread & 31, warp = thread >> 5;
+    if (!kBar) thread = threadIdx.y * blockDim.x + threadIdx.x;
+    const int lane = thread & 31, warp = thread >> 5;
     const int warps = T >> 5, first = warp & ~(warps - 1);
     if (lane == 0) red[slot][warp] = v;
     if (kBar)
-        named_barrier_sync(1, kBar);
+        named_barrier_sync(bar, kBar);
     else
         __syncthreads();
     const float *part = &red[slot][first];  // every thread adds the warps' sums, in the same order
@@ -277,12 +279,15 @@ __global__ void __launch_bounds__(kMaxT, V * N <= 8 ? 2 : 1) k_norm(const __grid
     }
 }
 
-// Many rows: persistent thread blocks fed by bulk copies, which a warp of its own
-// issues (kThreads others compute).  A step is G = kThreads / T rows; a ring of stages holds the x, residual and gate rows of the steps to come, so
-// the loads in flight do not depend on how many rows the registers hold.  Bulk copies
-// move whole 16-byte pieces: a row that starts or ends inside one is copied with its
-// surroundings (its neighbours' elements), except where that would leave the tensor.
-constexpr int kStreamStages = 8;
+// Many rows: one persistent thread block an SM, of up to three teams that share the weights
+// in shared memory and otherwise go their own ways (a block for each, with weights of its
+// own, left less room for rows: 8192 x 4096 bf16 with both norms 48.1 against 44.4 us).  A
+// team's steps of G = kThreads / T rows come by bulk copies that a warp of its own issues
+// (kThreads others compute): a ring of stages holds the x, residual and gate rows of the
+// steps to come, so the loads in flight do not depend on how many rows the registers hold.
+// Bulk copies move whole 16-byte pieces: a row that starts or ends inside one is copied with
+// its surroundings (its neighbours' elements), except where that would leave the tensor.
+constexpr int kStreamStages = 2;
 
 // Bytes of a stage: per tensor G rows, one after the other as in memory (`packed`: one
 // copy), or each in a place of its own.
@@ -314,35 +319,39 @@ struct Span {
     }
 };
 
-// Blocks an SM: three where 80 registers a thread and the ring allow it.
+// The most teams of a block that its registers hold.
 template <typename R, int V, int N, int kThreads>
-constexpr int stream_blocks() {
-    return kThreads > 256 ? 1 : V * N > 8 && (V < 8 || sizeof(R) == 4) ? 2 : 3;
+constexpr int stream_teams() {
+    return kThreads > 256 ? 1 : V * N > 16 || (V * N > 8 && (V < 8 || sizeof(R) == 4)) ? 2 : 3;
 }
 
 template <typename X, typename R, int V, int N, int kThreads, bool kFull>
-__global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads>())
+__global__ void __launch_bounds__((kThreads + 32) * stream_teams<R, V, N, kThreads>(), 1)
     k_norm_stream(const __grid_constant__ Params p, const int T, const int stages, uint64_t wait_cap_ns, int32_t *err) {
-    extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ __align__(16) float red[4][16];
-    __shared__ uint64_t full_bar[kStreamStages], empty_bar[kStreamStages];
+    constexpr int kTeams = stream_teams<R, V, N, kThreads>();
+    extern __shared__ __align__(128) uint8_t shared[];
+    __shared__ __align__(16) float red[kTeams][4][16];
+    __shared__ uint64_t full_bars[kTeams][kStreamStages], empty_bars[kTeams][kStreamStages];
     __shared__ int abort_word;
+    const int teams = blockDim.x / (kThreads + 32), team = threadIdx.x / (kThreads + 32), thread = threadIdx.x % (kThreads + 32);
+    uint64_t *const full_bar = full_bars[team], *const empty_bar = empty_bars[team];
     volatile int *abort_flag = &abort_word;
     int slot = 0;
-    const int lane = threadIdx.x & 31;
-    const int G = kThreads / T, g = threadIdx.x / T, tid = threadIdx.x & (T - 1);
+    const int lane = thread & 31;
+    const int G = kThreads / T, g = thread / T, tid = thread & (T - 1);
     const size_t steps = (p.rows + G - 1) / G;
     // a gate row of the rows themselves comes with them
     const bool row_gate = p.gate && p.gate_rows, packed_x = p.x_pitch == p.c, packed_r = p.res_pitch == p.c;
     const StreamRows lx(p.c, sizeof(X), G, packed_x, true), lr(p.c, sizeof(R), G, packed_r, p.has_res),
         lg(p.c, sizeof(X), G, false, row_gate);
     const uint32_t stage_bytes = lx.region + lr.region + lg.region;
+    uint8_t *const ring = shared + team * stages * stage_bytes;
     const uint32_t base = smem_u32(ring);
     const uint8_t *const x0 = (const uint8_t *)p.x, *const r0 = (const uint8_t *)p.res, *const g0 = (const uint8_t *)p.gate;
     const size_t x_pitch = p.x_pitch * sizeof(X), r_pitch = p.res_pitch * sizeof(R);
-    if (threadIdx.x == 0) {
+    if (thread == 0) {
         for (int s = 0; s < stages; s++) mbar_init(smem_u32(&full_bar[s]), 1), mbar_init(smem_u32(&empty_bar[s]), kThreads / 32);
-        abort_word = 0;
+        if (team == 0) abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -360,10 +369,12 @@ __global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads
     };
     pdl_wait();
     pdl_trigger();
-    if (threadIdx.x >= kThreads) {
+    // every block's first team before any second one
+    const size_t step0 = (size_t)team * gridDim.x + blockIdx.x, step_stride = (size_t)teams * gridDim.x;
+    if (thread >= kThreads) {
         int s = 0, issued = 0;
         uint32_t ph = 0;
-        for (size_t step = blockIdx.x; step < steps && !*abort_flag; step += gridDim.x) {
+        for (size_t step = step0; step < steps && !*abort_flag; step += step_stride) {
             if (issued >= stages) wait(&empty_bar[s], ph ^ 1u);
             __syncwarp();
             if (__any_sync(0xffffffffu, *abort_flag)) break;
@@ -425,7 +436,7 @@ __global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads
     // where all rows share it, the gate); w1: the weight of the next norm (both in shared
     // memory, 16 bytes of a thread beside its neighbour's: registers go to a third block
     // on the SM instead)
-    float *c0 = reinterpret_cast<float *>(ring + (size_t)stages * stage_bytes), *w1 = c0 + N * T * V;
+    float *c0 = reinterpret_cast<float *>(shared + (size_t)teams * stages * stage_bytes), *w1 = c0 + N * T * V;
     bool live[N];
     auto column = [&](int j) { return (uint32_t)(j * T + tid) * V; };
     auto kept = [&](const float *from, int j, float (&t)[V]) {
@@ -449,7 +460,7 @@ __global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads
 #pragma unroll
     for (int j = 0; j < N; j++) {
         live[j] = kFull || column(j) < p.c;
-        if (!live[j] || g) continue;
+        if (!live[j] || g || j % teams != team) continue;  // the teams share the columns
         float t[V];
         if (p.has_res) {
 #pragma unroll
@@ -473,7 +484,7 @@ __global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads
         if (p.w1) load_f32<V>(p.w1 + column(j), t);
         keep(w1, j, t);
     }
-    named_barrier_sync(1, kThreads);
+    named_barrier_sync(1 + kTeams, teams * kThreads);
     // (mean, 1 / root) of v over the row; elements past the row are 0
     auto statistics = [&](float (&v)[N][V], int kind) {
         if (kind == DW_NORM_LAYER) {
@@ -482,7 +493,7 @@ __global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads
             for (int j = 0; j < N; j++)
 #pragma unroll
                 for (int i = 0; i < V; i++) sum += v[j][i];
-            const float mean = row_sum<kThreads>(sum, T, red, slot) * p.inv_c;
+            const float mean = row_sum<kThreads>(sum, T, red[team], slot, thread, 1 + team) * p.inv_c;
 #pragma unroll
             for (int j = 0; j < N; j++)
 #pragma unroll
@@ -495,12 +506,11 @@ __global__ void __launch_bounds__(kThreads + 32, stream_blocks<R, V, N, kThreads
         for (int j = 0; j < N; j++) fma_all<V>(v[j], v[j], part);
 #pragma unroll
         for (int i = 0; i < V; i++) sq += part[i];
-        return __frsqrt_rn(fmaf(row_sum<kThreads>(sq, T, red, slot), p.inv_c, p.eps));
+        return __frsqrt_rn(fmaf(row_sum<kThreads>(sq, T, red[team], slot, thread, 1 + team), p.inv_c, p.eps));
     };
     int s = 0;
     uint32_t ph = 0;
-    size_t step = blockIdx.x;
-    for (; step < steps; step += gridDim.x) {
+    for (size_t step = step0; step < steps; step += step_stride) {
         wait(&full_bar[s], ph);
         const size_t row = step * G + g, row0 = packed_x ? step * G : row, rrow0 = packed_r ? step * G : row;
         const bool there = row < p.rows;
@@ -707,22 +717,25 @@ bool stream_as(dw_backend *be, const Params &p, int T, dw_status *st) {
                          StreamRows(p.c, sizeof(R), G, p.res_pitch == p.c, p.has_res).region +
                          StreamRows(p.c, sizeof(X), G, false, p.gate && p.gate_rows).region;
     const size_t weights = (size_t)T * N * V * 4 * 2;
-    // the most blocks an SM that have room for two steps each, or else for one
-    auto fits = [&](size_t blocks) {
-        const size_t room = kSmemBudget / blocks;
-        return room < weights + stage ? 0 : (int)std::min<size_t>(kStreamStages, (room - weights) / stage);
-    };
-    constexpr int kBlocks = stream_blocks<R, V, N, kThreads>();
-    // (two where a step is one long row with one reduction: blocks with less to wait for crowd
-    // the memory, 8192 x 4096 bf16 with a residual and one norm 49.8 against 43.2 us; with
-    // two norms three blocks 48.1, two 56.2)
-    const bool light = G == 1 && N > 1 && p.has_res && p.post == DW_NORM_NONE && p.pre != DW_NORM_LAYER;
-    const int per_sm = kBlocks == 3 && !light && fits(3) >= 2 ? 3 : kBlocks >= 2 && fits(2) >= 1 ? 2 : 1;
-    const int stages = std::min(fits(per_sm), light ? 3 : kStreamStages);
+    // Teams as registers and the ring allow, with two stages each where there is room: one
+    // fills while the other's values go to registers.  More copies in flight only get in
+    // each other's way (8192 x 4096 bf16, both norms, three teams: 1, 2, 3, 8 stages 47.5,
+    // 44.4, 46.0, 46.8 us; two teams 52.4), and so does a third team where little is
+    // computed: a whole row of 16-bit results from a residual and one norm (47.8 against
+    // 43.3 us with two; to MXFP4 47.0 against 54.7, rows of 4000 44.4 against 51.1).
+    const bool light = kFull && p.has_res && p.post == DW_NORM_NONE && p.pre != DW_NORM_LAYER && p.y_dtype != -2;
+    constexpr int kTeams = stream_teams<R, V, N, kThreads>();
+    const size_t room = kSmemBudget < weights ? 0 : kSmemBudget - weights, held = room / stage;
+    if (!held) return false;
+    const int teams = (int)std::min<size_t>(held, light ? std::min(kTeams, 2) : kTeams);
+    const int stages = (int)std::min<size_t>(held / teams, kStreamStages);
     const size_t steps = (p.rows + G - 1) / (size_t)G;
-    // with fewer steps than that nothing is there to fetch ahead (1000 x 1010 f32, 250 steps:
-    // 9.0 against 6.8 us by a block a row)
-    if (stages < 1 || steps < (size_t)be->sm_count * 2) return false;
+    // With few steps nothing is there to fetch ahead (1000 x 1010 f32, 250 steps: 9.0 against
+    // 6.8 us by a block a row; 296 x 4096 bf16 4.3 against 3.9, 400 rows 4.6 against 6.7).
+    // Of longer rows an SM holds only one such block (148 x 5120 4.7 against 4.1 us, 200 rows
+    // 4.9 against 7.0).
+    const bool few = V == 8 && p.c > 4096 ? p.rows <= (size_t)be->sm_count : steps < (size_t)be->sm_count * 2;
+    if (few) return false;
     static bool attr_set[16] = {};
     if (be->device < 16 && !attr_set[be->device]) {
         *st = dw_cuda_check(
@@ -730,8 +743,9 @@ bool stream_as(dw_backend *be, const Params &p, int T, dw_status *st) {
         if (*st != DW_OK) return true;
         attr_set[be->device] = true;
     }
-    const unsigned grid = (unsigned)std::min<size_t>(steps, (size_t)be->sm_count * per_sm);
-    *st = launch_dependent(be, "norm", kernel, grid, kThreads + 32, stages * stage + weights, 0, p, T, stages, be->wait_cap_ns, be->dev_err);
+    const unsigned grid = (unsigned)std::min<size_t>(steps, (size_t)be->sm_count);
+    *st = launch_dependent(be, "norm", kernel, grid, (kThreads + 32) * teams, teams * stages * stage + weights, 0, p, T, stages,
+                           be->wait_cap_ns, be->dev_err);
     return true;
 }
 
@@ -745,7 +759,11 @@ bool stream(dw_backend *be, const Params &p, int V, dw_status *st) {
         if ((size_t)T * 8 >= p.c) return stream_as<X, R, 8, 1, 256>(be, p, T, st);
         if ((size_t)T * 16 == p.c) return stream_as<X, R, 8, 2, 256, true>(be, p, T, st);
         if ((size_t)T * 16 >= p.c) return stream_as<X, R, 8, 2, 256>(be, p, T, st);
-        if ((size_t)512 * 16 >= p.c) return stream_as<X, R, 8, 2, 512>(be, p, 512, st);
+        // 4096 x 5120 and 4096 x 7168 bf16, both norms: 36.9 and 47.4 us, by rows of 512 threads 56.5
+        // and 59.3; 4096 x 8192 51.8, by 256 threads of 32 elements 51.8 and with one norm 48.4 against 43.9
+        if ((size_t)256 * 24 >= p.c) return stream_as<X, R, 8, 3, 256>(be, p, 256, st);
+        if ((size_t)512 * 16 == p.c) return stream_as<X, R, 8, 2, 512, true>(be, p, 512, st);
+        if ((size_t)256 * 32 >= p.c) return stream_as<X, R, 8, 4, 512>(be, p, 256, st);
         return stream_as<X, R, 8, 4, 512>(be, p, 512, st);
     }
     // an MXFP4 block is 32 / V threads (the same split for every y: the same sums)

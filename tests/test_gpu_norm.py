@@ -140,6 +140,17 @@ def test_norm_residual(be, dtype, res, rows, c, post, pre, gate_rows):
     np.testing.assert_array_equal(be.download_array(s2, np.uint8), be.download_array(s, np.uint8))
 
 
+@pytest.mark.parametrize("dtype,res", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("rows,c,post,pre,gate_rows", [(2000, 4096, RMS, RMS, 0), (2001, 4096, NONE, RMS, None),
+                                                       (149, 5120, RMS, RMS, 0), (901, 5128, LAYER, RMS, 1), (603, 6144, RMS, LAYER, 2),
+                                                       (605, 6152, RMS, RMS, 0), (151, 7168, LAYER, RMS, 3), (603, 8192, RMS, RMS, 1),
+                                                       (605, 8192, NONE, RMS, None), (152, 16384, NONE, RMS, None),
+                                                       (905, 4098, RMS, RMS, 0), (904, 1021, LAYER, RMS, 2),
+                                                       (40000, 64, NONE, RMS, None), (9000, 200, RMS, RMS, 0)])
+def test_rows_that_pass_through_the_ring_more_than_once(be, dtype, res, rows, c, post, pre, gate_rows):
+    test_norm_residual(be, dtype, res, rows, c, post, pre, gate_rows)
+
+
 @pytest.mark.parametrize("rows", [9, 700])
 @pytest.mark.parametrize("c", [200, 199])
 def test_pitches(be, rows, c):
