@@ -763,10 +763,17 @@ bool stream(dw_backend *be, const Params &p, int V, dw_status *st) {
         // and 59.3; 4096 x 8192 51.8, by 256 threads of 32 elements 51.8 and with one norm 48.4 against 43.9
         if ((size_t)256 * 24 >= p.c) return stream_as<X, R, 8, 3, 256>(be, p, 256, st);
         if ((size_t)512 * 16 == p.c) return stream_as<X, R, 8, 2, 512, true>(be, p, 512, st);
-        if ((size_t)256 * 32 >= p.c) return stream_as<X, R, 8, 4, 512>(be, p, 256, st);
+        if ((size_t)256 * 32 >= p.c) {
+            // two rows at once, where the ring has two stages of them (with f32 residuals it has one:
+            // 4096 x 7168 f32 109 against 87 us; R alone decides, so that a norm of `out` has its split)
+            if constexpr (sizeof(R) == 4) return stream_as<X, R, 8, 2, 512>(be, p, 512, st);
+            return stream_as<X, R, 8, 4, 512>(be, p, 256, st);
+        }
+        // (2048 x 11008 f32 68.6 us, with the registers and weights of 32 elements a thread 94.8)
+        if ((size_t)512 * 24 >= p.c) return stream_as<X, R, 8, 3, 512>(be, p, 512, st);
         return stream_as<X, R, 8, 4, 512>(be, p, 512, st);
     }
-    // an MXFP4 block is 32 / V threads (the same split for every y: the same sums)
+    // an MXFP4 block is 32 / V threads (here as above the same split for every y: the same sums)
     int T = 32 / V;
     while ((size_t)T * 16 < p.c && T < 256) T *= 2;
     if (V == 2) {
