@@ -162,6 +162,16 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax) {
     return (uint32_t)max((int)(amax >> 23) - 2, 0);
 }
 
+// The f32 bits of the largest |v| (a NaN where there is one), three to an instruction.
+template <int N>
+__device__ __forceinline__ uint32_t mx_amax(const float (&v)[N]) {
+    float m = fabsf(v[0]);
+    if constexpr (N % 2 == 0) asm("max.NaN.abs.f32 %0, %1, %2, %2;" : "=f"(m) : "f"(v[0]), "f"(v[N - 1]));
+#pragma unroll
+    for (int i = 1; i + 1 < N; i += 2) asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[i]), "f"(v[i + 1]));
+    return __float_as_uint(m);
+}
+
 // 1 / X (scale byte <= 252; 0 for the NaN scale, whose codes are 0).
 __device__ __forceinline__ float mx_inv_scale(uint32_t byte) {
     return byte == 0xFFu ? 0.0f : __uint_as_float((254u - byte) << 23);
@@ -231,10 +241,7 @@ __device__ __forceinline__ float mx_decode1(uint32_t c) {
 
 // 32 values of one thread -> 16 code bytes and the scale byte.
 __device__ __forceinline__ uint32_t mx_quantize32(const float (&v)[32], uint4 &codes) {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 32; i++) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    const uint32_t s = mx_scale_byte(amax);
+    const uint32_t s = mx_scale_byte(mx_amax(v));
     const float inv = mx_inv_scale(s);
     uint32_t c[4];
 #pragma unroll

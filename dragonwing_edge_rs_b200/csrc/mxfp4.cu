@@ -51,10 +51,10 @@ struct Place {
 template <typename T>
 __device__ __forceinline__ uint32_t amax8(const Raw<T, 8> &r) {
     if constexpr (sizeof(T) == 4) {
-        uint32_t m = 0;
+        float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = max(m, r.w[i] & 0x7FFFFFFFu);
-        return m;
+        for (int i = 0; i < 8; i++) v[i] = r.get(i);
+        return mx_amax(v);
     } else {
         // two to a word: magnitudes order like their bits
         uint32_t m = __vmaxu2(__vmaxu2(r.w[0] & 0x7FFF7FFFu, r.w[1] & 0x7FFF7FFFu),

@@ -795,12 +795,10 @@ __global__ void __launch_bounds__(kSkinnyThreads)
             for (int i = 0; i < 4; i++) v[i] = activate(v[i] + bias[i], p.act);
             const size_t row = j;
             if (p.out == 3) {
-                uint32_t amax = 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < 4; i++)
                     if (col + i >= p.n) v[i] = 0.0f;
-                    amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-                }
+                uint32_t amax = mx_amax(v);
 #pragma unroll
                 for (int o = 4; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
                 const uint32_t sb = mx_scale_byte(amax);

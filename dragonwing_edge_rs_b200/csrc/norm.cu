@@ -165,33 +165,31 @@ __device__ __forceinline__ void normalise(float (&v)[N][V], const bool (&live)[N
     }
 }
 
-// One group of V values as MXFP4: 32 / V neighbouring threads hold a block.
-template <int V>
-__device__ __forceinline__ void put_mxfp4(const float (&v)[V], size_t at, size_t row, bool there, const Params &p) {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < V; i++) amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+// One group of V values, from column `at` on, as MXFP4: 32 / V neighbouring threads hold a
+// block.  q, s: the codes of the row, its place in the first scale tile.
+template <int V, typename I>
+__device__ __forceinline__ void put_mxfp4(float (&v)[V], I at, uint8_t *q, uint8_t *s, bool there, const Params &p) {
+    uint32_t amax = mx_amax(v);
 #pragma unroll
     for (int o = 1; o < 32 / V; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     const uint32_t sb = mx_scale_byte(amax);
+    const I block = at / 32;
+    q += at / 2;
+    const float next = V == 1 ? __shfl_down_sync(0xffffffffu, v[0], 1) : 0.0f;
+    if (!there || block >= p.nb) return;
     const float inv = mx_inv_scale(sb);
-    const size_t block = at / 32;
-    uint8_t *dst = p.q + (row * p.nb * 32 + at) / 2;
+    scale_all<V>(v, inv);
     if constexpr (V == 8) {
-        float t[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) t[i] = v[i] * inv;
-        if (there && block < p.nb) *reinterpret_cast<uint32_t *>(dst) = sb == 0xFFu ? 0u : mx_codes8(t);
+        *reinterpret_cast<uint32_t *>(q) = sb == 0xFFu ? 0u : mx_codes8(v);
     } else if constexpr (V == 2) {
-        if (there && block < p.nb) *dst = sb == 0xFFu ? (uint8_t)0 : (uint8_t)mx_codes2(v[0] * inv, v[1] * inv);
+        *q = sb == 0xFFu ? (uint8_t)0 : (uint8_t)mx_codes2(v[0], v[1]);
     } else {
-        const float next = __shfl_down_sync(0xffffffffu, v[0], 1);
-        if ((threadIdx.x & 1) == 0 && there && block < p.nb) *dst = sb == 0xFFu ? (uint8_t)0 : (uint8_t)mx_codes2(v[0] * inv, next * inv);
+        if ((threadIdx.x & 1) == 0) *q = sb == 0xFFu ? (uint8_t)0 : (uint8_t)mx_codes2(v[0], next * inv);
     }
-    if ((at & 31) == 0 && there && block < p.nb) {
-        p.s[mx_scale_at(row, block, p.tiles)] = (uint8_t)sb;
+    if ((at & 31) == 0) {
+        s[(size_t)(block / 4) * 512 + block % 4] = (uint8_t)sb;
         if (block + 1 == p.nb)  // the places of the tile past the last block
-            for (size_t b = p.nb; b < p.tiles * 4; b++) p.s[mx_scale_at(row, b, p.tiles)] = 0;
+            for (size_t b = p.nb; b < p.tiles * 4; b++) s[b / 4 * 512 + b % 4] = 0;
     }
 }
 
@@ -264,7 +262,7 @@ __global__ void __launch_bounds__(kMaxT, V * N <= 8 ? 2 : 1) k_norm(const __grid
         for (int j = 0; j < N; j++) {
             const size_t at = ((size_t)j * T + tid) * V;
             if (p.y_dtype == -2) {
-                put_mxfp4<V>(v[j], at, row, true, p);
+                put_mxfp4<V>(v[j], (uint32_t)at, p.q + row * p.nb * 16, p.s + mx_scale_at(row, 0, p.tiles), true, p);
                 continue;
             }
             if (!live[j]) continue;
@@ -619,8 +617,9 @@ __global__ void __launch_bounds__((kThreads + 32) * stream_teams<R, V, N, kThrea
             }
         }
         if (p.y_dtype == -2) {
+            uint8_t *q = p.q + row * p.nb * 16, *sr = p.s + mx_scale_at(row, 0, p.tiles);
 #pragma unroll
-            for (int j = 0; j < N; j++) put_mxfp4<V>(v[j], column(j), row, there, p);
+            for (int j = 0; j < N; j++) put_mxfp4<V>(v[j], column(j), q, sr, there, p);
         } else if (there) {
             auto store = [&](auto *y) {
                 y += row * p.y_pitch;
@@ -696,7 +695,7 @@ __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Par
             if (p.pre != DW_NORM_NONE) v[0] = scaled(v[0], i, mean, rstd, p.w1, p.b1);
         }
         if (p.y_dtype == -2) {
-            put_mxfp4<1>(v, i, row, true, p);
+            put_mxfp4<1>(v, i, p.q + row * p.nb * 16, p.s + mx_scale_at(row, 0, p.tiles), true, p);
         } else if (i < p.c) {
             const size_t to = row * p.y_pitch + i;
             if (p.y_dtype == DW_F32)
