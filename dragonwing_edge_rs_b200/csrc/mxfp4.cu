@@ -18,8 +18,9 @@ constexpr int kThreads = 256;
 // loads in flight, and its addresses and bounds worked out once.  A thread block is
 // `ux` such units across and kThreads / (16 * ux) rows of a 32-row group down.  Both
 // kernels are near the issue rate, not only the memory's (8192 x 4096 f16 took 19.3 us
-// to quantise at 135 instructions for 8 values, 15.6 at 110, 13.7 now; its bytes take 13.2
-// at the copy rate).
+// to quantise at 135 instructions for 8 values, 15.6 at 110, 13.7 at 80).  With other
+// inputs each time, out of L2, that takes 15.2 us, by stores of single scale bytes 15.6;
+// its bytes take 13.2 at the copy rate.
 constexpr int kRows = 4;
 
 struct Shape {
@@ -31,7 +32,7 @@ struct Shape {
 
 struct Place {
     size_t row, col;  // of the first row's 8 values
-    size_t scale;     // byte of its block's scale; the next rows' are 4 bytes apart each
+    size_t scale;     // byte of the unit's 16 scales: four words, one for each row, of four blocks
     int rows;         // how many of the four rows there are
     bool whole;       // 8 values, loaded or stored at once
     __device__ __forceinline__ explicit Place(const Shape &p) {
@@ -41,7 +42,7 @@ struct Place {
         const size_t unit = ((size_t)blockIdx.y << p.lux) + u, tile = blockIdx.x >> (5 - lr);
         col = (unit << 7) + (threadIdx.x & 15) * 8;
         row = tile * 128 + r32;
-        scale = (tile * p.tiles + unit) * 512 + r32 * 16 + ((threadIdx.x & 15) >> 2);
+        scale = (tile * p.tiles + unit) * 512 + r32 * 16;
         rows = row >= p.rows ? 0 : (int)min((p.rows - row + 31) >> 5, (size_t)kRows);
         whole = p.vec && col + 8 <= p.k;
     }
@@ -160,8 +161,10 @@ __global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *__restrict
         }
     }
     uint8_t *dst = q + (at.row * p.nb * 32 + at.col) / 2;
-    s += at.scale;
-    const bool codes_here = at.col < p.nb * 32, scale_here = (threadIdx.x & 3) == 0 && at.col < p.tiles * 128;
+    s += at.scale;  // the unit's
+    const bool codes_here = at.col < p.nb * 32;
+    const int lane16 = threadIdx.x & 15;
+    uint32_t scales = 0;  // of block lane16 / 4 and row lane16 % 4
 #pragma unroll
     for (int i = 0; i < kRows; i++, dst += p.nb * 512) {
         uint32_t amax = amax8(raw[i]);
@@ -171,10 +174,14 @@ __global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *__restrict
         float v[8];
         scale8(raw[i], mx_inv_scale(sb), v);
         const uint32_t codes = sb == 0xFFu ? 0u : mx_codes8(v);
-        if (i >= at.rows) continue;
-        if (codes_here) *reinterpret_cast<uint32_t *>(dst) = codes;
-        if (scale_here) s[4 * i] = (uint8_t)sb;
+        if ((lane16 & 3) == i) scales = sb;
+        if (i < at.rows && codes_here) *reinterpret_cast<uint32_t *>(dst) = codes;
     }
+    // the unit's 16 scales: a row's four are a word, which the thread of that row stores
+    scales <<= 8 * (lane16 >> 2);
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 8);
+    if (lane16 < at.rows && at.col < p.tiles * 128) *reinterpret_cast<uint32_t *>(s + 4 * lane16) = scales;
 }
 
 template <typename T, bool kVec>
@@ -186,14 +193,19 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__
     if (kVec && at.col >= p.k) return;
     const uint8_t *src = q + (at.row * p.nb * 32 + at.col) / 2;
     s += at.scale;
-    uint32_t codes[kRows], sb[kRows];
+    uint32_t codes[kRows], sb[kRows] = {};
+    if (at.rows && at.col < p.k) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(s));
+        sb[0] = w.x, sb[1] = w.y, sb[2] = w.z, sb[3] = w.w;
+    }
 #pragma unroll
     for (int i = 0; i < kRows; i++, src += p.nb * 512) {
-        codes[i] = sb[i] = 0;
+        codes[i] = 0;
         if (i >= at.rows || at.col >= p.k) continue;
         codes[i] = __ldg(reinterpret_cast<const uint32_t *>(src));
-        sb[i] = __ldg(s + 4 * i);
     }
+#pragma unroll
+    for (int i = 0; i < kRows; i++) sb[i] = (sb[i] >> (8 * ((threadIdx.x & 15) >> 2))) & 0xFFu;
     if constexpr (!kVec) {
         // rows that start anywhere: the 16 threads of a unit write 16 neighbours at a time
         // (each its own 8, one by one, took 5.8 instead of 2.9 us for 1000 x 1010 f32)

@@ -9,7 +9,7 @@
 //
 // Bandwidth-bound: x, res and gate are read once, out and y written once.  Three forms:
 // persistent blocks that stream many rows through a ring (8192 x 4096 bf16 with both
-// norms 44.4 us, 6.0 TB/s; then the issue rate, 470 instructions a warp and row), a block
+// norms 44.4 us, 6.0 TB/s; near the issue rate too), a block
 // a row in registers for few (1 x 4096 2.3 us, latency), and a re-reading one for rows
 // over 16384.
 
