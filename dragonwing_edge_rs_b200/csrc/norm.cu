@@ -434,8 +434,8 @@ __global__ void __launch_bounds__((kThreads + 32) * stream_teams<R, V, N, kThrea
     }
     // c0: what the normalised x of a column is multiplied by (weight, residual scale and,
     // where all rows share it, the gate); w1: the weight of the next norm (both in shared
-    // memory, 16 bytes of a thread beside its neighbour's: registers go to a third block
-    // on the SM instead)
+    // memory, 16 bytes of a thread beside its neighbour's: registers go to a third team
+    // instead)
     float *c0 = reinterpret_cast<float *>(shared + (size_t)teams * stages * stage_bytes), *w1 = c0 + N * T * V;
     bool live[N];
     auto column = [&](int j) { return (uint32_t)(j * T + tid) * V; };
