@@ -309,11 +309,14 @@ struct Span {
         if (to < from) to = from;
     }
     __device__ __forceinline__ uint32_t bytes() const { return (uint32_t)(to - from); }
-    // The bytes at the tensor's ends that it leaves out (fewer than 16 at each).
+    // The bytes at the tensor's ends that it leaves out (fewer than 16 at each): by the calling
+    // thread's own stores, which later bulk copies into the same place have to come after.
     __device__ __forceinline__ void edges(uint8_t *dst, const uint8_t *src, uint32_t bytes) const {
         const uintptr_t a = (uintptr_t)src, e = a + bytes;
+        if (from <= a && to >= e) return;
         for (uintptr_t q = a; q < e && q < from; q++) dst[q - base] = *(const uint8_t *)q;
         for (uintptr_t q = to > a ? to : a; q < e; q++) dst[q - base] = *(const uint8_t *)q;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
 };
 
@@ -413,6 +416,7 @@ __global__ void __launch_bounds__((kThreads + 32) * stream_teams<R, V, N, kThrea
                     span.edges(ring + at, src, n);
                 });
                 bytes = __reduce_add_sync(0xffffffffu, bytes);
+                __syncwarp();  // every lane's edges come before the arrive (the sum orders no memory)
                 if (lane == 0) mbar_expect_tx(bar, bytes);
                 __syncwarp();
                 copies([&](const uint8_t *src, uint32_t n, const uint8_t *first, const uint8_t *last, uint32_t at) {
