@@ -153,8 +153,13 @@ __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 
 // silu(v) = v / (1 + e^-v) by ex2.approx and rcp.approx: a relative error of a few
 // 2^-24 plus |v| * 2^-24 (the exponent's rounding).  e^-v = inf gives v * 0 = -0.
+// A NaN stays one through either (a plain fmaxf would make it 0).
 __device__ __forceinline__ float activate(float v, int act) {
-    if (act == DW_EPI_RELU) return fmaxf(v, 0.0f);
+    if (act == DW_EPI_RELU) {
+        float r;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(0.0f));
+        return r;
+    }
     if (act == DW_EPI_SILU) {
         float r;
         asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + __expf(-v)));

@@ -537,7 +537,8 @@ DW_API dw_status dw_pack_scales_mxfp4(dw_backend *be, const dw_buf *scales, size
 /* y[m, n] = act(sum_k A[m, k] * B[n, k] + bias[n]): A an operand of m rows, B (a
  * weight, [out, in]) one of n rows, bias f32 [n] or NULL, act DW_EPI_NONE,
  * DW_EPI_RELU or DW_EPI_SILU in f32, y [m, n] of y_dtype, rounded once.  Sums are
- * f32, in an order that depends on m, n and k alone.  y overlaps no operand. */
+ * f32, in an order that depends on m, n and k alone.  A NaN stays NaN through every
+ * activation.  y overlaps no operand. */
 DW_API dw_status dw_gemm_mxfp4(dw_backend *be, const dw_buf *a_q, const dw_buf *a_s, const dw_buf *b_q, const dw_buf *b_s,
                                const dw_buf *bias, dw_buf *y, int y_dtype, size_t m, size_t n, size_t k, int act);
 /* The same with the result, unrounded, as an MXFP4 operand of m rows of n values:
