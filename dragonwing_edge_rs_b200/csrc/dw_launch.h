@@ -4,7 +4,9 @@
 // its writes are visible.  Each block then calls pdl_trigger(): not before pdl_wait()
 // (kernels waiting in a row would fill the SMs: quantise and dequantise of 1000 x 1010
 // f32 took 18 instead of 9 us), and after any tcgen05.alloc (a dependent block that
-// took tensor memory first would wait for a kernel that waits for it).
+// took tensor memory first would wait for a kernel that waits for it).  What such a kernel
+// reads may be written during its own life, so it reads by ordinary loads: no __ldg and no
+// `const T *__restrict__`, whose loads may be moved above the wait and past coherence.
 #pragma once
 
 #include <cstdlib>

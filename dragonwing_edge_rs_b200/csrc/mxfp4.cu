@@ -138,8 +138,8 @@ __device__ __forceinline__ void scale8(const Raw<T, 8> &r, float inv, float (&v)
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *__restrict__ x, uint8_t *__restrict__ q,
-                                                             uint8_t *__restrict__ s, const __grid_constant__ Shape p) {
+__global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *x, uint8_t *q, uint8_t *s,
+                                                             const __grid_constant__ Shape p) {
     pdl_wait();
     pdl_trigger();
     const Place at(p);
@@ -185,8 +185,8 @@ __global__ void __launch_bounds__(kThreads) k_quantize_mxfp4(const T *__restrict
 }
 
 template <typename T, bool kVec>
-__global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__restrict__ q, const uint8_t *__restrict__ s,
-                                                               T *__restrict__ y, const __grid_constant__ Shape p) {
+__global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *q, const uint8_t *s, T *y,
+                                                               const __grid_constant__ Shape p) {
     pdl_wait();
     pdl_trigger();
     const Place at(p);
@@ -195,14 +195,14 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__
     s += at.scale;
     uint32_t codes[kRows], sb[kRows] = {};
     if (at.rows && at.col < p.k) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(s));
+        const uint4 w = *reinterpret_cast<const uint4 *>(s);
         sb[0] = w.x, sb[1] = w.y, sb[2] = w.z, sb[3] = w.w;
     }
 #pragma unroll
     for (int i = 0; i < kRows; i++, src += p.nb * 512) {
         codes[i] = 0;
         if (i >= at.rows || at.col >= p.k) continue;
-        codes[i] = __ldg(reinterpret_cast<const uint32_t *>(src));
+        codes[i] = *reinterpret_cast<const uint32_t *>(src);
     }
 #pragma unroll
     for (int i = 0; i < kRows; i++) sb[i] = (sb[i] >> (8 * ((threadIdx.x & 15) >> 2))) & 0xFFu;
@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *__
 
 // Row-major scales [rows][nb] -> tiles; the places of a tile past the last block
 // get byte 0 (rows past the last are left as they are).  One thread per (row, tile).
-__global__ void __launch_bounds__(kThreads) k_pack_scales(const uint8_t *__restrict__ in, uint8_t *__restrict__ s,
-                                                          size_t rows, size_t nb, size_t tiles) {
+__global__ void __launch_bounds__(kThreads) k_pack_scales(const uint8_t *in, uint8_t *s, size_t rows, size_t nb,
+                                                          size_t tiles) {
     pdl_wait();
     pdl_trigger();
     const size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x;

@@ -182,13 +182,13 @@ __device__ __forceinline__ void finish32(float (&v)[32], size_t col, const GemmP
         if (col + 32 <= p.n && p.bias_vec) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float4 b = __ldg(reinterpret_cast<const float4 *>(p.bias + col) + i);
+                const float4 b = reinterpret_cast<const float4 *>(p.bias + col)[i];
                 v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < 32; i++)
-                if (col + i < p.n) v[i] += __ldg(p.bias + col + i);
+                if (col + i < p.n) v[i] += p.bias[col + i];
         }
     }
     if (p.act == DW_EPI_RELU) {
@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
         const size_t col = n0 + 4 * lane;
         float bias[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) bias[i] = p.bias && col + i < p.n ? __ldg(p.bias + col + i) : 0.0f;
+        for (int i = 0; i < 4; i++) bias[i] = p.bias && col + i < p.n ? p.bias[col + i] : 0.0f;
         const int rows = (int)p.m;
         for (int j = (int)rank + (int)S * warp; j < rows; j += (kSkinnyThreads / 32) * (int)S) {
             const uint32_t addr = smem_u32(part + j * 128 + 4 * lane);
