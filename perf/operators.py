@@ -190,6 +190,8 @@ def _gain(g, c):
 
 def prepare(case, seed):
     c = case
+    if own:
+        _open()
     g = torch.Generator(device="cuda").manual_seed(int(seed))
     dev = "cuda"
     s = {"case": c}
@@ -235,12 +237,18 @@ def _tile_bytes(rows, k):
     return ((rows + 127) // 128) * ((_blocks(k) + 3) // 4) * 512
 
 
-def _wrap(s):
+def _open():
+    """The backend, with its stream as torch's current one: inputs are made before the operators read them, and
+    what torch does with the outputs comes after them."""
     global _backend
     import dragonwing_edge_rs_b200 as dw
-    from dragonwing_edge_rs_b200 import ops
     if _backend is None:
         _backend = dw.CudaBackend(torch.cuda.current_device())
+    torch.cuda.set_stream(torch.cuda.ExternalStream(_backend.stream()))
+
+
+def _wrap(s):
+    from dragonwing_edge_rs_b200 import ops
     be, c = _backend, s["case"]
     s["b"] = b = {n: be.wrap(t.data_ptr(), ((t.shape[0] - 1) * t.stride(0) + t.shape[-1] if t.dim() == 2 else t.numel()) * t.element_size())
                   for n, t in s.items() if isinstance(t, torch.Tensor)}
