@@ -921,12 +921,13 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
     unsigned S = 1;
     const unsigned most = per_sm == 2 ? 8 : 4;
     while (S < most && 2 * S * tn <= (size_t)be->sm_count * 4 / 3 && 2 * (int)S <= p.k_blocks) S *= 2;
-    // The ring: no longer than a CTA's K blocks, and of three stages where the CTAs outnumber
-    // the SMs and have few blocks each: a third of them then fits beside two others, or
-    // the next launch's (11008 outputs, K 4096, one row 6.4 -> 5.3 us)
+    // The ring: no longer than a CTA's K blocks, and of at most three stages where the CTAs
+    // outnumber the SMs and have few blocks each: a third of them then fits beside two others,
+    // or the next launch's (11008 outputs, K 4096, one row 6.4 -> 5.5 us; 65536 outputs, K 256,
+    // where a ring of three stages would hold two that nothing fills: 5.2 -> 4.5 us)
     const int own = (p.k_blocks + (int)S - 1) / (int)S;
     p.stages = (int)std::min<size_t>(kSkinnyStages, ((kSmemLimit - 8192) / per_sm - 2048) / p.stage_bytes);
-    p.stages = std::min(p.stages, p.bn <= 32 && S * tn > (size_t)be->sm_count && own <= 8 ? 3 : own);
+    p.stages = std::min(p.stages, p.bn <= 32 && S * tn > (size_t)be->sm_count && own <= 8 ? std::min(own, 3) : own);
     // Tensor memory: accumulators and 16 columns a stage.  A CTA takes no larger share of an
     // SM's 512 columns than of its shared memory, so those that fit together, of this launch
     // and others, find columns: none waits for another's, which might itself wait for a
