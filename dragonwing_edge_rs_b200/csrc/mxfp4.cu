@@ -232,15 +232,9 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *q,
         const float X = mx_scale(sb[i]);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] *= X;
-        if (at.whole) {
-            Raw<T, 8> r;
-            r.set(v);
-            store_wide(r, dst);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (at.col + j < p.k) dst[j] = from_f32<T>(v[j]);
-        }
+        Raw<T, 8> r;  // all 8 lie in the row: k is a multiple of 8 here
+        r.set(v);
+        store_wide(r, dst);
     }
 }
 
