@@ -67,7 +67,8 @@ __device__ __forceinline__ uint32_t amax8(const Raw<T, 8> &r) {
 }
 
 // 8 elements from anywhere: the widest accesses that the address allows; 16-bit elements
-// at an odd place from the five words around them, where these lie in [first, last).
+// at an odd place from the five words around them, where these lie in [first, last)
+// (8192 x 4095 f16 22.9 us with its rows at every phase, 8192 x 4096 15.3).
 template <typename T>
 __device__ __forceinline__ void load_any(Raw<T, 8> &r, const T *src, const T *first, const T *last) {
     const uint32_t a = (uint32_t)(uintptr_t)src & 15;
@@ -208,7 +209,8 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *q,
     for (int i = 0; i < kRows; i++) sb[i] = (sb[i] >> (8 * ((threadIdx.x & 15) >> 2))) & 0xFFu;
     if constexpr (!kVec) {
         // rows that start anywhere: the 16 threads of a unit write 16 neighbours at a time
-        // (each its own 8, one by one, took 5.8 instead of 2.9 us for 1000 x 1010 f32)
+        // (each its own 8, one by one, took 5.8 instead of 2.6 us for 1000 x 1010 f32).  Two
+        // shuffles and a store an element: 8192 x 4095 f16 28.2 us, 8192 x 4096 15.0.
         const int lane16 = threadIdx.x & 15;
         const size_t col0 = at.col - lane16 * 8;
         T *dst = y + at.row * p.k + col0 + lane16;
@@ -239,7 +241,8 @@ __global__ void __launch_bounds__(kThreads) k_dequantize_mxfp4(const uint8_t *q,
 }
 
 // Row-major scales [rows][nb] -> tiles; the places of a tile past the last block
-// get byte 0 (rows past the last are left as they are).  One thread per (row, tile).
+// get byte 0 (rows past the last are left as they are).  One thread per (row, tile), four
+// byte loads each: 11008 x 4096 3.9 us against 0.4 for its bytes, once for a weight.
 __global__ void __launch_bounds__(kThreads) k_pack_scales(const uint8_t *in, uint8_t *s, size_t rows, size_t nb,
                                                           size_t tiles) {
     pdl_wait();

@@ -16,9 +16,11 @@
 // What bounds them (B200): with many rows each SM's intake from L2 -- a stage of 512 codes
 // is 70 KB for 256 x 256 outputs (0.63 us; 0.54 us at the tensor rate) and 52 KB for
 // 256 x 128 (0.36 us) -- and beyond one round of tiles the power limit; 8192^3 runs at
-// 5.7 PFLOP/s, 4096^3 at 4.5.  With few rows the weights' bytes and about 2.3 us of
-// launch, first copies and hand-offs: 11008 x 4096 (24 MB) 5.4 us from L2, 7.6 from HBM.
-// What a step of it cost and saved stands beside each part.
+// 5.4 to 5.7 PFLOP/s (193 to 205 us), 4096^3 at 4.4 (31 us), in a sustained loop at 3.8
+// (36 us).  With few rows the weights' bytes and about 2.3 us of
+// launch, first copies and hand-offs: 11008 x 4096 (24 MB) 5.5 us from L2, 7.6 from HBM.
+// What a step of it cost and saved stands beside each part: launches in a row in short
+// runs, measured when the step was made.
 //
 // Every mbarrier wait is bounded; on expiry the CTA records the failure, waits
 // (bounded) for its own copies and products in flight, frees its tensor memory
@@ -228,7 +230,9 @@ __device__ __forceinline__ void store64(uint32_t (&w)[16], size_t row, size_t co
         if (row0 + k < p.m) *reinterpret_cast<uint4 *>(dst + k * p.n) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
 }
 
-// What the epilogue stores: 0 f32, 1 f16, 2 bf16, 3 MXFP4.
+// What the epilogue stores: 0 f32, 1 f16, 2 bf16, 3 MXFP4.  Rows of y that do not start on
+// 16 bytes are written one element a lane, a row a lane (4096 x 4001 x 4096 f16 186 us,
+// 4096 x 4000 x 4096 31).
 template <int kOut>
 __device__ __forceinline__ void put32(float (&v)[32], size_t row, size_t col, const GemmParams &p, uint32_t &scale) {
     if constexpr (kOut == 3) {
@@ -955,7 +959,8 @@ dw_status launch_skinny(dw_backend *be, const MxGemmArgs &a) {
 
 }  // namespace
 
-// Which kernel, tile and split of K (times on B200, launches in a row, us):
+// Which kernel, tile and split of K (times on B200, launches in a row on the same operands
+// unless said, us; between the shapes named the rules are not measured):
 //   few rows: up to 64 (m 64, n 11008, k 4096: 7.7 against 9.5), or up to 128 where the
 //     pairs would have few tiles of a long K (m 128, k 4096: n 1000 5.8 against 7.0, n 4096
 //     6.9 against 6.5; k 11008, n 4096: 8.9 against 10.3);

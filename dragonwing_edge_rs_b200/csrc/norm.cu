@@ -9,9 +9,11 @@
 //
 // Bandwidth-bound: x, res and gate are read once, out and y written once.  Three forms:
 // persistent blocks that stream many rows through a ring (8192 x 4096 bf16 with both
-// norms 44.4 us, 6.0 TB/s; near the issue rate too), a block
+// norms 45.6 us, 5.9 TB/s; near the issue rate too), a block
 // a row in registers for few (1 x 4096 2.3 us, latency), and a re-reading one for rows
-// over 16384.
+// over 16384.  Times here and below are of launches in a row in short runs; the lower
+// clock of a sustained loop costs some 10% (50 us).  Those beside a choice compare its two
+// sides at the time it was made.
 
 #include <algorithm>
 
@@ -644,7 +646,9 @@ __global__ void __launch_bounds__((kThreads + 32) * stream_teams<R, V, N, kThrea
 }
 
 // Rows too long for registers: one thread block a row, elements read again for
-// each reduction (from L2) and `out` read back by the thread that wrote it.
+// each reduction (from L2) and `out` read back by the thread that wrote it.  Bound by its
+// single-element accesses, and by the SMs that few rows leave idle (both norms, bf16:
+// 64 x 40000 75 us against 3.2 for its bytes, 8192 x 20000 1038 against 203).
 template <typename X, typename R>
 __global__ void __launch_bounds__(kMaxT) k_norm_long(const __grid_constant__ Params p) {
     __shared__ __align__(16) float red[4][16];
