@@ -72,6 +72,30 @@ class DwNormDesc(ctypes.Structure):
         [("eps", ctypes.c_float), ("res_scale", ctypes.c_float)]
 
 
+class DwHeads(ctypes.Structure):
+    """dw_heads: [rows, heads, head_dim] inside wider rows (element offset, row pitch)."""
+    _fields_ = [("buf", ctypes.c_void_p), ("offset", ctypes.c_size_t), ("pitch", ctypes.c_size_t)]
+
+
+class DwHeadDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("q_heads", "kv_heads", "head_dim", "rot_dim", "dtype", "norm", "neighbours")] + \
+        [("eps", ctypes.c_float)]
+
+
+class DwKvCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("pages", ctypes.c_size_t)] + \
+        [(n, ctypes.c_int32) for n in ("kv_heads", "page_tokens", "head_dim")]
+
+
+class DwSequences(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("table", "lens", "starts")] + \
+        [(n, ctypes.c_size_t) for n in ("seqs", "tokens", "width")]
+
+
+class DwAttentionDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("q_heads", "dtype", "causal", "window")] + [("scale", ctypes.c_float)]
+
+
 # Every exported function with its argument types (restype is dw_status unless listed).
 vp, sz, i32, u32, f32 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_uint32, ctypes.c_float
 PDESC = ctypes.POINTER(DwConvDesc)
@@ -168,6 +192,14 @@ SIGNATURES = {
     "dw_norm_to_mxfp4": ([vp, ctypes.POINTER(DwNormDesc)] + [vp] * 5, i32),
     "dw_norm_residual": ([vp, ctypes.POINTER(DwNormDesc)] + [vp] * 9, i32),
     "dw_norm_residual_to_mxfp4": ([vp, ctypes.POINTER(DwNormDesc)] + [vp] * 10, i32),
+    # attention: head norms with the rotation, the paged 8-bit cache
+    "dw_prepare_rope": ([vp, ctypes.POINTER(ctypes.c_double), sz, PVP], i32),
+    "dw_norm_rope": ([vp, vp, sz] + [vp] * 8, i32),
+    "dw_kv_code_bytes": ([sz] * 4, sz),
+    "dw_kv_scale_bytes": ([sz] * 2, sz),
+    "dw_append_kv": ([vp] * 11, i32),
+    "dw_read_kv": ([vp, vp, vp, i32, vp, vp], i32),
+    "dw_attention_kv8": ([vp] * 6, i32),
     "dw_postprocess_yolo": ([vp, vp, sz, sz, sz, u32, u32, f32, f32, ctypes.c_int32, vp, vp, vp], i32),
 }
 

@@ -184,4 +184,35 @@ struct NormArgs {
 };
 dw_status launch_norm(dw_backend *be, const dw_norm_desc &d, const NormArgs &a);
 
+// The paged 8-bit key/value cache and the sequences of a call, as kernels see them.
+struct KvCache {
+    uint8_t *k, *v, *s;
+    uint32_t pages;
+    int heads, page, d;
+};
+struct Seqs {
+    const int32_t *table, *lens, *starts;  // starts: may be null
+    uint32_t seqs, tokens, width;
+};
+// [rows, heads, head_dim] in rows `pitch` elements apart; ptr null: absent.
+struct HeadRows {
+    void *ptr;
+    size_t pitch;
+};
+
+// heads.cu (head norms with the rotation, append to and read from the cache)
+struct HeadArgs {
+    HeadRows q, k, v, q_out, k_out;
+    const float *w_q, *w_k;
+    const uint64_t *rope;      // turns a position, fractions of 2^64; null: no rotation
+    const int32_t *positions;  // norm_rope alone
+};
+dw_status launch_norm_rope(dw_backend *be, const dw_head_desc &d, size_t tokens, const HeadArgs &a);
+dw_status launch_append_kv(dw_backend *be, const dw_head_desc &d, const KvCache &c, const Seqs &s, const HeadArgs &a);
+dw_status launch_read_kv(dw_backend *be, const KvCache &c, const Seqs &s, int dtype, const HeadRows &k, const HeadRows &v);
+
+// attention.cu (attention over the cache)
+dw_status launch_attention_kv8(dw_backend *be, const dw_attention_desc &d, const KvCache &c, const Seqs &s, const HeadRows &q,
+                               const HeadRows &out);
+
 }  // namespace dw

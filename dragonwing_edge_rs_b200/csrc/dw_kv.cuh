@@ -1,0 +1,110 @@
+// dw_kv.cuh -- device helpers of the paged 8-bit key/value cache: which rows and tokens a
+// sequence has, where its pages lie, and the e4m3 codes.
+//
+// A block (a page's tokens of one head) has one scale X = 2^e for its keys and one for its
+// values, held as the byte e + 127, e in [-64, 63].  The bounds keep every exponent that
+// attention forms from two of them inside f32.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "dw_device.cuh"
+
+namespace dw {
+
+constexpr int kKvMinExp = -64, kKvMaxExp = 63;
+
+__device__ __forceinline__ size_t kv_block(const KvCache &c, uint32_t page, int head) { return (size_t)page * c.heads + head; }
+__device__ __forceinline__ uint8_t *kv_codes(uint8_t *codes, const KvCache &c, uint32_t page, int head) {
+    return codes + kv_block(c, page, head) * (size_t)(c.page * c.d);
+}
+// A scale byte's exponent, whatever the byte.
+__device__ __forceinline__ int kv_exponent(uint32_t byte) { return min(max((int)byte - 127, kKvMinExp), kKvMaxExp); }
+__device__ __forceinline__ float kv_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The smallest e with amax <= 448 * 2^e; amax >= 0 finite, as f32 rounded to odd or exact
+// (448 * 2^e has an even last bit, so the rounding does not move a value past it).
+__device__ __forceinline__ int kv_scale_exponent(float amax) {
+    const uint32_t u = __float_as_uint(amax);  // 448 = 1.75 * 2^8
+    const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u);
+    return min(max(e, kKvMinExp), kKvMaxExp);
+}
+
+// Two f32 -> e4m3 codes (the first in the low byte), to nearest even, 448 at most, NaN 0x7F.
+__device__ __forceinline__ uint32_t e4m3_codes2(float a, float b) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The two codes of a half word as f16 values (exact).
+__device__ __forceinline__ uint32_t e4m3_to_f16x2(uint16_t c) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
+    return r;
+}
+__device__ __forceinline__ float2 e4m3_to_f32x2(uint16_t c) {
+    const uint32_t r = e4m3_to_f16x2(c);
+    __half2 h;
+    memcpy(&h, &r, 4);
+    return __half22float2(h);
+}
+
+// ---- sequences -----------------------------------------------------------------
+struct SeqRange {
+    int row0, n;  // its rows
+    int len;      // its tokens in the cache
+    __device__ __forceinline__ int position(int row) const { return len - n + (row - row0); }
+};
+
+__device__ __forceinline__ int seq_start(const Seqs &q, uint32_t s) {
+    if (!q.starts) return (int)(s * (q.tokens / q.seqs));
+    return min(max(q.starts[s], 0), (int)q.tokens);
+}
+
+__device__ __forceinline__ SeqRange seq_range(const Seqs &q, uint32_t s, int page, int32_t *err) {
+    SeqRange r;
+    const int most = (int)min((uint64_t)q.width * page, (uint64_t)0x7fffff00u), len = q.lens[s];
+    r.row0 = seq_start(q, s);
+    r.n = seq_start(q, s + 1) - r.row0;
+    r.len = min(max(len, 0), most);
+    bool bad = len != r.len || r.n < 0;
+    if (q.starts) bad |= q.starts[s] != r.row0 || q.starts[s + 1] != r.row0 + r.n;
+    if (bad) record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
+    r.n = max(r.n, 0);
+    return r;
+}
+
+// Items of work, cut from each sequence's rows: sequence s owns the items from start(s) *
+// per / size + extra * s on, which are at least floor(n * per / size) + extra.  A call launches
+// as many as its totals allow (they are known on the host, the sequences' own are not);
+// items that a sequence has too many are empty.
+__host__ __device__ inline size_t seq_items(size_t tokens, size_t seqs, int per, int size, int extra) {
+    return tokens * per / size + extra * seqs;
+}
+// The sequence of item w and its place there (below 0: of no sequence); a whole warp calls.
+__device__ __forceinline__ uint32_t seq_of_item(const Seqs &q, int64_t w, int per, int size, int extra, int64_t &place) {
+    const int lane = threadIdx.x & 31;
+    auto first = [&](uint32_t s) { return (int64_t)seq_start(q, s) * per / size + (int64_t)extra * s; };
+    uint32_t lo = 0, count = q.seqs;
+    while (count > 1) {  // the last of 32 evenly spaced ones that does not start behind w
+        const uint32_t step = (count + 31) / 32, at = (uint32_t)lane * step;
+        const uint32_t mask = __ballot_sync(0xffffffffu, at < count && first(lo + at) <= w) | 1u;
+        const uint32_t k = 31 - __clz(mask);
+        lo += k * step;
+        count = min(step, count - k * step);
+    }
+    place = w - first(lo);
+    return lo;
+}
+
+// The page of a sequence's token `t`, in bounds in any case.
+__device__ __forceinline__ uint32_t seq_page(const Seqs &q, const KvCache &c, uint32_t s, uint32_t index, int32_t *err) {
+    const uint32_t id = (uint32_t)q.table[(size_t)s * q.width + index];
+    if (id < c.pages) return id;
+    record_error(err, DW_DEV_BAD_ARG, 62, (int)s);
+    return 0;
+}
+
+}  // namespace dw

@@ -1114,3 +1114,227 @@ DW_API dw_status dw_norm_residual_to_mxfp4(dw_backend *be, const dw_norm_desc *d
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Attention: head norms with the rotation, the paged 8-bit cache, attention over it
+// ---------------------------------------------------------------------------
+
+namespace {
+
+// A present dw_heads of `rows` rows that reaches to its last element; *out its place.
+dw_status check_heads(dw_backend *be, const dw_heads *h, size_t rows, int heads, int d, int dtype, const char *op, const char *name,
+                      dw::HeadRows *out) {
+    if (!h || !h->buf) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %s is null", op, name);
+    const size_t width = (size_t)heads * d, pitch = h->pitch ? h->pitch : width, es = esize(dtype);
+    if (pitch < width) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %s pitch %zu is below the row's %zu", op, name, pitch, width);
+    if (!fits62(rows, pitch, es) || h->offset > ((size_t)1 << 60))
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %s is too large", op, name);
+    const size_t len = (h->offset + (rows - 1) * pitch + width) * es;
+    if (h->buf->len < len)
+        return dw_fail(be, DW_ERR_SIZE_MISMATCH, "%s: %s mismatch: needs %zu bytes, got %zu", op, name, len, h->buf->len);
+    DW_TRY(check_align(be, h->buf, es, op, name));
+    out->ptr = (char *)h->buf->ptr + h->offset * es, out->pitch = pitch;
+    return DW_OK;
+}
+
+// The head descriptor and the rotations' table.
+dw_status check_head_desc(dw_backend *be, const dw_head_desc *d, const dw_buf *rope, const char *op, dw::HeadArgs *a) {
+    if (!d) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: descriptor is null", op);
+    DW_TRY(check_dtype(be, d->dtype, op, "dtype"));
+    if (d->q_heads <= 0 || d->kv_heads <= 0 || d->q_heads > 65536 || d->kv_heads > 65536)
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: head counts must be 1 to 65536", op);
+    if (d->head_dim <= 0 || d->head_dim % 2 || d->head_dim > 512)
+        return dw_fail(be, DW_ERR_UNSUPPORTED, "%s: head_dim must be even and at most 512, not %d", op, d->head_dim);
+    if (d->rot_dim < 0 || d->rot_dim % 2 || d->rot_dim > d->head_dim)
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: rot_dim must be even and at most head_dim, not %d", op, d->rot_dim);
+    if (d->norm < DW_NORM_NONE || d->norm > DW_NORM_LAYER) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: unknown norm kind", op);
+    if (!(d->eps >= 0.0f)) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: eps must be >= 0", op);
+    if (d->rot_dim) {
+        DW_TRY(check_vec(be, rope, d->rot_dim / 2, 8, op, "rope"));
+        a->rope = (const uint64_t *)rope->ptr;
+    } else if (rope) {
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: rope is given but rot_dim is 0", op);
+    }
+    return DW_OK;
+}
+
+dw_status check_weight(dw_backend *be, const dw_head_desc *d, const dw_buf *w, const char *op, const float **out) {
+    if (!w) return DW_OK;
+    DW_TRY(check_vec(be, w, d->head_dim, 4, op, "norm weight"));
+    *out = (const float *)w->ptr;
+    return DW_OK;
+}
+
+dw_status check_cache(dw_backend *be, const dw_kv_cache *c, const char *op, dw::KvCache *out) {
+    if (!c || !c->k || !c->v || !c->scales) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: cache is null", op);
+    if (!c->pages || c->kv_heads <= 0 || c->kv_heads > 65536) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: pages and kv_heads must be positive", op);
+    if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128)
+        return dw_fail(be, DW_ERR_UNSUPPORTED, "%s: page_tokens must be 16, 32, 64 or 128, not %d", op, c->page_tokens);
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return dw_fail(be, DW_ERR_UNSUPPORTED, "%s: the cache's head_dim must be 64 or 128, not %d", op, c->head_dim);
+    if ((long double)c->pages * c->kv_heads * c->page_tokens > 2147483647.0L)
+        return dw_fail(be, DW_ERR_UNSUPPORTED, "%s: the cache holds more than 2^31 - 1 heads of tokens", op);
+    const size_t codes = dw_kv_code_bytes(c->pages, c->kv_heads, c->page_tokens, c->head_dim);
+    DW_TRY(check_len(be, c->k, codes, op, "keys"));
+    DW_TRY(check_len(be, c->v, codes, op, "values"));
+    DW_TRY(check_len(be, c->scales, dw_kv_scale_bytes(c->pages, c->kv_heads), op, "scales"));
+    DW_TRY(check_align(be, c->k, 16, op, "keys"));
+    DW_TRY(check_align(be, c->v, 16, op, "values"));
+    DW_TRY(check_align(be, c->scales, 2, op, "scales"));
+    out->k = (uint8_t *)c->k->ptr, out->v = (uint8_t *)c->v->ptr, out->s = (uint8_t *)c->scales->ptr;
+    out->pages = (uint32_t)c->pages, out->heads = c->kv_heads, out->page = c->page_tokens, out->d = c->head_dim;
+    return DW_OK;
+}
+
+dw_status check_seqs(dw_backend *be, const dw_sequences *s, int page, const char *op, dw::Seqs *out) {
+    if (!s) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: sequences are null", op);
+    DW_TRY(check_dims(be, s->seqs, s->tokens, op));
+    DW_TRY(check_dims(be, s->width, 1, op));
+    if (s->width > 0x7fffff00u / (unsigned)page) return dw_fail(be, DW_ERR_UNSUPPORTED, "%s: a sequence may have 2^31 tokens or more", op);
+    DW_TRY(need(be, s->table, op, "table"));
+    if (!fits62(s->seqs, s->width, 4)) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: table is too large", op);
+    DW_TRY(check_vec(be, s->table, s->seqs * s->width, 4, op, "table"));
+    DW_TRY(check_vec(be, s->lens, s->seqs, 4, op, "lens"));
+    if (s->starts)
+        DW_TRY(check_vec(be, s->starts, s->seqs + 1, 4, op, "starts"));
+    else if (s->tokens % s->seqs)
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %zu rows are no whole number for each of %zu sequences", op, s->tokens, s->seqs);
+    out->table = (const int32_t *)s->table->ptr, out->lens = (const int32_t *)s->lens->ptr;
+    out->starts = s->starts ? (const int32_t *)s->starts->ptr : nullptr;
+    out->seqs = (uint32_t)s->seqs, out->tokens = (uint32_t)s->tokens, out->width = (uint32_t)s->width;
+    return DW_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+DW_API size_t dw_kv_code_bytes(size_t pages, size_t kv_heads, size_t page_tokens, size_t head_dim) {
+    return pages * kv_heads * page_tokens * head_dim;
+}
+DW_API size_t dw_kv_scale_bytes(size_t pages, size_t kv_heads) { return pages * kv_heads * 2; }
+
+DW_API dw_status dw_prepare_rope(dw_backend *be, const double *freqs, size_t pairs, dw_buf **out) {
+    const char *op = "prepare_rope";
+    if (!be) return DW_ERR_INVALID_ARG;
+    DW_TRY(need(be, out, op, "out"));
+    *out = nullptr;
+    DW_TRY(need(be, freqs, op, "freqs"));
+    if (!pairs || pairs > 256) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: 1 to 256 pairs, not %zu", op, pairs);
+    uint64_t turns[256];
+    const long double two_pi = 6.283185307179586476925286766559005768L;
+    for (size_t i = 0; i < pairs; i++) {
+        if (!std::isfinite(freqs[i])) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: freqs[%zu] is not finite", op, i);
+        long double t = (long double)freqs[i] / two_pi;
+        t = (t - floorl(t)) * 18446744073709551616.0L;  // [0, 1) of a turn, in 2^-64; 1 (by rounding) is 0
+        turns[i] = t >= 18446744073709551616.0L ? 0 : (uint64_t)t;
+    }
+    dw_buf *b = nullptr;
+    DW_TRY(dw_alloc(be, pairs * 8, &b));
+    const dw_status st = dw_upload(be, b, turns, pairs * 8);
+    if (st != DW_OK) {
+        dw_free(be, b);
+        return st;
+    }
+    *out = b;
+    return DW_OK;
+}
+
+DW_API dw_status dw_norm_rope(dw_backend *be, const dw_head_desc *d, size_t tokens, const dw_heads *q, const dw_heads *k,
+                              const dw_buf *w_q, const dw_buf *w_k, const dw_buf *rope, const dw_buf *positions,
+                              const dw_heads *q_out, const dw_heads *k_out) {
+    const char *op = "norm_rope";
+    if (!be) return DW_ERR_INVALID_ARG;
+    dw::HeadArgs a{};
+    DW_TRY(check_head_desc(be, d, rope, op, &a));
+    DW_TRY(check_dims(be, tokens, 1, op));
+    if (!q && !k) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: neither q nor k is given", op);
+    if (!q != !q_out || !k != !k_out) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: an input and its output go together", op);
+    if (q) {
+        DW_TRY(check_heads(be, q, tokens, d->q_heads, d->head_dim, d->dtype, op, "q", &a.q));
+        DW_TRY(check_heads(be, q_out, tokens, d->q_heads, d->head_dim, d->dtype, op, "q_out", &a.q_out));
+    }
+    if (k) {
+        DW_TRY(check_heads(be, k, tokens, d->kv_heads, d->head_dim, d->dtype, op, "k", &a.k));
+        DW_TRY(check_heads(be, k_out, tokens, d->kv_heads, d->head_dim, d->dtype, op, "k_out", &a.k_out));
+    }
+    DW_TRY(check_weight(be, d, w_q, op, &a.w_q));
+    DW_TRY(check_weight(be, d, w_k, op, &a.w_k));
+    if (d->rot_dim) {
+        DW_TRY(check_vec(be, positions, tokens, 4, op, "positions"));
+        a.positions = (const int32_t *)positions->ptr;
+    }
+    cudaSetDevice(be->device);
+    return dw::launch_norm_rope(be, *d, tokens, a);
+}
+
+DW_API dw_status dw_append_kv(dw_backend *be, const dw_head_desc *d, const dw_kv_cache *cache, const dw_sequences *seqs,
+                              const dw_heads *k, const dw_heads *v, const dw_buf *w_k, const dw_buf *rope, const dw_heads *q,
+                              const dw_buf *w_q, const dw_heads *q_out) {
+    const char *op = "append_kv";
+    if (!be) return DW_ERR_INVALID_ARG;
+    dw::HeadArgs a{};
+    dw::KvCache c{};
+    dw::Seqs s{};
+    DW_TRY(check_head_desc(be, d, rope, op, &a));
+    DW_TRY(check_cache(be, cache, op, &c));
+    if (d->head_dim != c.d || d->kv_heads != c.heads)
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %d heads of %d do not go into a cache of %d heads of %d", op, d->kv_heads,
+                       d->head_dim, c.heads, c.d);
+    if (d->rot_dim % (c.d / 32)) return dw_fail(be, DW_ERR_UNSUPPORTED, "%s: rot_dim must be a multiple of %d, not %d", op, c.d / 32, d->rot_dim);
+    DW_TRY(check_seqs(be, seqs, c.page, op, &s));
+    DW_TRY(check_heads(be, k, s.tokens, c.heads, c.d, d->dtype, op, "k", &a.k));
+    DW_TRY(check_heads(be, v, s.tokens, c.heads, c.d, d->dtype, op, "v", &a.v));
+    DW_TRY(check_weight(be, d, w_k, op, &a.w_k));
+    if (!q != !q_out) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: q and q_out go together", op);
+    if (q) {
+        DW_TRY(check_heads(be, q, s.tokens, d->q_heads, c.d, d->dtype, op, "q", &a.q));
+        DW_TRY(check_heads(be, q_out, s.tokens, d->q_heads, c.d, d->dtype, op, "q_out", &a.q_out));
+        DW_TRY(check_weight(be, d, w_q, op, &a.w_q));
+    }
+    cudaSetDevice(be->device);
+    return dw::launch_append_kv(be, *d, c, s, a);
+}
+
+DW_API dw_status dw_read_kv(dw_backend *be, const dw_kv_cache *cache, const dw_sequences *seqs, int dtype, const dw_heads *k_out,
+                            const dw_heads *v_out) {
+    const char *op = "read_kv";
+    if (!be) return DW_ERR_INVALID_ARG;
+    dw::KvCache c{};
+    dw::Seqs s{};
+    dw::HeadRows k{}, v{};
+    DW_TRY(check_dtype(be, dtype, op, "dtype"));
+    DW_TRY(check_cache(be, cache, op, &c));
+    DW_TRY(check_seqs(be, seqs, c.page, op, &s));
+    if (!k_out && !v_out) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: neither k_out nor v_out is given", op);
+    if (k_out) DW_TRY(check_heads(be, k_out, s.tokens, c.heads, c.d, dtype, op, "k_out", &k));
+    if (v_out) DW_TRY(check_heads(be, v_out, s.tokens, c.heads, c.d, dtype, op, "v_out", &v));
+    cudaSetDevice(be->device);
+    return dw::launch_read_kv(be, c, s, dtype, k, v);
+}
+
+DW_API dw_status dw_attention_kv8(dw_backend *be, const dw_attention_desc *d, const dw_kv_cache *cache, const dw_sequences *seqs,
+                                  const dw_heads *q, const dw_heads *out) {
+    const char *op = "attention_kv8";
+    if (!be) return DW_ERR_INVALID_ARG;
+    if (!d) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: descriptor is null", op);
+    dw::KvCache c{};
+    dw::Seqs s{};
+    dw::HeadRows qr{}, outr{};
+    DW_TRY(check_cache(be, cache, op, &c));
+    DW_TRY(check_seqs(be, seqs, c.page, op, &s));
+    if (d->dtype != DW_F16 && d->dtype != DW_BF16) return dw_fail(be, DW_ERR_UNSUPPORTED, "%s: dtype must be F16 or BF16", op);
+    if (d->q_heads <= 0 || d->q_heads % c.heads)
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: %d query heads are no multiple of the cache's %d", op, d->q_heads, c.heads);
+    if (d->window < 0 || (d->window && !d->causal))
+        return dw_fail(be, DW_ERR_INVALID_ARG, "%s: a window is positive and needs causal", op);
+    if (!(d->scale >= 0.0f) || std::isinf(d->scale)) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: scale must be >= 0 and finite", op);
+    if ((long double)s.tokens * d->q_heads > 2147483647.0L)
+        return dw_fail(be, DW_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 query heads of rows", op);
+    DW_TRY(check_heads(be, q, s.tokens, d->q_heads, c.d, d->dtype, op, "q", &qr));
+    DW_TRY(check_heads(be, out, s.tokens, d->q_heads, c.d, d->dtype, op, "out", &outr));
+    cudaSetDevice(be->device);
+    return dw::launch_attention_kv8(be, *d, c, s, qr, outr);
+}
+
+}  // extern "C"

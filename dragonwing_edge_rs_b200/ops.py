@@ -435,6 +435,109 @@ def norm_residual_to_mxfp4(backend: CudaBackend, desc: NormDesc, x, w_post, b_po
 
 
 # ---------------------------------------------------------------------------
+# attention: head norms with the position rotation, a paged key/value cache in
+# 8 bits, attention over it (contracts in include/dw_cuda.h)
+# ---------------------------------------------------------------------------
+
+class Heads(L.DwHeads):
+    """[rows, heads, head_dim] inside wider rows of a buffer: from element `offset` on, rows
+    `pitch` elements apart (0: the heads' own width)."""
+
+    def __init__(self, buf: CudaBuffer, offset: int = 0, pitch: int = 0):
+        super().__init__(buf and buf.handle, offset, pitch)
+        self.keep = buf
+        self.ref = ctypes.addressof(self)
+
+
+class HeadDesc(L.DwHeadDesc):
+    """Which heads a row has, their type, norm and rotation (dw_head_desc)."""
+
+    def __init__(self, q_heads: int, kv_heads: int, head_dim: int, rot_dim: int, dtype: int, norm: int = NORM_NONE,
+                 eps: float = 1e-5, neighbours: bool = False):
+        super().__init__(q_heads, kv_heads, head_dim, rot_dim, dtype, norm, int(neighbours), eps)
+        self.ref = ctypes.addressof(self)
+
+
+class KvCache(L.DwKvCache):
+    """A paged key/value cache in 8 bits: codes of keys and values, scale bytes (dw_kv_cache)."""
+
+    def __init__(self, k: CudaBuffer, v: CudaBuffer, scales: CudaBuffer, pages: int, kv_heads: int, page_tokens: int,
+                 head_dim: int):
+        super().__init__(k and k.handle, v and v.handle, scales and scales.handle, pages, kv_heads, page_tokens, head_dim)
+        self.keep = (k, v, scales)
+        self.ref = ctypes.addressof(self)
+
+
+class Sequences(L.DwSequences):
+    """The sequences that a call's rows belong to: their pages, lengths and rows (dw_sequences)."""
+
+    def __init__(self, table: CudaBuffer, lens: CudaBuffer, starts, seqs: int, tokens: int, width: int):
+        super().__init__(table and table.handle, lens and lens.handle, starts and starts.handle, seqs, tokens, width)
+        self.keep = (table, lens, starts)
+        self.ref = ctypes.addressof(self)
+
+
+class AttentionDesc(L.DwAttentionDesc):
+    """Query heads, their type, the logits' scale and the mask (dw_attention_desc)."""
+
+    def __init__(self, q_heads: int, dtype: int, scale: float, causal: bool = True, window: int = 0):
+        super().__init__(q_heads, dtype, int(causal), window, scale)
+        self.ref = ctypes.addressof(self)
+
+
+def kv_code_bytes(pages: int, kv_heads: int, page_tokens: int, head_dim: int) -> int:
+    """Bytes of a cache's key (or value) codes."""
+    return int(L.load().dw_kv_code_bytes(pages, kv_heads, page_tokens, head_dim))
+
+
+def kv_scale_bytes(pages: int, kv_heads: int) -> int:
+    """Bytes of a cache's scales."""
+    return int(L.load().dw_kv_scale_bytes(pages, kv_heads))
+
+
+def prepare_rope(backend: CudaBackend, freqs) -> CudaBuffer:
+    """The rotations' table (once per model): freqs[i] is pair i's angle a position, in radians."""
+    f = np.ascontiguousarray(freqs, np.float64)
+    out = ctypes.c_void_p()
+    backend._check(L.load().dw_prepare_rope(backend.handle, f.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), f.size,
+                                            ctypes.byref(out)))
+    return CudaBuffer(backend, out, 8 * f.size)
+
+
+def norm_rope(backend: CudaBackend, desc: HeadDesc, tokens: int, q, k, w_q, w_k, rope, positions, q_out, k_out):
+    """Query and key heads of `tokens` rows, normed and turned by their positions, in one pass."""
+    st = L.load().dw_norm_rope(backend.handle, desc.ref, tokens, q and q.ref, k and k.ref, w_q and w_q.handle,
+                               w_k and w_k.handle, rope and rope.handle, positions and positions.handle,
+                               q_out and q_out.ref, k_out and k_out.ref)
+    if st:
+        backend._check(st)
+
+
+def append_kv(backend: CudaBackend, desc: HeadDesc, cache: KvCache, seqs: Sequences, k: Heads, v: Heads, w_k=None,
+              rope=None, q=None, w_q=None, q_out=None):
+    """Keys (normed, turned) and values of the rows into the cache; with q, the queries normed and turned to q_out."""
+    st = L.load().dw_append_kv(backend.handle, desc.ref, cache.ref, seqs.ref, k and k.ref, v and v.ref,
+                               w_k and w_k.handle, rope and rope.handle, q and q.ref, w_q and w_q.handle,
+                               q_out and q_out.ref)
+    if st:
+        backend._check(st)
+
+
+def read_kv(backend: CudaBackend, cache: KvCache, seqs: Sequences, dtype: int, k_out, v_out):
+    """The cached keys and values of the rows' positions, as `dtype` (either output may be None)."""
+    st = L.load().dw_read_kv(backend.handle, cache.ref, seqs.ref, dtype, k_out and k_out.ref, v_out and v_out.ref)
+    if st:
+        backend._check(st)
+
+
+def attention_kv8(backend: CudaBackend, desc: AttentionDesc, cache: KvCache, seqs: Sequences, q: Heads, out: Heads):
+    """Attention of the rows' query heads over their sequences' cached tokens."""
+    st = L.load().dw_attention_kv8(backend.handle, desc.ref, cache.ref, seqs.ref, q and q.ref, out and out.ref)
+    if st:
+        backend._check(st)
+
+
+# ---------------------------------------------------------------------------
 # YOLOv8 Detect tail and detection post-processing
 # (crates/dragonwing-onnx/src/postprocess.rs)
 # ---------------------------------------------------------------------------

@@ -584,6 +584,117 @@ DW_API dw_status dw_norm_residual_to_mxfp4(dw_backend *be, const dw_norm_desc *d
                                            const dw_buf *b_post, const dw_buf *gate, const dw_buf *residual, dw_buf *out,
                                            const dw_buf *w_pre, const dw_buf *b_pre, dw_buf *q, dw_buf *s);
 
+/* ---------------------------------------------------------------------- */
+/* Attention of a transformer block: head norms with the position rotation, */
+/* a paged key/value cache in 8 bits, attention over it                     */
+/* ---------------------------------------------------------------------- */
+/* Additions: the reference has no attention.  All work is asynchronous on the
+ * backend's stream; apart from dw_prepare_rope nothing here allocates or keeps a
+ * workspace, so every call may be captured, and a captured graph may be replayed
+ * after the contents (not the sizes) of any buffer changed.
+ *
+ * Rows are tokens.  A dw_heads is a tensor [rows, heads, head_dim] inside wider
+ * rows: element (r, h, i) is element offset + r * pitch + h * head_dim + i of buf
+ * (pitch 0: heads * head_dim).  The buffer reaches at least to its last element.
+ * A projection's packed rows are three of them on one buffer. */
+typedef struct dw_heads {
+    const dw_buf *buf;
+    size_t offset, pitch; /* elements */
+} dw_heads;
+
+/* Which heads a row has, their type, norm and rotation.  norm: dw_norm_kind over
+ * each head's head_dim values, with f32 weights [head_dim] (NULL: 1), before the
+ * rotation.  The first rot_dim values of a head are turned (even, 0: none): pair i
+ * is (i, i + rot_dim / 2), or with neighbours != 0 (2 i, 2 i + 1), and
+ * (a, b) becomes (a cos - b sin, a sin + b cos) of the angle position * freqs[i]. */
+typedef struct dw_head_desc {
+    int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads */
+    int32_t head_dim, rot_dim;
+    int32_t dtype; /* dw_dtype of rows in and out */
+    int32_t norm;
+    int32_t neighbours;
+    float eps; /* >= 0 */
+} dw_head_desc;
+
+/* Builds what the rotations read: freqs[pairs] in radians a position (host memory,
+ * finite), held as 64-bit fractions of a turn, so that an angle is exact to 2^-53 of
+ * its freq at every int32 position.  *out is a new buffer owned by the caller. */
+DW_API dw_status dw_prepare_rope(dw_backend *be, const double *freqs, size_t pairs, dw_buf **out);
+
+/* Query and key heads of `tokens` rows, normed and turned by their positions
+ * (int32 [tokens]; any sign) in one pass, in f32.  head_dim even, up to 512.  q or k
+ * (with its output) may be NULL; rope and positions are NULL where rot_dim is 0.  An
+ * output may be its own input; nothing else overlaps. */
+DW_API dw_status dw_norm_rope(dw_backend *be, const dw_head_desc *d, size_t tokens, const dw_heads *q, const dw_heads *k,
+                              const dw_buf *w_q, const dw_buf *w_k, const dw_buf *rope, const dw_buf *positions,
+                              const dw_heads *q_out, const dw_heads *k_out);
+
+/* A cache of `pages` pages, each of page_tokens tokens (16, 32, 64 or 128) of all
+ * kv_heads heads of head_dim values (64 or 128):
+ *   k, v    codes, [pages, kv_heads, page_tokens, head_dim] e4m3 bytes, 16-byte aligned;
+ *   scales  [pages, kv_heads, 2] bytes: of the keys and of the values of a block (a page's
+ *           tokens of one head); byte e + 127 stands for X = 2^e, e in -64..63.
+ * A value is its code times X.  X is the smallest power of two with max|v| <= 448 X over
+ * the block, and codes are rounded to nearest, ties to even (beyond 448 * 2^63 they stay
+ * there).  A token with a NaN or an infinity in its key or value has the key code 0x7F
+ * (NaN) and the value code 0 everywhere in that head, and no part in X: whoever sees it
+ * gets NaN, and nobody else.  Value codes are never NaN. */
+typedef struct dw_kv_cache {
+    dw_buf *k, *v, *scales;
+    size_t pages;
+    int32_t kv_heads, page_tokens, head_dim;
+} dw_kv_cache;
+
+DW_API size_t dw_kv_code_bytes(size_t pages, size_t kv_heads, size_t page_tokens, size_t head_dim);
+DW_API size_t dw_kv_scale_bytes(size_t pages, size_t kv_heads);
+
+/* The sequences that a call's rows belong to.  Sequence s has lens[s] tokens in the
+ * cache (after an append: its new ones included) in the pages table[s][0 ..], token t in
+ * page t / page_tokens of them.  Its rows are starts[s] .. starts[s + 1] - 1 (ascending,
+ * within `tokens`; none is allowed), or without starts tokens / seqs rows each; they are
+ * its last tokens: the i-th of its n rows is position lens[s] - n + i.  Rows of no sequence
+ * are neither read nor written, nor are table entries behind a sequence's last page.
+ * Positions below 0 (n > lens[s]) are no tokens of the cache.  Lengths, starts and pages that
+ * lie outside are not followed: dw_synchronize reports DW_ERR_DEVICE, and the call's
+ * results are not to be used. */
+typedef struct dw_sequences {
+    const dw_buf *table;  /* int32 [seqs, width] */
+    const dw_buf *lens;   /* int32 [seqs] */
+    const dw_buf *starts; /* int32 [seqs + 1], or NULL */
+    size_t seqs, tokens, width;
+} dw_sequences;
+
+/* Keys (normed with w_k and turned by their positions) and values into the cache, and
+ * where q is given the query heads, normed with w_q and turned, to q_out (which may be
+ * q).  rope is NULL where rot_dim is 0.  A block that tokens are added to keeps its X or
+ * takes a larger one, and the codes that it holds are then rounded again; the first token of a
+ * page makes the block anew.  Keys are computed in f64, so their codes are the
+ * definition's; queries in f32.  Two sequences may share pages that the call
+ * does not write. */
+DW_API dw_status dw_append_kv(dw_backend *be, const dw_head_desc *d, const dw_kv_cache *cache, const dw_sequences *seqs,
+                              const dw_heads *k, const dw_heads *v, const dw_buf *w_k, const dw_buf *rope,
+                              const dw_heads *q, const dw_buf *w_q, const dw_heads *q_out);
+
+/* The cached keys and values of the rows' positions, as `dtype` (f32 and bf16 hold them
+ * exactly); 0 at positions below 0.  k_out or v_out may be NULL. */
+DW_API dw_status dw_read_kv(dw_backend *be, const dw_kv_cache *cache, const dw_sequences *seqs, int dtype,
+                            const dw_heads *k_out, const dw_heads *v_out);
+
+/* out[r, h] = sum_j softmax_j(scale * q[r, h] . k_j) v_j over the tokens j that row r (at
+ * position p) sees: all of its sequence, with causal != 0 those up to p, with window > 0 (and
+ * causal) the last `window` of these.  Query head h reads cache head h / (q_heads /
+ * kv_heads).  A row that sees nothing gives 0.  q and out: DW_F16 or DW_BF16; products
+ * and sums are f32, the softmax's numerators are rounded to 11 bits before they meet the
+ * values.  The sums' order depends on the sizes and lengths alone.  out may be q itself. */
+typedef struct dw_attention_desc {
+    int32_t q_heads; /* a multiple of the cache's kv_heads */
+    int32_t dtype;
+    int32_t causal, window;
+    float scale; /* >= 0 */
+} dw_attention_desc;
+DW_API dw_status dw_attention_kv8(dw_backend *be, const dw_attention_desc *d, const dw_kv_cache *cache,
+                                  const dw_sequences *seqs, const dw_heads *q, const dw_heads *out);
+
 #ifdef __cplusplus
 }
 #endif
