@@ -19,7 +19,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "dw_kv.cuh"
+#include "dw_attend.cuh"
 #include "dw_launch.h"
 #include "dw_mxfp4.cuh"
 #include "dw_ptx.cuh"
@@ -31,19 +31,6 @@ constexpr int kTile = 32;  // tokens of a tile
 constexpr int kWarps = 4;
 constexpr int kStages = 2;
 constexpr float kHead = 14.0f;  // exponent of the largest weight
-
-struct AttendParams {
-    const void *q;
-    void *out;
-    size_t q_pitch, out_pitch;
-    int group;         // query heads of a cache head
-    int per_seq;       // blocks of rows of a sequence where all have as many; 0: by their starts
-    float scale_log2;  // scale * log2(e)
-    int causal, window;
-    bool vec;          // rows allow 16-byte accesses
-    uint64_t wait_cap_ns;
-    int32_t *err;
-};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -89,24 +76,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 // Column c of eight, as a place among the eight rows (or pieces) that it reads: rows of two
 // neighbouring columns lie four apart, which the copies' swizzle turns into other banks.
 __device__ __forceinline__ int spread(int c) { return (c & 1) * 4 + (c >> 1); }
-
-// (x, y) -> the sums' factor where the maximum goes from x to y (-inf: nothing so far).
-__device__ __forceinline__ float carry(float x, float y) { return x == y ? 1.0f : ex2_approx(x - y); }
-
-// A tile that does not start before `hi` or ends at `lo` or before is not visited; the rows'
-// own bounds decide token by token.
-struct Bounds {
-    int lo, hi;
-};
-__device__ __forceinline__ Bounds row_bounds(const AttendParams &p, const SeqRange &r, int token) {
-    const int pos = r.len - r.n + token;
-    Bounds b{0, r.len};
-    if (p.causal) {
-        b.hi = min(r.len, pos + 1);
-        if (p.window) b.lo = max(0, pos + 1 - p.window);
-    }
-    return b;
-}
 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kWarps * 32)
@@ -231,7 +200,7 @@ __global__ void __launch_bounds__(kWarps * 32)
             if constexpr (std::is_same_v<T, __nv_bfloat16>) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -126), 126);
+                e = query_exponent(top);
             }
             const float down = kv_pow2(-e);
             a_row[m][h] = p.scale_log2 * kv_pow2(e);
@@ -486,6 +455,7 @@ dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Se
     const size_t n = s.tokens / s.seqs;
     p.per_seq = s.starts ? 0 : (int)((n * p.group + R - 1) / R);
     const size_t items = s.starts ? seq_items(s.tokens, s.seqs, p.group, R, 1) : (size_t)p.per_seq * s.seqs, units = items * c.heads;
+    p.items = (uint32_t)items;
     // CTAs that share a block's tiles: as many as the GPU holds at once, each with a tile a warp at least
     const size_t most = ((size_t)s.width * c.page + kTile - 1) / kTile;
     unsigned S = 1;
@@ -519,6 +489,7 @@ dw_status launch_attention_kv8(dw_backend *be, const dw_attention_desc &d, const
     p.wait_cap_ns = be->wait_cap_ns, p.err = be->dev_err;
     auto with = [&](auto t) {
         using T = decltype(t);
+        if (s.tokens / s.seqs * p.group > 64) return c.d == 64 ? attend_prompt<T, 64>(be, p, c, s) : attend_prompt<T, 128>(be, p, c, s);
         return c.d == 64 ? attend_rows<T, 64>(be, p, c, s) : attend_rows<T, 128>(be, p, c, s);
     };
     return d.dtype == DW_F16 ? with(__half{}) : with(__nv_bfloat16{});

@@ -1,0 +1,506 @@
+// attention_prompt.cu -- attention over the paged 8-bit cache for many query rows (prompts and
+// pieces of them), on the tcgen05 tensor cores.  The mathematics is attention.cu's: weights
+// w_j = 2^(t_j - M + 7) with t_j = log2(e) scale q . k_j + ev_j, out = sum w_j code_j /
+// sum w_j 2^(-ev_j).  M is a maximum that lags: it moves (and what is summed so far is scaled)
+// only where a row's true one is more than 2^8 above, so w stays below 2^15, inside f16, and the
+// sums are rarely touched.
+//
+// A CTA has 256 rows (two tiles of 128: token by token the heads of a group) and goes through
+// tiles of 128 tokens:
+//   converters (4 warps)   codes of keys and values, from global memory through registers, as
+//                          f16 into shared memory (128-byte swizzled rows of 64 values);
+//   one issuing warp       S = Q K^T (128 x 128 x d) into tensor memory, O += P V with P from
+//                          tensor memory and V as it lies (tokens x values);
+//   2 x 4 softmax warps    a thread a row: S -> weights (f16, over S) and their sum.
+// While one row tile's weights are computed the other's products run.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "dw_attend.cuh"
+#include "dw_launch.h"
+#include "dw_mxfp4.cuh"
+#include "dw_ptx.cuh"
+#include "dw_tcgen05.cuh"
+
+namespace dw {
+namespace {
+
+constexpr int kRows = 256, kTile = 128;  // query rows of a CTA, tokens of a tile
+constexpr int kThreads = 512;
+constexpr int kStages = 2;
+constexpr float kHead = 7.0f, kLag = 8.0f;
+
+__device__ __forceinline__ bool wait_phase(uint64_t *barrier, uint32_t parity, const AttendParams &p, volatile int *abort_flag, int site) {
+    const uint32_t bar = smem_u32(barrier);
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+    for (;;) {
+        if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+        if (*abort_flag) return false;
+        if (globaltimer_ns() - t0 > p.wait_cap_ns) {
+            *abort_flag = 1;
+            record_error(p.err, DW_DEV_WAIT_EXPIRED, site, (int)parity);
+            return false;
+        }
+    }
+}
+// The same for a whole warp, with one answer.
+__device__ __forceinline__ bool wait_warp(uint64_t *barrier, uint32_t parity, const AttendParams &p, volatile int *abort_flag, int site) {
+    return __all_sync(0xffffffffu, wait_phase(barrier, parity, p, abort_flag, site));
+}
+
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
+}
+// One product of 128 x N x 16, by an elected lane: both operands in shared memory, or the first
+// in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t elected, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(elected)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t elected, uint64_t *bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(elected)
+        : "memory");
+}
+
+__device__ __forceinline__ void tm_ld32(uint32_t taddr, float (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+          "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+          "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tm_st32(uint32_t taddr, const float (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"f"(r[0]),
+        "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]),
+        "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]), "f"(r[19]), "f"(r[20]), "f"(r[21]),
+        "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]), "f"(r[28]), "f"(r[29]), "f"(r[30]), "f"(r[31]),
+        "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Values x tokens as they lie (rows of 64 values are tokens): the second operand's descriptor
+// where its columns, not its depth, run along the rows.  128-byte swizzle, 8 rows every 1024
+// bytes; the next 64 columns `next` bytes on.
+__device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t next) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Byte of the 16-byte piece `chunk` (0..7) of row r in a tile of swizzled 128-byte rows.
+__device__ __forceinline__ uint32_t swizzled(int r, int chunk) { return (uint32_t)(r * 128 + ((chunk ^ (r & 7)) << 4)); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_attend_prompt(const __grid_constant__ AttendParams p, const __grid_constant__ KvCache c, const __grid_constant__ Seqs sq) {
+    constexpr int kHalves = D / 64;                   // swizzled tiles of 64 values
+    constexpr uint32_t kHalf = kTile * 128;           // bytes of one
+    constexpr uint32_t kOperand = kHalves * kHalf;    // of 128 rows of queries, keys or values
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], drain;
+    __shared__ float2 scales[4][8];  // of a tile's 16-token groups: 2^ek, ev
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    volatile int *abort_flag = &abort_word;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+    uint8_t *const base = smem_raw + (smem - smem_u32(smem_raw));
+    const uint32_t q_at = 0, k_at = 2 * kOperand, v_at = k_at + kStages * kOperand;
+
+    pdl_wait();
+    // which rows of which sequence, which head: those that see most first
+    const uint32_t unit = blockIdx.x / (uint32_t)c.heads;
+    const int head = (int)(blockIdx.x % (uint32_t)c.heads);
+    int64_t place;
+    uint32_t s;
+    if (p.per_seq) {
+        s = unit % sq.seqs, place = p.per_seq - 1 - (int)(unit / sq.seqs);
+    } else {
+        s = seq_of_item(sq, p.items - 1 - unit, p.group, kRows, 1, place);
+    }
+    const SeqRange r = seq_range(sq, s, c.page, p.err);
+    const int rows_all = r.n * p.group, first = (int)min(place * kRows, (int64_t)0x7fffffff);
+    if (place < 0 || first >= rows_all) {
+        pdl_trigger();
+        return;
+    }
+    const int rows = min(kRows, rows_all - first);
+    auto token_of = [&](int row) { return (first + row) / p.group; };
+    const int lo = row_bounds(p, r, token_of(0)).lo;
+    const int tile0 = lo / kTile;
+    // tiles of either row tile: up to the last token that its last row sees
+    int tiles[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int hi = rows > t * 128 ? row_bounds(p, r, token_of(min(rows, t * 128 + 128) - 1)).hi : 0;
+        tiles[t] = max(0, (hi + kTile - 1) / kTile - tile0);
+    }
+    const int all = max(tiles[0], tiles[1]);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_u32(&q_full[i]), 4), mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&p_full[i]), 4), mbar_init(smem_u32(&o_full[i]), 1);
+        }
+        for (int i = 0; i < kStages; i++) {
+            mbar_init(smem_u32(&k_full[i]), 4), mbar_init(smem_u32(&k_empty[i]), 1);
+            mbar_init(smem_u32(&v_full[i]), 4), mbar_init(smem_u32(&v_empty[i]), 1);
+        }
+        mbar_init(smem_u32(&drain), 1);
+        abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_trigger();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);  // S of either row tile (128 columns each), then O
+
+    if (warp >= 12) {
+        // ---- converters: a thread has 16 codes of a row of each half of each of four groups of 32 rows
+        const int tid = threadIdx.x - 384, part = tid & 3, sub = tid >> 2;
+        uint4 kx[4 * kHalves], vx[4 * kHalves];
+        auto load = [&](uint4 (&x)[4 * kHalves], const uint8_t *codes, int tile) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int t = (tile0 + tile) * kTile + g * 32 + sub;
+#pragma unroll
+                for (int h = 0; h < kHalves; h++) x[g * kHalves + h] = make_uint4(0, 0, 0, 0);
+                if (t >= r.len) continue;  // no token: zeros, whatever the page holds there
+                const uint32_t page = seq_page(sq, c, s, (uint32_t)t / (uint32_t)c.page, p.err);
+                const uint4 *from = reinterpret_cast<const uint4 *>(codes + (kv_block(c, page, head) * c.page + t % c.page) * D) + part;
+#pragma unroll
+                for (int h = 0; h < kHalves; h++) x[g * kHalves + h] = from[4 * h];
+            }
+        };
+        auto store = [&](const uint4 (&x)[4 * kHalves], uint32_t at) {
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int h = 0; h < kHalves; h++) {
+                    const uint4 u = x[g * kHalves + h];
+                    const int row = g * 32 + sub;
+                    const uint32_t to = smem + at + h * kHalf;
+                    sts_v4(to + swizzled(row, 2 * part), make_uint4(e4m3_to_f16x2((uint16_t)u.x), e4m3_to_f16x2((uint16_t)(u.x >> 16)),
+                                                                   e4m3_to_f16x2((uint16_t)u.y), e4m3_to_f16x2((uint16_t)(u.y >> 16))));
+                    sts_v4(to + swizzled(row, 2 * part + 1), make_uint4(e4m3_to_f16x2((uint16_t)u.z), e4m3_to_f16x2((uint16_t)(u.z >> 16)),
+                                                                       e4m3_to_f16x2((uint16_t)u.w), e4m3_to_f16x2((uint16_t)(u.w >> 16))));
+                }
+        };
+        auto done = [&](uint64_t *bar) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(bar));
+        };
+        float2 sc = make_float2(0.0f, 0.0f);
+        auto load_scale = [&](int tile) {  // of group tid (0..7)
+            const int t = (tile0 + tile) * kTile + tid * 16;
+            sc = make_float2(1.0f, 0.0f);
+            if (tid >= 8 || t >= r.len) return;
+            const uint32_t page = seq_page(sq, c, s, (uint32_t)t / (uint32_t)c.page, p.err);
+            const uint8_t *b = c.s + kv_block(c, page, head) * 2;
+            sc = make_float2(kv_pow2(kv_exponent(b[0])), (float)kv_exponent(b[1]));
+        };
+        if (all) load(kx, c.k, 0), load_scale(0), load(vx, c.v, 0);
+        for (int j = 0; j < all; j++) {
+            const int st = j % kStages;
+            const uint32_t ph = (uint32_t)(j / kStages) & 1;
+            if (j >= kStages && !wait_warp(&k_empty[st], ph ^ 1, p, abort_flag, 71)) break;
+            store(kx, k_at + st * kOperand);
+            if (tid < 8) scales[j & 3][tid] = sc;
+            done(&k_full[st]);
+            if (j + 1 < all) load(kx, c.k, j + 1), load_scale(j + 1);
+            if (j >= kStages && !wait_warp(&v_empty[st], ph ^ 1, p, abort_flag, 72)) break;
+            store(vx, v_at + st * kOperand);
+            done(&v_full[st]);
+            if (j + 1 < all) load(vx, c.v, j + 1);
+        }
+    } else if (warp == 0) {
+        // ---- products
+        const uint32_t elected = elect_one();
+        constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | (8u << 24);
+        constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+        constexpr uint64_t hi = ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+        auto logits = [&](int t, int j) {
+            const uint32_t a = smem + q_at + t * kOperand, b = smem + k_at + (j % kStages) * kOperand;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                const uint32_t off = (uint32_t)(i / 4) * kHalf + (uint32_t)(i % 4) * 32;
+                mma_ss(elected, tmem + t * 128, smem_desc(a + off, hi), smem_desc(b + off, hi), idesc_s, i ? 1u : 0u);
+            }
+            commit(elected, &s_full[t]);
+        };
+        auto sums = [&](int t, int j) {
+            const uint32_t b = smem + v_at + (j % kStages) * kOperand;
+#pragma unroll
+            for (int i = 0; i < kTile / 16; i++)
+                mma_ts(elected, tmem + 256 + t * D, tmem + t * 128 + i * 8, desc_rows(b + i * 2048, kHalf), idesc_o, (j || i) ? 1u : 0u);
+        };
+        bool ok = true;
+        for (int t = 0; t < 2 && ok; t++)
+            if (tiles[t]) ok = wait_warp(&q_full[t], 0, p, abort_flag, 73);
+        for (int j = -1; j < all && ok; j++) {
+            // O += P V of tile j, S of tile j + 1
+            if (j + 1 < all) ok = wait_warp(&k_full[(j + 1) % kStages], (uint32_t)((j + 1) / kStages) & 1, p, abort_flag, 74);
+            if (ok && j >= 0) ok = wait_warp(&v_full[j % kStages], (uint32_t)(j / kStages) & 1, p, abort_flag, 75);
+            for (int t = 0; t < 2 && ok; t++) {
+                if (j >= 0 && j < tiles[t]) {
+                    ok = wait_warp(&p_full[t], (uint32_t)j & 1, p, abort_flag, 76);
+                    if (!ok) break;
+                    tc_fence_after();
+                    sums(t, j);
+                    if (j + 1 == tiles[t]) commit(elected, &o_full[t]);
+                }
+                tc_fence_after();
+                if (j + 1 < tiles[t]) logits(t, j + 1);
+            }
+            if (!ok) break;
+            if (j >= 0) commit(elected, &v_empty[j % kStages]);
+            if (j + 1 < all) commit(elected, &k_empty[(j + 1) % kStages]);
+        }
+        // products in flight end before the tensor memory is given back
+        commit(elected, &drain);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait_sleep(smem_u32(&drain), 0, 20000u) && globaltimer_ns() - t0 < p.wait_cap_ns) {
+        }
+    } else if (warp >= 4) {
+        // ---- softmax: a thread has a row
+        const int t = (warp - 4) >> 2, row = t * 128 + (warp & 3) * 32 + lane;
+        const bool there = row < rows;
+        const int at = first + row, token = there ? at / p.group : token_of(0);
+        Bounds b = row_bounds(p, r, token);
+        if (!there) b.hi = 0;
+        float a_row = p.scale_log2;
+        // the query row, in f16, to shared memory
+        if (tiles[t]) {
+            const T *src = (const T *)p.q + (size_t)(r.row0 + token) * p.q_pitch + (size_t)(head * p.group + at % p.group) * D;
+            auto piece = [&](int i) {
+                Raw<T, 8> x;
+                x.zero();
+                if (there && p.vec) {
+                    x.load(src + 8 * i);
+                } else if (there) {
+                    float u[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) u[e] = to_f32(src[8 * i + e]);
+                    x.set(u);
+                }
+                return x;
+            };
+            float down = 1.0f;
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) {
+                    const Raw<T, 8> x = piece(i);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x.get(e)));
+                }
+                const int e = query_exponent(top);
+                down = kv_pow2(-e), a_row *= kv_pow2(e);
+            }
+#pragma unroll
+            for (int i = 0; i < D / 8; i++) {
+                const Raw<T, 8> x = piece(i);
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = pack2<__half>(x.get(2 * e) * down, x.get(2 * e + 1) * down);
+                sts_v4(smem + q_at + t * kOperand + (i / 8) * kHalf + swizzled(row & 127, i & 7), make_uint4(w[0], w[1], w[2], w[3]));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&q_full[t]));
+        }
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_tm = tmem + t * 128 + lanes, o_tm = tmem + 256 + t * D + lanes;
+        // tokens that all of the warp's rows see, and those that any does
+        const int lo_all = __reduce_max_sync(0xffffffffu, b.lo), hi_all = __reduce_min_sync(0xffffffffu, b.hi);
+        float M = -INFINITY, L = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < tiles[t]; j++) {
+            const int t0 = (tile0 + j) * kTile;
+            if (!wait_warp(&s_full[t], (uint32_t)j & 1, p, abort_flag, 77)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const bool masked = t0 < lo_all || t0 + kTile > hi_all;
+            const int from = b.lo - t0, to = b.hi - t0;  // the row's columns of the tile
+            float top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                float x[32];
+                tm_ld32(s_tm + q * 32, x);
+                tc_wait_ld();
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const float2 sc = scales[j & 3][2 * q + g];
+                    const float a = a_row * sc.x;
+                    float m = -INFINITY;
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int col = 32 * q + 16 * g + i;
+                            if (col >= from && col < to) m = fmaxf(m, x[16 * g + i]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) m = fmaxf(m, x[16 * g + i]);
+                    }
+                    if (m != -INFINITY) top = fmaxf(top, fmaf(m, a, sc.y));
+                }
+            }
+            const bool moves = top > M + kLag || (M == -INFINITY && top != -INFINITY);
+            if (__any_sync(0xffffffffu, moves)) {
+                const float f = moves ? carry(M, top) : 1.0f;
+                if (moves) M = top;
+                L *= f;
+                if (j) {
+#pragma unroll
+                    for (int q = 0; q < D / 32; q++) {
+                        float x[32];
+                        tm_ld32(o_tm + q * 32, x);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[i] *= f;
+                        tm_st32(o_tm + q * 32, x);
+                    }
+                }
+            }
+            const float head_room = (M == -INFINITY ? 0.0f : -M) + kHead;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                float x[32];
+                uint32_t w[16];
+                tm_ld32(s_tm + q * 32, x);
+                tc_wait_ld();
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    const float2 sc = scales[j & 3][2 * q + g];
+                    const float a = a_row * sc.x, add = sc.y + head_room;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        float2 y = __ffma2_rn(make_float2(x[16 * g + i], x[16 * g + i + 1]), make_float2(a, a), make_float2(add, add));
+                        if (masked) {
+                            const int col = 32 * q + 16 * g + i;
+                            if (col < from || col >= to) y.x = -INFINITY;
+                            if (col + 1 < from || col + 1 >= to) y.y = -INFINITY;
+                        }
+                        y.x = ex2_approx(y.x), y.y = ex2_approx(y.y);
+                        sum += y.x + y.y;
+                        w[8 * g + i / 2] = pack2<__half>(y.x, y.y);
+                    }
+                    L = fmaf(sum, kv_pow2(-(int)sc.y), L);
+                }
+                tm_st16(s_tm + q * 16, w);
+            }
+            tm_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&p_full[t]));
+        }
+        if (tiles[t] && ok) ok = wait_warp(&o_full[t], 0, p, abort_flag, 78);
+        if (ok && rows > t * 128 + (warp & 3) * 32) {
+            tc_fence_after();
+            const float f = L == 0.0f ? 0.0f : 1.0f / L;
+            T *dst = (T *)p.out + (size_t)(r.row0 + token) * p.out_pitch + (size_t)(head * p.group + at % p.group) * D;
+#pragma unroll
+            for (int q = 0; q < D / 32; q++) {
+                float x[32];
+                if (tiles[t]) {
+                    tm_ld32(o_tm + q * 32, x);
+                    tc_wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) x[i] = 0.0f;
+                }
+                if (!there) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[e] = x[i + e] * f;
+                    if (p.vec) {
+                        Raw<T, 8> o;
+                        o.set(y);
+                        o.store(dst + q * 32 + i);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) dst[q * 32 + i + e] = from_f32<T>(y[e]);
+                    }
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace
+
+template <typename T, int D>
+dw_status attend_prompt(dw_backend *be, AttendParams p, const KvCache &c, const Seqs &s) {
+    auto kernel = k_attend_prompt<T, D>;
+    constexpr size_t smem = 1024 + (size_t)(2 + 2 * kStages) * kTile * D * 2;
+    const size_t n = s.tokens / s.seqs;
+    p.per_seq = s.starts ? 0 : (int)((n * p.group + kRows - 1) / kRows);
+    const size_t items = s.starts ? seq_items(s.tokens, s.seqs, p.group, kRows, 1) : (size_t)p.per_seq * s.seqs;
+    if (items * c.heads > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "attention_kv8: too many rows");
+    p.items = (uint32_t)items;
+    static bool attr_set[16] = {};
+    if (be->device < 16 && !attr_set[be->device]) {
+        dw_status st = dw_cuda_check(be, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                                     "attention_kv8 attributes");
+        if (st != DW_OK) return st;
+        attr_set[be->device] = true;
+    }
+    return launch_dependent(be, "attention_kv8 (prompt)", kernel, (unsigned)(items * c.heads), kThreads, smem, 0, p, c, s);
+}
+
+template dw_status attend_prompt<__half, 64>(dw_backend *, AttendParams, const KvCache &, const Seqs &);
+template dw_status attend_prompt<__half, 128>(dw_backend *, AttendParams, const KvCache &, const Seqs &);
+template dw_status attend_prompt<__nv_bfloat16, 64>(dw_backend *, AttendParams, const KvCache &, const Seqs &);
+template dw_status attend_prompt<__nv_bfloat16, 128>(dw_backend *, AttendParams, const KvCache &, const Seqs &);
+
+}  // namespace dw
