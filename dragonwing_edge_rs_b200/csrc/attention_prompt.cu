@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t kOperand = kHalves * kHalf;    // of 128 rows of queries, keys or values
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], drain;
-    __shared__ float2 scales[4][8];  // of a tile's 16-token groups: 2^ek, ev
+    __shared__ float4 scales[4][8];  // of a tile's 16-token groups: 2^ek, ev, 2^-ev
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
@@ -191,21 +191,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_trigger();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);  // S of either row tile (128 columns each), then O
 
+    // registers go to the softmax warps, which hold a row of logits each: (40 + 88 + 2 x 192) x 128 =
+    // the launch's 512 x 128
     if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // ---- converters: a thread has 16 codes of a row of each half of each of four groups of 32 rows
         const int tid = threadIdx.x - 384, part = tid & 3, sub = tid >> 2;
+        // (a row's page is looked up a tile ahead of its codes: in order they waited for one
+        // lookup after the other)
         uint4 kx[4 * kHalves], vx[4 * kHalves];
+        uint32_t page[4], ahead[4], scale_page = 0, scale_ahead = 0;
+        bool bad = false;
+        auto lookup = [&](int t) {  // the page of token t, in bounds in any case
+            if (t >= r.len) return 0u;
+            const uint32_t id = (uint32_t)sq.table[(size_t)s * sq.width + (uint32_t)t / (uint32_t)c.page];
+            bad |= id >= c.pages;
+            return id;
+        };
+        auto find = [&](int tile) {
+            const int t = (tile0 + tile) * kTile;
+#pragma unroll
+            for (int g = 0; g < 4; g++) ahead[g] = lookup(t + g * 32 + sub);
+            if (tid < 8) scale_ahead = lookup(t + tid * 16);
+        };
+        auto take = [&]() {
+#pragma unroll
+            for (int g = 0; g < 4; g++) page[g] = min(ahead[g], c.pages - 1);
+            scale_page = min(scale_ahead, c.pages - 1);
+        };
         auto load = [&](uint4 (&x)[4 * kHalves], const uint8_t *codes, int tile) {
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 const int t = (tile0 + tile) * kTile + g * 32 + sub;
+                const uint4 *from = reinterpret_cast<const uint4 *>(codes + (kv_block(c, page[g], head) * c.page + t % c.page) * D) + part;
 #pragma unroll
-                for (int h = 0; h < kHalves; h++) x[g * kHalves + h] = make_uint4(0, 0, 0, 0);
-                if (t >= r.len) continue;  // no token: zeros, whatever the page holds there
-                const uint32_t page = seq_page(sq, c, s, (uint32_t)t / (uint32_t)c.page, p.err);
-                const uint4 *from = reinterpret_cast<const uint4 *>(codes + (kv_block(c, page, head) * c.page + t % c.page) * D) + part;
-#pragma unroll
-                for (int h = 0; h < kHalves; h++) x[g * kHalves + h] = from[4 * h];
+                for (int h = 0; h < kHalves; h++)  // no token: zeros, whatever the page holds there
+                    x[g * kHalves + h] = t < r.len ? from[4 * h] : make_uint4(0, 0, 0, 0);
             }
         };
         auto store = [&](const uint4 (&x)[4 * kHalves], uint32_t at) {
@@ -227,30 +248,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(bar));
         };
-        float2 sc = make_float2(0.0f, 0.0f);
+        uint32_t sc = 0;
         auto load_scale = [&](int tile) {  // of group tid (0..7)
-            const int t = (tile0 + tile) * kTile + tid * 16;
-            sc = make_float2(1.0f, 0.0f);
-            if (tid >= 8 || t >= r.len) return;
-            const uint32_t page = seq_page(sq, c, s, (uint32_t)t / (uint32_t)c.page, p.err);
-            const uint8_t *b = c.s + kv_block(c, page, head) * 2;
-            sc = make_float2(kv_pow2(kv_exponent(b[0])), (float)kv_exponent(b[1]));
+            if (tid < 8) sc = *reinterpret_cast<const uint16_t *>(c.s + kv_block(c, scale_page, head) * 2);
         };
-        if (all) load(kx, c.k, 0), load_scale(0), load(vx, c.v, 0);
+        if (all) find(0), take(), load(kx, c.k, 0), load_scale(0), load(vx, c.v, 0);
+        if (all > 1) find(1);
         for (int j = 0; j < all; j++) {
             const int st = j % kStages;
             const uint32_t ph = (uint32_t)(j / kStages) & 1;
             if (j >= kStages && !wait_warp(&k_empty[st], ph ^ 1, p, abort_flag, 71)) break;
             store(kx, k_at + st * kOperand);
-            if (tid < 8) scales[j & 3][tid] = sc;
+            if (tid < 8) {
+                const int ve = kv_exponent(sc >> 8);
+                scales[j & 3][tid] = make_float4(kv_pow2(kv_exponent(sc & 255)), (float)ve, kv_pow2(-ve), 0.0f);
+            }
             done(&k_full[st]);
-            if (j + 1 < all) load(kx, c.k, j + 1), load_scale(j + 1);
+            if (j + 1 < all) {
+                take();
+                load(kx, c.k, j + 1), load_scale(j + 1);
+                if (j + 2 < all) find(j + 2);
+            }
             if (j >= kStages && !wait_warp(&v_empty[st], ph ^ 1, p, abort_flag, 72)) break;
             store(vx, v_at + st * kOperand);
             done(&v_full[st]);
             if (j + 1 < all) load(vx, c.v, j + 1);
         }
-    } else if (warp == 0) {
+        if (bad) record_error(p.err, DW_DEV_BAD_ARG, 62, (int)s);
+    } else if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 0) {
         // ---- products
         const uint32_t elected = elect_one();
         constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | (8u << 24);
@@ -298,7 +325,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait_sleep(smem_u32(&drain), 0, 20000u) && globaltimer_ns() - t0 < p.wait_cap_ns) {
         }
-    } else if (warp >= 4) {
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         // ---- softmax: a thread has a row
         const int t = (warp - 4) >> 2, row = t * 128 + (warp & 3) * 32 + lane;
         const bool there = row < rows;
@@ -359,77 +388,75 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             tc_fence_after();
-            const bool masked = t0 < lo_all || t0 + kTile > hi_all;
-            const int from = b.lo - t0, to = b.hi - t0;  // the row's columns of the tile
-            float top = -INFINITY;
+            float x[4][32];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                float x[32];
-                tm_ld32(s_tm + q * 32, x);
-                tc_wait_ld();
+            for (int q = 0; q < 4; q++) tm_ld32(s_tm + q * 32, x[q]);
+            tc_wait_ld();
+            // (a tile that some row sees in part takes code of its own: its compares and selects
+            // doubled the instructions of the others)
+            auto weights = [&](auto part) {
+                constexpr bool kPart = decltype(part)::value;
+                const int from = b.lo - t0, to = b.hi - t0;  // the row's columns of the tile
+                float top = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    const float2 sc = scales[j & 3][2 * q + g];
-                    const float a = a_row * sc.x;
+                for (int g = 0; g < 8; g++) {
                     float m = -INFINITY;
-                    if (masked) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int col = 32 * q + 16 * g + i;
-                            if (col >= from && col < to) m = fmaxf(m, x[16 * g + i]);
+                    for (int i = 0; i < 16; i++) {
+                        const float v = x[g / 2][16 * (g & 1) + i];
+                        const int col = 16 * g + i;
+                        if (!kPart || (col >= from && col < to)) m = fmaxf(m, v);
+                    }
+                    const float4 sc = scales[j & 3][g];
+                    if (!kPart || m != -INFINITY) top = fmaxf(top, fmaf(m, a_row * sc.x, sc.y));
+                }
+                const bool moves = top > M + kLag || (M == -INFINITY && top != -INFINITY);
+                if (__any_sync(0xffffffffu, moves)) {
+                    const float f = moves ? carry(M, top) : 1.0f;
+                    if (moves) M = top;
+                    L *= f;
+                    if (j) {
+#pragma unroll
+                        for (int q = 0; q < D / 32; q++) {
+                            float y[32];
+                            tm_ld32(o_tm + q * 32, y);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) y[i] *= f;
+                            tm_st32(o_tm + q * 32, y);
                         }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; i++) m = fmaxf(m, x[16 * g + i]);
-                    }
-                    if (m != -INFINITY) top = fmaxf(top, fmaf(m, a, sc.y));
-                }
-            }
-            const bool moves = top > M + kLag || (M == -INFINITY && top != -INFINITY);
-            if (__any_sync(0xffffffffu, moves)) {
-                const float f = moves ? carry(M, top) : 1.0f;
-                if (moves) M = top;
-                L *= f;
-                if (j) {
-#pragma unroll
-                    for (int q = 0; q < D / 32; q++) {
-                        float x[32];
-                        tm_ld32(o_tm + q * 32, x);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) x[i] *= f;
-                        tm_st32(o_tm + q * 32, x);
                     }
                 }
-            }
-            const float head_room = (M == -INFINITY ? 0.0f : -M) + kHead;
+                const float head_room = (M == -INFINITY ? 0.0f : -M) + kHead;
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                float x[32];
-                uint32_t w[16];
-                tm_ld32(s_tm + q * 32, x);
-                tc_wait_ld();
+                for (int q = 0; q < 4; q++) {
+                    uint32_t w[16];
 #pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    const float2 sc = scales[j & 3][2 * q + g];
-                    const float a = a_row * sc.x, add = sc.y + head_room;
-                    float sum = 0.0f;
+                    for (int g = 0; g < 2; g++) {
+                        const float4 sc = scales[j & 3][2 * q + g];
+                        const float a = a_row * sc.x, add = sc.y + head_room;
+                        float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        float2 y = __ffma2_rn(make_float2(x[16 * g + i], x[16 * g + i + 1]), make_float2(a, a), make_float2(add, add));
-                        if (masked) {
-                            const int col = 32 * q + 16 * g + i;
-                            if (col < from || col >= to) y.x = -INFINITY;
-                            if (col + 1 < from || col + 1 >= to) y.y = -INFINITY;
+                        for (int i = 0; i < 16; i += 2) {
+                            float2 y = __ffma2_rn(make_float2(x[q][16 * g + i], x[q][16 * g + i + 1]), make_float2(a, a), make_float2(add, add));
+                            if constexpr (kPart) {
+                                const int col = 32 * q + 16 * g + i;
+                                if (col < from || col >= to) y.x = -INFINITY;
+                                if (col + 1 < from || col + 1 >= to) y.y = -INFINITY;
+                            }
+                            y.x = ex2_approx(y.x), y.y = ex2_approx(y.y);
+                            sum = __fadd2_rn(sum, y);
+                            w[8 * g + i / 2] = pack2<__half>(y.x, y.y);
                         }
-                        y.x = ex2_approx(y.x), y.y = ex2_approx(y.y);
-                        sum += y.x + y.y;
-                        w[8 * g + i / 2] = pack2<__half>(y.x, y.y);
+                        L = fmaf(sum.x + sum.y, sc.z, L);
                     }
-                    L = fmaf(sum, kv_pow2(-(int)sc.y), L);
+                    tm_st16(s_tm + q * 16, w);
                 }
-                tm_st16(s_tm + q * 16, w);
-            }
+            };
+            if (t0 < lo_all || t0 + kTile > hi_all)
+                weights(std::true_type{});
+            else
+                weights(std::false_type{});
             tm_wait_st();
             tc_fence_before();
             __syncwarp();
