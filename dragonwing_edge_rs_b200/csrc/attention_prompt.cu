@@ -91,6 +91,14 @@ __device__ __forceinline__ void tm_ld32(uint32_t taddr, float (&r)[32]) {
         : "r"(taddr)
         : "memory");
 }
+__device__ __forceinline__ void tm_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tm_st32(uint32_t taddr, const float (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -109,6 +117,35 @@ __device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t (&r)[16])
         : "memory");
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A row's columns of tensor memory times f: f32, 32 columns at a time, or f16 pairs, 16.
+template <bool kPairs>
+__device__ __noinline__ void scale_columns(uint32_t taddr, int count, float f) {
+    tm_wait_st();
+#pragma unroll 1
+    for (int q = 0; q < count; q++) {
+        if constexpr (kPairs) {
+            uint32_t w[16];
+            tm_ld16(taddr + q * 16, w);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                __half2 h;
+                memcpy(&h, &w[i], 4);
+                const float2 v = __half22float2(h);
+                w[i] = pack2<__half>(v.x * f, v.y * f);
+            }
+            tm_st16(taddr + q * 16, w);
+        } else {
+            float x[32];
+            tm_ld32(taddr + q * 32, x);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i++) x[i] *= f;
+            tm_st32(taddr + q * 32, x);
+        }
+    }
+}
 
 // Values x tokens as they lie (rows of 64 values are tokens): the second operand's descriptor
 // where its columns, not its depth, run along the rows.  128-byte swizzle, 8 rows every 1024
@@ -191,10 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_trigger();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);  // S of either row tile (128 columns each), then O
 
-    // registers go to the softmax warps, which hold a row of logits each: (40 + 88 + 2 x 192) x 128 =
-    // the launch's 512 x 128
     if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // ---- converters: a thread has 16 codes of a row of each half of each of four groups of 32 rows
         const int tid = threadIdx.x - 384, part = tid & 3, sub = tid >> 2;
         // (a row's page is looked up a tile ahead of its codes: in order they waited for one
@@ -276,7 +310,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (bad) record_error(p.err, DW_DEV_BAD_ARG, 62, (int)s);
     } else if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
         // ---- products
         const uint32_t elected = elect_one();
@@ -327,7 +360,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         // ---- softmax: a thread has a row
         const int t = (warp - 4) >> 2, row = t * 128 + (warp & 3) * 32 + lane;
         const bool there = row < rows;
@@ -388,67 +420,62 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             tc_fence_after();
-            float x[4][32];
-#pragma unroll
-            for (int q = 0; q < 4; q++) tm_ld32(s_tm + q * 32, x[q]);
-            tc_wait_ld();
             // (a tile that some row sees in part takes code of its own: its compares and selects
             // doubled the instructions of the others)
             auto weights = [&](auto part) {
                 constexpr bool kPart = decltype(part)::value;
                 const int from = b.lo - t0, to = b.hi - t0;  // the row's columns of the tile
-                float top = -INFINITY;
+                float x[2][32];
+                tm_ld32(s_tm, x[0]);
 #pragma unroll
-                for (int g = 0; g < 8; g++) {
-                    float m = -INFINITY;
+                for (int q = 0; q < 4; q++) {  // 32 tokens at a time
+                    float(&v)[32] = x[q & 1];
+                    tc_wait_ld();
+                    if (q < 3) tm_ld32(s_tm + (q + 1) * 32, x[(q + 1) & 1]);
+                    const float4 sc[2] = {scales[j & 3][2 * q], scales[j & 3][2 * q + 1]};
+                    const float a[2] = {a_row * sc[0].x, a_row * sc[1].x};
+                    float top = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float v = x[g / 2][16 * (g & 1) + i];
-                        const int col = 16 * g + i;
-                        if (!kPart || (col >= from && col < to)) m = fmaxf(m, v);
-                    }
-                    const float4 sc = scales[j & 3][g];
-                    if (!kPart || m != -INFINITY) top = fmaxf(top, fmaf(m, a_row * sc.x, sc.y));
-                }
-                const bool moves = top > M + kLag || (M == -INFINITY && top != -INFINITY);
-                if (__any_sync(0xffffffffu, moves)) {
-                    const float f = moves ? carry(M, top) : 1.0f;
-                    if (moves) M = top;
-                    L *= f;
-                    if (j) {
+                    for (int g = 0; g < 2; g++) {
+                        float m = -INFINITY;
 #pragma unroll
-                        for (int q = 0; q < D / 32; q++) {
-                            float y[32];
-                            tm_ld32(o_tm + q * 32, y);
-                            tc_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; i++) y[i] *= f;
-                            tm_st32(o_tm + q * 32, y);
+                        for (int i = 16 * g; i < 16 * g + 16; i += 2) {
+                            if constexpr (kPart) {
+                                if (32 * q + i >= from && 32 * q + i < to) m = fmaxf(m, v[i]);
+                                if (32 * q + i + 1 >= from && 32 * q + i + 1 < to) m = fmaxf(m, v[i + 1]);
+                            } else {
+                                m = fmaxf(m, fmaxf(v[i], v[i + 1]));
+                            }
                         }
+                        if (!kPart || m != -INFINITY) top = fmaxf(top, fmaf(m, a[g], sc[g].y));
                     }
-                }
-                const float head_room = (M == -INFINITY ? 0.0f : -M) + kHead;
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
+                    if (__any_sync(0xffffffffu, top > M + kLag)) {
+                        // M moves, to a whole number: what is scaled stays exact
+                        tc_wait_ld();
+                        const float next = top > M + kLag ? ceilf(top) : M, f = carry(M, next);
+                        M = next;
+                        L *= f;
+                        if (j) scale_columns<false>(o_tm, D / 32, f);
+                        if (q) scale_columns<true>(s_tm, q, f);
+                    }
+                    const float head_room = (M == -INFINITY ? 0.0f : -M) + kHead;
                     uint32_t w[16];
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
-                        const float4 sc = scales[j & 3][2 * q + g];
-                        const float a = a_row * sc.x, add = sc.y + head_room;
+                        const float add = sc[g].y + head_room;
                         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            float2 y = __ffma2_rn(make_float2(x[q][16 * g + i], x[q][16 * g + i + 1]), make_float2(a, a), make_float2(add, add));
+                        for (int i = 16 * g; i < 16 * g + 16; i += 2) {
+                            float2 y = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(a[g], a[g]), make_float2(add, add));
                             if constexpr (kPart) {
-                                const int col = 32 * q + 16 * g + i;
-                                if (col < from || col >= to) y.x = -INFINITY;
-                                if (col + 1 < from || col + 1 >= to) y.y = -INFINITY;
+                                if (32 * q + i < from || 32 * q + i >= to) y.x = -INFINITY;
+                                if (32 * q + i + 1 < from || 32 * q + i + 1 >= to) y.y = -INFINITY;
                             }
                             y.x = ex2_approx(y.x), y.y = ex2_approx(y.y);
                             sum = __fadd2_rn(sum, y);
-                            w[8 * g + i / 2] = pack2<__half>(y.x, y.y);
+                            w[i / 2] = pack2<__half>(y.x, y.y);
                         }
-                        L = fmaf(sum.x + sum.y, sc.z, L);
+                        L = fmaf(sum.x + sum.y, sc[g].z, L);
                     }
                     tm_st16(s_tm + q * 16, w);
                 }
