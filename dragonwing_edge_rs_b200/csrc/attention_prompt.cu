@@ -6,13 +6,15 @@
 // sums are rarely touched.
 //
 // A CTA has 256 rows (two tiles of 128: token by token the heads of a group) and goes through
-// tiles of 128 tokens:
+// tiles of 64 tokens:
 //   converters (4 warps)   codes of keys and values, from global memory through registers, as
 //                          f16 into shared memory (128-byte swizzled rows of 64 values);
-//   one issuing warp       S = Q K^T (128 x 128 x d) into tensor memory, O += P V with P from
+//   one issuing warp       S = Q K^T (128 x 64 x d) into tensor memory, O += P V with P from
 //                          tensor memory and V as it lies (tokens x values);
 //   2 x 4 softmax warps    a thread a row: S -> weights (f16, over S) and their sum.
-// While one row tile's weights are computed the other's products run.
+// Tensor memory holds O of both row tiles (256 columns) and two S of each: the next logits are
+// there when a tile's weights are done.  (Tiles of 128 tokens leave room for one S of each; a
+// row tile then waited for its own products, 1450 of 4700 cycles.)
 
 #include <algorithm>
 #include <type_traits>
@@ -26,14 +28,18 @@
 namespace dw {
 namespace {
 
-constexpr int kRows = 256, kTile = 128;  // query rows of a CTA, tokens of a tile
+constexpr int kRows = 256, kTile = 64;  // query rows of a CTA, tokens of a tile
+constexpr int kGroups = kTile / 16;     // of tokens that share scales
 constexpr int kThreads = 512;
-constexpr int kStages = 2;
+constexpr int kStages = 4;   // of keys and of values
 constexpr float kHead = 7.0f, kLag = 8.0f;
+constexpr int kEvery = 4;  // of that many pairs of weights one is computed by exp2_fma
 
 __device__ __forceinline__ bool wait_phase(uint64_t *barrier, uint32_t parity, const AttendParams &p, volatile int *abort_flag, int site) {
     const uint32_t bar = smem_u32(barrier);
-    if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (int i = 0; i < 16; i++)  // nearly every wait ends here, without a look at the clock
+        if (mbar_try_wait_sleep(bar, parity, 2000u)) return true;
     const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
     for (;;) {
@@ -91,14 +97,6 @@ __device__ __forceinline__ void tm_ld32(uint32_t taddr, float (&r)[32]) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tm_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
 __device__ __forceinline__ void tm_st32(uint32_t taddr, const float (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -118,32 +116,40 @@ __device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t (&r)[16])
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A row's columns of tensor memory times f: f32, 32 columns at a time, or f16 pairs, 16.
-template <bool kPairs>
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x of two values without the special-function unit, whose 16 results a cycle are what the
+// weights wait for: x = n + f, f in [-1/2, 1/2], a polynomial of degree 4 for 2^f (equal ripples,
+// relative error 2.6e-6) and n added to its exponent.  Below 2^-126 it gives 2^-126; x at most
+// 127, no NaN.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    const float2 magic = make_float2(kMagic, kMagic), lowest = make_float2(-126.0f, -126.0f);
+    x.x = fmaxf(x.x, lowest.x), x.y = fmaxf(x.y, lowest.y);
+    const float2 t = __fadd2_rn(x, magic);  // n in the low bits
+    const float2 f = __fadd2_rn(x, __ffma2_rn(t, make_float2(-1.0f, -1.0f), magic));
+    auto both = [](float c) { return make_float2(c, c); };
+    float2 r = __ffma2_rn(f, both(0x1.3997d6p-7f), both(0x1.ca1440p-5f));
+    r = __ffma2_rn(r, f, both(0x1.ec06dap-3f));
+    r = __ffma2_rn(r, f, both(0x1.62e0dcp-1f));
+    r = __ffma2_rn(r, f, both(0x1.ffffe8p-1f));
+    return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// A row's columns of tensor memory times f.
 __device__ __noinline__ void scale_columns(uint32_t taddr, int count, float f) {
-    tm_wait_st();
 #pragma unroll 1
     for (int q = 0; q < count; q++) {
-        if constexpr (kPairs) {
-            uint32_t w[16];
-            tm_ld16(taddr + q * 16, w);
-            tc_wait_ld();
+        float x[32];
+        tm_ld32(taddr + q * 32, x);
+        tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                __half2 h;
-                memcpy(&h, &w[i], 4);
-                const float2 v = __half22float2(h);
-                w[i] = pack2<__half>(v.x * f, v.y * f);
-            }
-            tm_st16(taddr + q * 16, w);
-        } else {
-            float x[32];
-            tm_ld32(taddr + q * 32, x);
-            tc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; i++) x[i] *= f;
-            tm_st32(taddr + q * 32, x);
-        }
+        for (int i = 0; i < 32; i++) x[i] *= f;
+        tm_st32(taddr + q * 32, x);
     }
 }
 
@@ -161,11 +167,11 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attend_prompt(const __grid_constant__ AttendParams p, const __grid_constant__ KvCache c, const __grid_constant__ Seqs sq) {
     constexpr int kHalves = D / 64;                   // swizzled tiles of 64 values
-    constexpr uint32_t kHalf = kTile * 128;           // bytes of one
-    constexpr uint32_t kOperand = kHalves * kHalf;    // of 128 rows of queries, keys or values
+    constexpr uint32_t kHalf = kTile * 128, kOperand = kHalves * kHalf;    // bytes of one, of a tile's keys or values
+    constexpr uint32_t kQHalf = 128 * 128, kQOperand = kHalves * kQHalf;   // the same of a row tile's queries
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], drain;
-    __shared__ float4 scales[4][8];  // of a tile's 16-token groups: 2^ek, ev, 2^-ev
+    __shared__ uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], drain;
+    __shared__ float4 scales[8][kGroups];  // of eight tiles: 2^ek, ev, 2^-ev
     __shared__ float row_scale[kRows];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
@@ -173,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     uint8_t *const base = smem_raw + (smem - smem_u32(smem_raw));
-    const uint32_t q_at = 0, k_at = 2 * kOperand, v_at = k_at + kStages * kOperand;
+    const uint32_t q_at = 0, k_at = 2 * kQOperand, v_at = k_at + kStages * kOperand;
 
     pdl_wait();
     // which rows of which sequence, which head: those that see most first
@@ -207,8 +213,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(smem_u32(&q_full[i]), 4), mbar_init(smem_u32(&s_full[i]), 1);
-            mbar_init(smem_u32(&p_full[i]), 4), mbar_init(smem_u32(&o_full[i]), 1);
+            mbar_init(smem_u32(&q_full[i]), 4), mbar_init(smem_u32(&s_full[i][0]), 1), mbar_init(smem_u32(&s_full[i][1]), 1);
+            mbar_init(smem_u32(&p_full[i][0]), 4), mbar_init(smem_u32(&p_full[i][1]), 4), mbar_init(smem_u32(&o_done[i][0]), 1), mbar_init(smem_u32(&o_done[i][1]), 1);
         }
         for (int i = 0; i < kStages; i++) {
             mbar_init(smem_u32(&k_full[i]), 4), mbar_init(smem_u32(&k_empty[i]), 1);
@@ -227,55 +233,58 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     pdl_trigger();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);  // S of either row tile (128 columns each), then O
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);  // two S of 64 columns of each row tile, then O
 
     if (warp >= 12) {
-        // ---- converters: a thread has 16 codes of a row of each half of each of four groups of 32 rows
+        // ---- converters: a thread has 16 codes of each half of a row in each of two groups of 32 rows
         const int tid = threadIdx.x - 384, part = tid & 3, sub = tid >> 2;
+        constexpr int kG = kTile / 32, kN = kG * kHalves;
+        const int shift = 31 - __clz(c.page);  // pages hold a power of two of tokens
         // (a row's page is looked up a tile ahead of its codes: in order they waited for one
         // lookup after the other)
-        uint4 kx[4 * kHalves], vx[4 * kHalves];
-        uint32_t page[4], ahead[4], scale_page = 0, scale_ahead = 0;
+        uint4 kx[kN], vx[kN];
+        uint32_t page[kG], ahead[kG], scale_page = 0, scale_ahead = 0;
         bool bad = false;
         auto lookup = [&](int t) {  // the page of token t, in bounds in any case
             if (t >= r.len) return 0u;
-            const uint32_t id = (uint32_t)sq.table[(size_t)s * sq.width + (uint32_t)t / (uint32_t)c.page];
+            const uint32_t id = (uint32_t)sq.table[(size_t)s * sq.width + (uint32_t)(t >> shift)];
             bad |= id >= c.pages;
             return id;
         };
         auto find = [&](int tile) {
             const int t = (tile0 + tile) * kTile;
 #pragma unroll
-            for (int g = 0; g < 4; g++) ahead[g] = lookup(t + g * 32 + sub);
-            if (tid < 8) scale_ahead = lookup(t + tid * 16);
+            for (int g = 0; g < kG; g++) ahead[g] = lookup(t + g * 32 + sub);
+            if (tid < kGroups) scale_ahead = lookup(t + tid * 16);
         };
         auto take = [&]() {
 #pragma unroll
-            for (int g = 0; g < 4; g++) page[g] = min(ahead[g], c.pages - 1);
+            for (int g = 0; g < kG; g++) page[g] = min(ahead[g], c.pages - 1);
             scale_page = min(scale_ahead, c.pages - 1);
         };
-        auto load = [&](uint4 (&x)[4 * kHalves], const uint8_t *codes, int tile) {
+        auto load = [&](uint4 (&x)[kN], const uint8_t *codes, int tile) {
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
+            for (int g = 0; g < kG; g++) {
                 const int t = (tile0 + tile) * kTile + g * 32 + sub;
-                const uint4 *from = reinterpret_cast<const uint4 *>(codes + (kv_block(c, page[g], head) * c.page + t % c.page) * D) + part;
+                const uint32_t row = ((page[g] * (uint32_t)c.heads + (uint32_t)head) << shift) + (uint32_t)(t & (c.page - 1));
+                const uint4 *from = reinterpret_cast<const uint4 *>(codes + (size_t)row * D) + part;
 #pragma unroll
                 for (int h = 0; h < kHalves; h++)  // no token: zeros, whatever the page holds there
                     x[g * kHalves + h] = t < r.len ? from[4 * h] : make_uint4(0, 0, 0, 0);
             }
         };
-        auto store = [&](const uint4 (&x)[4 * kHalves], uint32_t at) {
+        auto store = [&](const uint4 (&x)[kN], uint32_t at) {
+            // (row & 7 is the same in every group)
+            const uint32_t to = smem + at + swizzled(sub, 2 * part), to1 = smem + at + swizzled(sub, 2 * part + 1);
 #pragma unroll
-            for (int g = 0; g < 4; g++)
+            for (int g = 0; g < kG; g++)
 #pragma unroll
                 for (int h = 0; h < kHalves; h++) {
                     const uint4 u = x[g * kHalves + h];
-                    const int row = g * 32 + sub;
-                    const uint32_t to = smem + at + h * kHalf;
-                    sts_v4(to + swizzled(row, 2 * part), make_uint4(e4m3_to_f16x2((uint16_t)u.x), e4m3_to_f16x2((uint16_t)(u.x >> 16)),
-                                                                   e4m3_to_f16x2((uint16_t)u.y), e4m3_to_f16x2((uint16_t)(u.y >> 16))));
-                    sts_v4(to + swizzled(row, 2 * part + 1), make_uint4(e4m3_to_f16x2((uint16_t)u.z), e4m3_to_f16x2((uint16_t)(u.z >> 16)),
-                                                                       e4m3_to_f16x2((uint16_t)u.w), e4m3_to_f16x2((uint16_t)(u.w >> 16))));
+                    sts_v4(to + h * kHalf + g * 4096, make_uint4(e4m3_to_f16x2((uint16_t)u.x), e4m3_to_f16x2((uint16_t)(u.x >> 16)),
+                                                                 e4m3_to_f16x2((uint16_t)u.y), e4m3_to_f16x2((uint16_t)(u.y >> 16))));
+                    sts_v4(to1 + h * kHalf + g * 4096, make_uint4(e4m3_to_f16x2((uint16_t)u.z), e4m3_to_f16x2((uint16_t)(u.z >> 16)),
+                                                                  e4m3_to_f16x2((uint16_t)u.w), e4m3_to_f16x2((uint16_t)(u.w >> 16))));
                 }
         };
         auto done = [&](uint64_t *bar) {
@@ -284,24 +293,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(smem_u32(bar));
         };
         uint32_t sc = 0;
-        auto load_scale = [&](int tile) {  // of group tid (0..7)
-            if (tid < 8) sc = *reinterpret_cast<const uint16_t *>(c.s + kv_block(c, scale_page, head) * 2);
+        auto load_scale = [&]() {  // of group tid
+            if (tid < kGroups) sc = *reinterpret_cast<const uint16_t *>(c.s + kv_block(c, scale_page, head) * 2);
         };
-        if (all) find(0), take(), load(kx, c.k, 0), load_scale(0), load(vx, c.v, 0);
+        if (all) find(0), take(), load(kx, c.k, 0), load_scale(), load(vx, c.v, 0);
         if (all > 1) find(1);
         for (int j = 0; j < all; j++) {
             const int st = j % kStages;
             const uint32_t ph = (uint32_t)(j / kStages) & 1;
             if (j >= kStages && !wait_warp(&k_empty[st], ph ^ 1, p, abort_flag, 71)) break;
             store(kx, k_at + st * kOperand);
-            if (tid < 8) {
+            if (tid < kGroups) {
                 const int ve = kv_exponent(sc >> 8);
-                scales[j & 3][tid] = make_float4(kv_pow2(kv_exponent(sc & 255)), (float)ve, kv_pow2(-ve), 0.0f);
+                scales[j & 7][tid] = make_float4(kv_pow2(kv_exponent(sc & 255)), (float)ve, kv_pow2(-ve), 0.0f);
             }
             done(&k_full[st]);
             if (j + 1 < all) {
                 take();
-                load(kx, c.k, j + 1), load_scale(j + 1);
+                load(kx, c.k, j + 1), load_scale();
                 if (j + 2 < all) find(j + 2);
             }
             if (j >= kStages && !wait_warp(&v_empty[st], ph ^ 1, p, abort_flag, 72)) break;
@@ -318,41 +327,46 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
         constexpr uint64_t hi = ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
         auto logits = [&](int t, int j) {
-            const uint32_t a = smem + q_at + t * kOperand, b = smem + k_at + (j % kStages) * kOperand;
+            const uint32_t a = smem + q_at + t * kQOperand, b = smem + k_at + (j % kStages) * kOperand;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) {
-                const uint32_t off = (uint32_t)(i / 4) * kHalf + (uint32_t)(i % 4) * 32;
-                mma_ss(elected, tmem + t * 128, smem_desc(a + off, hi), smem_desc(b + off, hi), idesc_s, i ? 1u : 0u);
+                const uint32_t in = (uint32_t)(i % 4) * 32;
+                mma_ss(elected, tmem + (2 * t + (j & 1)) * kTile, smem_desc(a + (i / 4) * kQHalf + in, hi), smem_desc(b + (i / 4) * kHalf + in, hi),
+                       idesc_s, i ? 1u : 0u);
             }
-            commit(elected, &s_full[t]);
+            commit(elected, &s_full[t][j & 1]);
         };
         auto sums = [&](int t, int j) {
             const uint32_t b = smem + v_at + (j % kStages) * kOperand;
 #pragma unroll
             for (int i = 0; i < kTile / 16; i++)
-                mma_ts(elected, tmem + 256 + t * D, tmem + t * 128 + i * 8, desc_rows(b + i * 2048, kHalf), idesc_o, (j || i) ? 1u : 0u);
+                mma_ts(elected, tmem + 256 + t * D, tmem + (2 * t + (j & 1)) * kTile + i * 8, desc_rows(b + i * 2048, kHalf), idesc_o,
+                       (j || i) ? 1u : 0u);
+            commit(elected, &o_done[t][j & 1]);
         };
+        auto phase = [](int j) { return (uint32_t)(j / kStages) & 1; };
         bool ok = true;
         for (int t = 0; t < 2 && ok; t++)
             if (tiles[t]) ok = wait_warp(&q_full[t], 0, p, abort_flag, 73);
-        for (int j = -1; j < all && ok; j++) {
-            // O += P V of tile j, S of tile j + 1
-            if (j + 1 < all) ok = wait_warp(&k_full[(j + 1) % kStages], (uint32_t)((j + 1) / kStages) & 1, p, abort_flag, 74);
-            if (ok && j >= 0) ok = wait_warp(&v_full[j % kStages], (uint32_t)(j / kStages) & 1, p, abort_flag, 75);
+        for (int j = -2; j < all && ok; j++) {
+            // O += P V of tile j, then S of tile j + 2 in the place of what these weights were made of
+            const int k = j + 2;
+            if (j >= 0) ok = wait_warp(&v_full[j % kStages], phase(j), p, abort_flag, 75);
             for (int t = 0; t < 2 && ok; t++) {
                 if (j >= 0 && j < tiles[t]) {
-                    ok = wait_warp(&p_full[t], (uint32_t)j & 1, p, abort_flag, 76);
+                    ok = wait_warp(&p_full[t][j & 1], (uint32_t)(j >> 1) & 1, p, abort_flag, 76);
                     if (!ok) break;
                     tc_fence_after();
                     sums(t, j);
-                    if (j + 1 == tiles[t]) commit(elected, &o_full[t]);
                 }
+                if (k < all && t == 0) ok = wait_warp(&k_full[k % kStages], phase(k), p, abort_flag, 74);
+                if (!ok) break;
                 tc_fence_after();
-                if (j + 1 < tiles[t]) logits(t, j + 1);
+                if (k < tiles[t]) logits(t, k);
             }
             if (!ok) break;
             if (j >= 0) commit(elected, &v_empty[j % kStages]);
-            if (j + 1 < all) commit(elected, &k_empty[(j + 1) % kStages]);
+            if (k < all) commit(elected, &k_empty[k % kStages]);
         }
         // products in flight end before the tensor memory is given back
         commit(elected, &drain);
@@ -376,21 +390,28 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i0 = 0; i0 < kPer; i0 += 8) {
                 Raw<T, 8> x[8];
+                auto source = [&](int i) {  // in bounds in any case
+                    const int at = first + min(row0 + (i0 + i) * (32 / kPer), rows - 1);
+                    return (const T *)p.q + (size_t)(r.row0 + at / p.group) * p.q_pitch + (size_t)(head * p.group + at % p.group) * D + 8 * piece;
+                };
+                if (p.vec) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int row = row0 + (i0 + i) * (32 / kPer), at = first + row;
-                    x[i].zero();
-                    if (row >= rows) continue;
-                    const T *src = (const T *)p.q + (size_t)(r.row0 + at / p.group) * p.q_pitch + (size_t)(head * p.group + at % p.group) * D + 8 * piece;
-                    if (p.vec) {
-                        x[i].load(src);
-                    } else {
+                    for (int i = 0; i < 8; i++) x[i].load(source(i));
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < 8; i++) {
+                        const T *src = source(i);
                         float u[8];
 #pragma unroll
                         for (int e = 0; e < 8; e++) u[e] = to_f32(src[e]);
-                        x[i].set(u);
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            if (k == i) x[k].set(u);
                     }
                 }
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (row0 + (i0 + i) * (32 / kPer) >= rows) x[i].zero();
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const int row = row0 + (i0 + i) * (32 / kPer);
@@ -408,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint32_t w[4];
 #pragma unroll
                     for (int e = 0; e < 4; e++) w[e] = pack2<__half>(x[i].get(2 * e) * down, x[i].get(2 * e + 1) * down);
-                    sts_v4(smem + q_at + t * kOperand + (piece / 8) * kHalf + swizzled(row & 127, piece & 7), make_uint4(w[0], w[1], w[2], w[3]));
+                    sts_v4(smem + q_at + t * kQOperand + (piece / 8) * kQHalf + swizzled(row & 127, piece & 7), make_uint4(w[0], w[1], w[2], w[3]));
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -417,14 +438,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (std::is_same_v<T, __nv_bfloat16>) a_row *= row_scale[row];
         }
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_tm = tmem + t * 128 + lanes, o_tm = tmem + 256 + t * D + lanes;
+        const uint32_t s0_tm = tmem + 2 * t * kTile + lanes, o_tm = tmem + 256 + t * D + lanes;
         // tokens that all of the warp's rows see, and those that any does
         const int lo_all = __reduce_max_sync(0xffffffffu, b.lo), hi_all = __reduce_min_sync(0xffffffffu, b.hi);
         float M = -INFINITY, L = 0.0f;
         bool ok = true;
         for (int j = 0; j < tiles[t]; j++) {
             const int t0 = (tile0 + j) * kTile;
-            if (!wait_warp(&s_full[t], (uint32_t)j & 1, p, abort_flag, 77)) {
+            if (!wait_warp(&s_full[t][j & 1], (uint32_t)(j >> 1) & 1, p, abort_flag, 77)) {
                 ok = false;
                 break;
             }
@@ -434,57 +455,66 @@ __global__ void __launch_bounds__(kThreads, 1)
             auto weights = [&](auto part) {
                 constexpr bool kPart = decltype(part)::value;
                 const int from = b.lo - t0, to = b.hi - t0;  // the row's columns of the tile
-                float x[2][32];
-                tm_ld32(s_tm, x[0]);
+                const uint32_t s_tm = s0_tm + (j & 1) * kTile;
+                float x[kTile / 32][32];
 #pragma unroll
-                for (int q = 0; q < 4; q++) {  // 32 tokens at a time
-                    float(&v)[32] = x[q & 1];
-                    tc_wait_ld();
-                    if (q < 3) tm_ld32(s_tm + (q + 1) * 32, x[(q + 1) & 1]);
-                    const float4 sc[2] = {scales[j & 3][2 * q], scales[j & 3][2 * q + 1]};
-                    const float a[2] = {a_row * sc[0].x, a_row * sc[1].x};
-                    float top = -INFINITY;
+                for (int q = 0; q < kTile / 32; q++) tm_ld32(s_tm + q * 32, x[q]);
+                float4 sc[kGroups];
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        float m = -INFINITY;
+                for (int g = 0; g < kGroups; g++) sc[g] = scales[j & 7][g], sc[g].x *= a_row;
+                tc_wait_ld();
+                // the largest exponent; NaN where there is one (M then becomes NaN, and all that the row sums)
+                float top = -INFINITY;
 #pragma unroll
-                        for (int i = 16 * g; i < 16 * g + 16; i += 2) {
-                            if constexpr (kPart) {
-                                if (32 * q + i >= from && 32 * q + i < to) m = fmaxf(m, v[i]);
-                                if (32 * q + i + 1 >= from && 32 * q + i + 1 < to) m = fmaxf(m, v[i + 1]);
-                            } else {
-                                m = fmaxf(m, fmaxf(v[i], v[i + 1]));
-                            }
-                        }
-                        if (!kPart || m != -INFINITY) top = fmaxf(top, fmaf(m, a[g], sc[g].y));
+                for (int g = 0; g < kGroups; g++) {
+                    const float *v = x[g / 2] + 16 * (g & 1);
+                    if constexpr (kPart) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (16 * g + i >= from && 16 * g + i < to) top = max_nan(top, top, fmaf(v[i], sc[g].x, sc[g].y));
+                    } else {
+                        float m = max_nan(v[0], v[1], v[2]), n = max_nan(v[3], v[4], v[5]);
+#pragma unroll
+                        for (int i = 6; i < 14; i += 4) m = max_nan(m, v[i], v[i + 1]), n = max_nan(n, v[i + 2], v[i + 3]);
+                        m = max_nan(m, v[14], v[15]);
+                        top = max_nan(top, top, fmaf(max_nan(m, n, n), sc[g].x, sc[g].y));
                     }
-                    if (__any_sync(0xffffffffu, top > M + kLag)) {
-                        // M moves, to a whole number: what is scaled stays exact
-                        tc_wait_ld();
-                        const float next = top > M + kLag ? ceilf(top) : M, f = carry(M, next);
-                        M = next;
-                        L *= f;
-                        if (j) scale_columns<false>(o_tm, D / 32, f);
-                        if (q) scale_columns<true>(s_tm, q, f);
+                }
+                if (__any_sync(0xffffffffu, !(top <= M + kLag))) {
+                    // M moves, to a whole number: what is scaled stays exact
+                    const float next = top <= M + kLag ? M : ceilf(top), f = carry(M, next);
+                    M = next;
+                    L *= f;
+                    if (j) {
+                        // (that of tile j - 2 is done, or its place would not hold these logits)
+                        ok = wait_warp(&o_done[t][(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, p, abort_flag, 79);
+                        tc_fence_after();
+                        scale_columns(o_tm, D / 32, f);
                     }
-                    const float head_room = (M == -INFINITY ? 0.0f : -M) + kHead;
+                }
+                const float head_room = (M == -INFINITY ? 0.0f : -M) + kHead;
+#pragma unroll
+                for (int q = 0; q < kTile / 32; q++) {
                     uint32_t w[16];
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
-                        const float add = sc[g].y + head_room;
+                        const float a = sc[2 * q + g].x, add = sc[2 * q + g].y + head_room;
                         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int i = 16 * g; i < 16 * g + 16; i += 2) {
-                            float2 y = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(a[g], a[g]), make_float2(add, add));
+                            float2 y = __ffma2_rn(make_float2(x[q][i], x[q][i + 1]), make_float2(a, a), make_float2(add, add));
                             if constexpr (kPart) {
                                 if (32 * q + i < from || 32 * q + i >= to) y.x = -INFINITY;
                                 if (32 * q + i + 1 < from || 32 * q + i + 1 >= to) y.y = -INFINITY;
                             }
-                            y.x = ex2_approx(y.x), y.y = ex2_approx(y.y);
+                            if (!kPart && i / 2 % kEvery == kEvery - 1)
+                                y = exp2_fma(y);
+                            else
+                                y.x = ex2_approx(y.x), y.y = ex2_approx(y.y);
                             sum = __fadd2_rn(sum, y);
                             w[i / 2] = pack2<__half>(y.x, y.y);
                         }
-                        L = fmaf(sum.x + sum.y, sc[g].z, L);
+                        L = fmaf(sum.x + sum.y, sc[2 * q + g].z, L);
                     }
                     tm_st16(s_tm + q * 16, w);
                 }
@@ -493,12 +523,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 weights(std::true_type{});
             else
                 weights(std::false_type{});
+            if (!ok) break;
             tm_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&p_full[t]));
+            if (lane == 0) mbar_arrive(smem_u32(&p_full[t][j & 1]));
         }
-        if (tiles[t] && ok) ok = wait_warp(&o_full[t], 0, p, abort_flag, 78);
+        if (tiles[t] && ok) {
+            const int last = tiles[t] - 1;
+            ok = wait_warp(&o_done[t][last & 1], (uint32_t)(last >> 1) & 1, p, abort_flag, 78);
+        }
         if (ok && rows > t * 128 + (warp & 3) * 32) {
             tc_fence_after();
             const float f = L == 0.0f ? 0.0f : 1.0f / L;
@@ -545,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, int D>
 dw_status attend_prompt(dw_backend *be, AttendParams p, const KvCache &c, const Seqs &s) {
     auto kernel = k_attend_prompt<T, D>;
-    constexpr size_t smem = 1024 + (size_t)(2 + 2 * kStages) * kTile * D * 2;
+    constexpr size_t smem = 1024 + (size_t)(2 * 128 + 2 * kStages * kTile) * D * 2;
     const size_t n = s.tokens / s.seqs;
     p.per_seq = s.starts ? 0 : (int)((n * p.group + kRows - 1) / kRows);
     const size_t items = s.starts ? seq_items(s.tokens, s.seqs, p.group, kRows, 1) : (size_t)p.per_seq * s.seqs;
