@@ -9,7 +9,8 @@
 // tiles of 64 tokens:
 //   converters (4 warps)   codes of keys and values, from global memory through registers, as
 //                          f16 into shared memory (128-byte swizzled rows of 64 values);
-//   one issuing warp       S = Q K^T (128 x 64 x d) into tensor memory, O += P V with P from
+//   2 issuing warps        (one for each row tile: what one waits for, the other's products fill)
+//                          S = Q K^T (128 x 64 x d) into tensor memory, O += P V with P from
 //                          tensor memory and V as it lies (tokens x values);
 //   2 x 4 softmax warps    a thread a row: S -> weights (f16, over S) and their sum.
 // Tensor memory holds O of both row tiles (256 columns) and two S of each: the next logits are
@@ -37,9 +38,11 @@ constexpr int kEvery = 4;  // of that many pairs of weights one is computed by e
 
 __device__ __forceinline__ bool wait_phase(uint64_t *barrier, uint32_t parity, const AttendParams &p, volatile int *abort_flag, int site) {
     const uint32_t bar = smem_u32(barrier);
+    // nearly every wait ends here, without a look at the clock (a wait with a time to sleep wakes
+    // up late)
 #pragma unroll 1
-    for (int i = 0; i < 16; i++)  // nearly every wait ends here, without a look at the clock
-        if (mbar_try_wait_sleep(bar, parity, 2000u)) return true;
+    for (int i = 0; i < 4096; i++)
+        if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
     for (;;) {
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t kHalf = kTile * 128, kOperand = kHalves * kHalf;    // bytes of one, of a tile's keys or values
     constexpr uint32_t kQHalf = 128 * 128, kQOperand = kHalves * kQHalf;   // the same of a row tile's queries
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], drain;
+    __shared__ uint64_t q_full[2], s_full[2][2], p_full[2][2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], drain[2];
     __shared__ float4 scales[8][kGroups];  // of eight tiles: 2^ek, ev, 2^-ev
     __shared__ float row_scale[kRows];
     __shared__ uint32_t tmem_slot;
@@ -214,18 +217,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(smem_u32(&q_full[i]), 4), mbar_init(smem_u32(&s_full[i][0]), 1), mbar_init(smem_u32(&s_full[i][1]), 1);
-            mbar_init(smem_u32(&p_full[i][0]), 4), mbar_init(smem_u32(&p_full[i][1]), 4), mbar_init(smem_u32(&o_done[i][0]), 1), mbar_init(smem_u32(&o_done[i][1]), 1);
+            mbar_init(smem_u32(&p_full[i][0]), 4), mbar_init(smem_u32(&p_full[i][1]), 4), mbar_init(smem_u32(&drain[i]), 1);
         }
         for (int i = 0; i < kStages; i++) {
-            mbar_init(smem_u32(&k_full[i]), 4), mbar_init(smem_u32(&k_empty[i]), 1);
-            mbar_init(smem_u32(&v_full[i]), 4), mbar_init(smem_u32(&v_empty[i]), 1);
+            mbar_init(smem_u32(&k_full[i]), 4), mbar_init(smem_u32(&k_empty[i]), 2);
+            mbar_init(smem_u32(&v_full[i]), 4), mbar_init(smem_u32(&v_empty[i]), 2);
         }
-        mbar_init(smem_u32(&drain), 1);
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 1) {
+    if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -240,10 +242,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int tid = threadIdx.x - 384, part = tid & 3, sub = tid >> 2;
         constexpr int kG = kTile / 32, kN = kG * kHalves;
         const int shift = 31 - __clz(c.page);  // pages hold a power of two of tokens
-        // (a row's page is looked up a tile ahead of its codes: in order they waited for one
-        // lookup after the other)
-        uint4 kx[kN], vx[kN];
-        uint32_t page[kG], ahead[kG], scale_page = 0, scale_ahead = 0;
+        // Codes are loaded two tiles ahead, and a row's page looked up a tile before that: a load takes
+        // some 800 cycles, a lookup as many before it.
+        struct Pages {
+            uint32_t row[kG], group;  // of the thread's rows; of group tid
+        } ahead{};
+        struct Codes {
+            uint4 k[kN], v[kN];
+            uint32_t scales;  // of group tid
+        } x0, x1;
         bool bad = false;
         auto lookup = [&](int t) {  // the page of token t, in bounds in any case
             if (t >= r.len) return 0u;
@@ -251,27 +258,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             bad |= id >= c.pages;
             return id;
         };
-        auto find = [&](int tile) {
+        auto find = [&](Pages &g, int tile) {
             const int t = (tile0 + tile) * kTile;
 #pragma unroll
-            for (int g = 0; g < kG; g++) ahead[g] = lookup(t + g * 32 + sub);
-            if (tid < kGroups) scale_ahead = lookup(t + tid * 16);
+            for (int i = 0; i < kG; i++) g.row[i] = lookup(t + i * 32 + sub);
+            if (tid < kGroups) g.group = lookup(t + tid * 16);
         };
-        auto take = [&]() {
-#pragma unroll
-            for (int g = 0; g < kG; g++) page[g] = min(ahead[g], c.pages - 1);
-            scale_page = min(scale_ahead, c.pages - 1);
-        };
-        auto load = [&](uint4 (&x)[kN], const uint8_t *codes, int tile) {
+        auto load = [&](uint4 (&x)[kN], const uint8_t *codes, const Pages &pg, int tile) {
 #pragma unroll
             for (int g = 0; g < kG; g++) {
                 const int t = (tile0 + tile) * kTile + g * 32 + sub;
-                const uint32_t row = ((page[g] * (uint32_t)c.heads + (uint32_t)head) << shift) + (uint32_t)(t & (c.page - 1));
+                const uint32_t row = ((min(pg.row[g], c.pages - 1) * (uint32_t)c.heads + (uint32_t)head) << shift) + (uint32_t)(t & (c.page - 1));
                 const uint4 *from = reinterpret_cast<const uint4 *>(codes + (size_t)row * D) + part;
 #pragma unroll
                 for (int h = 0; h < kHalves; h++)  // no token: zeros, whatever the page holds there
                     x[g * kHalves + h] = t < r.len ? from[4 * h] : make_uint4(0, 0, 0, 0);
             }
+        };
+        auto load_scales = [&](Codes &x, const Pages &pg) {
+            if (tid < kGroups) x.scales = *reinterpret_cast<const uint16_t *>(c.s + kv_block(c, min(pg.group, c.pages - 1), head) * 2);
         };
         auto store = [&](const uint4 (&x)[kN], uint32_t at) {
             // (row & 7 is the same in every group)
@@ -292,89 +297,78 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(bar));
         };
-        uint32_t sc = 0;
-        auto load_scale = [&]() {  // of group tid
-            if (tid < kGroups) sc = *reinterpret_cast<const uint16_t *>(c.s + kv_block(c, scale_page, head) * 2);
-        };
-        if (all) find(0), take(), load(kx, c.k, 0), load_scale(), load(vx, c.v, 0);
-        if (all > 1) find(1);
-        for (int j = 0; j < all; j++) {
+        Pages second{};
+        if (all) find(ahead, 0);
+        if (all > 1) find(second, 1);
+        if (all) load(x0.k, c.k, ahead, 0), load_scales(x0, ahead), load(x0.v, c.v, ahead, 0);
+        if (all > 1) load(x1.k, c.k, second, 1), load_scales(x1, second), load(x1.v, c.v, second, 1);
+        if (all > 2) find(ahead, 2);
+        auto convert = [&](int j, Codes &x) {
             const int st = j % kStages;
             const uint32_t ph = (uint32_t)(j / kStages) & 1;
-            if (j >= kStages && !wait_warp(&k_empty[st], ph ^ 1, p, abort_flag, 71)) break;
-            store(kx, k_at + st * kOperand);
+            if (j >= kStages && !wait_warp(&k_empty[st], ph ^ 1, p, abort_flag, 71)) return false;
+            store(x.k, k_at + st * kOperand);
             if (tid < kGroups) {
-                const int ve = kv_exponent(sc >> 8);
-                scales[j & 7][tid] = make_float4(kv_pow2(kv_exponent(sc & 255)), (float)ve, kv_pow2(-ve), 0.0f);
+                const int ve = kv_exponent(x.scales >> 8);
+                scales[j & 7][tid] = make_float4(kv_pow2(kv_exponent(x.scales & 255)), (float)ve, kv_pow2(-ve), 0.0f);
             }
             done(&k_full[st]);
-            if (j + 1 < all) {
-                take();
-                load(kx, c.k, j + 1), load_scale();
-                if (j + 2 < all) find(j + 2);
-            }
-            if (j >= kStages && !wait_warp(&v_empty[st], ph ^ 1, p, abort_flag, 72)) break;
-            store(vx, v_at + st * kOperand);
+            const Pages now = ahead;
+            if (j + 2 < all) load(x.k, c.k, now, j + 2), load_scales(x, now);
+            if (j + 3 < all) find(ahead, j + 3);
+            if (j >= kStages && !wait_warp(&v_empty[st], ph ^ 1, p, abort_flag, 72)) return false;
+            store(x.v, v_at + st * kOperand);
             done(&v_full[st]);
-            if (j + 1 < all) load(vx, c.v, j + 1);
-        }
+            if (j + 2 < all) load(x.v, c.v, now, j + 2);
+            return true;
+        };
+        for (int j = 0; j < all; j += 2)
+            if (!convert(j, x0) || (j + 1 < all && !convert(j + 1, x1))) break;
         if (bad) record_error(p.err, DW_DEV_BAD_ARG, 62, (int)s);
-    } else if (warp < 4) {
-        if (warp == 0) {
-        // ---- products
+    } else if (warp < 2) {
+        // ---- products of row tile t: S of tile j + 2 goes to the place of what the weights of tile j were made of
+        const int t = warp;
         const uint32_t elected = elect_one();
         constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | (8u << 24);
         constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
         constexpr uint64_t hi = ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-        auto logits = [&](int t, int j) {
-            const uint32_t a = smem + q_at + t * kQOperand, b = smem + k_at + (j % kStages) * kOperand;
-#pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                const uint32_t in = (uint32_t)(i % 4) * 32;
-                mma_ss(elected, tmem + (2 * t + (j & 1)) * kTile, smem_desc(a + (i / 4) * kQHalf + in, hi), smem_desc(b + (i / 4) * kHalf + in, hi),
-                       idesc_s, i ? 1u : 0u);
-            }
-            commit(elected, &s_full[t][j & 1]);
-        };
-        auto sums = [&](int t, int j) {
-            const uint32_t b = smem + v_at + (j % kStages) * kOperand;
-#pragma unroll
-            for (int i = 0; i < kTile / 16; i++)
-                mma_ts(elected, tmem + 256 + t * D, tmem + (2 * t + (j & 1)) * kTile + i * 8, desc_rows(b + i * 2048, kHalf), idesc_o,
-                       (j || i) ? 1u : 0u);
-            commit(elected, &o_done[t][j & 1]);
-        };
         auto phase = [](int j) { return (uint32_t)(j / kStages) & 1; };
-        bool ok = true;
-        for (int t = 0; t < 2 && ok; t++)
-            if (tiles[t]) ok = wait_warp(&q_full[t], 0, p, abort_flag, 73);
+        bool ok = !tiles[t] || wait_warp(&q_full[t], 0, p, abort_flag, 73);
         for (int j = -2; j < all && ok; j++) {
-            // O += P V of tile j, then S of tile j + 2 in the place of what these weights were made of
             const int k = j + 2;
+            const bool sums = j >= 0 && j < tiles[t], logits = k < tiles[t];
+            // (stages of tiles that only the other row tile needs are waited for and given back too)
             if (j >= 0) ok = wait_warp(&v_full[j % kStages], phase(j), p, abort_flag, 75);
-            for (int t = 0; t < 2 && ok; t++) {
-                if (j >= 0 && j < tiles[t]) {
-                    ok = wait_warp(&p_full[t][j & 1], (uint32_t)(j >> 1) & 1, p, abort_flag, 76);
-                    if (!ok) break;
-                    tc_fence_after();
-                    sums(t, j);
-                }
-                if (k < all && t == 0) ok = wait_warp(&k_full[k % kStages], phase(k), p, abort_flag, 74);
-                if (!ok) break;
-                tc_fence_after();
-                if (k < tiles[t]) logits(t, k);
-            }
+            if (k < all && ok) ok = wait_warp(&k_full[k % kStages], phase(k), p, abort_flag, 74);
+            if (sums && ok) ok = wait_warp(&p_full[t][j & 1], (uint32_t)(j >> 1) & 1, p, abort_flag, 76);
             if (!ok) break;
+            tc_fence_after();
+            const uint32_t s_tm = tmem + (2 * t + (j & 1)) * kTile;
+            if (sums) {
+                const uint32_t b = smem + v_at + (j % kStages) * kOperand;
+#pragma unroll
+                for (int i = 0; i < kTile / 16; i++)
+                    mma_ts(elected, tmem + 256 + t * D, s_tm + i * 8, desc_rows(b + i * 2048, kHalf), idesc_o, (j || i) ? 1u : 0u);
+            }
+            if (logits) {
+                const uint32_t a = smem + q_at + t * kQOperand, b = smem + k_at + (k % kStages) * kOperand;
+#pragma unroll
+                for (int i = 0; i < D / 16; i++) {
+                    const uint32_t in = (uint32_t)(i % 4) * 32;
+                    mma_ss(elected, s_tm, smem_desc(a + (i / 4) * kQHalf + in, hi), smem_desc(b + (i / 4) * kHalf + in, hi), idesc_s, i ? 1u : 0u);
+                }
+            }
+            // also without logits (behind the last tile): the sums up to tile j are done then
+            if (k < tiles[t] + 2) commit(elected, &s_full[t][j & 1]);
             if (j >= 0) commit(elected, &v_empty[j % kStages]);
             if (k < all) commit(elected, &k_empty[k % kStages]);
         }
         // products in flight end before the tensor memory is given back
-        commit(elected, &drain);
+        commit(elected, &drain[t]);
         const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait_sleep(smem_u32(&drain), 0, 20000u) && globaltimer_ns() - t0 < p.wait_cap_ns) {
+        while (!mbar_try_wait_sleep(smem_u32(&drain[t]), 0, 20000u) && globaltimer_ns() - t0 < p.wait_cap_ns) {
         }
-        }
-    } else {
+    } else if (warp >= 4) {
         // ---- softmax: a thread has a row
         const int t = (warp - 4) >> 2, row = t * 128 + (warp & 3) * 32 + lane;
         const bool there = row < rows;
@@ -486,8 +480,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     M = next;
                     L *= f;
                     if (j) {
-                        // (that of tile j - 2 is done, or its place would not hold these logits)
-                        ok = wait_warp(&o_done[t][(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1, p, abort_flag, 79);
+                        // the sums up to tile j - 1 are done when the logits of tile j + 1 are there
+                        ok = wait_warp(&s_full[t][(j + 1) & 1], (uint32_t)((j + 1) >> 1) & 1, p, abort_flag, 79);
                         tc_fence_after();
                         scale_columns(o_tm, D / 32, f);
                     }
@@ -529,10 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&p_full[t][j & 1]));
         }
-        if (tiles[t] && ok) {
-            const int last = tiles[t] - 1;
-            ok = wait_warp(&o_done[t][last & 1], (uint32_t)(last >> 1) & 1, p, abort_flag, 78);
-        }
+        if (tiles[t] && ok) ok = wait_warp(&s_full[t][(tiles[t] + 1) & 1], (uint32_t)((tiles[t] + 1) >> 1) & 1, p, abort_flag, 78);
         if (ok && rows > t * 128 + (warp & 3) * 32) {
             tc_fence_after();
             const float f = L == 0.0f ? 0.0f : 1.0f / L;
@@ -568,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 2) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
