@@ -3,16 +3,19 @@
 //   out = sum_j softmax_j(scale * q . k_j) v_j
 // A block's keys are codes times 2^ek, its values codes times 2^ev.  With t_j = log2(e) scale
 // q . k_j + ev_j and M = max t_j over the tokens so far,
-//   w_j = 2^(t_j - M + 14),  out = sum_j w_j code_j / sum_j w_j 2^(-ev_j):
-// the value scale rides in the exponent, so the products see codes alone, and 14 puts the
-// largest w at 2^14, which leaves the small ones of a long softmax 38 binary places in f16.
+//   w_j = 2^(t_j - M + 11),  out = sum_j w_j code_j / sum_j w_j 2^(-ev_j):
+// the value scale rides in the exponent, so the products see codes alone.  M lags: it moves, to
+// a whole number, where a row's true maximum is more than 2^4 above, so the largest w stays
+// below 2^15, inside f16, and the smallest keep 31 binary places and more below it.
 // The 11 bits that a w keeps are the one rounding beyond f32 (codes and f16 queries are exact
 // in f16; a bf16 query row is taken times a power of two that puts its largest value near 2^15).
 //
-// A warp owns 16 (or 32) rows, token by token the heads of a group that share a cache head, and
+// A warp owns 8 NT rows, token by token the heads of a group that share a cache head, and
 // goes through tiles of 32 tokens that its own TMA copies bring into its own ring of stages: no
 // barrier but the copies' own before the end.  Codes become f16 in registers on the way into
-// mma.sync (m16n8k16), in the layout that the copies' swizzle makes free of bank conflicts.  The
+// mma.sync (m16n8k16).  Tokens, and then values, take the 16-row side and the rows the 8-column
+// side (S^T = K Q^T, O^T = V^T P^T): with rows on the 16 side a group of four wasted three
+// quarters of the products.  The copies' swizzle keeps all reads free of bank conflicts.  The
 // warps of a CTA and the CTAs of a cluster share a sequence's tiles in turn and join their sums
 // through shared memory, in a fixed order.  Bound by the cache's bytes.
 
@@ -30,7 +33,7 @@ namespace {
 constexpr int kTile = 32;  // tokens of a tile
 constexpr int kWarps = 4;
 constexpr int kStages = 2;
-constexpr float kHead = 14.0f;  // exponent of the largest weight
+constexpr float kHead = 11.0f, kLag = 4.0f;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -77,19 +80,28 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 // neighbouring columns lie four apart, which the copies' swizzle turns into other banks.
 __device__ __forceinline__ int spread(int c) { return (c & 1) * 4 + (c >> 1); }
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kWarps * 32)
+// 8 x 8 f16 of a warp, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     k_attend_rows(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                   const __grid_constant__ AttendParams p, const __grid_constant__ KvCache c, const __grid_constant__ Seqs sq) {
-    constexpr int R = 16 * MT, KS = D / 16, kBytes = kTile * D;  // rows, steps of a logit, bytes of a tile's keys
-    constexpr int NT = D / 8, kPieces = D / 64;                  // column tiles of the output; 16-byte pieces of a lane's keys
+    constexpr int R = 8 * NT, KS = D / 16, kBytes = kTile * D;  // rows, steps of a logit, bytes of a tile's keys
+    constexpr int VT = D / 16, kPieces = D / 64;                // row tiles of the output; 16-byte pieces of a lane's keys
+    constexpr int kRing = kStages * 2 * kBytes;
+    static_assert(R * D * 4 <= kRing, "a warp's sums lie over its ring");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ uint64_t full[kWarps][kStages];
     __shared__ uint32_t scales[kWarps][kStages];
     __shared__ float part_m[kWarps][R], part_l[kWarps][R], all_m[R], all_l[R];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
     uint8_t *const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    uint8_t *const ring = smem + warp * kStages * 2 * kBytes;
+    uint8_t *const ring = smem + warp * kRing;
     const uint32_t S = cluster_size(), rank = cluster_rank();
     if (lane == 0) {
         for (int i = 0; i < kStages; i++) mbar_init(smem_u32(&full[warp][i]), 1);
@@ -108,6 +120,16 @@ __global__ void __launch_bounds__(kWarps * 32)
     } else {
         s = seq_of_item(sq, item, p.group, R, 1, place);
     }
+    // (without a window the first tiles' pages are looked up before the length is known)
+    const bool two = c.page < kTile;
+    const int shift = 31 - __clz(c.page);  // pages hold a power of two of tokens
+    const int step = (int)S * kWarps, gid = (int)rank * kWarps + warp;
+    uint32_t guess[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint32_t index = (uint32_t)((gid + lane * step) * kTile + 16 * h) >> shift;
+        guess[h] = !p.window && index < sq.width ? (uint32_t)sq.table[(size_t)s * sq.width + index] : 0u;
+    }
     const SeqRange r = seq_range(sq, s, c.page, p.err);
     const int rows_all = r.n * p.group, first = (int)min(place * R, (int64_t)0x7fffffff);
     if (place < 0 || first >= rows_all) return;
@@ -116,205 +138,222 @@ __global__ void __launch_bounds__(kWarps * 32)
     // tokens that every row sees: tiles inside need no mask
     const int lo_all = row_bounds(p, r, token_b).lo, hi_all = row_bounds(p, r, token_a).hi;
     const int tile0 = lo / kTile, tiles = hi > lo ? (hi + kTile - 1) / kTile - tile0 : 0;
-    const int step = (int)S * kWarps, gid = (int)rank * kWarps + warp;
     const int mine = tiles > gid ? (tiles - gid + step - 1) / step : 0;  // tiles of this warp
 
-    // The pages of 32 of the warp's tiles and their scale bytes, a tile a lane (two pages where
-    // they hold 16 tokens); those of the next 32 are loaded on the way, the pages and then the
+    // Where 32 of the warp's tiles lie (a tile a lane, two pages where they hold 16 tokens) and
+    // their scale bytes; those of the next 32 are loaded on the way, the pages and then the
     // scales, each well before it is used.
-    const bool two = c.page < kTile;
     struct Pages {
-        uint32_t page[2], scale[2];
+        uint32_t page[2];
+        int row[2];  // of the codes
+        uint32_t scale;
     } now{}, next{};
+    auto places = [&](Pages &b, int t) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            b.row[h] = (int)(((b.page[h] * (uint32_t)c.heads + (uint32_t)head) << shift) + (uint32_t)((t + 16 * h) & (c.page - 1)));
+    };
     auto fetch_pages = [&](Pages &b, int base) {
         const int i = base + lane, t = (tile0 + gid + i * step) * kTile;
         if (i >= mine) return;
-        b.page[0] = seq_page(sq, c, s, (uint32_t)t / (uint32_t)c.page, p.err);
-        b.page[1] = two && t + 16 < r.len ? seq_page(sq, c, s, (uint32_t)(t + 16) / (uint32_t)c.page, p.err) : b.page[0];
+        b.page[0] = seq_page(sq, c, s, (uint32_t)t >> shift, p.err);
+        b.page[1] = two && t + 16 < r.len ? seq_page(sq, c, s, (uint32_t)(t + 16) >> shift, p.err) : b.page[0];
+        places(b, t);
     };
     auto fetch_scales = [&](Pages &b, int base) {
         if (base + lane >= mine) return;
-#pragma unroll
-        for (int h = 0; h < 2; h++) b.scale[h] = *reinterpret_cast<const uint16_t *>(c.s + kv_block(c, b.page[h], head) * 2);
+        const uint16_t *from = reinterpret_cast<const uint16_t *>(c.s);
+        b.scale = from[kv_block(c, b.page[0], head)] | (uint32_t)from[kv_block(c, b.page[1], head)] << 16;
     };
-    const int box = two ? 16 : kTile;
     auto issue = [&](int i) {  // the copies of the warp's tile i, and its scales' place
-        const int t = (tile0 + gid + i * step) * kTile, stage = i % kStages;
+        const int stage = i % kStages;
         if ((i & 31) == 0 && i) now = next;
-        const uint32_t pg0 = __shfl_sync(0xffffffffu, now.page[0], i & 31), pg1 = __shfl_sync(0xffffffffu, now.page[1], i & 31);
+        const int row0 = __shfl_sync(0xffffffffu, now.row[0], i & 31), row1 = __shfl_sync(0xffffffffu, now.row[1], i & 31);
         if (lane == 0) {
             const uint32_t bar = smem_u32(&full[warp][stage]), dst = smem_u32(ring + stage * 2 * kBytes);
-            const bool second = two && t + 16 < r.len;
-            mbar_expect_tx(bar, 2 * (second || !two ? kBytes : kBytes / 2));
-            const int row0 = (int)(((size_t)pg0 * c.heads + head) * c.page) + t % c.page;
+            const bool second = two && (tile0 + gid + i * step) * kTile + 16 < r.len;
+            mbar_expect_tx(bar, two && !second ? kBytes : 2 * kBytes);
             tma_load_2d(dst, &tmap_k, bar, 0, row0);
             tma_load_2d(dst + kBytes, &tmap_v, bar, 0, row0);
             if (second) {
-                const int row1 = (int)(((size_t)pg1 * c.heads + head) * c.page);
-                tma_load_2d(dst + box * D, &tmap_k, bar, 0, row1);
-                tma_load_2d(dst + kBytes + box * D, &tmap_v, bar, 0, row1);
+                tma_load_2d(dst + 16 * D, &tmap_k, bar, 0, row1);
+                tma_load_2d(dst + kBytes + 16 * D, &tmap_v, bar, 0, row1);
             }
         }
-        if (lane == (i & 31)) scales[warp][stage] = now.scale[0] | now.scale[1] << 16;
+        if (lane == (i & 31)) scales[warp][stage] = now.scale;
         if ((i & 31) == 8) fetch_pages(next, (i & ~31) + 32);
         if ((i & 31) == 20) fetch_scales(next, (i & ~31) + 32);
     };
-    fetch_pages(now, 0);
+    if (p.window) {
+        fetch_pages(now, 0);
+    } else if (lane < mine) {
+        const int t = (gid + lane * step) * kTile;
+        const bool second = two && t + 16 < r.len;
+        if (guess[0] >= c.pages || (second && guess[1] >= c.pages)) record_error(p.err, DW_DEV_BAD_ARG, 62, (int)s);
+        now.page[0] = min(guess[0], c.pages - 1), now.page[1] = second ? min(guess[1], c.pages - 1) : now.page[0];
+        places(now, t);
+    }
     fetch_scales(now, 0);
     for (int i = 0; i < min(kStages, mine); i++) issue(i);
 
-    // queries: step ks = 4 i + w of a logit takes the key values 16 (quad + 4 i) + 4 w .. + 3 of a lane
-    uint32_t qf[MT][KS][4];
-    float a_row[MT][2];  // what a logit of a row is multiplied by, but for its block's scale
-    int my_lo[MT][2], my_hi[MT][2];
+    // queries: step ks = 4 j + w of a logit takes the values 16 (quad + 4 j) + 4 w .. + 3 of a lane
+    uint32_t qf[NT][KS][2];
+    float a_row[NT][2];  // of rows 2 quad and 2 quad + 1: what a logit is multiplied by, but for its block's scale
+    int my_lo[NT][2], my_hi[NT][2];
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int n = 0; n < NT; n++) {
+        const int row = n * 8 + g, at = first + min(row, rows - 1);
+        const T *src = (const T *)p.q + (size_t)(r.row0 + at / p.group) * p.q_pitch + (size_t)(head * p.group + at % p.group) * D;
+        Raw<T, 8> x[2 * kPieces];
+        if (p.vec) {
+#pragma unroll
+            for (int j = 0; j < 2 * kPieces; j++) x[j].load(src + 16 * (quad + 4 * (j / 2)) + 8 * (j & 1));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2 * kPieces; j++) {
+                float u[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) u[e] = to_f32(src[16 * (quad + 4 * (j / 2)) + 8 * (j & 1) + e]);
+                x[j].set(u);
+            }
+        }
+        float a = p.scale_log2, down = 1.0f;
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            float top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2 * kPieces; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j].get(e)));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = query_exponent(top);
+            down = kv_pow2(-e), a *= kv_pow2(e);
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * kPieces; j++)
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                qf[n][2 * j + w][0] = pack2<__half>(x[j].get(4 * w) * down, x[j].get(4 * w + 1) * down);
+                qf[n][2 * j + w][1] = pack2<__half>(x[j].get(4 * w + 2) * down, x[j].get(4 * w + 3) * down);
+            }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int row = m * 16 + h * 8 + g, at = first + row;
-            const bool there = row < rows;
-            const int token = there ? at / p.group : token_a;
-            const Bounds b = row_bounds(p, r, token);
-            my_lo[m][h] = b.lo, my_hi[m][h] = there ? b.hi : 0;
-            const T *src = (const T *)p.q + (size_t)(r.row0 + token) * p.q_pitch + (size_t)(head * p.group + at % p.group) * D;
-            float v[kPieces][16], top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kPieces; i++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 8) {
-                    Raw<T, 8> x;
-                    x.zero();
-                    const T *from = src + 16 * (quad + 4 * i) + e;
-                    if (there && p.vec)
-                        x.load(from);
-                    else if (there) {
-                        float u[8];
-#pragma unroll
-                        for (int j = 0; j < 8; j++) u[j] = to_f32(from[j]);
-                        x.set(u);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[i][e + j] = x.get(j), top = fmaxf(top, fabsf(v[i][e + j]));
-                }
-            int e = 0;
-            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                e = query_exponent(top);
-            }
-            const float down = kv_pow2(-e);
-            a_row[m][h] = p.scale_log2 * kv_pow2(e);
-#pragma unroll
-            for (int i = 0; i < kPieces; i++)
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    qf[m][4 * i + w][h] = pack2<__half>(v[i][4 * w] * down, v[i][4 * w + 1] * down);
-                    qf[m][4 * i + w][2 + h] = pack2<__half>(v[i][4 * w + 2] * down, v[i][4 * w + 3] * down);
-                }
+            const int mine_row = n * 8 + 2 * quad + h;
+            const Bounds b = row_bounds(p, r, (first + min(mine_row, rows - 1)) / p.group);
+            my_lo[n][h] = b.lo, my_hi[n][h] = mine_row < rows ? b.hi : 0;
+            a_row[n][h] = __shfl_sync(0xffffffffu, a, 4 * (2 * quad + h));
         }
+    }
 
-    float o[MT][NT][4], M[MT][2], L[MT][2];
+    float o[NT][VT][4], M[NT][2], L[NT][2];
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
+    for (int n = 0; n < NT; n++) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) M[m][h] = -INFINITY, L[m][h] = 0.0f;
+        for (int h = 0; h < 2; h++) M[n][h] = -INFINITY, L[n][h] = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int v = 0; v < VT; v++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[m][n][e] = 0.0f;
+            for (int e = 0; e < 4; e++) o[n][v][e] = 0.0f;
     }
 
     // Waits, with a limit, for the copies of the warp's tile i.
     auto landed = [&](int i) {
         const uint32_t bar = smem_u32(&full[warp][i % kStages]), parity = (uint32_t)(i / kStages) & 1;
-        bool done = mbar_try_wait(bar, parity);
-        if (__all_sync(0xffffffffu, done)) return true;
+        // nearly every wait ends here (one with a time to sleep wakes up late)
+#pragma unroll 1
+        for (int k = 0; k < 4096; k++)
+            if (mbar_try_wait(bar, parity)) return true;
         const uint64_t t0 = globaltimer_ns();
-        while (!__all_sync(0xffffffffu, done)) {
-            if (!done) done = mbar_try_wait_sleep(bar, parity, 20000u);
-            if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > p.wait_cap_ns)) return false;
-        }
+        while (!mbar_try_wait_sleep(bar, parity, 20000u))
+            if (globaltimer_ns() - t0 > p.wait_cap_ns) return false;
         return true;
     };
     __syncwarp();
     for (int i = 0; i < mine; i++) {
         const int stage = i % kStages, t = (tile0 + gid + i * step) * kTile;
-        if (!landed(i)) {
+        if (!__all_sync(0xffffffffu, landed(i))) {
             if (lane == 0) record_error(p.err, DW_DEV_WAIT_EXPIRED, 51, i);
             for (int j = i; j < min(i + kStages, mine); j++) landed(j);  // nothing more is issued
             break;
         }
         const uint8_t *ks = ring + stage * 2 * kBytes, *vs = ks + kBytes;
         const uint32_t sc = scales[warp][stage];  // of the tile's (up to two) blocks
-        // ---- logits
-        float x[MT][4][4];
+        // ---- logits: 16 tokens a row tile, row c of eight the token spread(c)
+        float x[NT][2][4];
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+            for (int m = 0; m < 2; m++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) x[m][n][e] = 0.0f;
-            const int row = 8 * n + spread(g);
+                for (int e = 0; e < 4; e++) x[n][m][e] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < kPieces; j++) {
+        for (int j = 0; j < kPieces; j++) {
+            uint32_t kw[4][4];
+#pragma unroll
+            for (int b = 0; b < 4; b++) {  // eight tokens
+                const int row = 8 * b + spread(g);
                 const int piece = D == 128 ? (quad + 4 * j) ^ (row & 7) : quad ^ ((row >> 1) & 3);
                 const uint4 k = *reinterpret_cast<const uint4 *>(ks + row * D + piece * 16);
-                const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const uint32_t b0 = e4m3_to_f16x2((uint16_t)kw[w]), b1 = e4m3_to_f16x2((uint16_t)(kw[w] >> 16));
-#pragma unroll
-                    for (int m = 0; m < MT; m++) mma_f16(x[m][n], qf[m][4 * j + w], b0, b1);
-                }
+                kw[b][0] = k.x, kw[b][1] = k.y, kw[b][2] = k.z, kw[b][3] = k.w;
             }
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+#pragma unroll
+                for (int m = 0; m < 2; m++) {
+                    const uint32_t a[4] = {e4m3_to_f16x2((uint16_t)kw[2 * m][w]), e4m3_to_f16x2((uint16_t)kw[2 * m + 1][w]),
+                                           e4m3_to_f16x2((uint16_t)(kw[2 * m][w] >> 16)), e4m3_to_f16x2((uint16_t)(kw[2 * m + 1][w] >> 16))};
+#pragma unroll
+                    for (int n = 0; n < NT; n++) mma_f16(x[n][m], a, qf[n][4 * j + w][0], qf[n][4 * j + w][1]);
+                }
         }
         // ---- weights
         const int ve[2] = {kv_exponent(sc >> 8 & 255), kv_exponent(sc >> 24)};
         const float ka[2] = {kv_pow2(kv_exponent(sc & 255)), kv_pow2(kv_exponent(sc >> 16 & 255))};
         const bool masked = t < lo_all || t + kTile > hi_all;
-        uint32_t pf[MT][4][2];
+        uint32_t pf[NT][4];  // f16 weights of eight tokens (values of a row together)
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int n = 0; n < NT; n++) {
+            float top[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                float top = -INFINITY;
+                top[h] = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const float a = a_row[m][h] * ka[n / 2], b = (float)ve[n / 2];
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float &v = x[m][n][2 * h + e];
-                        v = fmaf(v, a, b);
-                        if (masked) {
-                            const int at = t + 8 * n + quad + 4 * e;  // columns 2 quad, 2 quad + 1
-                            if (at < my_lo[m][h] || at >= my_hi[m][h]) v = -INFINITY;
-                        }
-                        top = fmaxf(top, v);
+                for (int b = 0; b < 4; b++) {
+                    float &v = x[n][b / 2][2 * (b & 1) + h];
+                    v = fmaf(v, a_row[n][h] * ka[b / 2], (float)ve[b / 2]);
+                    if (masked) {
+                        const int at = t + 8 * b + spread(g);
+                        if (at < my_lo[n][h] || at >= my_hi[n][h]) v = -INFINITY;
                     }
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float now_m = fmaxf(M[m][h], top);
-                if (now_m != M[m][h]) {
-                    const float f = carry(M[m][h], now_m);
-                    M[m][h] = now_m;
-                    L[m][h] *= f;
-#pragma unroll
-                    for (int n = 0; n < NT; n++) o[m][n][2 * h] *= f, o[m][n][2 * h + 1] *= f;
-                }
-                const float base = (now_m == -INFINITY ? 0.0f : -now_m) + kHead;
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int n = 2 * b; n < 2 * b + 2; n++) {
-                        const float w0 = ex2_approx(x[m][n][2 * h] + base), w1 = ex2_approx(x[m][n][2 * h + 1] + base);
-                        sum += w0 + w1;
-                        pf[m][n][h] = pack2<__half>(w0, w1);
-                    }
-                    L[m][h] = fmaf(sum, kv_pow2(-ve[b]), L[m][h]);
+                    top[h] = fmaxf(top[h], v);
                 }
             }
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+                for (int h = 0; h < 2; h++) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
+            if (__any_sync(0xffffffffu, top[0] > M[n][0] + kLag || top[1] > M[n][1] + kLag)) {
+                // M moves, to a whole number: what is scaled stays exact
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float to = top[h] > M[n][h] + kLag ? ceilf(top[h]) : M[n][h], f = carry(M[n][h], to);
+                    M[n][h] = to;
+                    L[n][h] *= f;
+#pragma unroll
+                    for (int v = 0; v < VT; v++) o[n][v][h] *= f, o[n][v][2 + h] *= f;
+                }
+            }
+            float w[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float base = (M[n][h] == -INFINITY ? 0.0f : -M[n][h]) + kHead;
+#pragma unroll
+                for (int b = 0; b < 4; b++) w[h][b] = ex2_approx(x[n][b / 2][2 * (b & 1) + h] + base);
+                L[n][h] = fmaf(w[h][0] + w[h][1], kv_pow2(-ve[0]), fmaf(w[h][2] + w[h][3], kv_pow2(-ve[1]), L[n][h]));
+            }
+#pragma unroll
+            for (int b = 0; b < 4; b++) pf[n][b] = transposed(pack2<__half>(w[0][b], w[1][b]));
+        }
         // ---- values
         const bool tail = t + kTile > r.len;
 #pragma unroll
@@ -337,20 +376,16 @@ __global__ void __launch_bounds__(kWarps * 32)
                 }
             }
 #pragma unroll
-            for (int w = 0; w < D / 32; w++) {
-                const uint32_t b[2][2] = {{__byte_perm(v[0][w], v[1][w], 0x5140), __byte_perm(v[0][w], v[1][w], 0x7362)},
-                                          {__byte_perm(v[2][w], v[3][w], 0x5140), __byte_perm(v[2][w], v[3][w], 0x7362)}};
+            for (int w = 0; w < D / 32; w++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t b0 = e4m3_to_f16x2((uint16_t)(b[0][e / 2] >> (16 * (e % 2))));
-                    const uint32_t b1 = e4m3_to_f16x2((uint16_t)(b[1][e / 2] >> (16 * (e % 2))));
+                for (int e = 0; e < 2; e++) {  // the lane's values 4 w + 2 e and the next, of two tokens each
+                    const uint32_t b0 = __byte_perm(v[0][w], v[1][w], e ? 0x7362 : 0x5140);
+                    const uint32_t b1 = __byte_perm(v[2][w], v[3][w], e ? 0x7362 : 0x5140);
+                    const uint32_t a[4] = {e4m3_to_f16x2((uint16_t)b0), e4m3_to_f16x2((uint16_t)(b0 >> 16)), e4m3_to_f16x2((uint16_t)b1),
+                                           e4m3_to_f16x2((uint16_t)(b1 >> 16))};
 #pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        const uint32_t a[4] = {pf[m][2 * j][0], pf[m][2 * j][1], pf[m][2 * j + 1][0], pf[m][2 * j + 1][1]};
-                        mma_f16(o[m][4 * w + e], a, b0, b1);
-                    }
+                    for (int n = 0; n < NT; n++) mma_f16(o[n][2 * w + e], a, pf[n][2 * j], pf[n][2 * j + 1]);
                 }
-            }
         }
         __syncwarp();  // the stage has been read
         if (i + kStages < mine) issue(i + kStages);
@@ -359,25 +394,21 @@ __global__ void __launch_bounds__(kWarps * 32)
     // ---- join: the warps' sums, then those of the cluster's CTAs.  A warp leaves its sums in its
     // ring (its copies have all landed).
     float *const part = reinterpret_cast<float *>(ring);  // [R][D]
+    __syncwarp();
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            float l = L[m][h];
-            l += __shfl_xor_sync(0xffffffffu, l, 1);
-            l += __shfl_xor_sync(0xffffffffu, l, 2);
-            const int row = m * 16 + h * 8 + g;
-            if (quad == 0) part_m[warp][row] = M[m][h], part_l[warp][row] = l;
-            // column 2 quad + e of output tile n is value n of the lane's piece
+            float l = L[n][h];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int col = 2 * quad + e;
-                const int at = D == 128 ? spread(col) * 16 : (2 * ((col >> 1) & 1) + (col >> 2)) * 16 + (col & 1) * 8;
+            for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+            const int row = n * 8 + 2 * quad + h;
+            if (g == 0) part_m[warp][row] = M[n][h], part_l[warp][row] = l;
+            const int at = D == 128 ? spread(g) * 16 : (2 * ((g >> 1) & 1) + (g >> 2)) * 16 + (g & 1) * 8;
 #pragma unroll
-                for (int n = 0; n < NT; n += 4)
-                    *reinterpret_cast<float4 *>(part + row * D + at + n) =
-                        make_float4(o[m][n][2 * h + e], o[m][n + 1][2 * h + e], o[m][n + 2][2 * h + e], o[m][n + 3][2 * h + e]);
-            }
+            for (int v = 0; v < VT; v += 2)
+                *reinterpret_cast<float4 *>(part + row * D + at + 2 * v) =
+                    make_float4(o[n][v][h], o[n][v][2 + h], o[n][v + 1][h], o[n][v + 1][2 + h]);
         }
     __syncthreads();
     constexpr int kQuads = D / 4;
@@ -396,7 +427,6 @@ __global__ void __launch_bounds__(kWarps * 32)
         }
     };
     float *const part0 = reinterpret_cast<float *>(smem);
-    constexpr int kRing = kStages * 2 * kBytes / 4;  // floats of a warp's ring
     for (int i = threadIdx.x; i < rows * kQuads; i += kWarps * 32) {
         const int row = i / kQuads, at = i % kQuads * 4;
         float m = -INFINITY, l = 0.0f;
@@ -406,7 +436,7 @@ __global__ void __launch_bounds__(kWarps * 32)
 #pragma unroll
         for (int w = 0; w < kWarps; w++) {
             const float f = carry(part_m[w][row], m);
-            const float4 u = *reinterpret_cast<const float4 *>(part0 + w * kRing + row * D + at);
+            const float4 u = *reinterpret_cast<const float4 *>(part0 + w * (kRing / 4) + row * D + at);
             l = fmaf(part_l[w][row], f, l);
             v.x = fmaf(u.x, f, v.x), v.y = fmaf(u.y, f, v.y), v.z = fmaf(u.z, f, v.z), v.w = fmaf(u.w, f, v.w);
         }
@@ -447,10 +477,10 @@ bool code_map(dw_backend *be, CUtensorMap *map, const uint8_t *codes, const KvCa
                                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Seqs &s) {
-    constexpr int R = 16;
-    auto kernel = k_attend_rows<T, D, 1>;
+    constexpr int R = 8 * NT;
+    auto kernel = k_attend_rows<T, D, NT>;
     constexpr size_t smem = 1024 + (size_t)kWarps * kStages * 2 * kTile * D;
     const size_t n = s.tokens / s.seqs;
     p.per_seq = s.starts ? 0 : (int)((n * p.group + R - 1) / R);
@@ -459,7 +489,7 @@ dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Se
     // CTAs that share a block's tiles: as many as the GPU holds at once, each with a tile a warp at least
     const size_t most = ((size_t)s.width * c.page + kTile - 1) / kTile;
     unsigned S = 1;
-    while (S < 8 && units * 2 * S <= (size_t)be->sm_count * 2 && (size_t)2 * S * kWarps <= most) S *= 2;
+    while (S < 8 && units * 2 * S <= (size_t)be->sm_count * 6 && (size_t)2 * S * kWarps <= most) S *= 2;
     if (units * S > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "attention_kv8: too many rows");
     CUtensorMap tk, tv;
     const int box = std::min(c.page, kTile);
@@ -473,6 +503,14 @@ dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Se
         attr_set[be->device] = true;
     }
     return launch_dependent(be, "attention_kv8", kernel, (unsigned)(units * S), kWarps * 32, smem, S, tk, tv, p, c, s);
+}
+
+template <typename T, int D>
+dw_status attend(dw_backend *be, const AttendParams &p, const KvCache &c, const Seqs &s) {
+    const size_t rows = (s.tokens + s.seqs - 1) / s.seqs * p.group;  // of a sequence, on average
+    if (rows > 64) return attend_prompt<T, D>(be, p, c, s);
+    if (rows <= 8) return attend_rows<T, D, 1>(be, p, c, s);
+    return rows <= 16 ? attend_rows<T, D, 2>(be, p, c, s) : attend_rows<T, D, 3>(be, p, c, s);
 }
 
 }  // namespace
@@ -489,8 +527,7 @@ dw_status launch_attention_kv8(dw_backend *be, const dw_attention_desc &d, const
     p.wait_cap_ns = be->wait_cap_ns, p.err = be->dev_err;
     auto with = [&](auto t) {
         using T = decltype(t);
-        if (s.tokens / s.seqs * p.group > 64) return c.d == 64 ? attend_prompt<T, 64>(be, p, c, s) : attend_prompt<T, 128>(be, p, c, s);
-        return c.d == 64 ? attend_rows<T, 64>(be, p, c, s) : attend_rows<T, 128>(be, p, c, s);
+        return c.d == 64 ? attend<T, 64>(be, p, c, s) : attend<T, 128>(be, p, c, s);
     };
     return d.dtype == DW_F16 ? with(__half{}) : with(__nv_bfloat16{});
 }
