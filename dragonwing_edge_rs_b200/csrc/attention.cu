@@ -11,11 +11,12 @@
 // in f16; a bf16 query row is taken times a power of two that puts its largest value near 2^15).
 //
 // A warp owns 8 NT rows, token by token the heads of a group that share a cache head, and
-// goes through tiles of 32 tokens that its own TMA copies bring into its own ring of stages: no
-// barrier but the copies' own before the end.  Codes become f16 in registers on the way into
+// goes through tiles of 32 tokens that its own asynchronous copies bring into its own ring of
+// stages: no barrier before the end (a TMA copy of a tile and its barrier took a warp 600 of
+// 2200 cycles to issue; 16 copies of 16 bytes a lane take 100).  Codes become f16 in registers on the way into
 // mma.sync (m16n8k16).  Tokens, and then values, take the 16-row side and the rows the 8-column
 // side (S^T = K Q^T, O^T = V^T P^T): with rows on the 16 side a group of four wasted three
-// quarters of the products.  The copies' swizzle keeps all reads free of bank conflicts.  The
+// quarters of the products.  The copies swizzle the rows, so that all reads are free of bank conflicts.  The
 // warps of a CTA and the CTAs of a cluster share a sequence's tiles in turn and join their sums
 // through shared memory, in a fixed order.  Bound by the cache's bytes.
 
@@ -33,6 +34,7 @@ namespace {
 constexpr int kTile = 32;  // tokens of a tile
 constexpr int kWarps = 4;
 constexpr int kStages = 2;
+constexpr unsigned kMaxShare = 8;  // CTAs that share a sequence
 constexpr float kHead = 11.0f, kLag = 4.0f;
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -77,7 +79,7 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 }
 
 // Column c of eight, as a place among the eight rows (or pieces) that it reads: rows of two
-// neighbouring columns lie four apart, which the copies' swizzle turns into other banks.
+// neighbouring columns lie four apart, which the rows' swizzle turns into other banks.
 __device__ __forceinline__ int spread(int c) { return (c & 1) * 4 + (c >> 1); }
 
 // 8 x 8 f16 of a warp, transposed.
@@ -89,25 +91,17 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
-    k_attend_rows(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                  const __grid_constant__ AttendParams p, const __grid_constant__ KvCache c, const __grid_constant__ Seqs sq) {
+    k_attend_rows(const __grid_constant__ AttendParams p, const __grid_constant__ KvCache c, const __grid_constant__ Seqs sq) {
     constexpr int R = 8 * NT, KS = D / 16, kBytes = kTile * D;  // rows, steps of a logit, bytes of a tile's keys
     constexpr int VT = D / 16, kPieces = D / 64;                // row tiles of the output; 16-byte pieces of a lane's keys
     constexpr int kRing = kStages * 2 * kBytes;
     static_assert(R * D * 4 <= kRing, "a warp's sums lie over its ring");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ uint64_t full[kWarps][kStages];
     __shared__ uint32_t scales[kWarps][kStages];
     __shared__ float part_m[kWarps][R], part_l[kWarps][R], all_m[R], all_l[R];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
-    uint8_t *const smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    uint8_t *const ring = smem + warp * kRing;
+    uint8_t *const ring = smem_raw + warp * kRing;
     const uint32_t S = cluster_size(), rank = cluster_rank();
-    if (lane == 0) {
-        for (int i = 0; i < kStages; i++) mbar_init(smem_u32(&full[warp][i]), 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncwarp();
     pdl_wait();
     pdl_trigger();
     // which rows of which sequence, which head
@@ -130,10 +124,30 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         const uint32_t index = (uint32_t)((gid + lane * step) * kTile + 16 * h) >> shift;
         guess[h] = !p.window && index < sq.width ? (uint32_t)sq.table[(size_t)s * sq.width + index] : 0u;
     }
-    const SeqRange r = seq_range(sq, s, c.page, p.err);
-    const int rows_all = r.n * p.group, first = (int)min(place * R, (int64_t)0x7fffffff);
+    const int row0 = seq_start(sq, s), rows_all = max(0, seq_start(sq, s + 1) - row0) * p.group, first = (int)min(place * R, (int64_t)0x7fffffff);
     if (place < 0 || first >= rows_all) return;
-    const int rows = min(R, rows_all - first), token_a = first / p.group, token_b = (first + rows - 1) / p.group;
+    const int rows = min(R, rows_all - first);
+    // the query rows: a lane has the values 16 (quad + 4 j) .. + 15 of row g of eight
+    Raw<T, 8> qx[NT][2 * kPieces];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int at = first + min(n * 8 + g, rows - 1);
+        const T *src = (const T *)p.q + (size_t)(row0 + at / p.group) * p.q_pitch + (size_t)(head * p.group + at % p.group) * D;
+        if (p.vec) {
+#pragma unroll
+            for (int j = 0; j < 2 * kPieces; j++) qx[n][j].load(src + 16 * (quad + 4 * (j / 2)) + 8 * (j & 1));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2 * kPieces; j++) {
+                float u[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) u[e] = to_f32(src[16 * (quad + 4 * (j / 2)) + 8 * (j & 1) + e]);
+                qx[n][j].set(u);
+            }
+        }
+    }
+    const SeqRange r = seq_range(sq, s, c.page, p.err);
+    const int token_a = first / p.group, token_b = (first + rows - 1) / p.group;
     const int lo = row_bounds(p, r, token_a).lo, hi = row_bounds(p, r, token_b).hi;
     // tokens that every row sees: tiles inside need no mask
     const int lo_all = row_bounds(p, r, token_b).lo, hi_all = row_bounds(p, r, token_a).hi;
@@ -145,13 +159,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     // scales, each well before it is used.
     struct Pages {
         uint32_t page[2];
-        int row[2];  // of the codes
+        uint32_t row[2];  // of the codes, where 16 tokens begin
         uint32_t scale;
     } now{}, next{};
     auto places = [&](Pages &b, int t) {
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            b.row[h] = (int)(((b.page[h] * (uint32_t)c.heads + (uint32_t)head) << shift) + (uint32_t)((t + 16 * h) & (c.page - 1)));
+            b.row[h] = ((b.page[h] * (uint32_t)c.heads + (uint32_t)head) << shift) + (uint32_t)((t + 16 * h) & (c.page - 1));
     };
     auto fetch_pages = [&](Pages &b, int base) {
         const int i = base + lane, t = (tile0 + gid + i * step) * kTile;
@@ -165,24 +179,37 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         const uint16_t *from = reinterpret_cast<const uint16_t *>(c.s);
         b.scale = from[kv_block(c, b.page[0], head)] | (uint32_t)from[kv_block(c, b.page[1], head)] << 16;
     };
-    auto issue = [&](int i) {  // the copies of the warp's tile i, and its scales' place
-        const int stage = i % kStages;
-        if ((i & 31) == 0 && i) now = next;
-        const int row0 = __shfl_sync(0xffffffffu, now.row[0], i & 31), row1 = __shfl_sync(0xffffffffu, now.row[1], i & 31);
-        if (lane == 0) {
-            const uint32_t bar = smem_u32(&full[warp][stage]), dst = smem_u32(ring + stage * 2 * kBytes);
-            const bool second = two && (tile0 + gid + i * step) * kTile + 16 < r.len;
-            mbar_expect_tx(bar, two && !second ? kBytes : 2 * kBytes);
-            tma_load_2d(dst, &tmap_k, bar, 0, row0);
-            tma_load_2d(dst + kBytes, &tmap_v, bar, 0, row0);
-            if (second) {
-                tma_load_2d(dst + 16 * D, &tmap_k, bar, 0, row1);
-                tma_load_2d(dst + kBytes + 16 * D, &tmap_v, bar, 0, row1);
+    // The copies of the warp's tile i (nothing behind the last: every turn makes a group), and its
+    // scales' place.  Lane l of copy k has piece l % kLine of row kLines k + l / kLine; a piece lies
+    // where its place in the 128-byte line, xor the line modulo 8 (of 64-byte rows: the pair of rows
+    // modulo 4), says.
+    constexpr int kLine = D / 16, kLines = 32 / kLine;  // 16-byte pieces of a row, rows of a copy
+    const int c_row = lane / kLine, c_piece = lane % kLine;
+    uint32_t c_to[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int row = k * kLines + c_row;
+        c_to[k] = smem_u32(ring) + row * D + (D == 128 ? c_piece ^ (row & 7) : c_piece ^ ((row >> 1) & 3)) * 16;
+    }
+    auto issue = [&](int i) {
+        if (i < mine) {
+            const uint32_t stage = (uint32_t)(i % kStages) * 2 * kBytes;
+            if ((i & 31) == 0 && i) now = next;
+            const uint32_t at0 = __shfl_sync(0xffffffffu, now.row[0], i & 31), at1 = __shfl_sync(0xffffffffu, now.row[1], i & 31);
+            const size_t from[2] = {(size_t)at0 * D + lane * 16, (size_t)at1 * D + lane * 16};
+#pragma unroll
+            for (int k = 0; k < kTile / kLines; k++) {
+                constexpr int kHalfCopies = kTile / kLines / 2;
+                const size_t at = from[k / kHalfCopies] + (k % kHalfCopies) * 512;
+                const uint32_t to = c_to[k & 1] + stage + (k & ~1) * 512;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(c.k + at) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + kBytes), "l"(c.v + at) : "memory");
             }
+            if (lane == (i & 31)) scales[warp][i % kStages] = now.scale;
+            if ((i & 31) == 8) fetch_pages(next, (i & ~31) + 32);
+            if ((i & 31) == 20) fetch_scales(next, (i & ~31) + 32);
         }
-        if (lane == (i & 31)) scales[warp][stage] = now.scale;
-        if ((i & 31) == 8) fetch_pages(next, (i & ~31) + 32);
-        if ((i & 31) == 20) fetch_scales(next, (i & ~31) + 32);
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if (p.window) {
         fetch_pages(now, 0);
@@ -194,7 +221,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
         places(now, t);
     }
     fetch_scales(now, 0);
-    for (int i = 0; i < min(kStages, mine); i++) issue(i);
+    for (int i = 0; i < kStages; i++) issue(i);
 
     // queries: step ks = 4 j + w of a logit takes the values 16 (quad + 4 j) + 4 w .. + 3 of a lane
     uint32_t qf[NT][KS][2];
@@ -202,21 +229,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     int my_lo[NT][2], my_hi[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int row = n * 8 + g, at = first + min(row, rows - 1);
-        const T *src = (const T *)p.q + (size_t)(r.row0 + at / p.group) * p.q_pitch + (size_t)(head * p.group + at % p.group) * D;
-        Raw<T, 8> x[2 * kPieces];
-        if (p.vec) {
-#pragma unroll
-            for (int j = 0; j < 2 * kPieces; j++) x[j].load(src + 16 * (quad + 4 * (j / 2)) + 8 * (j & 1));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 2 * kPieces; j++) {
-                float u[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) u[e] = to_f32(src[16 * (quad + 4 * (j / 2)) + 8 * (j & 1) + e]);
-                x[j].set(u);
-            }
-        }
+        const Raw<T, 8>(&x)[2 * kPieces] = qx[n];
         float a = p.scale_log2, down = 1.0f;
         if constexpr (std::is_same_v<T, __nv_bfloat16>) {
             float top = 0.0f;
@@ -256,26 +269,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
             for (int e = 0; e < 4; e++) o[n][v][e] = 0.0f;
     }
 
-    // Waits, with a limit, for the copies of the warp's tile i.
-    auto landed = [&](int i) {
-        const uint32_t bar = smem_u32(&full[warp][i % kStages]), parity = (uint32_t)(i / kStages) & 1;
-        // nearly every wait ends here (one with a time to sleep wakes up late)
-#pragma unroll 1
-        for (int k = 0; k < 4096; k++)
-            if (mbar_try_wait(bar, parity)) return true;
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait_sleep(bar, parity, 20000u))
-            if (globaltimer_ns() - t0 > p.wait_cap_ns) return false;
-        return true;
-    };
-    __syncwarp();
     for (int i = 0; i < mine; i++) {
         const int stage = i % kStages, t = (tile0 + gid + i * step) * kTile;
-        if (!__all_sync(0xffffffffu, landed(i))) {
-            if (lane == 0) record_error(p.err, DW_DEV_WAIT_EXPIRED, 51, i);
-            for (int j = i; j < min(i + kStages, mine); j++) landed(j);  // nothing more is issued
-            break;
-        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        __syncwarp();  // every lane's copies of the tile are there
         const uint8_t *ks = ring + stage * 2 * kBytes, *vs = ks + kBytes;
         const uint32_t sc = scales[warp][stage];  // of the tile's (up to two) blocks
         // ---- logits: 16 tokens a row tile, row c of eight the token spread(c)
@@ -388,13 +385,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
                 }
         }
         __syncwarp();  // the stage has been read
-        if (i + kStages < mine) issue(i + kStages);
+        issue(i + kStages);
     }
 
     // ---- join: the warps' sums, then those of the cluster's CTAs.  A warp leaves its sums in its
     // ring (its copies have all landed).
     float *const part = reinterpret_cast<float *>(ring);  // [R][D]
-    __syncwarp();
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -426,7 +422,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
             for (int i = 0; i < 4; i++) dst[i] = from_f32<T>(y[i]);
         }
     };
-    float *const part0 = reinterpret_cast<float *>(smem);
+    float *const part0 = reinterpret_cast<float *>(smem_raw);
     for (int i = threadIdx.x; i < rows * kQuads; i += kWarps * 32) {
         const int row = i / kQuads, at = i % kQuads * 4;
         float m = -INFINITY, l = 0.0f;
@@ -451,37 +447,32 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     cluster_sync();
     for (int i = (int)rank * kWarps * 32 + threadIdx.x; i < rows * kQuads; i += (int)S * kWarps * 32) {
         const int row = i / kQuads, at = i % kQuads * 4;
-        float m = -INFINITY, l = 0.0f;
-        for (uint32_t k = 0; k < S; k++) m = fmaxf(m, ld_peer(all_m + row, k));
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t k = 0; k < S; k++) {
-            const float f = carry(ld_peer(all_m + row, k), m);
-            const float4 u = ld_peer4(part0 + row * D + at, k);
-            l = fmaf(ld_peer(all_l + row, k), f, l);
-            v.x = fmaf(u.x, f, v.x), v.y = fmaf(u.y, f, v.y), v.z = fmaf(u.z, f, v.z), v.w = fmaf(u.w, f, v.w);
+        // all at once: one after the other they took 2000 cycles
+        float pm[kMaxShare], pl[kMaxShare], m = -INFINITY, l = 0.0f;
+        float4 pv[kMaxShare], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxShare; k++)
+            if (k < S) pm[k] = ld_peer(all_m + row, k), pl[k] = ld_peer(all_l + row, k), pv[k] = ld_peer4(part0 + row * D + at, k);
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxShare; k++)
+            if (k < S) m = fmaxf(m, pm[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxShare; k++) {
+            if (k >= S) continue;
+            const float f = carry(pm[k], m);
+            l = fmaf(pl[k], f, l);
+            v.x = fmaf(pv[k].x, f, v.x), v.y = fmaf(pv[k].y, f, v.y), v.z = fmaf(pv[k].z, f, v.z), v.w = fmaf(pv[k].w, f, v.w);
         }
         store(row, at, v, l);
     }
     cluster_sync_relaxed();  // no CTA leaves while its sums may be read
 }
 
-// Codes as a 2-D byte tensor [tokens of all pages and heads][d]; a box is `rows` tokens.
-bool code_map(dw_backend *be, CUtensorMap *map, const uint8_t *codes, const KvCache &c, int rows) {
-    cuuint64_t dims[2] = {(cuuint64_t)c.d, (cuuint64_t)c.pages * c.heads * c.page};
-    cuuint64_t strides[1] = {(cuuint64_t)c.d};
-    cuuint32_t box[2] = {(cuuint32_t)c.d, (cuuint32_t)rows};
-    cuuint32_t estr[2] = {1, 1};
-    return be->encode_tiled && be->encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), dims, strides, box,
-                                                estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                                c.d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int D, int NT>
 dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Seqs &s) {
     constexpr int R = 8 * NT;
     auto kernel = k_attend_rows<T, D, NT>;
-    constexpr size_t smem = 1024 + (size_t)kWarps * kStages * 2 * kTile * D;
+    constexpr size_t smem = (size_t)kWarps * kStages * 2 * kTile * D;
     const size_t n = s.tokens / s.seqs;
     p.per_seq = s.starts ? 0 : (int)((n * p.group + R - 1) / R);
     const size_t items = s.starts ? seq_items(s.tokens, s.seqs, p.group, R, 1) : (size_t)p.per_seq * s.seqs, units = items * c.heads;
@@ -489,12 +480,8 @@ dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Se
     // CTAs that share a block's tiles: as many as the GPU holds at once, each with a tile a warp at least
     const size_t most = ((size_t)s.width * c.page + kTile - 1) / kTile;
     unsigned S = 1;
-    while (S < 8 && units * 2 * S <= (size_t)be->sm_count * 6 && (size_t)2 * S * kWarps <= most) S *= 2;
+    while (S < kMaxShare && units * 2 * S <= (size_t)be->sm_count * 6 && (size_t)2 * S * kWarps <= most) S *= 2;
     if (units * S > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "attention_kv8: too many rows");
-    CUtensorMap tk, tv;
-    const int box = std::min(c.page, kTile);
-    if (!code_map(be, &tk, c.k, c, box) || !code_map(be, &tv, c.v, c, box))
-        return dw_fail(be, DW_ERR_DEVICE, "attention_kv8: tensor map rejected");
     static bool attr_set[16] = {};
     if (be->device < 16 && !attr_set[be->device]) {
         dw_status st = dw_cuda_check(be, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
@@ -502,7 +489,7 @@ dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Se
         if (st != DW_OK) return st;
         attr_set[be->device] = true;
     }
-    return launch_dependent(be, "attention_kv8", kernel, (unsigned)(units * S), kWarps * 32, smem, S, tk, tv, p, c, s);
+    return launch_dependent(be, "attention_kv8", kernel, (unsigned)(units * S), kWarps * 32, smem, S, p, c, s);
 }
 
 template <typename T, int D>
