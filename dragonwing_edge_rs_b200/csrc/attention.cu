@@ -32,7 +32,6 @@ namespace dw {
 namespace {
 
 constexpr int kTile = 32;  // tokens of a tile
-constexpr int kWarps = 4;
 constexpr int kStages = 2;
 constexpr unsigned kMaxShare = 8;  // CTAs that share a sequence
 constexpr float kHead = 11.0f, kLag = 4.0f;
@@ -89,8 +88,8 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     return y;
 }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
+template <typename T, int D, int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2)
     k_attend_rows(const __grid_constant__ AttendParams p, const __grid_constant__ KvCache c, const __grid_constant__ Seqs sq) {
     constexpr int R = 8 * NT, KS = D / 16, kBytes = kTile * D;  // rows, steps of a logit, bytes of a tile's keys
     constexpr int VT = D / 16, kPieces = D / 64;                // row tiles of the output; 16-byte pieces of a lane's keys
@@ -468,20 +467,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2)
     cluster_sync_relaxed();  // no CTA leaves while its sums may be read
 }
 
-template <typename T, int D, int NT>
-dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Seqs &s) {
-    constexpr int R = 8 * NT;
-    auto kernel = k_attend_rows<T, D, NT>;
+template <typename T, int D, int NT, int kWarps>
+dw_status launch_rows(dw_backend *be, const AttendParams &p, const KvCache &c, const Seqs &s, size_t units, unsigned S) {
+    auto kernel = k_attend_rows<T, D, NT, kWarps>;
     constexpr size_t smem = (size_t)kWarps * kStages * 2 * kTile * D;
-    const size_t n = s.tokens / s.seqs;
-    p.per_seq = s.starts ? 0 : (int)((n * p.group + R - 1) / R);
-    const size_t items = s.starts ? seq_items(s.tokens, s.seqs, p.group, R, 1) : (size_t)p.per_seq * s.seqs, units = items * c.heads;
-    p.items = (uint32_t)items;
-    // CTAs that share a block's tiles: as many as the GPU holds at once, each with a tile a warp at least
-    const size_t most = ((size_t)s.width * c.page + kTile - 1) / kTile;
-    unsigned S = 1;
-    while (S < kMaxShare && units * 2 * S <= (size_t)be->sm_count * 6 && (size_t)2 * S * kWarps <= most) S *= 2;
-    if (units * S > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "attention_kv8: too many rows");
     static bool attr_set[16] = {};
     if (be->device < 16 && !attr_set[be->device]) {
         dw_status st = dw_cuda_check(be, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
@@ -490,6 +479,31 @@ dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Se
         attr_set[be->device] = true;
     }
     return launch_dependent(be, "attention_kv8", kernel, (unsigned)(units * S), kWarps * 32, smem, S, p, c, s);
+}
+
+template <typename T, int D, int NT>
+dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Seqs &s) {
+    constexpr int R = 8 * NT;
+    const size_t n = s.tokens / s.seqs, sms = (size_t)be->sm_count;
+    p.per_seq = s.starts ? 0 : (int)((n * p.group + R - 1) / R);
+    const size_t items = s.starts ? seq_items(s.tokens, s.seqs, p.group, R, 1) : (size_t)p.per_seq * s.seqs, units = items * c.heads;
+    if (units * kMaxShare > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "attention_kv8: too many rows");
+    p.items = (uint32_t)items;
+    // S CTAs share a unit's tiles (as many as the longest sequence can have), each with a tile a warp at least.
+    // Few units: CTAs of eight warps, one an SM (one token, 8 heads, 32000 tokens 24 us, by four warps 29; 8
+    // sequences of up to 2000 tokens 10.2 and 11.1).
+    // More: CTAs of four, until the GPU is full (16 sequences of up to 4000 tokens with 20 rows: S = 1, 2, 4, 8
+    // 49.9, 40.1, 43.8, 60 us), and with few rows beyond, for the balance of long and short sequences, while a
+    // warp keeps six tiles (64 sequences of up to 8192: 1, 2, 4 105.8, 95.7, 93.9).
+    const size_t most = ((size_t)s.width * c.page + kTile - 1) / kTile;
+    unsigned S = 1;
+    if (units * 2 <= sms) {
+        while (S < kMaxShare && units * 2 * S <= sms && (size_t)2 * S * 8 <= most) S *= 2;
+        return launch_rows<T, D, NT, 8>(be, p, c, s, units, S);
+    }
+    const size_t held = sms * (NT == 1 ? 3 : 2);
+    while (S < kMaxShare && (units * 2 * S <= held ? 2 * S * 4 <= most : NT == 1 && units * 2 * S <= 5 * held && 2 * S * 4 * 6 <= most)) S *= 2;
+    return launch_rows<T, D, NT, 4>(be, p, c, s, units, S);
 }
 
 template <typename T, int D>
