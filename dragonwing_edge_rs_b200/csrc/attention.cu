@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2
         const uint32_t index = (uint32_t)((gid + lane * step) * kTile + 16 * h) >> shift;
         guess[h] = !p.window && index < sq.width ? (uint32_t)sq.table[(size_t)s * sq.width + index] : 0u;
     }
-    const int row0 = seq_start(sq, s), rows_all = max(0, seq_start(sq, s + 1) - row0) * p.group, first = (int)min(place * R, (int64_t)0x7fffffff);
+    int row0;
+    const int rows_all = seq_rows(sq, s, row0, p.err) * p.group, first = (int)min(place * R, (int64_t)0x7fffffff);
     if (place < 0 || first >= rows_all) return;
     const int rows = min(R, rows_all - first);
     // the query rows: a lane has the values 16 (quad + 4 j) .. + 15 of row g of eight

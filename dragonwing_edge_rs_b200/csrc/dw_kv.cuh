@@ -63,16 +63,20 @@ __device__ __forceinline__ int seq_start(const Seqs &q, uint32_t s) {
     return min(max(q.starts[s], 0), (int)q.tokens);
 }
 
+// The rows of a sequence, its starts checked.
+__device__ __forceinline__ int seq_rows(const Seqs &q, uint32_t s, int &row0, int32_t *err) {
+    row0 = seq_start(q, s);
+    const int end = seq_start(q, s + 1);
+    if (q.starts && (end < row0 || q.starts[s] != row0 || q.starts[s + 1] != end)) record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
+    return max(end - row0, 0);
+}
+
 __device__ __forceinline__ SeqRange seq_range(const Seqs &q, uint32_t s, int page, int32_t *err) {
     SeqRange r;
     const int most = (int)min((uint64_t)q.width * page, (uint64_t)0x7fffff00u), len = q.lens[s];
-    r.row0 = seq_start(q, s);
-    r.n = seq_start(q, s + 1) - r.row0;
+    r.n = seq_rows(q, s, r.row0, err);
     r.len = min(max(len, 0), most);
-    bool bad = len != r.len || r.n < 0;
-    if (q.starts) bad |= q.starts[s] != r.row0 || q.starts[s + 1] != r.row0 + r.n;
-    if (bad) record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
-    r.n = max(r.n, 0);
+    if (len != r.len) record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
     return r;
 }
 

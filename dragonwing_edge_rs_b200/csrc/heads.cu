@@ -90,35 +90,45 @@ __device__ __forceinline__ void norm_rope_row(const HeadParams &p, size_t row, i
         const Slot<E> slot(c, p.rot, p.neighbours);
         live[j] = 2 * E * c < p.d;
         a[j] = slot.a, b[j] = slot.b, turns[j] = slot.turns && live[j];
-#pragma unroll
-        for (int i = 0; i < E; i++)
-            if (turns[j]) turn_f32(p.rope[c * E + i], position, cs[j][i], sn[j][i]);
     }
-    auto source = [&](int h) {
-        return h < p.hq ? (const T *)p.q + row * p.q_pitch + (size_t)h * p.d : (const T *)p.k + row * p.k_pitch + (size_t)(h - p.hq) * p.d;
-    };
-    Raw<T, E> ra[J], rb[J];
-    auto load = [&](int h) {
+    // Two groups' values are on their way while one is computed (with one the loads in flight were
+    // too few: 8192 x 40 heads of 128 bf16 49.6 us).
+    struct Group {
+        Raw<T, E> a[J], b[J];
+    } g0, g1;
+    auto load = [&](Group &x, int h) {
         if (h >= heads) return;
-        const T *x = source(h);
+        const T *from = h < p.hq ? (const T *)p.q + row * p.q_pitch + (size_t)h * p.d : (const T *)p.k + row * p.k_pitch + (size_t)(h - p.hq) * p.d;
 #pragma unroll
         for (int j = 0; j < J; j++)
-            if (live[j]) ra[j].load(x + a[j]), rb[j].load(x + b[j]);
+            if (live[j]) x.a[j].load(from + a[j]), x.b[j].load(from + b[j]);
     };
     int h = first * per + lane / p.group, weights = -1;
     const int end = min((first + p.chunk) * per, (heads + per - 1) / per * per);
-    load(h);
-    for (; h < end; h += per) {
+    load(g0, h);
+    if (h + per < end) load(g1, h + per);
+#pragma unroll
+    for (int j = 0; j < J; j++)
+#pragma unroll
+        for (int i = 0; i < E; i++)
+            if (turns[j]) turn_f32(p.rope[(sub + j * p.group) * E + i], position, cs[j][i], sn[j][i]);
+    auto sum = [&](float x) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            if (o < p.group) x += __shfl_xor_sync(0xffffffffu, x, o);
+        return x;
+    };
+    auto one = [&](Group &x) {
         float v[J][2 * E];
         const bool there = h < heads;
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
             for (int i = 0; i < E; i++) {
-                v[j][i] = there && live[j] ? ra[j].get(i) : 0.0f;
-                v[j][E + i] = there && live[j] ? rb[j].get(i) : 0.0f;
+                v[j][i] = there && live[j] ? x.a[j].get(i) : 0.0f;
+                v[j][E + i] = there && live[j] ? x.b[j].get(i) : 0.0f;
             }
-        if (h + per < end) load(h + per);
+        if (h + 2 * per < end) load(x, h + 2 * per);
         if (p.norm != DW_NORM_NONE) {
             const int kind = h < p.hq ? 0 : 1;
             if (kind != weights) {
@@ -132,12 +142,6 @@ __device__ __forceinline__ void norm_rope_row(const HeadParams &p, size_t row, i
                         w[j][E + i] = from && live[j] ? from[b[j] + i] : 1.0f;
                     }
             }
-            auto sum = [&](float x) {
-#pragma unroll
-                for (int o = 16; o; o >>= 1)
-                    if (o < p.group) x += __shfl_xor_sync(0xffffffffu, x, o);
-                return x;
-            };
             if (p.norm == DW_NORM_LAYER) {
                 float m = 0.0f;
 #pragma unroll
@@ -161,21 +165,27 @@ __device__ __forceinline__ void norm_rope_row(const HeadParams &p, size_t row, i
 #pragma unroll
                 for (int i = 0; i < 2 * E; i++) v[j][i] *= rstd * w[j][i];
         }
-        if (!there) continue;
-        T *out = h < p.hq ? (T *)p.q_out + row * p.qo_pitch + (size_t)h * p.d : (T *)p.k_out + row * p.ko_pitch + (size_t)(h - p.hq) * p.d;
+        if (there) {
+            T *out = h < p.hq ? (T *)p.q_out + row * p.qo_pitch + (size_t)h * p.d : (T *)p.k_out + row * p.ko_pitch + (size_t)(h - p.hq) * p.d;
 #pragma unroll
-        for (int j = 0; j < J; j++) {
-            if (!live[j]) continue;
-            if (turns[j]) rotate<E, float>(v[j], cs[j], sn[j], p.neighbours);
-            float lo[E], hi[E];
+            for (int j = 0; j < J; j++) {
+                if (!live[j]) continue;
+                if (turns[j]) rotate<E, float>(v[j], cs[j], sn[j], p.neighbours);
+                float lo[E], hi[E];
 #pragma unroll
-            for (int i = 0; i < E; i++) lo[i] = v[j][i], hi[i] = v[j][E + i];
-            Raw<T, E> r;
-            r.set(lo);
-            r.store(out + a[j]);
-            r.set(hi);
-            r.store(out + b[j]);
+                for (int i = 0; i < E; i++) lo[i] = v[j][i], hi[i] = v[j][E + i];
+                Raw<T, E> r;
+                r.set(lo);
+                r.store(out + a[j]);
+                r.set(hi);
+                r.store(out + b[j]);
+            }
         }
+        h += per;
+    };
+    while (h < end) {
+        one(g0);
+        if (h < end) one(g1);
     }
 }
 
@@ -190,11 +200,18 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ 
 
 // ---- append ------------------------------------------------------------------------
 // A block of threads has one head of one page that rows are written to, a warp eight of its
-// tokens, a lane 2 E = d / 32 values of each.  Keys are computed in f64 and kept as f32 rounded
-// to odd (a last bit of 1 where anything was cut off), which rounds to e4m3 as the f64 would:
-// the cached codes are the definition's own, whatever hardware or order computed them.  A
-// warp's tokens follow each other, so the angles after the first come by one complex product
-// each.  The blocks behind those of the pages norm and turn query rows.
+// tokens, a lane 2 E = d / 32 values of each.  The cached codes are the definition's own: keys
+// are computed in f32, with a bound on what that can be off, and where a value within the bound
+// of its own would get another code (some token in 300) the token is computed again in f64
+// (everything in f64 took 17 us of a 4096-token prompt's 23).  An f64 key is kept as f32 rounded to
+// odd (a last bit of 1 where anything was cut off), which rounds to e4m3 as the f64 would.
+// The blocks behind those of the pages norm and turn query rows.
+//
+// The bound: in units of 2^-24, a sum of squares by lanes' chains of 4 and 5 levels is off by 9
+// of itself, the root of its mean and the reciprocal by 7 then, times a weight and the value 2
+// more; a cosine and a sine by 8 (the angle's own rounding is below 4), their products and the
+// sum by 4, of the pair's size: 21, taken as 64.
+constexpr float kKeyErr = 64.0f / 16777216.0f;
 constexpr int kWarpTokens = 8;
 
 __device__ __forceinline__ float round_to_odd(double v) {
@@ -246,50 +263,92 @@ __device__ __forceinline__ void rescale_codes(uint8_t *p, float f) {
     }
 }
 
+// The 2 E key values of a lane of one token, normed and turned, in f64.
+template <typename T, int E>
+__device__ __noinline__ bool exact_key(const HeadParams &p, const T *k, const Slot<E> slot, int64_t position, float (&out)[2 * E]) {
+    float lo[E], hi[E];
+    load_values<T, E>(k + slot.a, p.vec, lo);
+    load_values<T, E>(k + slot.b, p.vec, hi);
+    double x[2 * E], cs[E], sn[E];
+#pragma unroll
+    for (int j = 0; j < E; j++) x[j] = lo[j], x[E + j] = hi[j];
+    if (p.norm != DW_NORM_NONE) {
+        if (p.norm == DW_NORM_LAYER) {
+            double m = 0.0;
+#pragma unroll
+            for (int j = 0; j < 2 * E; j++) m += x[j];
+            m = warp_sum(m) / p.d;
+#pragma unroll
+            for (int j = 0; j < 2 * E; j++) x[j] -= m;
+        }
+        double sq = 0.0;
+#pragma unroll
+        for (int j = 0; j < 2 * E; j++) sq = fma(x[j], x[j], sq);
+        const double rstd = 1.0 / sqrt(warp_sum(sq) / p.d + (double)p.eps);
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            x[j] *= rstd * (p.w_k ? (double)p.w_k[slot.a + j] : 1.0);
+            x[E + j] *= rstd * (p.w_k ? (double)p.w_k[slot.b + j] : 1.0);
+        }
+    }
+    if (slot.turns) {
+#pragma unroll
+        for (int j = 0; j < E; j++) turn_f64(p.rope[(threadIdx.x & 31) * E + j], position, cs[j], sn[j]);
+        rotate<E, double>(x, cs, sn, p.neighbours);
+    }
+    bool ok = true;
+#pragma unroll
+    for (int j = 0; j < 2 * E; j++) ok = ok && isfinite(x[j]), out[j] = round_to_odd(x[j]);
+    return ok;
+}
+
+// The place of item w of rows whose sequences have as many each.
+__device__ __forceinline__ uint32_t seq_and_place(const Seqs &q, uint32_t w, uint32_t each, int per, int size, int extra, int64_t &place) {
+    if (q.starts) return seq_of_item(q, w, per, size, extra, place);
+    place = w % each;
+    return w / each;
+}
+
 template <typename T, int E, int QE, int QJ>
 __global__ void __launch_bounds__(512)
     k_append(const __grid_constant__ HeadParams p, const __grid_constant__ KvCache c, const __grid_constant__ Seqs q,
-             const uint32_t page_blocks, int32_t *err) {
-    __shared__ uint32_t top[2][16];
+             const uint32_t page_blocks, const uint32_t each_rows, const uint32_t each_pages, int32_t *err) {
+    __shared__ uint32_t top[3][16];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32;
     pdl_wait();
     pdl_trigger();
     if (blockIdx.x >= page_blocks) {
         const size_t unit = (size_t)(blockIdx.x - page_blocks) * warps + warp;
-        const int64_t row = (int64_t)(unit / p.chunks);
+        const size_t row = unit / p.chunks;
         if (row >= p.tokens) return;
         int64_t place;
-        const uint32_t s = seq_of_item(q, row, 1, 1, 0, place);
+        const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place);
         const SeqRange r = seq_range(q, s, c.page, err);
         if (place < 0 || place >= r.n) return;
         HeadParams pq = p;
         pq.hk = 0;
-        norm_rope_row<T, QE, QJ>(pq, (size_t)row, r.position((int)row), (int)(unit % p.chunks) * p.chunk);
+        norm_rope_row<T, QE, QJ>(pq, row, r.position((int)row), (int)(unit % p.chunks) * p.chunk);
         return;
     }
     const int head = (int)(blockIdx.x % p.hk);
     int64_t place;
-    const uint32_t s = seq_of_item(q, blockIdx.x / p.hk, 1, c.page, 2, place);
+    const uint32_t s = seq_and_place(q, blockIdx.x / p.hk, each_pages, 1, c.page, 2, place);
     const SeqRange r = seq_range(q, s, c.page, err);
+    const int shift = 31 - __clz(c.page);   // pages hold a power of two of tokens
     const int first = max(r.len - r.n, 0);  // the sequence's first new token
-    const int64_t begin = (first / c.page + place) * c.page;
+    const int64_t begin = ((first >> shift) + place) << shift;
     if (place < 0 || first >= r.len || begin >= r.len) return;
     const int t0 = max(first, (int)begin), t1 = (int)min((int64_t)r.len, begin + c.page);
-    const uint32_t page = seq_page(q, c, s, (uint32_t)(begin / c.page), err);
-    uint8_t *const scale = c.s + kv_block(c, page, head) * 2;
-    const bool has_old = t0 > begin;
-    const int k_old = has_old ? kv_exponent(scale[0]) : kKvMinExp, v_old = has_old ? kv_exponent(scale[1]) : kKvMinExp;
-    uint8_t *const kc = kv_codes(c.k, c, page, head), *const vc = kv_codes(c.v, c, page, head);
-
     const int w0 = (int)begin + warp * kWarpTokens;  // the warp's first token
     const Slot<E> slot(lane, p.rot, p.neighbours);
     const T *const kp = (const T *)p.k + (size_t)head * p.d, *const vp = (const T *)p.v + (size_t)head * p.d;
+    auto row_of = [&](int t) { return (size_t)r.row0 + (t - (r.len - r.n)); };
     float kv[kWarpTokens][2 * E], vv[kWarpTokens][2 * E];
 #pragma unroll
     for (int i = 0; i < kWarpTokens; i++) {
         const int t = w0 + i;
         if (t < t0 || t >= t1) continue;
-        const size_t row = (size_t)r.row0 + (t - (r.len - r.n));
+        const size_t row = row_of(t);
         float lo[E], hi[E];
         load_values<T, E>(kp + row * p.k_pitch + slot.a, p.vec, lo);
         load_values<T, E>(kp + row * p.k_pitch + slot.b, p.vec, hi);
@@ -300,70 +359,112 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
         for (int j = 0; j < E; j++) vv[i][j] = lo[j], vv[i][E + j] = hi[j];
     }
-    double cs[E], sn[E], cs1[E], sn1[E], w[2 * E];
+    const uint32_t page = seq_page(q, c, s, (uint32_t)(begin >> shift), err);
+    uint8_t *const scale = c.s + kv_block(c, page, head) * 2;
+    const bool has_old = t0 > begin;
+    const int k_old = has_old ? kv_exponent(scale[0]) : kKvMinExp, v_old = has_old ? kv_exponent(scale[1]) : kKvMinExp;
+    uint8_t *const kc = kv_codes(c.k, c, page, head), *const vc = kv_codes(c.v, c, page, head);
+    uint64_t turn[E];
+    float w[2 * E];
+    const bool any = w0 < t1 && w0 + kWarpTokens > t0, weighs = p.norm != DW_NORM_NONE && p.w_k;
 #pragma unroll
     for (int j = 0; j < E; j++) {
-        const bool weighs = p.norm != DW_NORM_NONE && p.w_k;
-        w[j] = weighs ? (double)p.w_k[slot.a + j] : 1.0, w[E + j] = weighs ? (double)p.w_k[slot.b + j] : 1.0;
-        cs[j] = cs1[j] = 1.0, sn[j] = sn1[j] = 0.0;
-        if (slot.turns && w0 < t1 && w0 + kWarpTokens > t0) {
-            const uint64_t f = p.rope[lane * E + j];
-            turn_f64(f, max(w0, t0), cs[j], sn[j]);
-            if (min(w0 + kWarpTokens, t1) - max(w0, t0) > 1) turn_f64(f, 1, cs1[j], sn1[j]);
-        }
+        turn[j] = slot.turns && any ? p.rope[lane * E + j] : 0;
+        w[j] = weighs && any ? p.w_k[slot.a + j] : 1.0f, w[E + j] = weighs && any ? p.w_k[slot.b + j] : 1.0f;
     }
-    float kmax = 0.0f, vmax = 0.0f;
-    uint32_t poison = 0;
+    // largest |key| less and plus what it can be off, largest |value|; tokens that are no numbers;
+    // tokens that are exact already
+    float k_low = 0.0f, k_high = 0.0f, vmax = 0.0f, err_of[kWarpTokens][E];
+    uint32_t poison = 0, exact = 0;
 #pragma unroll
     for (int i = 0; i < kWarpTokens; i++) {
         const int t = w0 + i;
         if (t < t0 || t >= t1) continue;
-        double x[2 * E];
+        float x[2 * E], rms = 1.0f;
 #pragma unroll
         for (int j = 0; j < 2 * E; j++) x[j] = kv[i][j];
-        if (p.norm != DW_NORM_NONE) {
-            if (p.norm == DW_NORM_LAYER) {
-                double m = 0.0;
+        if (p.norm == DW_NORM_RMS) {
+            float sq = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 2 * E; j++) m += x[j];
-                m = warp_sum(m) / p.d;
+            for (int j = 0; j < 2 * E; j++) sq = fmaf(x[j], x[j], sq);
 #pragma unroll
-                for (int j = 0; j < 2 * E; j++) x[j] -= m;
-            }
-            double sq = 0.0;
-#pragma unroll
-            for (int j = 0; j < 2 * E; j++) sq = fma(x[j], x[j], sq);
-            const double rstd = 1.0 / sqrt(warp_sum(sq) / p.d + (double)p.eps);
+            for (int o = 16; o; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+            rms = fmaf(sq, p.inv_d, p.eps);
+            const float rstd = __frsqrt_rn(rms);
 #pragma unroll
             for (int j = 0; j < 2 * E; j++) x[j] *= rstd * w[j];
         }
-        if (slot.turns) rotate<E, double>(x, cs, sn, p.neighbours);
-        bool ok = true;
-        float km = 0.0f, vm = 0.0f;
+        float cs[E], sn[E];
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            // what the two values of a pair can be off
+            const float pair = p.neighbours ? fabsf(x[2 * j]) + fabsf(x[2 * j + 1]) : fabsf(x[j]) + fabsf(x[E + j]);
+            err_of[i][j] = p.norm == DW_NORM_NONE && !slot.turns ? 0.0f : kKeyErr * pair;
+            if (slot.turns) turn_f32(turn[j], t, cs[j], sn[j]);
+        }
+        if (slot.turns) rotate<E, float>(x, cs, sn, p.neighbours);
+        float low = 0.0f, high = 0.0f, vm = 0.0f;
+        bool fine = p.norm != DW_NORM_LAYER && rms > 1e-30f && rms < 1e30f, ok = true;
 #pragma unroll
         for (int j = 0; j < 2 * E; j++) {
-            ok = ok && isfinite(x[j]) && isfinite(vv[i][j]);
-            kv[i][j] = round_to_odd(x[j]);
-            km = fmaxf(km, fabsf(kv[i][j])), vm = fmaxf(vm, fabsf(vv[i][j]));
+            const float off = p.neighbours ? err_of[i][j / 2] : err_of[i][j % E];
+            low = fmaxf(low, fabsf(x[j]) - off), high = fmaxf(high, fabsf(x[j]) + off);
+            fine = fine && fabsf(x[j]) + off < 1e38f;
+            vm = fmaxf(vm, fabsf(vv[i][j]));
+            ok = ok && isfinite(vv[i][j]);
         }
+        if (!__all_sync(0xffffffffu, fine)) {
+            float f[2 * E];
+            const bool number = exact_key<T, E>(p, kp + row_of(t) * p.k_pitch, slot, t, f);
+            ok = ok && number, exact |= 1u << i;
+            low = high = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2 * E; j++) x[j] = f[j], low = high = fmaxf(high, fabsf(f[j]));
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * E; j++) kv[i][j] = x[j];
         if (__all_sync(0xffffffffu, ok))
-            kmax = fmaxf(kmax, km), vmax = fmaxf(vmax, vm);
+            k_low = fmaxf(k_low, low), k_high = fmaxf(k_high, high), vmax = fmaxf(vmax, vm);
         else
             poison |= 1u << i;
-#pragma unroll
-        for (int j = 0; j < E; j++) {  // the next token's angle
-            const double cn = cs[j] * cs1[j] - sn[j] * sn1[j];
-            sn[j] = sn[j] * cs1[j] + cs[j] * sn1[j];
-            cs[j] = cn;
-        }
     }
-    kmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(kmax)));
-    vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vmax)));
-    if (lane == 0) top[0][warp] = __float_as_uint(kmax), top[1][warp] = __float_as_uint(vmax);
-    __syncthreads();
-    uint32_t km = 0, vm = 0;
-    for (int i = 0; i < warps; i++) km = max(km, top[0][i]), vm = max(vm, top[1][i]);
-    const int ke = max(kv_scale_exponent(__uint_as_float(km)), k_old), ve = max(kv_scale_exponent(__uint_as_float(vm)), v_old);
+    uint32_t km[3] = {__float_as_uint(k_low), __float_as_uint(k_high), __float_as_uint(vmax)};
+    auto block_max = [&](int from) {
+#pragma unroll
+        for (int n = from; n < 3; n++) {
+            km[n] = __reduce_max_sync(0xffffffffu, km[n]);
+            if (lane == 0) top[n][warp] = km[n];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = from; n < 3; n++)
+            for (int i = 0; i < warps; i++) km[n] = max(km[n], top[n][i]);
+    };
+    block_max(0);
+    int ke = kv_scale_exponent(__uint_as_float(km[1]));
+    if (ke != kv_scale_exponent(__uint_as_float(km[0]))) {  // the largest key lies at a border: every token in f64
+        k_high = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWarpTokens; i++) {
+            const int t = w0 + i;
+            if (t < t0 || t >= t1 || (poison >> i & 1)) continue;
+            if (!(exact >> i & 1)) {
+                float f[2 * E];
+                exact_key<T, E>(p, kp + row_of(t) * p.k_pitch, slot, t, f);
+#pragma unroll
+                for (int j = 0; j < 2 * E; j++) kv[i][j] = f[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 2 * E; j++) k_high = fmaxf(k_high, fabsf(kv[i][j]));
+        }
+        exact = 0xFFu;
+        __syncthreads();
+        km[1] = __float_as_uint(k_high);
+        block_max(1);
+        ke = kv_scale_exponent(__uint_as_float(km[1]));
+    }
+    ke = max(ke, k_old);
+    const int ve = max(kv_scale_exponent(__uint_as_float(km[2])), v_old);
     const float k_inv = kv_pow2(-ke), v_inv = kv_pow2(-ve);
     if (threadIdx.x == 0) scale[0] = (uint8_t)(ke + 127), scale[1] = (uint8_t)(ve + 127);
 #pragma unroll
@@ -375,6 +476,22 @@ __global__ void __launch_bounds__(512)
             if (ve != v_old) rescale_codes<E>(vr + 2 * E * lane, kv_pow2(v_old - ve));
         } else if (t < t1) {
             const bool bad = poison >> i & 1;
+            if (!bad && !(exact >> i & 1)) {
+                // a value that is off by all it can be: the same code?
+                bool same = true;
+#pragma unroll
+                for (int j = 0; j < 2 * E; j++) {
+                    const float off = p.neighbours ? err_of[i][j / 2] : err_of[i][j % E];
+                    const uint32_t two = e4m3_codes2((kv[i][j] - off) * k_inv, (kv[i][j] + off) * k_inv);
+                    same = same && (two & 255) == (two >> 8);
+                }
+                if (!__all_sync(0xffffffffu, same)) {
+                    float f[2 * E];
+                    exact_key<T, E>(p, kp + row_of(t) * p.k_pitch, slot, t, f);
+#pragma unroll
+                    for (int j = 0; j < 2 * E; j++) kv[i][j] = f[j];
+                }
+            }
             float lo[E], hi[E], all[2 * E];
 #pragma unroll
             for (int j = 0; j < E; j++) {
@@ -391,49 +508,54 @@ __global__ void __launch_bounds__(512)
 }
 
 // ---- read --------------------------------------------------------------------------
-// A warp has a row's keys or values, a lane 8 values at a time.
+// A warp has a row's keys or values, a lane 16 of them at a time.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    k_read(const __grid_constant__ KvCache c, const __grid_constant__ Seqs q, T *k_out, T *v_out, size_t k_pitch, size_t v_pitch,
-           const bool vec, int32_t *err) {
+    k_read(const __grid_constant__ KvCache c, const __grid_constant__ Seqs q, const uint32_t each_rows, T *k_out, T *v_out, size_t k_pitch,
+           size_t v_pitch, const bool vec, int32_t *err) {
     const int lane = threadIdx.x & 31;
     const size_t unit = (size_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
     pdl_wait();
     pdl_trigger();
-    const int64_t row = (int64_t)(unit / 2);
+    const size_t row = unit / 2;
     const bool values = unit & 1;
     T *out = values ? v_out : k_out;
     if (row >= q.tokens || !out) return;
     int64_t place;
-    const uint32_t s = seq_of_item(q, row, 1, 1, 0, place);
+    const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place);
     const SeqRange r = seq_range(q, s, c.page, err);
     if (place < 0 || place >= r.n) return;
-    out += (size_t)row * (values ? v_pitch : k_pitch);
-    const int t = r.position((int)row);
-    const uint32_t page = t < 0 ? 0 : seq_page(q, c, s, (uint32_t)t / (uint32_t)c.page, err);
-    for (int i = lane * 8; i < c.heads * c.d; i += 256) {
-        const int head = i / c.d;
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = 0.0f;
+    out += row * (values ? v_pitch : k_pitch);
+    const int t = r.position((int)row), shift = 31 - __clz(c.page), d_shift = 31 - __clz(c.d);  // powers of two
+    const uint32_t page = t < 0 ? 0 : seq_page(q, c, s, (uint32_t)t >> shift, err);
+    const uint8_t *const codes = (values ? c.v : c.k) + ((kv_block(c, page, 0) << shift) + (t & (c.page - 1))) * c.d;
+    const uint8_t *const scales = c.s + kv_block(c, page, 0) * 2 + values;
+#pragma unroll 2
+    for (int i = lane * 16; i < c.heads << d_shift; i += 512) {
+        const int head = i >> d_shift;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        float x = 0.0f;
         if (t >= 0) {
-            const uint8_t *codes = kv_codes(values ? c.v : c.k, c, page, head) + (t % c.page) * c.d + i % c.d;
-            const float x = kv_pow2(kv_exponent(c.s[kv_block(c, page, head) * 2 + values]));
-            const uint2 w = *reinterpret_cast<const uint2 *>(codes);
-            const uint32_t ws[2] = {w.x, w.y};
+            w = *reinterpret_cast<const uint4 *>(codes + ((size_t)head << (shift + d_shift)) + (i & (c.d - 1)));
+            x = kv_pow2(kv_exponent(scales[2 * head]));
+        }
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float v[8];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float2 f = e4m3_to_f32x2((uint16_t)(ws[j / 2] >> (16 * (j % 2))));
+                const float2 f = e4m3_to_f32x2((uint16_t)(ws[2 * h + j / 2] >> (16 * (j % 2))));
                 v[2 * j] = f.x * x, v[2 * j + 1] = f.y * x;
             }
-        }
-        if (vec) {
-            Raw<T, 8> o;
-            o.set(v);
-            o.store(out + i);
-        } else {
+            if (vec) {
+                Raw<T, 8> o;
+                o.set(v);
+                o.store(out + i + 8 * h);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 8; j++) out[i + j] = from_f32<T>(v[j]);
+                for (int j = 0; j < 8; j++) out[i + 8 * h + j] = from_f32<T>(v[j]);
+            }
         }
     }
 }
@@ -494,7 +616,9 @@ template <typename T, int E>
 dw_status append(dw_backend *be, HeadParams p, const KvCache &c, const Seqs &s, const HeadArgs &a) {
     p.vec = aligned(a.k, sizeof(T), E * sizeof(T)) && aligned(a.v, sizeof(T), E * sizeof(T));
     const unsigned threads = (unsigned)(c.page / kWarpTokens * 32);
-    const size_t pages = seq_items(s.tokens, s.seqs, 1, c.page, 2) * p.hk;
+    // pages that n rows can lie in, from anywhere in the first
+    const size_t n = s.tokens / s.seqs, each = (n + c.page - 2) / c.page + 1;
+    const size_t pages = (s.starts ? seq_items(s.tokens, s.seqs, 1, c.page, 2) : each * s.seqs) * p.hk;
     auto go = [&](auto kernel, int QE, int QJ) {
         size_t blocks = pages;
         p.chunks = 1;
@@ -503,7 +627,8 @@ dw_status append(dw_backend *be, HeadParams p, const KvCache &c, const Seqs &s, 
             blocks += ((size_t)p.tokens * p.chunks + threads / 32 - 1) / (threads / 32);
         }
         if (blocks > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "append_kv: too many rows");
-        return launch_dependent(be, "append_kv", kernel, (unsigned)blocks, threads, 0, 0, p, c, s, (uint32_t)pages, be->dev_err);
+        return launch_dependent(be, "append_kv", kernel, (unsigned)blocks, threads, 0, 0, p, c, s, (uint32_t)pages, (uint32_t)n,
+                                (uint32_t)each, be->dev_err);
     };
     if (wide<T>(p, {a.q, a.q_out})) return go(k_append<T, E, kWide<T>, 1>, kWide<T>, 1);
     return go(k_append<T, E, 1, E>, 1, E);
@@ -534,7 +659,7 @@ dw_status launch_read_kv(dw_backend *be, const KvCache &c, const Seqs &s, int dt
     auto go = [&](auto t) {
         using T = decltype(t);
         const bool vec = aligned(k, sizeof(T), 16) && aligned(v, sizeof(T), 16);
-        return launch_dependent(be, "read_kv", k_read<T>, (unsigned)blocks, kThreads, 0, 0, c, s, (T *)k.ptr, (T *)v.ptr, k.pitch, v.pitch,
+        return launch_dependent(be, "read_kv", k_read<T>, (unsigned)blocks, kThreads, 0, 0, c, s, s.tokens / s.seqs, (T *)k.ptr, (T *)v.ptr, k.pitch, v.pitch,
                                 vec, be->dev_err);
     };
     if (dtype == DW_F32) return go(float{});
