@@ -10,6 +10,7 @@
 // All are bound by the bytes of the rows, in short calls by latency.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "dw_kv.cuh"
 #include "dw_launch.h"
@@ -31,7 +32,7 @@ struct HeadParams {
     int hq, hk, d, rot, norm;
     float eps, inv_d;
     int group, chunk, chunks;  // lanes of a head, head groups of a warp, warps of a row
-    bool neighbours, vec;
+    bool neighbours, vec, whole;  // whole: heads turn whole
 };
 
 __device__ __forceinline__ void turn_f32(uint64_t freq, int64_t position, float &c, float &s) {
@@ -189,6 +190,137 @@ __device__ __forceinline__ void norm_rope_row(const HeadParams &p, size_t row, i
     }
 }
 
+// The same for heads that turn whole and fill their lanes (d = 2 E * 32 / kPer; kPer heads a
+// group): a lane keeps the products of weights and angles, so that a value is
+// rstd * (a * (w_a cos) - b * (w_b sin)), and finds one in kPer of its angles, the others by
+// shuffles.  (By norm_rope_row 8192 x 40 heads of 128 bf16 took 49 us, bound by its instructions.)
+template <typename T, int E, int kPer>
+__device__ __forceinline__ void rope_row(const HeadParams &p, size_t row, int64_t position, int first) {
+    constexpr int kGroup = 32 / kPer, kMine = E > kPer ? E / kPer : 1, kD = 2 * E * kGroup;
+    const int lane = threadIdx.x & 31, sub = lane % kGroup, in = lane / kGroup;
+    const int qg = (p.hq + kPer - 1) / kPer, kg = (p.hk + kPer - 1) / kPer, end = min(first + p.chunk, qg + kg);
+    const bool nb = p.neighbours;
+    const int a = nb ? 2 * E * sub : E * sub, b = nb ? a + E : kD / 2 + E * sub;
+    struct Group {
+        Raw<T, E> a, b;
+    } g0, g1;
+    // group g of the row: its heads of q, or of k
+    auto place = [&](const void *q, size_t q_pitch, const void *k, size_t k_pitch, int g, bool &there) {
+        const bool key = g >= qg;
+        const int h = (key ? g - qg : g) * kPer + in, heads = key ? p.hk : p.hq;
+        there = h < heads;
+        return (T *)(key ? k : q) + row * (key ? k_pitch : q_pitch) + (size_t)min(h, heads - 1) * kD;
+    };
+    auto load = [&](Group &x, int g) {
+        bool there;
+        const T *from = place(p.q, p.q_pitch, p.k, p.k_pitch, g, there);
+        x.a.load(from + a), x.b.load(from + b);
+    };
+    load(g0, first);
+    if (first + 1 < end) load(g1, first + 1);
+    float mc[kMine], ms[kMine], cs[E], sn[E];
+#pragma unroll
+    for (int m = 0; m < kMine; m++)
+        if (in + m * kPer < E) turn_f32(p.rope[sub * E + in + m * kPer], position, mc[m], ms[m]);
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        cs[i] = __shfl_sync(0xffffffffu, mc[i / kPer], i % kPer * kGroup + sub);
+        sn[i] = __shfl_sync(0xffffffffu, ms[i / kPer], i % kPer * kGroup + sub);
+    }
+    // halves: pair i is values i and E + i of a lane; neighbours: values 2 i and 2 i + 1
+    auto A = [&](const float (&v)[2 * E], int i) { return nb ? v[2 * i] : v[i]; };
+    auto B = [&](const float (&v)[2 * E], int i) { return nb ? v[2 * i + 1] : v[E + i]; };
+    auto some = [&](int from, int to, const float *weights) {
+        if (from >= to) return;
+        float ac[E], bs[E], as[E], bc[E];
+        {
+            float w[2 * E];
+#pragma unroll
+            for (int i = 0; i < E; i++) w[i] = weights ? weights[a + i] : 1.0f, w[E + i] = weights ? weights[b + i] : 1.0f;
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                ac[i] = A(w, i) * cs[i], as[i] = A(w, i) * sn[i];
+                bc[i] = B(w, i) * cs[i], bs[i] = -(B(w, i) * sn[i]);
+            }
+        }
+        auto sum = [&](float x) {
+#pragma unroll
+            for (int o = 1; o < kGroup; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+            return x;
+        };
+        auto one = [&](Group &x, int g) {
+            float v[2 * E];
+#pragma unroll
+            for (int i = 0; i < E; i++) v[i] = x.a.get(i), v[E + i] = x.b.get(i);
+            if (g + 2 < end) load(x, g + 2);
+            if (p.norm != DW_NORM_NONE) {
+                if (p.norm == DW_NORM_LAYER) {
+                    float m = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 2 * E; i++) m += v[i];
+                    m = sum(m) * p.inv_d;
+#pragma unroll
+                    for (int i = 0; i < 2 * E; i++) v[i] -= m;
+                }
+                float2 sq = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int i = 0; i < 2 * E; i += 2) sq = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(v[i], v[i + 1]), sq);
+                const float rstd = __frsqrt_rn(fmaf(sum(sq.x + sq.y), p.inv_d, p.eps));
+#pragma unroll
+                for (int i = 0; i < 2 * E; i += 2) {
+                    const float2 r = __fmul2_rn(make_float2(v[i], v[i + 1]), make_float2(rstd, rstd));
+                    v[i] = r.x, v[i + 1] = r.y;
+                }
+            }
+            float y[2 * E];
+            auto turn = [&](auto near) {  // two pairs to an instruction
+                constexpr bool kNear = decltype(near)::value;
+#pragma unroll
+                for (int i = 0; i < E; i += 2) {
+                    const int a0 = kNear ? 2 * i : i, a1 = kNear ? 2 * i + 2 : i + 1, b0 = kNear ? 2 * i + 1 : E + i, b1 = kNear ? 2 * i + 3 : E + i + 1;
+                    const float2 va = make_float2(v[a0], v[a1]), vb = make_float2(v[b0], v[b1]);
+                    const float2 ya = __ffma2_rn(va, make_float2(ac[i], ac[i + 1]), __fmul2_rn(vb, make_float2(bs[i], bs[i + 1])));
+                    const float2 yb = __ffma2_rn(va, make_float2(as[i], as[i + 1]), __fmul2_rn(vb, make_float2(bc[i], bc[i + 1])));
+                    y[a0] = ya.x, y[a1] = ya.y, y[b0] = yb.x, y[b1] = yb.y;
+                }
+            };
+            if (nb)
+                turn(std::true_type{});
+            else
+                turn(std::false_type{});
+            bool there;
+            T *out = place(p.q_out, p.qo_pitch, p.k_out, p.ko_pitch, g, there);
+            if (!there) return;
+            float lo[E], hi[E];
+#pragma unroll
+            for (int i = 0; i < E; i++) lo[i] = y[i], hi[i] = y[E + i];
+            Raw<T, E> r;
+            r.set(lo);
+            r.store(out + a);
+            r.set(hi);
+            r.store(out + b);
+        };
+        // groups alternate between the two places, whichever of q and k they are of
+        int g = from;
+        if ((g - first) & 1) one(g1, g++);
+        while (g < to) {
+            one(g0, g++);
+            if (g < to) one(g1, g++);
+        }
+    };
+    some(first, min(end, qg), p.w_q);
+    some(max(first, qg), end, p.w_k);
+}
+
+template <typename T, int E, int kPer>
+__global__ void __launch_bounds__(kThreads) k_rope(const __grid_constant__ HeadParams p) {
+    pdl_wait();
+    pdl_trigger();
+    const size_t unit = (size_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32, row = unit / p.chunks;
+    if (row >= p.tokens) return;
+    rope_row<T, E, kPer>(p, row, p.positions[row], (int)(unit % p.chunks) * p.chunk);
+}
+
 template <typename T, int E, int J>
 __global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ HeadParams p) {
     pdl_wait();
@@ -202,16 +334,17 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ 
 // A block of threads has one head of one page that rows are written to, a warp eight of its
 // tokens, a lane 2 E = d / 32 values of each.  The cached codes are the definition's own: keys
 // are computed in f32, with a bound on what that can be off, and where a value within the bound
-// of its own would get another code (some token in 300) the token is computed again in f64
+// of its own would get another code (some token in 100) the token is computed again in f64
 // (everything in f64 took 17 us of a 4096-token prompt's 23).  An f64 key is kept as f32 rounded to
 // odd (a last bit of 1 where anything was cut off), which rounds to e4m3 as the f64 would.
 // The blocks behind those of the pages norm and turn query rows.
 //
 // The bound: in units of 2^-24, a sum of squares by lanes' chains of 4 and 5 levels is off by 9
 // of itself, the root of its mean and the reciprocal by 7 then, times a weight and the value 2
-// more; a cosine and a sine by 8 (the angle's own rounding is below 4), their products and the
-// sum by 4, of the pair's size: 21, taken as 64.
-constexpr float kKeyErr = 64.0f / 16777216.0f;
+// more; a cosine and a sine of the first token by 8 (the angle's own rounding is below 4) and at
+// each of up to seven steps to the next by 8 of the step's and 4 of the products and sum, 92;
+// their products with the values and the sum by 4, of the pair's size: 105, taken as 128.
+constexpr float kKeyErr = 128.0f / 16777216.0f;
 constexpr int kWarpTokens = 8;
 
 __device__ __forceinline__ float round_to_odd(double v) {
@@ -327,7 +460,11 @@ __global__ void __launch_bounds__(512)
         if (place < 0 || place >= r.n) return;
         HeadParams pq = p;
         pq.hk = 0;
-        norm_rope_row<T, QE, QJ>(pq, row, r.position((int)row), (int)(unit % p.chunks) * p.chunk);
+        const int from = (int)(unit % p.chunks) * p.chunk;
+        if constexpr (QJ == 0)
+            rope_row<T, QE, QE / E>(pq, row, r.position((int)row), from);
+        else
+            norm_rope_row<T, QE, QJ>(pq, row, r.position((int)row), from);
         return;
     }
     const int head = (int)(blockIdx.x % p.hk);
@@ -364,12 +501,16 @@ __global__ void __launch_bounds__(512)
     const bool has_old = t0 > begin;
     const int k_old = has_old ? kv_exponent(scale[0]) : kKvMinExp, v_old = has_old ? kv_exponent(scale[1]) : kKvMinExp;
     uint8_t *const kc = kv_codes(c.k, c, page, head), *const vc = kv_codes(c.v, c, page, head);
-    uint64_t turn[E];
-    float w[2 * E];
+    float w[2 * E], cs[E], sn[E], cs1[E], sn1[E];
     const bool any = w0 < t1 && w0 + kWarpTokens > t0, weighs = p.norm != DW_NORM_NONE && p.w_k;
 #pragma unroll
     for (int j = 0; j < E; j++) {
-        turn[j] = slot.turns && any ? p.rope[lane * E + j] : 0;
+        cs[j] = cs1[j] = 1.0f, sn[j] = sn1[j] = 0.0f;
+        if (slot.turns && any) {  // of the warp's first token, and of a step from token to token
+            const uint64_t f = p.rope[lane * E + j];
+            turn_f32(f, max(w0, t0), cs[j], sn[j]);
+            if (min(w0 + kWarpTokens, t1) - max(w0, t0) > 1) turn_f32(f, 1, cs1[j], sn1[j]);
+        }
         w[j] = weighs && any ? p.w_k[slot.a + j] : 1.0f, w[E + j] = weighs && any ? p.w_k[slot.b + j] : 1.0f;
     }
     // largest |key| less and plus what it can be off, largest |value|; tokens that are no numbers;
@@ -394,15 +535,18 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
             for (int j = 0; j < 2 * E; j++) x[j] *= rstd * w[j];
         }
-        float cs[E], sn[E];
 #pragma unroll
         for (int j = 0; j < E; j++) {
             // what the two values of a pair can be off
             const float pair = p.neighbours ? fabsf(x[2 * j]) + fabsf(x[2 * j + 1]) : fabsf(x[j]) + fabsf(x[E + j]);
             err_of[i][j] = p.norm == DW_NORM_NONE && !slot.turns ? 0.0f : kKeyErr * pair;
-            if (slot.turns) turn_f32(turn[j], t, cs[j], sn[j]);
         }
         if (slot.turns) rotate<E, float>(x, cs, sn, p.neighbours);
+#pragma unroll
+        for (int j = 0; j < E; j++) {  // the next token's angle
+            const float cn = fmaf(cs[j], cs1[j], -sn[j] * sn1[j]);
+            sn[j] = fmaf(sn[j], cs1[j], cs[j] * sn1[j]), cs[j] = cn;
+        }
         float low = 0.0f, high = 0.0f, vm = 0.0f;
         bool fine = p.norm != DW_NORM_LAYER && rms > 1e-30f && rms < 1e30f, ok = true;
 #pragma unroll
@@ -571,16 +715,17 @@ HeadParams params(const dw_head_desc &d, size_t tokens, const HeadArgs &a) {
     p.hq = a.q.ptr ? d.q_heads : 0, p.hk = a.k.ptr ? d.kv_heads : 0;
     p.d = d.head_dim, p.rot = d.rot_dim, p.norm = d.norm;
     p.eps = d.eps, p.inv_d = 1.0f / (float)d.head_dim, p.neighbours = d.neighbours != 0;
+    p.whole = d.rot_dim == d.head_dim;
     return p;
 }
 
 // The lanes of a head with E values in a piece and J slots a lane, and how the heads of a row
 // are shared out: few rows give each warp one group of heads, many rows all of a row's, so that
 // its angles are computed once.
-void split(const dw_backend *be, HeadParams &p, int heads, int E, int J) {
+void split(const dw_backend *be, HeadParams &p, int E, int J) {
     p.group = 1;
     while (p.group * 2 * E * J < p.d) p.group *= 2;
-    const int per = 32 / p.group, groups = (heads + per - 1) / per;
+    const int per = 32 / p.group, groups = (p.hq + per - 1) / per + (p.hk + per - 1) / per;
     const size_t warps = (size_t)be->sm_count * 32;  // that the GPU holds at about this many registers
     p.chunk = (int)std::max<size_t>(1, std::min<size_t>(groups, (size_t)p.tokens * groups / warps));
     p.chunks = (groups + p.chunk - 1) / p.chunk;
@@ -600,13 +745,18 @@ bool wide(const HeadParams &p, std::initializer_list<HeadRows> rows) {
 
 template <typename T>
 dw_status norm_rope(dw_backend *be, HeadParams p, const HeadArgs &a) {
-    const int heads = p.hq + p.hk;
     auto go = [&](auto kernel, int E, int J) {
-        split(be, p, heads, E, J);
+        split(be, p, E, J);
         const size_t blocks = ((size_t)p.tokens * p.chunks + kThreads / 32 - 1) / (kThreads / 32);
         if (blocks > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "norm_rope: too many rows");
         return launch_dependent(be, "norm_rope", kernel, (unsigned)blocks, kThreads, 0, 0, p);
     };
+    if (wide<T>(p, {a.q, a.k, a.q_out, a.k_out})) {
+        constexpr int E = kWide<T>;
+        if (p.whole && p.d == 16 * E) return go(k_rope<T, E, 4>, E, 1);
+        if (p.whole && p.d == 8 * E) return go(k_rope<T, E, 8>, E, 1);
+        if (p.whole && p.d == 32 * E) return go(k_rope<T, E, 2>, E, 1);
+    }
     if (wide<T>(p, {a.q, a.k, a.q_out, a.k_out})) return go(k_norm_rope<T, kWide<T>, 1>, kWide<T>, 1);
     if (p.d <= 128) return go(k_norm_rope<T, 1, 2>, 1, 2);
     return go(k_norm_rope<T, 1, 8>, 1, 8);
@@ -623,13 +773,17 @@ dw_status append(dw_backend *be, HeadParams p, const KvCache &c, const Seqs &s, 
         size_t blocks = pages;
         p.chunks = 1;
         if (p.hq) {
-            split(be, p, p.hq, QE, QJ);
+            HeadParams queries = p;
+            queries.hk = 0;
+            split(be, queries, QE, QJ ? QJ : 1);
+            p.group = queries.group, p.chunk = queries.chunk, p.chunks = queries.chunks;
             blocks += ((size_t)p.tokens * p.chunks + threads / 32 - 1) / (threads / 32);
         }
         if (blocks > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "append_kv: too many rows");
         return launch_dependent(be, "append_kv", kernel, (unsigned)blocks, threads, 0, 0, p, c, s, (uint32_t)pages, (uint32_t)n,
                                 (uint32_t)each, be->dev_err);
     };
+    if (wide<T>(p, {a.q, a.q_out}) && p.whole) return go(k_append<T, E, kWide<T>, 0>, kWide<T>, 1);
     if (wide<T>(p, {a.q, a.q_out})) return go(k_append<T, E, kWide<T>, 1>, kWide<T>, 1);
     return go(k_append<T, E, 1, E>, 1, E);
 }
