@@ -204,7 +204,7 @@ struct HeadRows {
 struct HeadArgs {
     HeadRows q, k, v, q_out, k_out;
     const float *w_q, *w_k;
-    const uint64_t *rope;      // turns a position, fractions of 2^64; null: no rotation
+    const uint64_t *rope;      // per pair: turns a position in 2^-64; then f64 cos and sin of one; null: no rotation
     const int32_t *positions;  // norm_rope alone
 };
 dw_status launch_norm_rope(dw_backend *be, const dw_head_desc &d, size_t tokens, const HeadArgs &a);

@@ -332,19 +332,13 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ 
 
 // ---- append ------------------------------------------------------------------------
 // A block of threads has one head of one page that rows are written to, a warp eight of its
-// tokens, a lane 2 E = d / 32 values of each.  The cached codes are the definition's own: keys
-// are computed in f32, with a bound on what that can be off, and where a value within the bound
-// of its own would get another code (some token in 100) the token is computed again in f64
-// (everything in f64 took 17 us of a 4096-token prompt's 23).  An f64 key is kept as f32 rounded to
-// odd (a last bit of 1 where anything was cut off), which rounds to e4m3 as the f64 would.
-// The blocks behind those of the pages norm and turn query rows.
-//
-// The bound: in units of 2^-24, a sum of squares by lanes' chains of 4 and 5 levels is off by 9
-// of itself, the root of its mean and the reciprocal by 7 then, times a weight and the value 2
-// more; a cosine and a sine of the first token by 8 (the angle's own rounding is below 4) and at
-// each of up to seven steps to the next by 8 of the step's and 4 of the products and sum, 92;
-// their products with the values and the sum by 4, of the pair's size: 105, taken as 128.
-constexpr float kKeyErr = 128.0f / 16777216.0f;
+// tokens, a lane 2 E = d / 32 values of each.  Keys are computed in f64 and kept, in shared
+// memory, as f32 rounded to odd (a last bit of 1 where anything was cut off), which rounds to
+// e4m3 as the f64 would: the cached codes are the definition's own, whatever hardware or order
+// computed them.  (f32 with a bound, and f64 where that leaves two codes open, took longer: the
+// bound has to hold for the pair, and one token in five had a value too small beside its
+// partner.)  A warp's tokens follow each other, so the angles after the first come by one
+// complex product each.  The blocks behind those of the pages norm and turn query rows.
 constexpr int kWarpTokens = 8;
 
 __device__ __forceinline__ float round_to_odd(double v) {
@@ -396,45 +390,6 @@ __device__ __forceinline__ void rescale_codes(uint8_t *p, float f) {
     }
 }
 
-// The 2 E key values of a lane of one token, normed and turned, in f64.
-template <typename T, int E>
-__device__ __noinline__ bool exact_key(const HeadParams &p, const T *k, const Slot<E> slot, int64_t position, float (&out)[2 * E]) {
-    float lo[E], hi[E];
-    load_values<T, E>(k + slot.a, p.vec, lo);
-    load_values<T, E>(k + slot.b, p.vec, hi);
-    double x[2 * E], cs[E], sn[E];
-#pragma unroll
-    for (int j = 0; j < E; j++) x[j] = lo[j], x[E + j] = hi[j];
-    if (p.norm != DW_NORM_NONE) {
-        if (p.norm == DW_NORM_LAYER) {
-            double m = 0.0;
-#pragma unroll
-            for (int j = 0; j < 2 * E; j++) m += x[j];
-            m = warp_sum(m) / p.d;
-#pragma unroll
-            for (int j = 0; j < 2 * E; j++) x[j] -= m;
-        }
-        double sq = 0.0;
-#pragma unroll
-        for (int j = 0; j < 2 * E; j++) sq = fma(x[j], x[j], sq);
-        const double rstd = 1.0 / sqrt(warp_sum(sq) / p.d + (double)p.eps);
-#pragma unroll
-        for (int j = 0; j < E; j++) {
-            x[j] *= rstd * (p.w_k ? (double)p.w_k[slot.a + j] : 1.0);
-            x[E + j] *= rstd * (p.w_k ? (double)p.w_k[slot.b + j] : 1.0);
-        }
-    }
-    if (slot.turns) {
-#pragma unroll
-        for (int j = 0; j < E; j++) turn_f64(p.rope[(threadIdx.x & 31) * E + j], position, cs[j], sn[j]);
-        rotate<E, double>(x, cs, sn, p.neighbours);
-    }
-    bool ok = true;
-#pragma unroll
-    for (int j = 0; j < 2 * E; j++) ok = ok && isfinite(x[j]), out[j] = round_to_odd(x[j]);
-    return ok;
-}
-
 // The place of item w of rows whose sequences have as many each.
 __device__ __forceinline__ uint32_t seq_and_place(const Seqs &q, uint32_t w, uint32_t each, int per, int size, int extra, int64_t &place) {
     if (q.starts) return seq_of_item(q, w, per, size, extra, place);
@@ -446,7 +401,8 @@ template <typename T, int E, int QE, int QJ>
 __global__ void __launch_bounds__(512)
     k_append(const __grid_constant__ HeadParams p, const __grid_constant__ KvCache c, const __grid_constant__ Seqs q,
              const uint32_t page_blocks, const uint32_t each_rows, const uint32_t each_pages, int32_t *err) {
-    __shared__ uint32_t top[3][16];
+    extern __shared__ float keys[];  // [page][d], as lanes have them
+    __shared__ uint32_t top[2][16];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, warps = blockDim.x / 32;
     pdl_wait();
     pdl_trigger();
@@ -479,175 +435,131 @@ __global__ void __launch_bounds__(512)
     const int w0 = (int)begin + warp * kWarpTokens;  // the warp's first token
     const Slot<E> slot(lane, p.rot, p.neighbours);
     const T *const kp = (const T *)p.k + (size_t)head * p.d, *const vp = (const T *)p.v + (size_t)head * p.d;
+    // the rows of a token of the warp; those that are not its own are not looked at
     auto row_of = [&](int t) { return (size_t)r.row0 + (t - (r.len - r.n)); };
-    float kv[kWarpTokens][2 * E], vv[kWarpTokens][2 * E];
-#pragma unroll
-    for (int i = 0; i < kWarpTokens; i++) {
-        const int t = w0 + i;
-        if (t < t0 || t >= t1) continue;
-        const size_t row = row_of(t);
-        float lo[E], hi[E];
-        load_values<T, E>(kp + row * p.k_pitch + slot.a, p.vec, lo);
-        load_values<T, E>(kp + row * p.k_pitch + slot.b, p.vec, hi);
-#pragma unroll
-        for (int j = 0; j < E; j++) kv[i][j] = lo[j], kv[i][E + j] = hi[j];
-        load_values<T, E>(vp + row * p.v_pitch + 2 * E * lane, p.vec, lo);
-        load_values<T, E>(vp + row * p.v_pitch + 2 * E * lane + E, p.vec, hi);
-#pragma unroll
-        for (int j = 0; j < E; j++) vv[i][j] = lo[j], vv[i][E + j] = hi[j];
-    }
     const uint32_t page = seq_page(q, c, s, (uint32_t)(begin >> shift), err);
     uint8_t *const scale = c.s + kv_block(c, page, head) * 2;
     const bool has_old = t0 > begin;
     const int k_old = has_old ? kv_exponent(scale[0]) : kKvMinExp, v_old = has_old ? kv_exponent(scale[1]) : kKvMinExp;
     uint8_t *const kc = kv_codes(c.k, c, page, head), *const vc = kv_codes(c.v, c, page, head);
-    float w[2 * E], cs[E], sn[E], cs1[E], sn1[E];
-    const bool any = w0 < t1 && w0 + kWarpTokens > t0, weighs = p.norm != DW_NORM_NONE && p.w_k;
-#pragma unroll
-    for (int j = 0; j < E; j++) {
-        cs[j] = cs1[j] = 1.0f, sn[j] = sn1[j] = 0.0f;
-        if (slot.turns && any) {  // of the warp's first token, and of a step from token to token
-            const uint64_t f = p.rope[lane * E + j];
-            turn_f32(f, max(w0, t0), cs[j], sn[j]);
-            if (min(w0 + kWarpTokens, t1) - max(w0, t0) > 1) turn_f32(f, 1, cs1[j], sn1[j]);
-        }
-        w[j] = weighs && any ? p.w_k[slot.a + j] : 1.0f, w[E + j] = weighs && any ? p.w_k[slot.b + j] : 1.0f;
-    }
-    // largest |key| less and plus what it can be off, largest |value|; tokens that are no numbers;
-    // tokens that are exact already
-    float k_low = 0.0f, k_high = 0.0f, vmax = 0.0f, err_of[kWarpTokens][E];
-    uint32_t poison = 0, exact = 0;
-#pragma unroll
-    for (int i = 0; i < kWarpTokens; i++) {
-        const int t = w0 + i;
-        if (t < t0 || t >= t1) continue;
-        float x[2 * E], rms = 1.0f;
-#pragma unroll
-        for (int j = 0; j < 2 * E; j++) x[j] = kv[i][j];
-        if (p.norm == DW_NORM_RMS) {
-            float sq = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 2 * E; j++) sq = fmaf(x[j], x[j], sq);
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-            rms = fmaf(sq, p.inv_d, p.eps);
-            const float rstd = __frsqrt_rn(rms);
-#pragma unroll
-            for (int j = 0; j < 2 * E; j++) x[j] *= rstd * w[j];
-        }
+    const int from = max(w0, t0), to = min(w0 + kWarpTokens, t1);
+    float kmax = 0.0f, vmax = 0.0f;
+    uint32_t poison = 0;
+    if (from < to) {
+        double cs[E], sn[E], cs1[E], sn1[E];
+        float w[2 * E];
+        const bool weighs = p.norm != DW_NORM_NONE && p.w_k;
 #pragma unroll
         for (int j = 0; j < E; j++) {
-            // what the two values of a pair can be off
-            const float pair = p.neighbours ? fabsf(x[2 * j]) + fabsf(x[2 * j + 1]) : fabsf(x[j]) + fabsf(x[E + j]);
-            err_of[i][j] = p.norm == DW_NORM_NONE && !slot.turns ? 0.0f : kKeyErr * pair;
+            w[j] = weighs ? p.w_k[slot.a + j] : 1.0f, w[E + j] = weighs ? p.w_k[slot.b + j] : 1.0f;
+            cs[j] = cs1[j] = 1.0, sn[j] = sn1[j] = 0.0;
+            if (slot.turns) {
+                const int pair = lane * E + j, pairs = p.rot / 2;
+                turn_f64(p.rope[pair], from, cs[j], sn[j]);
+                const double *const step = reinterpret_cast<const double *>(p.rope + pairs);
+                cs1[j] = step[pair], sn1[j] = step[pairs + pair];
+            }
         }
-        if (slot.turns) rotate<E, float>(x, cs, sn, p.neighbours);
+        constexpr int kBatch = 4;  // tokens whose loads are in flight
+#pragma unroll 1
+        for (int t4 = from; t4 < to; t4 += kBatch) {
+            float kv[kBatch][2 * E], vv[kBatch][2 * E];
 #pragma unroll
-        for (int j = 0; j < E; j++) {  // the next token's angle
-            const float cn = fmaf(cs[j], cs1[j], -sn[j] * sn1[j]);
-            sn[j] = fmaf(sn[j], cs1[j], cs[j] * sn1[j]), cs[j] = cn;
-        }
-        float low = 0.0f, high = 0.0f, vm = 0.0f;
-        bool fine = p.norm != DW_NORM_LAYER && rms > 1e-30f && rms < 1e30f, ok = true;
+            for (int i = 0; i < kBatch; i++) {
+                const size_t row = row_of(min(t4 + i, to - 1));
+                float lo[E], hi[E];
+                load_values<T, E>(kp + row * p.k_pitch + slot.a, p.vec, lo);
+                load_values<T, E>(kp + row * p.k_pitch + slot.b, p.vec, hi);
 #pragma unroll
-        for (int j = 0; j < 2 * E; j++) {
-            const float off = p.neighbours ? err_of[i][j / 2] : err_of[i][j % E];
-            low = fmaxf(low, fabsf(x[j]) - off), high = fmaxf(high, fabsf(x[j]) + off);
-            fine = fine && fabsf(x[j]) + off < 1e38f;
-            vm = fmaxf(vm, fabsf(vv[i][j]));
-            ok = ok && isfinite(vv[i][j]);
-        }
-        if (!__all_sync(0xffffffffu, fine)) {
-            float f[2 * E];
-            const bool number = exact_key<T, E>(p, kp + row_of(t) * p.k_pitch, slot, t, f);
-            ok = ok && number, exact |= 1u << i;
-            low = high = 0.0f;
+                for (int j = 0; j < E; j++) kv[i][j] = lo[j], kv[i][E + j] = hi[j];
+                load_values<T, E>(vp + row * p.v_pitch + 2 * E * lane, p.vec, lo);
+                load_values<T, E>(vp + row * p.v_pitch + 2 * E * lane + E, p.vec, hi);
 #pragma unroll
-            for (int j = 0; j < 2 * E; j++) x[j] = f[j], low = high = fmaxf(high, fabsf(f[j]));
-        }
-#pragma unroll
-        for (int j = 0; j < 2 * E; j++) kv[i][j] = x[j];
-        if (__all_sync(0xffffffffu, ok))
-            k_low = fmaxf(k_low, low), k_high = fmaxf(k_high, high), vmax = fmaxf(vmax, vm);
-        else
-            poison |= 1u << i;
-    }
-    uint32_t km[3] = {__float_as_uint(k_low), __float_as_uint(k_high), __float_as_uint(vmax)};
-    auto block_max = [&](int from) {
-#pragma unroll
-        for (int n = from; n < 3; n++) {
-            km[n] = __reduce_max_sync(0xffffffffu, km[n]);
-            if (lane == 0) top[n][warp] = km[n];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int n = from; n < 3; n++)
-            for (int i = 0; i < warps; i++) km[n] = max(km[n], top[n][i]);
-    };
-    block_max(0);
-    int ke = kv_scale_exponent(__uint_as_float(km[1]));
-    if (ke != kv_scale_exponent(__uint_as_float(km[0]))) {  // the largest key lies at a border: every token in f64
-        k_high = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kWarpTokens; i++) {
-            const int t = w0 + i;
-            if (t < t0 || t >= t1 || (poison >> i & 1)) continue;
-            if (!(exact >> i & 1)) {
-                float f[2 * E];
-                exact_key<T, E>(p, kp + row_of(t) * p.k_pitch, slot, t, f);
-#pragma unroll
-                for (int j = 0; j < 2 * E; j++) kv[i][j] = f[j];
+                for (int j = 0; j < E; j++) vv[i][j] = lo[j], vv[i][E + j] = hi[j];
             }
 #pragma unroll
-            for (int j = 0; j < 2 * E; j++) k_high = fmaxf(k_high, fabsf(kv[i][j]));
-        }
-        exact = 0xFFu;
-        __syncthreads();
-        km[1] = __float_as_uint(k_high);
-        block_max(1);
-        ke = kv_scale_exponent(__uint_as_float(km[1]));
-    }
-    ke = max(ke, k_old);
-    const int ve = max(kv_scale_exponent(__uint_as_float(km[2])), v_old);
-    const float k_inv = kv_pow2(-ke), v_inv = kv_pow2(-ve);
-    if (threadIdx.x == 0) scale[0] = (uint8_t)(ke + 127), scale[1] = (uint8_t)(ve + 127);
+            for (int i = 0; i < kBatch; i++) {
+                const int t = t4 + i;
+                if (t >= to) break;
+                double x[2 * E];
 #pragma unroll
-    for (int i = 0; i < kWarpTokens; i++) {
-        const int t = w0 + i;
-        uint8_t *const kr = kc + (t - (int)begin) * p.d, *const vr = vc + (t - (int)begin) * p.d;
-        if (t < t0) {
-            if (ke != k_old) rescale_codes<E>(kr + 2 * E * lane, kv_pow2(k_old - ke));
-            if (ve != v_old) rescale_codes<E>(vr + 2 * E * lane, kv_pow2(v_old - ve));
-        } else if (t < t1) {
-            const bool bad = poison >> i & 1;
-            if (!bad && !(exact >> i & 1)) {
-                // a value that is off by all it can be: the same code?
-                bool same = true;
+                for (int j = 0; j < 2 * E; j++) x[j] = kv[i][j];
+                if (p.norm != DW_NORM_NONE) {
+                    if (p.norm == DW_NORM_LAYER) {
+                        double m = 0.0;
+#pragma unroll
+                        for (int j = 0; j < 2 * E; j++) m += x[j];
+                        m = warp_sum(m) / p.d;
+#pragma unroll
+                        for (int j = 0; j < 2 * E; j++) x[j] -= m;
+                    }
+                    double sq = 0.0;
+#pragma unroll
+                    for (int j = 0; j < 2 * E; j++) sq = fma(x[j], x[j], sq);
+                    const double rstd = rsqrt(warp_sum(sq) / p.d + (double)p.eps);
+#pragma unroll
+                    for (int j = 0; j < 2 * E; j++) x[j] *= rstd * w[j];
+                }
+                if (slot.turns) rotate<E, double>(x, cs, sn, p.neighbours);
+                bool ok = true;
+                float km = 0.0f, vm = 0.0f, y[2 * E];
 #pragma unroll
                 for (int j = 0; j < 2 * E; j++) {
-                    const float off = p.neighbours ? err_of[i][j / 2] : err_of[i][j % E];
-                    const uint32_t two = e4m3_codes2((kv[i][j] - off) * k_inv, (kv[i][j] + off) * k_inv);
-                    same = same && (two & 255) == (two >> 8);
+                    ok = ok && isfinite(x[j]) && isfinite(vv[i][j]);
+                    y[j] = round_to_odd(x[j]);
+                    km = fmaxf(km, fabsf(y[j])), vm = fmaxf(vm, fabsf(vv[i][j]));
                 }
-                if (!__all_sync(0xffffffffu, same)) {
-                    float f[2 * E];
-                    exact_key<T, E>(p, kp + row_of(t) * p.k_pitch, slot, t, f);
+                if (__all_sync(0xffffffffu, ok))
+                    kmax = fmaxf(kmax, km), vmax = fmaxf(vmax, vm);
+                else
+                    poison |= 1u << (t - w0);
+                float *const place = keys + (t - (int)begin) * p.d + lane * 2 * E;
 #pragma unroll
-                    for (int j = 0; j < 2 * E; j++) kv[i][j] = f[j];
+                for (int j = 0; j < 2 * E; j++) place[j] = y[j];
+#pragma unroll
+                for (int j = 0; j < E; j++) {  // the next token's angle
+                    const double cn = cs[j] * cs1[j] - sn[j] * sn1[j];
+                    sn[j] = sn[j] * cs1[j] + cs[j] * sn1[j];
+                    cs[j] = cn;
                 }
             }
-            float lo[E], hi[E], all[2 * E];
-#pragma unroll
-            for (int j = 0; j < E; j++) {
-                lo[j] = bad ? __uint_as_float(0x7FC00000u) : kv[i][j] * k_inv;
-                hi[j] = bad ? __uint_as_float(0x7FC00000u) : kv[i][E + j] * k_inv;
-            }
-#pragma unroll
-            for (int j = 0; j < 2 * E; j++) all[j] = bad ? 0.0f : vv[i][j] * v_inv;
-            store_codes<E>(kr + slot.a, lo);
-            store_codes<E>(kr + slot.b, hi);
-            store_codes<2 * E>(vr + 2 * E * lane, all);
         }
+    }
+    kmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(kmax)));
+    vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vmax)));
+    if (lane == 0) top[0][warp] = __float_as_uint(kmax), top[1][warp] = __float_as_uint(vmax);
+    __syncthreads();
+    uint32_t km = 0, vm = 0;
+    for (int i = 0; i < warps; i++) km = max(km, top[0][i]), vm = max(vm, top[1][i]);
+    const int ke = max(kv_scale_exponent(__uint_as_float(km)), k_old), ve = max(kv_scale_exponent(__uint_as_float(vm)), v_old);
+    const float k_inv = kv_pow2(-ke), v_inv = kv_pow2(-ve);
+    if (threadIdx.x == 0) scale[0] = (uint8_t)(ke + 127), scale[1] = (uint8_t)(ve + 127);
+    if (ke != k_old || ve != v_old)  // the codes that the block holds are rounded again
+        for (int t = w0; t < min(w0 + kWarpTokens, t0); t++) {
+            uint8_t *const kr = kc + (t - (int)begin) * p.d, *const vr = vc + (t - (int)begin) * p.d;
+            if (ke != k_old) rescale_codes<E>(kr + 2 * E * lane, kv_pow2(k_old - ke));
+            if (ve != v_old) rescale_codes<E>(vr + 2 * E * lane, kv_pow2(v_old - ve));
+        }
+#pragma unroll 4
+    for (int t = from; t < to; t++) {
+        uint8_t *const kr = kc + (t - (int)begin) * p.d, *const vr = vc + (t - (int)begin) * p.d;
+        const bool bad = poison >> (t - w0) & 1;
+        const float *const place = keys + (t - (int)begin) * p.d + lane * 2 * E;
+        const T *const v = vp + row_of(t) * p.v_pitch + 2 * E * lane;
+        float lo[E], hi[E], all[2 * E];
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+            lo[j] = bad ? __uint_as_float(0x7FC00000u) : place[j] * k_inv;
+            hi[j] = bad ? __uint_as_float(0x7FC00000u) : place[E + j] * k_inv;
+        }
+        float v0[E], v1[E];
+        load_values<T, E>(v, p.vec, v0);
+        load_values<T, E>(v + E, p.vec, v1);
+#pragma unroll
+        for (int j = 0; j < E; j++) all[j] = bad ? 0.0f : v0[j] * v_inv, all[E + j] = bad ? 0.0f : v1[j] * v_inv;
+        store_codes<E>(kr + slot.a, lo);
+        store_codes<E>(kr + slot.b, hi);
+        store_codes<2 * E>(vr + 2 * E * lane, all);
     }
 }
 
@@ -780,7 +692,13 @@ dw_status append(dw_backend *be, HeadParams p, const KvCache &c, const Seqs &s, 
             blocks += ((size_t)p.tokens * p.chunks + threads / 32 - 1) / (threads / 32);
         }
         if (blocks > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "append_kv: too many rows");
-        return launch_dependent(be, "append_kv", kernel, (unsigned)blocks, threads, 0, 0, p, c, s, (uint32_t)pages, (uint32_t)n,
+        const size_t smem = (size_t)c.page * c.d * 4;
+        if (smem > 48 * 1024)
+            if (dw_status st = dw_cuda_check(be, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                                             "append_kv attributes");
+                st != DW_OK)
+                return st;
+        return launch_dependent(be, "append_kv", kernel, (unsigned)blocks, threads, smem, 0, p, c, s, (uint32_t)pages, (uint32_t)n,
                                 (uint32_t)each, be->dev_err);
     };
     if (wide<T>(p, {a.q, a.q_out}) && p.whole) return go(k_append<T, E, kWide<T>, 0>, kWide<T>, 1);

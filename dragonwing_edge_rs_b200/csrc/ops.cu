@@ -3,6 +3,7 @@
 // then dispatch to the kernels.
 
 #include <cmath>
+#include <cstring>
 #include <vector>
 
 #include "dw_internal.h"
@@ -1150,7 +1151,9 @@ dw_status check_head_desc(dw_backend *be, const dw_head_desc *d, const dw_buf *r
     if (d->norm < DW_NORM_NONE || d->norm > DW_NORM_LAYER) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: unknown norm kind", op);
     if (!(d->eps >= 0.0f)) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: eps must be >= 0", op);
     if (d->rot_dim) {
-        DW_TRY(check_vec(be, rope, d->rot_dim / 2, 8, op, "rope"));
+        DW_TRY(need(be, rope, op, "rope"));
+        DW_TRY(check_len(be, rope, (size_t)d->rot_dim / 2 * 24, op, "rope"));
+        DW_TRY(check_align(be, rope, 8, op, "rope"));
         a->rope = (const uint64_t *)rope->ptr;
     } else if (rope) {
         return dw_fail(be, DW_ERR_INVALID_ARG, "%s: rope is given but rot_dim is 0", op);
@@ -1221,17 +1224,19 @@ DW_API dw_status dw_prepare_rope(dw_backend *be, const double *freqs, size_t pai
     *out = nullptr;
     DW_TRY(need(be, freqs, op, "freqs"));
     if (!pairs || pairs > 256) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: 1 to 256 pairs, not %zu", op, pairs);
-    uint64_t turns[256];
+    uint64_t turns[3 * 256];  // fractions of a turn, then cosines and sines of one step, as f64
     const long double two_pi = 6.283185307179586476925286766559005768L;
     for (size_t i = 0; i < pairs; i++) {
         if (!std::isfinite(freqs[i])) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: freqs[%zu] is not finite", op, i);
         long double t = (long double)freqs[i] / two_pi;
         t = (t - floorl(t)) * 18446744073709551616.0L;  // [0, 1) of a turn, in 2^-64; 1 (by rounding) is 0
         turns[i] = t >= 18446744073709551616.0L ? 0 : (uint64_t)t;
+        const double c = (double)cosl((long double)freqs[i]), s = (double)sinl((long double)freqs[i]);
+        memcpy(&turns[pairs + i], &c, 8), memcpy(&turns[2 * pairs + i], &s, 8);
     }
     dw_buf *b = nullptr;
-    DW_TRY(dw_alloc(be, pairs * 8, &b));
-    const dw_status st = dw_upload(be, b, turns, pairs * 8);
+    DW_TRY(dw_alloc(be, pairs * 24, &b));
+    const dw_status st = dw_upload(be, b, turns, pairs * 24);
     if (st != DW_OK) {
         dw_free(be, b);
         return st;

@@ -501,7 +501,7 @@ def prepare_rope(backend: CudaBackend, freqs) -> CudaBuffer:
     out = ctypes.c_void_p()
     backend._check(L.load().dw_prepare_rope(backend.handle, f.ctypes.data_as(ctypes.POINTER(ctypes.c_double)), f.size,
                                             ctypes.byref(out)))
-    return CudaBuffer(backend, out, 8 * f.size)
+    return CudaBuffer(backend, out, L.load().dw_buf_len(out))
 
 
 def norm_rope(backend: CudaBackend, desc: HeadDesc, tokens: int, q, k, w_q, w_k, rope, positions, q_out, k_out):
