@@ -346,12 +346,6 @@ __device__ __forceinline__ float round_to_odd(double v) {
     return __uint_as_float(__float_as_uint(f) | (uint32_t)((__double2loint(v) & 0x1FFFFFFF) != 0));
 }
 
-__device__ __forceinline__ double warp_sum(double v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 template <typename T, int E>
 __device__ __forceinline__ void load_values(const T *p, bool vec, float (&v)[E]) {
     if (vec) {
@@ -447,7 +441,8 @@ __global__ void __launch_bounds__(512)
     uint32_t poison = 0;
     if (from < to) {
         double cs[E], sn[E], cs1[E], sn1[E];
-        float w[2 * E];
+        double w[2 * E];
+        const double inv_d = 1.0 / (64 * E);  // a power of two
         const bool weighs = p.norm != DW_NORM_NONE && p.w_k;
 #pragma unroll
         for (int j = 0; j < E; j++) {
@@ -460,9 +455,8 @@ __global__ void __launch_bounds__(512)
                 cs1[j] = step[pair], sn1[j] = step[pairs + pair];
             }
         }
-        constexpr int kBatch = 4;  // tokens whose loads are in flight
-#pragma unroll 1
-        for (int t4 = from; t4 < to; t4 += kBatch) {
+        auto some = [&](const int t4, auto count) {
+            constexpr int kBatch = decltype(count)::value;
             float kv[kBatch][2 * E], vv[kBatch][2 * E];
 #pragma unroll
             for (int i = 0; i < kBatch; i++) {
@@ -477,45 +471,68 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
                 for (int j = 0; j < E; j++) vv[i][j] = lo[j], vv[i][E + j] = hi[j];
             }
+            // the batch's tokens side by side (one after the other each waited for its own sums; what
+            // lies behind the last is computed too, and left)
+            double x[kBatch][2 * E];
+#pragma unroll
+            for (int i = 0; i < kBatch; i++)
+#pragma unroll
+                for (int j = 0; j < 2 * E; j++) x[i][j] = kv[i][j];
+            if (p.norm != DW_NORM_NONE) {
+                double sum[kBatch];
+                auto sums = [&]() {
+#pragma unroll
+                    for (int o = 16; o; o >>= 1)
+#pragma unroll
+                        for (int i = 0; i < kBatch; i++) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+                };
+                if (p.norm == DW_NORM_LAYER) {
+#pragma unroll
+                    for (int i = 0; i < kBatch; i++) {
+                        sum[i] = 0.0;
+#pragma unroll
+                        for (int j = 0; j < 2 * E; j++) sum[i] += x[i][j];
+                    }
+                    sums();
+#pragma unroll
+                    for (int i = 0; i < kBatch; i++)
+#pragma unroll
+                        for (int j = 0; j < 2 * E; j++) x[i][j] -= sum[i] * inv_d;
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch; i++) {
+                    sum[i] = 0.0;
+#pragma unroll
+                    for (int j = 0; j < 2 * E; j++) sum[i] = fma(x[i][j], x[i][j], sum[i]);
+                }
+                sums();
+#pragma unroll
+                for (int i = 0; i < kBatch; i++) {
+                    const double rstd = rsqrt(fma(sum[i], inv_d, (double)p.eps));
+#pragma unroll
+                    for (int j = 0; j < 2 * E; j++) x[i][j] *= rstd * w[j];
+                }
+            }
 #pragma unroll
             for (int i = 0; i < kBatch; i++) {
-                const int t = t4 + i;
-                if (t >= to) break;
-                double x[2 * E];
-#pragma unroll
-                for (int j = 0; j < 2 * E; j++) x[j] = kv[i][j];
-                if (p.norm != DW_NORM_NONE) {
-                    if (p.norm == DW_NORM_LAYER) {
-                        double m = 0.0;
-#pragma unroll
-                        for (int j = 0; j < 2 * E; j++) m += x[j];
-                        m = warp_sum(m) / p.d;
-#pragma unroll
-                        for (int j = 0; j < 2 * E; j++) x[j] -= m;
-                    }
-                    double sq = 0.0;
-#pragma unroll
-                    for (int j = 0; j < 2 * E; j++) sq = fma(x[j], x[j], sq);
-                    const double rstd = rsqrt(warp_sum(sq) / p.d + (double)p.eps);
-#pragma unroll
-                    for (int j = 0; j < 2 * E; j++) x[j] *= rstd * w[j];
-                }
-                if (slot.turns) rotate<E, double>(x, cs, sn, p.neighbours);
+                const int t = min(t4 + i, to - 1);
+                const bool in = t4 + i < to;
+                if (slot.turns) rotate<E, double>(x[i], cs, sn, p.neighbours);
                 bool ok = true;
                 float km = 0.0f, vm = 0.0f, y[2 * E];
 #pragma unroll
                 for (int j = 0; j < 2 * E; j++) {
-                    ok = ok && isfinite(x[j]) && isfinite(vv[i][j]);
-                    y[j] = round_to_odd(x[j]);
+                    ok = ok && isfinite(x[i][j]) && isfinite(vv[i][j]);
+                    y[j] = round_to_odd(x[i][j]);
                     km = fmaxf(km, fabsf(y[j])), vm = fmaxf(vm, fabsf(vv[i][j]));
                 }
-                if (__all_sync(0xffffffffu, ok))
-                    kmax = fmaxf(kmax, km), vmax = fmaxf(vmax, vm);
-                else
-                    poison |= 1u << (t - w0);
+                const bool number = __all_sync(0xffffffffu, ok);
+                if (in && number) kmax = fmaxf(kmax, km), vmax = fmaxf(vmax, vm);
+                if (in && !number) poison |= 1u << (t - w0);
                 float *const place = keys + (t - (int)begin) * p.d + lane * 2 * E;
 #pragma unroll
-                for (int j = 0; j < 2 * E; j++) place[j] = y[j];
+                for (int j = 0; j < 2 * E; j++)
+                    if (in) place[j] = y[j];
 #pragma unroll
                 for (int j = 0; j < E; j++) {  // the next token's angle
                     const double cn = cs[j] * cs1[j] - sn[j] * sn1[j];
@@ -523,6 +540,12 @@ __global__ void __launch_bounds__(512)
                     cs[j] = cn;
                 }
             }
+        };
+        if (to - from == 1) {
+            some(from, std::integral_constant<int, 1>{});
+        } else {
+#pragma unroll 1
+            for (int t4 = from; t4 < to; t4 += 4) some(t4, std::integral_constant<int, 4>{});
         }
     }
     kmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(kmax)));
