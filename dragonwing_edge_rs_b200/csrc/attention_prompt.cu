@@ -34,7 +34,6 @@ constexpr int kGroups = kTile / 16;     // of tokens that share scales
 constexpr int kThreads = 512;
 constexpr int kStages = 4;   // of keys and of values
 constexpr float kHead = 7.0f, kLag = 8.0f;
-constexpr int kEvery = 4;  // of that many pairs of weights one is computed by exp2_fma
 
 __device__ __forceinline__ bool wait_phase(uint64_t *barrier, uint32_t parity, const AttendParams &p, volatile int *abort_flag, int site) {
     const uint32_t bar = smem_u32(barrier);
@@ -123,24 +122,6 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-
-// 2^x of two values without the special-function unit, whose 16 results a cycle are what the
-// weights wait for: x = n + f, f in [-1/2, 1/2], a polynomial of degree 4 for 2^f (equal ripples,
-// relative error 2.6e-6) and n added to its exponent.  Below 2^-126 it gives 2^-126; x at most
-// 127, no NaN.
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-    const float2 magic = make_float2(kMagic, kMagic), lowest = make_float2(-126.0f, -126.0f);
-    x.x = fmaxf(x.x, lowest.x), x.y = fmaxf(x.y, lowest.y);
-    const float2 t = __fadd2_rn(x, magic);  // n in the low bits
-    const float2 f = __fadd2_rn(x, __ffma2_rn(t, make_float2(-1.0f, -1.0f), magic));
-    auto both = [](float c) { return make_float2(c, c); };
-    float2 r = __ffma2_rn(f, both(0x1.3997d6p-7f), both(0x1.ca1440p-5f));
-    r = __ffma2_rn(r, f, both(0x1.ec06dap-3f));
-    r = __ffma2_rn(r, f, both(0x1.62e0dcp-1f));
-    r = __ffma2_rn(r, f, both(0x1.ffffe8p-1f));
-    return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23)),
-                       __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23)));
 }
 
 // A row's columns of tensor memory times f.
@@ -379,25 +360,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The warp's 32 query rows, in f16, to shared memory: kPer lanes a row, eight rows of a lane
         // in flight (a row a thread, its pieces one after the other, took 13000 cycles).
         if (tiles[t]) {
-            constexpr int kPer = D / 8;
+            constexpr int kPer = D / 8, kStep = 32 / kPer;
             const int piece = lane % kPer, row0 = t * 128 + (warp & 3) * 32 + lane / kPer;
+            int token = (first + row0) / p.group, in = (first + row0) % p.group;  // of the lane's next row
+            const T *src = nullptr;
+            auto source = [&](int row) {  // of its rows in turn; behind the last, the last one's
+                if (row < rows) src = (const T *)p.q + (size_t)(r.row0 + token) * p.q_pitch + (size_t)(head * p.group + in) * D + 8 * piece;
+                in += kStep;
+                while (in >= p.group) in -= p.group, token++;
+                return src;
+            };
+            src = (const T *)p.q + (size_t)(r.row0 + token_of(0)) * p.q_pitch + (size_t)(head * p.group + first % p.group) * D;
 #pragma unroll
             for (int i0 = 0; i0 < kPer; i0 += 8) {
                 Raw<T, 8> x[8];
-                auto source = [&](int i) {  // in bounds in any case
-                    const int at = first + min(row0 + (i0 + i) * (32 / kPer), rows - 1);
-                    return (const T *)p.q + (size_t)(r.row0 + at / p.group) * p.q_pitch + (size_t)(head * p.group + at % p.group) * D + 8 * piece;
-                };
                 if (p.vec) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i].load(source(i));
+                    for (int i = 0; i < 8; i++) x[i].load(source(row0 + (i0 + i) * kStep));
                 } else {
 #pragma unroll 1
                     for (int i = 0; i < 8; i++) {
-                        const T *src = source(i);
+                        const T *from = source(row0 + (i0 + i) * kStep);
                         float u[8];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) u[e] = to_f32(src[e]);
+                        for (int e = 0; e < 8; e++) u[e] = to_f32(from[e]);
 #pragma unroll
                         for (int k = 0; k < 8; k++)
                             if (k == i) x[k].set(u);
@@ -405,10 +391,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    if (row0 + (i0 + i) * (32 / kPer) >= rows) x[i].zero();
+                    if (row0 + (i0 + i) * kStep >= rows) x[i].zero();
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const int row = row0 + (i0 + i) * (32 / kPer);
+                    const int row = row0 + (i0 + i) * kStep;
                     float down = 1.0f;
                     if constexpr (std::is_same_v<T, __nv_bfloat16>) {
                         float top = 0.0f;
@@ -501,10 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 if (32 * q + i < from || 32 * q + i >= to) y.x = -INFINITY;
                                 if (32 * q + i + 1 < from || 32 * q + i + 1 >= to) y.y = -INFINITY;
                             }
-                            if (!kPart && i / 2 % kEvery == kEvery - 1)
-                                y = exp2_fma(y);
-                            else
-                                y.x = ex2_approx(y.x), y.y = ex2_approx(y.y);
+                            y.x = ex2_approx(y.x), y.y = ex2_approx(y.y);
                             sum = __fadd2_rn(sum, y);
                             w[i / 2] = pack2<__half>(y.x, y.y);
                         }
