@@ -370,46 +370,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                 while (in >= p.group) in -= p.group, token++;
                 return src;
             };
-            src = (const T *)p.q + (size_t)(r.row0 + token_of(0)) * p.q_pitch + (size_t)(head * p.group + first % p.group) * D;
-#pragma unroll
-            for (int i0 = 0; i0 < kPer; i0 += 8) {
-                Raw<T, 8> x[8];
+            src = (const T *)p.q + (size_t)(r.row0 + token_of(0)) * p.q_pitch + (size_t)(head * p.group + first % p.group) * D + 8 * piece;
+            // all of a lane's pieces at once to their places (by way of registers, four or eight in flight,
+            // they took 7000 cycles), bf16 rows turned into f16 there
+            auto place = [&](int row) { return smem + q_at + t * kQOperand + (piece / 8) * kQHalf + swizzled(row & 127, piece & 7); };
+#pragma unroll 4
+            for (int i = 0; i < kPer; i++) {
+                const int row = row0 + i * kStep;
+                const T *from = source(row);
                 if (p.vec) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i].load(source(row0 + (i0 + i) * kStep));
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place(row)), "l"(from) : "memory");
                 } else {
-#pragma unroll 1
-                    for (int i = 0; i < 8; i++) {
-                        const T *from = source(row0 + (i0 + i) * kStep);
-                        float u[8];
+                    Raw<T, 8> x;
+                    float u[8];
 #pragma unroll
-                        for (int e = 0; e < 8; e++) u[e] = to_f32(from[e]);
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            if (k == i) x[k].set(u);
-                    }
+                    for (int e = 0; e < 8; e++) u[e] = to_f32(from[e]);
+                    x.set(u);
+                    sts_v4(place(row), make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]));
                 }
+            }
+            asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll 1
+                for (int i0 = 0; i0 < kPer; i0 += 4) {
+                    Raw<T, 8> x[4];
+                    float top[4];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (row0 + (i0 + i) * kStep >= rows) x[i].zero();
+                    for (int i = 0; i < 4; i++) {
+                        const uint4 v = lds_v4(place(row0 + (i0 + i) * kStep));
+                        x[i].w[0] = v.x, x[i].w[1] = v.y, x[i].w[2] = v.z, x[i].w[3] = v.w, top[i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int row = row0 + (i0 + i) * kStep;
-                    float down = 1.0f;
-                    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-                        float top = 0.0f;
+                        for (int e = 0; e < 8; e++) top[i] = fmaxf(top[i], fabsf(x[i].get(e)));
+                    }
 #pragma unroll
-                        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i].get(e)));
+                    for (int o = kPer / 2; o; o >>= 1)
 #pragma unroll
-                        for (int o = kPer / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        const int e = query_exponent(top);
-                        down = kv_pow2(-e);
+                        for (int i = 0; i < 4; i++) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int row = row0 + (i0 + i) * kStep, e = query_exponent(top[i]);
+                        const float down = kv_pow2(-e);
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) w[k] = pack2<__half>(x[i].get(2 * k) * down, x[i].get(2 * k + 1) * down);
+                        sts_v4(place(row), make_uint4(w[0], w[1], w[2], w[3]));
                         if (piece == 0) row_scale[row] = kv_pow2(e);
                     }
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) w[e] = pack2<__half>(x[i].get(2 * e) * down, x[i].get(2 * e + 1) * down);
-                    sts_v4(smem + q_at + t * kQOperand + (piece / 8) * kQHalf + swizzled(row & 127, piece & 7), make_uint4(w[0], w[1], w[2], w[3]));
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
