@@ -32,7 +32,7 @@ struct HeadParams {
     int hq, hk, d, rot, norm;
     float eps, inv_d;
     int group, chunk, chunks;  // lanes of a head, head groups of a warp, warps of a row
-    bool neighbours, vec, whole;  // whole: heads turn whole
+    bool neighbours, whole;  // whole: heads turn whole
 };
 
 __device__ __forceinline__ void turn_f32(uint64_t freq, int64_t position, float &c, float &s) {
@@ -346,9 +346,9 @@ __device__ __forceinline__ float round_to_odd(double v) {
     return __uint_as_float(__float_as_uint(f) | (uint32_t)((__double2loint(v) & 0x1FFFFFFF) != 0));
 }
 
-template <typename T, int E>
-__device__ __forceinline__ void load_values(const T *p, bool vec, float (&v)[E]) {
-    if (vec) {
+template <typename T, int E, bool kVec>
+__device__ __forceinline__ void load_values(const T *p, float (&v)[E]) {
+    if constexpr (kVec) {
         Raw<T, E> r;
         r.load(p);
 #pragma unroll
@@ -391,7 +391,7 @@ __device__ __forceinline__ uint32_t seq_and_place(const Seqs &q, uint32_t w, uin
     return w / each;
 }
 
-template <typename T, int E, int QE, int QJ>
+template <typename T, int E, int QE, int QJ, bool kVec>
 __global__ void __launch_bounds__(512)
     k_append(const __grid_constant__ HeadParams p, const __grid_constant__ KvCache c, const __grid_constant__ Seqs q,
              const uint32_t page_blocks, const uint32_t each_rows, const uint32_t each_pages, int32_t *err) {
@@ -429,14 +429,16 @@ __global__ void __launch_bounds__(512)
     const int w0 = (int)begin + warp * kWarpTokens;  // the warp's first token
     const Slot<E> slot(lane, p.rot, p.neighbours);
     const T *const kp = (const T *)p.k + (size_t)head * p.d, *const vp = (const T *)p.v + (size_t)head * p.d;
-    // the rows of a token of the warp; those that are not its own are not looked at
-    auto row_of = [&](int t) { return (size_t)r.row0 + (t - (r.len - r.n)); };
     const uint32_t page = seq_page(q, c, s, (uint32_t)(begin >> shift), err);
     uint8_t *const scale = c.s + kv_block(c, page, head) * 2;
     const bool has_old = t0 > begin;
     const int k_old = has_old ? kv_exponent(scale[0]) : kKvMinExp, v_old = has_old ? kv_exponent(scale[1]) : kKvMinExp;
     uint8_t *const kc = kv_codes(c.k, c, page, head), *const vc = kv_codes(c.v, c, page, head);
     const int from = max(w0, t0), to = min(w0 + kWarpTokens, t1);
+    // the lane's places in the rows of the warp's first token
+    const size_t row = (size_t)r.row0 + (from - (r.len - r.n));
+    const T *const ka = kp + row * p.k_pitch + slot.a, *const va = vp + row * p.v_pitch + 2 * E * lane;
+    const int half = slot.b - slot.a;
     float kmax = 0.0f, vmax = 0.0f;
     uint32_t poison = 0;
     if (from < to) {
@@ -460,16 +462,14 @@ __global__ void __launch_bounds__(512)
             float kv[kBatch][2 * E], vv[kBatch][2 * E];
 #pragma unroll
             for (int i = 0; i < kBatch; i++) {
-                const size_t row = row_of(min(t4 + i, to - 1));
+                const uint32_t n = (uint32_t)(min(t4 + i, to - 1) - from);
+                const T *const k = ka + n * p.k_pitch;
                 float lo[E], hi[E];
-                load_values<T, E>(kp + row * p.k_pitch + slot.a, p.vec, lo);
-                load_values<T, E>(kp + row * p.k_pitch + slot.b, p.vec, hi);
+                load_values<T, E, kVec>(k, lo);
+                load_values<T, E, kVec>(k + half, hi);
 #pragma unroll
                 for (int j = 0; j < E; j++) kv[i][j] = lo[j], kv[i][E + j] = hi[j];
-                load_values<T, E>(vp + row * p.v_pitch + 2 * E * lane, p.vec, lo);
-                load_values<T, E>(vp + row * p.v_pitch + 2 * E * lane + E, p.vec, hi);
-#pragma unroll
-                for (int j = 0; j < E; j++) vv[i][j] = lo[j], vv[i][E + j] = hi[j];
+                load_values<T, 2 * E, kVec>(va + n * p.v_pitch, vv[i]);
             }
             // the batch's tokens side by side (one after the other each waited for its own sums; what
             // lies behind the last is computed too, and left)
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(512)
                 const bool number = __all_sync(0xffffffffu, ok);
                 if (in && number) kmax = fmaxf(kmax, km), vmax = fmaxf(vmax, vm);
                 if (in && !number) poison |= 1u << (t - w0);
-                float *const place = keys + (t - (int)begin) * p.d + lane * 2 * E;
+                float *const place = keys + (uint32_t)(t - (int)begin) * (64 * E) + lane * 2 * E;
 #pragma unroll
                 for (int j = 0; j < 2 * E; j++)
                     if (in) place[j] = y[j];
@@ -565,21 +565,19 @@ __global__ void __launch_bounds__(512)
         }
 #pragma unroll 4
     for (int t = from; t < to; t++) {
-        uint8_t *const kr = kc + (t - (int)begin) * p.d, *const vr = vc + (t - (int)begin) * p.d;
+        const uint32_t in = (uint32_t)(t - (int)begin) * (64 * E);
+        uint8_t *const kr = kc + in, *const vr = vc + in;
         const bool bad = poison >> (t - w0) & 1;
-        const float *const place = keys + (t - (int)begin) * p.d + lane * 2 * E;
-        const T *const v = vp + row_of(t) * p.v_pitch + 2 * E * lane;
+        const float *const place = keys + in + lane * 2 * E;
         float lo[E], hi[E], all[2 * E];
 #pragma unroll
         for (int j = 0; j < E; j++) {
             lo[j] = bad ? __uint_as_float(0x7FC00000u) : place[j] * k_inv;
             hi[j] = bad ? __uint_as_float(0x7FC00000u) : place[E + j] * k_inv;
         }
-        float v0[E], v1[E];
-        load_values<T, E>(v, p.vec, v0);
-        load_values<T, E>(v + E, p.vec, v1);
+        load_values<T, 2 * E, kVec>(va + (uint32_t)(t - from) * p.v_pitch, all);
 #pragma unroll
-        for (int j = 0; j < E; j++) all[j] = bad ? 0.0f : v0[j] * v_inv, all[E + j] = bad ? 0.0f : v1[j] * v_inv;
+        for (int j = 0; j < 2 * E; j++) all[j] = bad ? 0.0f : all[j] * v_inv;
         store_codes<E>(kr + slot.a, lo);
         store_codes<E>(kr + slot.b, hi);
         store_codes<2 * E>(vr + 2 * E * lane, all);
@@ -699,7 +697,7 @@ dw_status norm_rope(dw_backend *be, HeadParams p, const HeadArgs &a) {
 
 template <typename T, int E>
 dw_status append(dw_backend *be, HeadParams p, const KvCache &c, const Seqs &s, const HeadArgs &a) {
-    p.vec = aligned(a.k, sizeof(T), E * sizeof(T)) && aligned(a.v, sizeof(T), E * sizeof(T));
+    const bool vec = aligned(a.k, sizeof(T), E * sizeof(T)) && aligned(a.v, sizeof(T), 2 * E * sizeof(T));
     const unsigned threads = (unsigned)(c.page / kWarpTokens * 32);
     // pages that n rows can lie in, from anywhere in the first
     const size_t n = s.tokens / s.seqs, each = (n + c.page - 2) / c.page + 1;
@@ -724,9 +722,9 @@ dw_status append(dw_backend *be, HeadParams p, const KvCache &c, const Seqs &s, 
         return launch_dependent(be, "append_kv", kernel, (unsigned)blocks, threads, smem, 0, p, c, s, (uint32_t)pages, (uint32_t)n,
                                 (uint32_t)each, be->dev_err);
     };
-    if (wide<T>(p, {a.q, a.q_out}) && p.whole) return go(k_append<T, E, kWide<T>, 0>, kWide<T>, 1);
-    if (wide<T>(p, {a.q, a.q_out})) return go(k_append<T, E, kWide<T>, 1>, kWide<T>, 1);
-    return go(k_append<T, E, 1, E>, 1, E);
+    if (vec && wide<T>(p, {a.q, a.q_out}) && p.whole) return go(k_append<T, E, kWide<T>, 0, true>, kWide<T>, 1);
+    if (vec && wide<T>(p, {a.q, a.q_out})) return go(k_append<T, E, kWide<T>, 1, true>, kWide<T>, 1);
+    return go(k_append<T, E, 1, E, false>, 1, E);
 }
 
 }  // namespace
