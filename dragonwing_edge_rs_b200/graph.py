@@ -49,7 +49,9 @@ class CompiledOp:
     Resize, QuantizeU8, Dequantize, YoloDetect (the Detect head's tail),
     YoloPostprocess (postprocess_yolo), the fp16 ops, and the 4-bit block's:
     NormResidual, QuantizeMxfp4, DequantizeMxfp4 and GemmMxfp4 (an MXFP4 operand is a pair of
-    u8 tensors, codes and scales)."""
+    u8 tensors, codes and scales), and those of its attention: AppendKv and AttentionKv8 (a paged
+    cache is three u8 tensors, codes of keys and values and scales; sequences are two or three
+    i32 ones, table, lens and starts)."""
 
     name: str
     op_type: str
@@ -404,6 +406,62 @@ class F16GraphBuilder:
         residual, a = self.norm_residual(x, residual, post, quantized=True)
         h = self.gemm_mxfp4(a, rows, c, f, act=L.EPI_SILU, quantized=True)
         return self.gemm_mxfp4(h, rows, f, c), residual
+
+    # ---- attention over a paged 8-bit cache: packed rows [rows, (hq + 2 hk) * d] of f16
+    def kv_cache(self, name, pages, kv_heads, page_tokens, head_dim):
+        """A cache as graph inputs (state that stays between runs; graphs that share it are given its buffers):
+        (codes of keys, of values, scales)."""
+        codes = (pages, kv_heads, page_tokens, head_dim)
+        cache = tuple(self.g.add_tensor(f"{name}_{t}", s, "u8") for t, s in (("k", codes), ("v", codes), ("s", (pages, kv_heads, 2))))
+        self.g.inputs += cache
+        return cache
+
+    def sequences(self, name, seqs, width, ragged=False):
+        """The sequences of the rows as graph inputs: their pages [seqs, width], lengths [seqs] and, where they have
+        different numbers of rows, where those start [seqs + 1]."""
+        shapes = {"table": (seqs, width), "lens": (seqs,)}
+        if ragged:
+            shapes["starts"] = (seqs + 1,)
+        out = tuple(self.g.add_tensor(f"{name}_{t}", s, "i32") for t, s in shapes.items())
+        self.g.inputs += out
+        return out
+
+    def append_kv(self, qkv, cache, seqs, hq, norm=L.NORM_RMS, theta=10000.0, rot=None, neighbours=False, eps=1e-5, name=None):
+        """Keys (normed, turned) and values of packed rows into the cache; the queries, normed and turned."""
+        g = self.g
+        name = name or self._name("append")
+        _, hk, _, d = g.tensors[cache[0]].shape
+        rows = g.tensors[qkv].shape[0]
+        rot = d if rot is None else rot
+        for tag in ("_wq", "_wk") if norm != L.NORM_NONE else ():
+            g.initializers[name + tag] = self.rng.normal(1.0, 0.1, d).astype(np.float32)
+        q = g.add_tensor(name + "_q", (rows, hq * d), "f16")
+        g.ops.append(CompiledOp(name, "AppendKv", [qkv, *cache, *seqs], [q],
+                                {"hq": hq, "norm": norm, "rot": rot, "theta": theta, "neighbours": neighbours, "eps": eps}))
+        return q
+
+    def attention_kv8(self, q, cache, seqs, scale=None, causal=True, window=0, name=None):
+        """Attention of the query rows over their sequences' cached tokens."""
+        g = self.g
+        name = name or self._name("attention")
+        d = g.tensors[cache[0]].shape[3]
+        rows, width = g.tensors[q].shape
+        y = g.add_tensor(name + "_out", (rows, width), "f16")
+        g.ops.append(CompiledOp(name, "AttentionKv8", [q, *cache, *seqs], [y],
+                                {"hq": width // d, "scale": d ** -0.5 if scale is None else scale, "causal": causal, "window": window}))
+        return y
+
+    def attention_mxfp4(self, x, residual, cache, seqs, hq, post=L.NORM_NONE, norm=L.NORM_RMS, window=0):
+        """An attention block: x (the branch before) joins the residual, is normalised and quantised, goes through
+        the packed projection, the cache and attention, and is quantised again for the projection back:
+        (branch, residual)."""
+        g = self.g
+        rows, c = g.tensors[x].shape
+        _, hk, _, d = g.tensors[cache[0]].shape
+        residual, a = self.norm_residual(x, residual, post, quantized=True)
+        qkv = self.gemm_mxfp4(a, rows, c, (hq + 2 * hk) * d)
+        y = self.attention_kv8(self.append_kv(qkv, cache, seqs, hq, norm), cache, seqs, window=window)
+        return self.gemm_mxfp4(self.quantize_mxfp4(y), rows, hq * d, c), residual
 
     def output_f32(self, x, name):
         g = self.g
@@ -1175,7 +1233,8 @@ class CudaGraphRuntime:
     """Executes a Graph on one GPU (VulkanGraphRuntime::new / set_input_bytes /
     run / get_output_bytes, vulkan_runtime.rs:115, 359)."""
 
-    def __init__(self, graph: Graph, backend: CudaBackend, fuse: bool = True, residual_i8: bool = False):
+    def __init__(self, graph: Graph, backend: CudaBackend, fuse: bool = True, residual_i8: bool = False, buffers=None):
+        """buffers: CudaBuffers of other owners for tensors, by name (a cache that several graphs share)."""
         if fuse:
             graph = lower_for_device(graph, residual_i8=residual_i8)
         self.graph = graph
@@ -1185,8 +1244,11 @@ class CudaGraphRuntime:
         self._cgraph = None
         self._slot_graphs = []
         for name, t in graph.tensors.items():
+            given = (buffers or {}).get(name)
+            if given is not None and (name in graph.views or given.len_bytes() != t.nbytes):
+                raise BackendError(L.DW_ERR_SIZE_MISMATCH, f"buffer given for {name}: {given.len_bytes()} bytes, not {t.nbytes}")
             if name not in graph.views:
-                self.bufs[name] = backend.alloc(t.nbytes)
+                self.bufs[name] = given if given is not None else backend.alloc(t.nbytes)
         consts = {}
         for name, arr in graph.initializers.items():
             consts[name] = backend.upload_array(np.ascontiguousarray(arr))
@@ -1382,6 +1444,25 @@ class CudaGraphRuntime:
             y = [bufs[o] for o in op.outputs[1:]]
             fn = ops.norm_residual_to_mxfp4 if len(y) == 2 else ops.norm_residual
             return lambda: fn(be, desc, x, w0, None, None, r, out, w1, None, *y)
+        if t in ("AppendKv", "AttentionKv8"):
+            pr, T = op.params, self.graph.tensors
+            x, (k, v, s), seqs = op.inputs[0], op.inputs[1:4], op.inputs[4:]
+            pages, hk, page, d = T[k].shape
+            cache = ops.KvCache(bufs[k], bufs[v], bufs[s], pages, hk, page, d)
+            rows, (n, width) = T[x].shape[0], T[seqs[0]].shape
+            sq = ops.Sequences(bufs[seqs[0]], bufs[seqs[1]], bufs[seqs[2]] if len(seqs) > 2 else None, n, rows, width)
+            y = ops.Heads(bufs[op.outputs[0]])
+            if t == "AttentionKv8":
+                desc = ops.AttentionDesc(pr["hq"], ops.F16, pr["scale"], pr["causal"], pr["window"])
+                q = ops.Heads(bufs[x])
+                return lambda: ops.attention_kv8(be, desc, cache, sq, q, y)
+            rot, pitch = pr["rot"], T[x].shape[1]
+            desc = ops.HeadDesc(pr["hq"], hk, d, rot, ops.F16, pr["norm"], pr["eps"], pr["neighbours"])
+            rope = self._cached(op.name + "_rope", lambda: ops.prepare_rope(
+                be, pr["theta"] ** (-2.0 * np.arange(rot // 2) / rot))) if rot else None
+            q, hs, vs = (ops.Heads(bufs[x], o * d, pitch) for o in (0, pr["hq"], pr["hq"] + hk))
+            wq, wk = consts.get(op.name + "_wq"), consts.get(op.name + "_wk")
+            return lambda: ops.append_kv(be, desc, cache, sq, hs, vs, wk, rope, q, wq, y)
         if t == "CastF16ToF32":
             x, y = bufs[op.inputs[0]], bufs[op.outputs[0]]
             return lambda: ops.cast_f16_to_f32(be, x, y)
