@@ -33,43 +33,7 @@ namespace {
 
 constexpr int kTile = 32;  // tokens of a tile
 constexpr int kStages = 2;
-constexpr unsigned kMaxShare = 8;  // CTAs that share a sequence
 constexpr float kHead = 11.0f, kLag = 4.0f;
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void cluster_sync_relaxed() {
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ float ld_peer(const float *p, uint32_t rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_addr(p, rank)) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 ld_peer4(const float *p, uint32_t rank) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(peer_addr(p, rank))
-                 : "memory");
-    return v;
-}
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -447,22 +411,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2
     cluster_sync();
     for (int i = (int)rank * kWarps * 32 + threadIdx.x; i < rows * kQuads; i += (int)S * kWarps * 32) {
         const int row = i / kQuads, at = i % kQuads * 4;
-        // all at once: one after the other they took 2000 cycles
-        float pm[kMaxShare], pl[kMaxShare], m = -INFINITY, l = 0.0f;
-        float4 pv[kMaxShare], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (uint32_t k = 0; k < kMaxShare; k++)
-            if (k < S) pm[k] = ld_peer(all_m + row, k), pl[k] = ld_peer(all_l + row, k), pv[k] = ld_peer4(part0 + row * D + at, k);
-#pragma unroll
-        for (uint32_t k = 0; k < kMaxShare; k++)
-            if (k < S) m = fmaxf(m, pm[k]);
-#pragma unroll
-        for (uint32_t k = 0; k < kMaxShare; k++) {
-            if (k >= S) continue;
-            const float f = carry(pm[k], m);
-            l = fmaf(pl[k], f, l);
-            v.x = fmaf(pv[k].x, f, v.x), v.y = fmaf(pv[k].y, f, v.y), v.z = fmaf(pv[k].z, f, v.z), v.w = fmaf(pv[k].w, f, v.w);
-        }
+        float l;
+        const float4 v = join_sums(all_m + row, all_l + row, part0 + row * D + at, S, l);
         store(row, at, v, l);
     }
     cluster_sync_relaxed();  // no CTA leaves while its sums may be read
@@ -490,27 +440,36 @@ dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Se
     const size_t items = s.starts ? seq_items(s.tokens, s.seqs, p.group, R, 1) : (size_t)p.per_seq * s.seqs, units = items * c.heads;
     if (units * kMaxShare > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "attention_kv8: too many rows");
     p.items = (uint32_t)items;
-    // S CTAs share a unit's tiles (as many as the longest sequence can have), each with a tile a warp at least.
-    // Few units: CTAs of eight warps, one an SM (one token, 8 heads, 32000 tokens 24 us, by four warps 29; 8
-    // sequences of up to 2000 tokens 10.2 and 11.1).
-    // More: CTAs of four, until the GPU is full (16 sequences of up to 4000 tokens with 20 rows: S = 1, 2, 4, 8
-    // 49.9, 40.1, 43.8, 60 us), and with few rows beyond, for the balance of long and short sequences, while a
-    // warp keeps six tiles (64 sequences of up to 8192: 1, 2, 4 105.8, 95.7, 93.9).
+    // S CTAs share a unit's tiles (`most`: as many as the longest sequence can have).  While an SM for each unit is
+    // there: CTAs of eight warps, as many as SMs, each with a tile a warp at least (one row, 8 heads: over 8000
+    // tokens S = 1, 2, 4, 8 38, 23, 15, 11 us; 8 sequences of 4000 22, 16.6, 23, 39, by four warps 28, 19, 20,
+    // 25; 16 sequences 25, 32, 42, 70, by four warps 30, 32, 37, 38).
+    // More units: CTAs of four warps, several an SM.  With few rows they too share, for the balance of long and
+    // short sequences, while a warp keeps twelve tiles of the longest (64 sequences of up to 8192: 105, 96, 94, 126
+    // us, by eight warps 98, 107, 153, 270; 32 of 2000 31, 36, 37, 50, by eight 30, 41, 62, 115).
     const size_t most = ((size_t)s.width * c.page + kTile - 1) / kTile;
     unsigned S = 1;
-    if (units * 2 <= sms) {
+    if (units <= sms) {
         while (S < kMaxShare && units * 2 * S <= sms && (size_t)2 * S * 8 <= most) S *= 2;
         return launch_rows<T, D, NT, 8>(be, p, c, s, units, S);
     }
-    const size_t held = sms * (NT == 1 ? 3 : 2);
-    while (S < kMaxShare && (units * 2 * S <= held ? 2 * S * 4 <= most : NT == 1 && units * 2 * S <= 5 * held && 2 * S * 4 * 6 <= most)) S *= 2;
+    while (NT == 1 && S < kMaxShare && units * 2 * S <= 15 * sms && 2 * S * 4 * 12 <= most) S *= 2;
     return launch_rows<T, D, NT, 4>(be, p, c, s, units, S);
 }
 
 template <typename T, int D>
 dw_status attend(dw_backend *be, const AttendParams &p, const KvCache &c, const Seqs &s) {
     const size_t rows = (s.tokens + s.seqs - 1) / s.seqs * p.group;  // of a sequence, on average
-    if (rows > 64) return attend_prompt<T, D>(be, p, c, s);
+    // Up to 24 rows a warp has them all.  With more the cache would be read again for every 24; the
+    // kernel of many rows has 256 in a CTA, at the price of one CTA an SM and a longer start, and of
+    // the products of 128 rows, however few there are (8 heads, us, this one's first: 20 rows of 16
+    // sequences of up to 4000 tokens 40 and 75; 24 rows over 8000 tokens 19 and 22; 32 rows 35 and 22;
+    // 64 rows of 16 sequences of 1000 42 and 26; 256 rows over 8000 72 and 33).  Between 24 and 48 it
+    // gains only where CTAs are few and share the tokens (40 rows of 16 sequences of 4000 72 and
+    // 83; 48 rows of 64 of 1000 87 and 92, of one of 8000 36 and 22).
+    if (rows > 48 || (rows > 24 && s.seqs * c.heads * 2 <= (size_t)be->sm_count)) return attend_prompt<T, D>(be, p, c, s);
+    // (fewer rows than it has places cost a warp products and registers: one row of 64 sequences of up
+    // to 8192 tokens 94 us by 8 places, 129 by 16, 182 by 24; 8 rows over 8000 tokens 11.1, 13.9, 18.2)
     if (rows <= 8) return attend_rows<T, D, 1>(be, p, c, s);
     return rows <= 16 ? attend_rows<T, D, 2>(be, p, c, s) : attend_rows<T, D, 3>(be, p, c, s);
 }

@@ -13,6 +13,7 @@
 //                          S = Q K^T (128 x 64 x d) into tensor memory, O += P V with P from
 //                          tensor memory and V as it lies (tokens x values);
 //   2 x 4 softmax warps    a thread a row: S -> weights (f16, over S) and their sum.
+// Where units (a CTA's rows and a cache head) are few, the CTAs of a cluster share their tokens.
 // Tensor memory holds O of both row tiles (256 columns) and two S of each: the next logits are
 // there when a tile's weights are done.  (Tiles of 128 tokens leave room for one S of each; a
 // row tile then waited for its own products, 1450 of 4700 cycles.)
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ uint64_t q_full[2], s_full[2][2], p_full[2][2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], drain[2];
     __shared__ float4 scales[8][kGroups];  // of eight tiles: 2^ek, ev, 2^-ev
-    __shared__ float row_scale[kRows];
+    __shared__ float row_scale[kRows], all_m[kRows], all_l[kRows];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int *abort_flag = &abort_word;
@@ -166,8 +167,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     pdl_wait();
     // which rows of which sequence, which head: those that see most first
-    const uint32_t unit = blockIdx.x / (uint32_t)c.heads;
-    const int head = (int)(blockIdx.x % (uint32_t)c.heads);
+    const uint32_t S = cluster_size(), rank = cluster_rank(), block = blockIdx.x / S;
+    const uint32_t unit = block / (uint32_t)c.heads;
+    const int head = (int)(block % (uint32_t)c.heads);
     int64_t place;
     uint32_t s;
     if (p.per_seq) {
@@ -184,13 +186,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rows = min(kRows, rows_all - first);
     auto token_of = [&](int row) { return (first + row) / p.group; };
     const int lo = row_bounds(p, r, token_of(0)).lo;
-    const int tile0 = lo / kTile;
+    int tile0 = lo / kTile;
     // tiles of either row tile: up to the last token that its last row sees
     int tiles[2];
 #pragma unroll
     for (int t = 0; t < 2; t++) {
         const int hi = rows > t * 128 ? row_bounds(p, r, token_of(min(rows, t * 128 + 128) - 1)).hi : 0;
         tiles[t] = max(0, (hi + kTile - 1) / kTile - tile0);
+    }
+    if (S > 1) {  // this CTA's share of them
+        const int share = (max(tiles[0], tiles[1]) + (int)S - 1) / (int)S, from = (int)rank * share;
+        tile0 += from;
+#pragma unroll
+        for (int t = 0; t < 2; t++) tiles[t] = min(max(tiles[t] - from, 0), share);
     }
     const int all = max(tiles[0], tiles[1]);
 
@@ -217,6 +225,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_trigger();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);  // two S of 64 columns of each row tile, then O
 
+    // a softmax thread's row: sums, maximum (as the last phase needs them)
+    float M = -INFINITY, L = 0.0f;
+    bool ok = true;
     if (warp >= 12) {
         // ---- converters: a thread has 16 codes of each half of a row in each of two groups of 32 rows
         const int tid = threadIdx.x - 384, part = tid & 3, sub = tid >> 2;
@@ -313,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
         constexpr uint64_t hi = ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
         auto phase = [](int j) { return (uint32_t)(j / kStages) & 1; };
-        bool ok = !tiles[t] || wait_warp(&q_full[t], 0, p, abort_flag, 73);
+        ok = !tiles[t] || wait_warp(&q_full[t], 0, p, abort_flag, 73);
         for (int j = -2; j < all && ok; j++) {
             const int k = j + 2;
             const bool sums = j >= 0 && j < tiles[t], logits = k < tiles[t];
@@ -425,8 +436,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t s0_tm = tmem + 2 * t * kTile + lanes, o_tm = tmem + 256 + t * D + lanes;
         // tokens that all of the warp's rows see, and those that any does
         const int lo_all = __reduce_max_sync(0xffffffffu, b.lo), hi_all = __reduce_min_sync(0xffffffffu, b.hi);
-        float M = -INFINITY, L = 0.0f;
-        bool ok = true;
         for (int j = 0; j < tiles[t]; j++) {
             const int t0 = (tile0 + j) * kTile;
             if (!wait_warp(&s_full[t][j & 1], (uint32_t)(j >> 1) & 1, p, abort_flag, 77)) {
@@ -505,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) mbar_arrive(smem_u32(&p_full[t][j & 1]));
         }
         if (tiles[t] && ok) ok = wait_warp(&s_full[t][(tiles[t] + 1) & 1], (uint32_t)((tiles[t] + 1) >> 1) & 1, p, abort_flag, 78);
-        if (ok && rows > t * 128 + (warp & 3) * 32) {
+        if (ok && rows > t * 128 + (warp & 3) * 32 && S == 1) {
             tc_fence_after();
             const float f = L == 0.0f ? 0.0f : 1.0f / L;
             T *dst = (T *)p.out + (size_t)(r.row0 + token) * p.out_pitch + (size_t)(head * p.group + at % p.group) * D;
@@ -537,6 +546,49 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
+    if (S > 1) {
+        // ---- join: each CTA leaves its sums in shared memory, over its queries and stages
+        float *const part = reinterpret_cast<float *>(base);  // [256][D], a row's 16-byte pieces xor the row modulo 8
+        auto piece_at = [&](int row, int piece) { return part + row * D + (piece ^ (row & 7)) * 4; };
+        __syncthreads();  // all products are done
+        if (warp >= 4 && warp < 12) {
+            const int t = (warp - 4) >> 2, row = t * 128 + (warp & 3) * 32 + lane;
+            all_m[row] = M, all_l[row] = L;
+            tc_fence_after();
+            if (tiles[t]) {
+#pragma unroll
+                for (int q = 0; q < D / 32; q++) {
+                    float x[32];
+                    tm_ld32(tmem + 256 + t * D + ((uint32_t)((warp & 3) * 32) << 16) + q * 32, x);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        *reinterpret_cast<float4 *>(piece_at(row, q * 8 + i)) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                }
+            } else {
+#pragma unroll 4
+                for (int i = 0; i < D / 4; i++) *reinterpret_cast<float4 *>(piece_at(row, i)) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+        cluster_sync();
+        for (int i = (int)rank * kThreads + threadIdx.x; i < rows * (D / 4); i += (int)S * kThreads) {
+            const int row = i / (D / 4), piece = i % (D / 4);
+            float l;
+            const float4 v = join_sums(all_m + row, all_l + row, piece_at(row, piece), S, l);
+            const float f = l == 0.0f ? 0.0f : 1.0f / l, y[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+            const int at = first + row;
+            T *dst = (T *)p.out + (size_t)(r.row0 + at / p.group) * p.out_pitch + (size_t)(head * p.group + at % p.group) * D + piece * 4;
+            if (p.vec) {
+                Raw<T, 4> o;
+                o.set(y);
+                o.store(dst);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) dst[e] = from_f32<T>(y[e]);
+            }
+        }
+        cluster_sync_relaxed();  // no CTA leaves while its sums may be read
+    }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -564,7 +616,12 @@ dw_status attend_prompt(dw_backend *be, AttendParams p, const KvCache &c, const 
         if (st != DW_OK) return st;
         attr_set[be->device] = true;
     }
-    return launch_dependent(be, "attention_kv8 (prompt)", kernel, (unsigned)(items * c.heads), kThreads, smem, 0, p, c, s);
+    // S CTAs share a unit's tiles while an SM each is there and four tiles each (256 rows over 8000 tokens, 8
+    // heads: S = 1, 2, 4, 8 145, 83, 47, 33 us; 300 rows and tokens: with shares of two tiles 16.3, without 14.5)
+    const size_t units = items * c.heads, most = ((size_t)s.width * c.page + kTile - 1) / kTile;
+    unsigned S = 1;
+    while (S < kMaxShare && units * 2 * S <= (size_t)be->sm_count && 2 * S * 4 <= most) S *= 2;
+    return launch_dependent(be, "attention_kv8 (prompt)", kernel, (unsigned)(units * S), kThreads, smem, S, p, c, s);
 }
 
 template dw_status attend_prompt<__half, 64>(dw_backend *, AttendParams, const KvCache &, const Seqs &);

@@ -4,6 +4,7 @@
 #include <cstdint>
 
 #include "dw_kv.cuh"
+#include "dw_ptx.cuh"
 
 namespace dw {
 
@@ -42,6 +43,70 @@ __device__ __forceinline__ float carry(float x, float y) { return x == y ? 1.0f 
 // [2^14, 2^15): nothing overflows and what falls below f16's smallest step is 2^-39 of it.
 __device__ __forceinline__ int query_exponent(float top) {
     return min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -126), 126);
+}
+
+// ---- sums of several CTAs -----------------------------------------------------------
+// The CTAs of a cluster go through shares of a sequence's tokens and join their sums through
+// shared memory, in the order of their ranks.
+constexpr unsigned kMaxShare = 8;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float ld_peer(const float *p, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_addr(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_peer4(const float *p, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(peer_addr(p, rank))
+                 : "memory");
+    return v;
+}
+
+
+// Four values of a row's sum, and what to divide them by, over all CTAs: each has a maximum, the
+// sum of the weights and sums of the values at these places.  (All loads at once: one after the
+// other they took 2000 cycles.)
+__device__ __forceinline__ float4 join_sums(const float *m_at, const float *l_at, const float *v_at, uint32_t S, float &l) {
+    float pm[kMaxShare], pl[kMaxShare], m = -INFINITY;
+    float4 pv[kMaxShare], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (uint32_t k = 0; k < kMaxShare; k++)
+        if (k < S) pm[k] = ld_peer(m_at, k), pl[k] = ld_peer(l_at, k), pv[k] = ld_peer4(v_at, k);
+#pragma unroll
+    for (uint32_t k = 0; k < kMaxShare; k++)
+        if (k < S) m = fmaxf(m, pm[k]);
+    l = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < kMaxShare; k++) {
+        if (k >= S) continue;
+        const float f = carry(pm[k], m);
+        l = fmaf(pl[k], f, l);
+        v.x = fmaf(pv[k].x, f, v.x), v.y = fmaf(pv[k].y, f, v.y), v.z = fmaf(pv[k].z, f, v.z), v.w = fmaf(pv[k].w, f, v.w);
+    }
+    return v;
 }
 
 // attention_prompt.cu

@@ -113,6 +113,19 @@ def test_prompts(be, dtype, page, d, hk, group, lens, n):
         attend(t, hk * group, dtype, n, causal=False, gap=16)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("page,d,hk,group,lens,n", [(64, 128, 1, 4, [4000], [70]), (16, 64, 2, 5, [1500], [60]), (32, 128, 1, 3, [2100, 900, 65], [20, 100, 61]),
+                                                    (128, 64, 1, 1, [3000, 40], [257, 3]), (64, 128, 1, 1, [600], [49])])
+def test_pieces_of_prompts_behind_long_caches(be, dtype, page, d, hk, group, lens, n):
+    """Few blocks of many rows: the CTAs of a cluster share a block's tokens, some with tiles of one half of the rows
+    alone or with none."""
+    t = filled(be, page + d + len(n), lens, hk, page, d)
+    attend(t, hk * group, dtype, n, in_place=True)
+    attend(t, hk * group, dtype, n, uniform=len(n) == 1, gap=5, offset=3, in_place=True)
+    attend(t, hk * group, dtype, n, window=300, extra=2)
+    attend(t, hk * group, dtype, n, causal=False, gap=8)
+
+
 def test_more_rows_than_tokens(be):
     """Rows before the first position see nothing."""
     t = filled(be, 1, [3, 0, 70], 1, 16, 64)
