@@ -444,12 +444,15 @@ dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Se
     // there: CTAs of eight warps, as many as SMs, each with a tile a warp at least (one row, 8 heads: over 8000
     // tokens S = 1, 2, 4, 8 38, 23, 15, 11 us; 8 sequences of 4000 22, 16.6, 23, 39, by four warps 28, 19, 20,
     // 25; 16 sequences 25, 32, 42, 70, by four warps 30, 32, 37, 38).
-    // More units: CTAs of four warps, several an SM.  With few rows they too share, for the balance of long and
-    // short sequences, while a warp keeps twelve tiles of the longest (64 sequences of up to 8192: 105, 96, 94, 126
-    // us, by eight warps 98, 107, 153, 270; 32 of 2000 31, 36, 37, 50, by eight 30, 41, 62, 115).
+    // With few rows the same up to two units an SM (32 sequences of up to 2000 22.4, of 2000 29.9; by four warps
+    // 26.3 and 30.5, two sharing 21.9 and 35.9); with more they fall behind (32 sequences of 2000, 16 rows each 37,
+    // by four warps 31).
+    // More units: CTAs of four warps, several an SM.  With few rows they share too, for the balance of long and
+    // short sequences, while a warp keeps twelve tiles of the longest (64 sequences of up to 8192: 106, 95, 94, 126
+    // us, by eight warps 98, 107, 153, 270).
     const size_t most = ((size_t)s.width * c.page + kTile - 1) / kTile;
     unsigned S = 1;
-    if (units <= sms) {
+    if (units <= (NT == 1 ? 2 : 1) * sms) {
         while (S < kMaxShare && units * 2 * S <= sms && (size_t)2 * S * 8 <= most) S *= 2;
         return launch_rows<T, D, NT, 8>(be, p, c, s, units, S);
     }
