@@ -92,8 +92,8 @@ __device__ __forceinline__ void norm_rope_row(const HeadParams &p, size_t row, i
         live[j] = 2 * E * c < p.d;
         a[j] = slot.a, b[j] = slot.b, turns[j] = slot.turns && live[j];
     }
-    // Two groups' values are on their way while one is computed (with one the loads in flight were
-    // too few: 8192 x 40 heads of 128 bf16 49.6 us).
+    // Two groups' values are on their way while one is computed (8192 x 40 heads of 128 bf16 49.3 us,
+    // 49.6 with one: the instructions are the bound).
     struct Group {
         Raw<T, E> a[J], b[J];
     } g0, g1;
@@ -190,10 +190,12 @@ __device__ __forceinline__ void norm_rope_row(const HeadParams &p, size_t row, i
     }
 }
 
+constexpr int kAhead = 4;
+
 // The same for heads that turn whole and fill their lanes (d = 2 E * 32 / kPer; kPer heads a
 // group): a lane keeps the products of weights and angles, so that a value is
 // rstd * (a * (w_a cos) - b * (w_b sin)), and finds one in kPer of its angles, the others by
-// shuffles.  (By norm_rope_row 8192 x 40 heads of 128 bf16 took 49 us, bound by its instructions.)
+// XX
 template <typename T, int E, int kPer>
 __device__ __forceinline__ void rope_row(const HeadParams &p, size_t row, int64_t position, int first) {
     constexpr int kGroup = 32 / kPer, kMine = E > kPer ? E / kPer : 1, kD = 2 * E * kGroup;
@@ -203,7 +205,7 @@ __device__ __forceinline__ void rope_row(const HeadParams &p, size_t row, int64_
     const int a = nb ? 2 * E * sub : E * sub, b = nb ? a + E : kD / 2 + E * sub;
     struct Group {
         Raw<T, E> a, b;
-    } g0, g1;
+    } groups[kAhead];
     // group g of the row: its heads of q, or of k
     auto place = [&](const void *q, size_t q_pitch, const void *k, size_t k_pitch, int g, bool &there) {
         const bool key = g >= qg;
@@ -216,8 +218,9 @@ __device__ __forceinline__ void rope_row(const HeadParams &p, size_t row, int64_
         const T *from = place(p.q, p.q_pitch, p.k, p.k_pitch, g, there);
         x.a.load(from + a), x.b.load(from + b);
     };
-    load(g0, first);
-    if (first + 1 < end) load(g1, first + 1);
+#pragma unroll
+    for (int n = 0; n < kAhead; n++)
+        if (first + n < end) load(groups[n], first + n);
     float mc[kMine], ms[kMine], cs[E], sn[E];
 #pragma unroll
     for (int m = 0; m < kMine; m++)
@@ -230,86 +233,84 @@ __device__ __forceinline__ void rope_row(const HeadParams &p, size_t row, int64_
     // halves: pair i is values i and E + i of a lane; neighbours: values 2 i and 2 i + 1
     auto A = [&](const float (&v)[2 * E], int i) { return nb ? v[2 * i] : v[i]; };
     auto B = [&](const float (&v)[2 * E], int i) { return nb ? v[2 * i + 1] : v[E + i]; };
-    auto some = [&](int from, int to, const float *weights) {
-        if (from >= to) return;
-        float ac[E], bs[E], as[E], bc[E];
-        {
-            float w[2 * E];
+    float ac[E], bs[E], as[E], bc[E];
+    auto weigh = [&](const float *weights) {
+        float w[2 * E];
 #pragma unroll
-            for (int i = 0; i < E; i++) w[i] = weights ? weights[a + i] : 1.0f, w[E + i] = weights ? weights[b + i] : 1.0f;
+        for (int i = 0; i < E; i++) w[i] = weights ? weights[a + i] : 1.0f, w[E + i] = weights ? weights[b + i] : 1.0f;
 #pragma unroll
-            for (int i = 0; i < E; i++) {
-                ac[i] = A(w, i) * cs[i], as[i] = A(w, i) * sn[i];
-                bc[i] = B(w, i) * cs[i], bs[i] = -(B(w, i) * sn[i]);
-            }
-        }
-        auto sum = [&](float x) {
-#pragma unroll
-            for (int o = 1; o < kGroup; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            return x;
-        };
-        auto one = [&](Group &x, int g) {
-            float v[2 * E];
-#pragma unroll
-            for (int i = 0; i < E; i++) v[i] = x.a.get(i), v[E + i] = x.b.get(i);
-            if (g + 2 < end) load(x, g + 2);
-            if (p.norm != DW_NORM_NONE) {
-                if (p.norm == DW_NORM_LAYER) {
-                    float m = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 2 * E; i++) m += v[i];
-                    m = sum(m) * p.inv_d;
-#pragma unroll
-                    for (int i = 0; i < 2 * E; i++) v[i] -= m;
-                }
-                float2 sq = make_float2(0.0f, 0.0f);
-#pragma unroll
-                for (int i = 0; i < 2 * E; i += 2) sq = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(v[i], v[i + 1]), sq);
-                const float rstd = __frsqrt_rn(fmaf(sum(sq.x + sq.y), p.inv_d, p.eps));
-#pragma unroll
-                for (int i = 0; i < 2 * E; i += 2) {
-                    const float2 r = __fmul2_rn(make_float2(v[i], v[i + 1]), make_float2(rstd, rstd));
-                    v[i] = r.x, v[i + 1] = r.y;
-                }
-            }
-            float y[2 * E];
-            auto turn = [&](auto near) {  // two pairs to an instruction
-                constexpr bool kNear = decltype(near)::value;
-#pragma unroll
-                for (int i = 0; i < E; i += 2) {
-                    const int a0 = kNear ? 2 * i : i, a1 = kNear ? 2 * i + 2 : i + 1, b0 = kNear ? 2 * i + 1 : E + i, b1 = kNear ? 2 * i + 3 : E + i + 1;
-                    const float2 va = make_float2(v[a0], v[a1]), vb = make_float2(v[b0], v[b1]);
-                    const float2 ya = __ffma2_rn(va, make_float2(ac[i], ac[i + 1]), __fmul2_rn(vb, make_float2(bs[i], bs[i + 1])));
-                    const float2 yb = __ffma2_rn(va, make_float2(as[i], as[i + 1]), __fmul2_rn(vb, make_float2(bc[i], bc[i + 1])));
-                    y[a0] = ya.x, y[a1] = ya.y, y[b0] = yb.x, y[b1] = yb.y;
-                }
-            };
-            if (nb)
-                turn(std::true_type{});
-            else
-                turn(std::false_type{});
-            bool there;
-            T *out = place(p.q_out, p.qo_pitch, p.k_out, p.ko_pitch, g, there);
-            if (!there) return;
-            float lo[E], hi[E];
-#pragma unroll
-            for (int i = 0; i < E; i++) lo[i] = y[i], hi[i] = y[E + i];
-            Raw<T, E> r;
-            r.set(lo);
-            r.store(out + a);
-            r.set(hi);
-            r.store(out + b);
-        };
-        // groups alternate between the two places, whichever of q and k they are of
-        int g = from;
-        if ((g - first) & 1) one(g1, g++);
-        while (g < to) {
-            one(g0, g++);
-            if (g < to) one(g1, g++);
+        for (int i = 0; i < E; i++) {
+            ac[i] = A(w, i) * cs[i], as[i] = A(w, i) * sn[i];
+            bc[i] = B(w, i) * cs[i], bs[i] = -(B(w, i) * sn[i]);
         }
     };
-    some(first, min(end, qg), p.w_q);
-    some(max(first, qg), end, p.w_k);
+    auto sum = [&](float x) {
+#pragma unroll
+        for (int o = 1; o < kGroup; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        return x;
+    };
+    auto one = [&](Group &x, int g) {
+        float v[2 * E];
+#pragma unroll
+        for (int i = 0; i < E; i++) v[i] = x.a.get(i), v[E + i] = x.b.get(i);
+        if (g + kAhead < end) load(x, g + kAhead);
+        if (p.norm != DW_NORM_NONE) {
+            if (p.norm == DW_NORM_LAYER) {
+                float m = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 2 * E; i++) m += v[i];
+                m = sum(m) * p.inv_d;
+#pragma unroll
+                for (int i = 0; i < 2 * E; i++) v[i] -= m;
+            }
+            float2 sq = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < 2 * E; i += 2) sq = __ffma2_rn(make_float2(v[i], v[i + 1]), make_float2(v[i], v[i + 1]), sq);
+            const float rstd = __frsqrt_rn(fmaf(sum(sq.x + sq.y), p.inv_d, p.eps));
+#pragma unroll
+            for (int i = 0; i < 2 * E; i += 2) {
+                const float2 r = __fmul2_rn(make_float2(v[i], v[i + 1]), make_float2(rstd, rstd));
+                v[i] = r.x, v[i + 1] = r.y;
+            }
+        }
+        float y[2 * E];
+        auto turn = [&](auto near) {  // two pairs to an instruction
+            constexpr bool kNear = decltype(near)::value;
+#pragma unroll
+            for (int i = 0; i < E; i += 2) {
+                const int a0 = kNear ? 2 * i : i, a1 = kNear ? 2 * i + 2 : i + 1, b0 = kNear ? 2 * i + 1 : E + i, b1 = kNear ? 2 * i + 3 : E + i + 1;
+                const float2 va = make_float2(v[a0], v[a1]), vb = make_float2(v[b0], v[b1]);
+                const float2 ya = __ffma2_rn(va, make_float2(ac[i], ac[i + 1]), __fmul2_rn(vb, make_float2(bs[i], bs[i + 1])));
+                const float2 yb = __ffma2_rn(va, make_float2(as[i], as[i + 1]), __fmul2_rn(vb, make_float2(bc[i], bc[i + 1])));
+                y[a0] = ya.x, y[a1] = ya.y, y[b0] = yb.x, y[b1] = yb.y;
+            }
+        };
+        if (nb)
+            turn(std::true_type{});
+        else
+            turn(std::false_type{});
+        bool there;
+        T *out = place(p.q_out, p.qo_pitch, p.k_out, p.ko_pitch, g, there);
+        if (!there) return;
+        float lo[E], hi[E];
+#pragma unroll
+        for (int i = 0; i < E; i++) lo[i] = y[i], hi[i] = y[E + i];
+        Raw<T, E> r;
+        r.set(lo);
+        r.store(out + a);
+        r.set(hi);
+        r.store(out + b);
+    };
+    weigh(first < qg ? p.w_q : p.w_k);
+    for (int base = first; base < end; base += kAhead) {
+#pragma unroll
+        for (int n = 0; n < kAhead; n++) {
+            const int g = base + n;
+            if (g >= end) break;
+            if (g == qg && g != first) weigh(p.w_k);
+            one(groups[n], g);
+        }
+    }
 }
 
 template <typename T, int E, int kPer>
@@ -653,14 +654,16 @@ HeadParams params(const dw_head_desc &d, size_t tokens, const HeadArgs &a) {
 }
 
 // The lanes of a head with E values in a piece and J slots a lane, and how the heads of a row
-// are shared out: few rows give each warp one group of heads, many rows all of a row's, so that
-// its angles are computed once.
+// are shared out: a warp has all of a row's, so that its angles are computed once, unless the
+// rows are fewer than the warps that the GPU holds at about this many registers (ten groups,
+// all by one warp and one a warp: 1 row 6.0 and 2.3 us, 256 rows 7.2 and 4.3, shared by this
+// rule 3.6, 1024 rows 7.3, 9.9 and 5.7, 2048 rows 8.9 and 17).
 void split(const dw_backend *be, HeadParams &p, int E, int J) {
     p.group = 1;
     while (p.group * 2 * E * J < p.d) p.group *= 2;
     const int per = 32 / p.group, groups = (p.hq + per - 1) / per + (p.hk + per - 1) / per;
-    const size_t warps = (size_t)be->sm_count * 32;  // that the GPU holds at about this many registers
-    p.chunk = (int)std::max<size_t>(1, std::min<size_t>(groups, (size_t)p.tokens * groups / warps));
+    const int parts = (int)std::min<size_t>(groups, std::max<size_t>(1, (size_t)be->sm_count * 16 / p.tokens));
+    p.chunk = (groups + parts - 1) / parts;
     p.chunks = (groups + p.chunk - 1) / p.chunk;
 }
 
