@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(512)
         double cs[E], sn[E], cs1[E], sn1[E];
         double w[2 * E];
         const double inv_d = 1.0 / (64 * E);  // a power of two
-        const bool weighs = p.norm != DW_NORM_NONE && p.w_k;
+        const bool weighs = p.w_k;
 #pragma unroll
         for (int j = 0; j < E; j++) {
             w[j] = weighs ? p.w_k[slot.a + j] : 1.0f, w[E + j] = weighs ? p.w_k[slot.b + j] : 1.0f;
@@ -644,7 +644,8 @@ HeadParams params(const dw_head_desc &d, size_t tokens, const HeadArgs &a) {
     HeadParams p{};
     p.q = a.q.ptr, p.k = a.k.ptr, p.v = a.v.ptr, p.q_out = a.q_out.ptr, p.k_out = a.k_out.ptr;
     p.q_pitch = a.q.pitch, p.k_pitch = a.k.pitch, p.v_pitch = a.v.pitch, p.qo_pitch = a.q_out.pitch, p.ko_pitch = a.k_out.pitch;
-    p.w_q = a.w_q, p.w_k = a.w_k, p.rope = a.rope, p.positions = a.positions;
+    if (d.norm != DW_NORM_NONE) p.w_q = a.w_q, p.w_k = a.w_k;  // (without a norm nothing weighs)
+    p.rope = a.rope, p.positions = a.positions;
     p.tokens = (uint32_t)tokens;
     p.hq = a.q.ptr ? d.q_heads : 0, p.hk = a.k.ptr ? d.kv_heads : 0;
     p.d = d.head_dim, p.rot = d.rot_dim, p.norm = d.norm;

@@ -603,7 +603,7 @@ typedef struct dw_heads {
 } dw_heads;
 
 /* Which heads a row has, their type, norm and rotation.  norm: dw_norm_kind over
- * each head's head_dim values, with f32 weights [head_dim] (NULL: 1), before the
+ * each head's head_dim values, with f32 weights [head_dim] (NULL: 1; without a norm they are not used), before the
  * rotation.  The first rot_dim values of a head are turned (even, 0: none): pair i
  * is (i, i + rot_dim / 2), or with neighbours != 0 (2 i, 2 i + 1), and
  * (a, b) becomes (a cos - b sin, a sin + b cos) of the angle position * freqs[i]. */

@@ -88,6 +88,34 @@ def test_norm_rope(be, dtype, case):
         assert (diff <= tol).all(), (diff / tol).max()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,rot", [(64, 64), (128, 128), (128, 64)])
+def test_without_a_norm_nothing_weighs(be, dtype, d, rot):
+    """Weights that a call without a norm gets change nothing, in any of its outputs."""
+    t = Setup(be, d + rot, 2, 60, 2, 16, d)
+    hq, n = 4, [40, 20]
+    x, xv = put(be, t.rng.normal(0, 1, (sum(n), hq + 4, d)), dtype)
+    rows, pos = xv.reshape(sum(n), hq + 4, d), np.r_[np.arange(40), np.arange(20)].astype(np.int32)
+    w, rope = be.upload_array(np.full(d, 3, np.float32)), ops.prepare_rope(be, freqs(rot))
+    want = K.turn(rows[:, :hq], pos, freqs(rot), rot, False)
+    tol = rope_tolerance(rows[:, :hq], 0, None, 1e-5, want, rot, False, dtype)
+    desc = ops.HeadDesc(hq, 2, d, rot, R.DTYPES[dtype], 0)
+    out = be.alloc(want.size * (4 if dtype == "f32" else 2))
+
+    def close():
+        assert (np.abs(values(be.download_array(out, np.uint8), dtype).reshape(want.shape) - want) <= tol).all()
+    at = lambda h: ops.Heads(x, h * d, (hq + 4) * d)
+    ops.norm_rope(be, desc, sum(n), at(0), None, w, w, rope, be.upload_array(pos), ops.Heads(out), None)
+    close()
+    t.lens[:] = n
+    seqs, caches = t.sequences(n), []
+    for weight in (None, w):
+        ops.append_kv(be, desc, t.cache, seqs, at(hq), at(hq + 2), weight, rope, at(0), weight, ops.Heads(out))
+        close()
+        caches.append(np.concatenate([be.download_array(b, np.uint8) for b in (t.k, t.v, t.s)]))
+    np.testing.assert_array_equal(*caches)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_norm_rope_in_place_and_alone(be, dtype):
     n, hq, d = 37, 5, 128
