@@ -618,7 +618,7 @@ typedef struct dw_head_desc {
 
 /* Builds what the rotations read: freqs[pairs] in radians a position (host memory,
  * finite), held as 64-bit fractions of a turn, so that an angle is exact to 2^-53 of
- * its freq at every int32 position.  *out is a new buffer owned by the caller. */
+ * its freq at every int32 position, with cosine and sine of one position's step.  *out is a new buffer owned by the caller. */
 DW_API dw_status dw_prepare_rope(dw_backend *be, const double *freqs, size_t pairs, dw_buf **out);
 
 /* Query and key heads of `tokens` rows, normed and turned by their positions
