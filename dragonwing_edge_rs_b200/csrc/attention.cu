@@ -7,7 +7,7 @@
 // the value scale rides in the exponent, so the products see codes alone.  M lags: it moves, to
 // a whole number, where a row's true maximum is more than 2^4 above, so the largest w stays
 // below 2^15, inside f16, and the smallest keep 31 binary places and more below it.
-// The 11 bits that a w keeps are the one rounding beyond f32 (codes and f16 queries are exact
+// The 11 bits that a w is cut to, in both sums, are the one loss beyond f32 (codes and f16 queries are exact
 // in f16; a bf16 query row is taken times a power of two that puts its largest value near 2^15).
 //
 // A warp owns 8 NT rows, token by token the heads of a group that share a cache head, and
@@ -304,16 +304,18 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2
                     for (int v = 0; v < VT; v++) o[n][v][h] *= f, o[n][v][2 + h] *= f;
                 }
             }
-            float w[2][4];
+            float base[2];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const float base = (M[n][h] == -INFINITY ? 0.0f : -M[n][h]) + kHead;
+            for (int h = 0; h < 2; h++) base[h] = (M[n][h] == -INFINITY ? 0.0f : -M[n][h]) + kHead;
+            float2 sum[2] = {};
 #pragma unroll
-                for (int b = 0; b < 4; b++) w[h][b] = ex2_approx(x[n][b / 2][2 * (b & 1) + h] + base);
-                L[n][h] = fmaf(w[h][0] + w[h][1], kv_pow2(-ve[0]), fmaf(w[h][2] + w[h][3], kv_pow2(-ve[1]), L[n][h]));
+            for (int b = 0; b < 4; b++) {
+                const float2 w = eleven_bits(ex2_approx(x[n][b / 2][2 * (b & 1)] + base[0]), ex2_approx(x[n][b / 2][2 * (b & 1) + 1] + base[1]));
+                sum[b / 2] = __fadd2_rn(sum[b / 2], w);
+                pf[n][b] = transposed(pack2<__half>(w.x, w.y));
             }
-#pragma unroll
-            for (int b = 0; b < 4; b++) pf[n][b] = transposed(pack2<__half>(w[0][b], w[1][b]));
+            L[n][0] = fmaf(sum[0].x, kv_pow2(-ve[0]), fmaf(sum[1].x, kv_pow2(-ve[1]), L[n][0]));
+            L[n][1] = fmaf(sum[0].y, kv_pow2(-ve[0]), fmaf(sum[1].y, kv_pow2(-ve[1]), L[n][1]));
         }
         // ---- values
         const bool tail = t + kTile > r.len;

@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int i = 16 * g; i < 16 * g + 16; i += 2) {
                             float2 y = __ffma2_rn(make_float2(x[q][i], x[q][i + 1]), make_float2(a, a), make_float2(add, add));
-                            y.x = ex2_approx(y.x), y.y = ex2_approx(y.y);
+                            y = eleven_bits(ex2_approx(y.x), ex2_approx(y.y));
                             sum = __fadd2_rn(sum, y);
                             w[i / 2] = pack2<__half>(y.x, y.y);
                         }

@@ -39,6 +39,14 @@ __device__ __forceinline__ Bounds row_bounds(const AttendParams &p, const SeqRan
 // (x, y) -> the sums' factor where the maximum goes from x to y (-inf: nothing so far).
 __device__ __forceinline__ float carry(float x, float y) { return x == y ? 1.0f : ex2_approx(x - y); }
 
+// Weights cut to the 11 bits that f16 keeps, but with f32's exponents (a block of small values has
+// weights far below f16's range that count in the sum of weights).  Both sums take these, so only
+// what the cuts differ by between a row's tokens is an error, as much as of a rounding to nearest, and
+// a row of one token is exact; with the uncut ones in the sum of weights it was half as much again.
+__device__ __forceinline__ float2 eleven_bits(float x, float y) {
+    return make_float2(__uint_as_float(__float_as_uint(x) & ~0x1FFFu), __uint_as_float(__float_as_uint(y) & ~0x1FFFu));
+}
+
 // A bf16 query row goes to f16 times 2^-e, which puts its largest magnitude `top` into
 // [2^14, 2^15): nothing overflows and what falls below f16's smallest step is 2^-39 of it.
 __device__ __forceinline__ int query_exponent(float top) {

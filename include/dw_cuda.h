@@ -684,8 +684,8 @@ DW_API dw_status dw_read_kv(dw_backend *be, const dw_kv_cache *cache, const dw_s
  * position p) sees: all of its sequence, with causal != 0 those up to p, with window > 0 (and
  * causal) the last `window` of these.  Query head h reads cache head h / (q_heads /
  * kv_heads).  A row that sees nothing gives 0.  q and out: DW_F16 or DW_BF16; products
- * and sums are f32, the softmax's numerators are rounded to 11 bits before they meet the
- * values.  The sums' order depends on the sizes and lengths alone.  out may be q itself. */
+ * and sums are f32, the softmax's weights are cut to 11 bits, in numerator and
+ * denominator.  The sums' order depends on the sizes and lengths alone.  out may be q itself. */
 typedef struct dw_attention_desc {
     int32_t q_heads; /* a multiple of the cache's kv_heads */
     int32_t dtype;

@@ -23,10 +23,12 @@ def be():
 def tolerance(want, mean, big, mass, length, d, dtype):
     """A logit: d exact products summed in f32 with at most a whole last place lost in each of d / 8 sums, of their
     absolute sum; its scaling, the value scale's addition and the maximum's: four roundings of |t| + 64 + 14 in units
-    of log2; 2^x 2^-22.  A weight is off by that, twice (numerator and denominator), and once by half a step of f16.
+    of log2; 2^x 2^-22.  A weight is off by that, twice (numerator and denominator), and by its cut to 11 bits: both sums
+    take the cut weights w (1 - e), 0 <= e < 2^-10, and sum w (v - out) = 0, so sum w (e - 2^-11) (v - out) / sum w, at
+    most 2^-11 (mean + |out|), is what that does.
     The values' sum: at most a whole last place in each of length / 8 + 32 sums and joins.  Then the result's rounding."""
     weight = 2.0 ** -11 + 2 * (d / 8 * 2.0 ** -23 * mass + 4 * 2.0 ** -23 * (2 * big + 78) + 2.0 ** -22)
-    tol = (weight * 1.1 + (length / 8 + 32) * 2.0 ** -23) * mean
+    tol = (weight * 1.1 + (length / 8 + 32) * 2.0 ** -23) * mean + 2.0 ** -11 * np.abs(want)
     floor = {"f16": 2.0 ** -25, "bf16": 1e-40}[dtype]
     return tol + HALF_STEP[dtype] * (np.abs(want) + tol) + floor + length * 2.0 ** -38 * np.nan_to_num(mean).max(initial=0.0)
 
