@@ -7,7 +7,8 @@
 // Angles: a frequency is a 64-bit fraction of a turn, so position * frequency modulo a turn is
 // one integer product, exact however far the position.
 //
-// All are bound by the bytes of the rows, in short calls by latency.
+// Rotations and reads of many rows are bound by their bytes and the loads in flight, appends by
+// the chain from a page's lookup to its codes, short calls by latency.
 
 #include <algorithm>
 #include <type_traits>
@@ -339,7 +340,8 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ 
 // computed them.  (f32 with a bound, and f64 where that leaves two codes open, took longer: the
 // bound has to hold for the pair, and one token in five had a value too small beside its
 // partner.)  A warp's tokens follow each other, so the angles after the first come by one
-// complex product each.  The blocks behind those of the pages norm and turn query rows.
+// complex product each.  The blocks behind those of the pages norm and turn query rows.  (4096
+// tokens, 8 heads of 128 bf16: 17.5 us, 25 MB; with 32 query heads 29.3, 92 MB.)
 constexpr int kWarpTokens = 8;
 
 __device__ __forceinline__ float round_to_odd(double v) {
@@ -586,7 +588,8 @@ __global__ void __launch_bounds__(512)
 }
 
 // ---- read --------------------------------------------------------------------------
-// A warp has a row's keys or values, a lane 16 of them at a time.
+// A warp has a row's keys or values, a lane 16 of them at a time (4096 rows of 8 heads of 128 bf16
+// 7.5 us, 25 MB).
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_read(const __grid_constant__ KvCache c, const __grid_constant__ Seqs q, const uint32_t each_rows, T *k_out, T *v_out, size_t k_pitch,
