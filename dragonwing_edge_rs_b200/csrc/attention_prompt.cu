@@ -552,6 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- join: each CTA leaves its sums in shared memory, over its queries and stages
         float *const part = reinterpret_cast<float *>(base);  // [256][D], a row's 16-byte pieces xor the row modulo 8
         auto piece_at = [&](int row, int piece) { return part + row * D + (piece ^ (row & 7)) * 4; };
+        __syncwarp();
         __syncthreads();  // all products are done
         if (warp >= 4 && warp < 12) {
             const int t = (warp - 4) >> 2, row = t * 128 + (warp & 3) * 32 + lane;

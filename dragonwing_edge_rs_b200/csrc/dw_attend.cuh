@@ -69,9 +69,11 @@ __device__ __forceinline__ uint32_t cluster_size() {
     return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_sync_relaxed() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {

@@ -608,7 +608,7 @@ typedef struct dw_heads {
  * is (i, i + rot_dim / 2), or with neighbours != 0 (2 i, 2 i + 1), and
  * (a, b) becomes (a cos - b sin, a sin + b cos) of the angle position * freqs[i]. */
 typedef struct dw_head_desc {
-    int32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads */
+    int32_t q_heads, kv_heads;
     int32_t head_dim, rot_dim;
     int32_t dtype; /* dw_dtype of rows in and out */
     int32_t norm;
