@@ -253,3 +253,35 @@ def test_shared_pages_and_two_backends(be):
         be.synchronize(), other.synchronize()
         for out in outs:
             np.testing.assert_array_equal(be.download_array(out, np.uint8), want)
+
+
+@pytest.mark.parametrize("n", [20, 90])
+def test_captured_pieces_of_prompts_beside_another_backend(be, n):
+    """Few and many rows whose tokens a cluster shares: a captured call, replayed at other lengths (one of them 0, one
+    shorter than its rows), gives the eager call's bits while another backend makes the same calls."""
+    t = filled(be, n, [2500, 1700], 1, 32, 128)
+    lib, up, bytes_ = ops.L.load(), be.upload_array, 2 * n * 2 * 128 * 2
+    q = up(t.rng.normal(0, 1, bytes_ // 2).astype(np.float16))
+    lens, table = up(t.lens), up(t.pages)
+    seqs = ops.Sequences(table, lens, None, 2, 2 * n, t.width)
+    desc = ops.AttentionDesc(2, ops.F16, 128 ** -0.5)
+    a, b, c = (be.alloc(bytes_) for _ in range(3))
+    g = ctypes.c_void_p()
+    be._check(lib.dw_capture_begin(be.handle))
+    ops.attention_kv8(be, desc, t.cache, seqs, ops.Heads(q), ops.Heads(a))
+    be._check(lib.dw_capture_end(be.handle, ctypes.byref(g)))
+    with dw.CudaBackend(0) as other:
+        for now in ([2500, 1700], [1, 1700], [0, 64], [n - 1, n], [2499, 3]):
+            be.upload(lens, np.asarray(now, np.int32))
+            be.synchronize()
+            for _ in range(5):
+                be._check(lib.dw_graph_launch(be.handle, g))
+                ops.attention_kv8(other, desc, t.cache, seqs, ops.Heads(q), ops.Heads(c))
+            ops.attention_kv8(be, desc, t.cache, seqs, ops.Heads(q), ops.Heads(b))
+            be.synchronize(), other.synchronize()
+            want = be.download_array(b, np.uint8)
+            np.testing.assert_array_equal(be.download_array(a, np.uint8), want)
+            np.testing.assert_array_equal(be.download_array(c, np.uint8), want)
+            t.lens[:], t.starts = now, np.array([0, n, 2 * n])
+            check(t, desc, "f16", n, values(be.download_array(q, np.uint8), "f16").reshape(2 * n, 2, 128), values(want, "f16").reshape(2 * n, 2, 128))
+    lib.dw_graph_destroy(g)
