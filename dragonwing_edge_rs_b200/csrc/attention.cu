@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2
     if (p.per_seq) {
         s = item / (uint32_t)p.per_seq, place = item % (uint32_t)p.per_seq;
     } else {
-        s = seq_of_item(sq, item, p.group, R, 1, place);
+        s = seq_of_item(sq, item, p.group, R, 1, place, p.err);
     }
     // (without a window the first tiles' pages are looked up before the length is known)
     const bool two = c.page < kTile;

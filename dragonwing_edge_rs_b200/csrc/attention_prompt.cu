@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (p.per_seq) {
         s = unit % sq.seqs, place = p.per_seq - 1 - (int)(unit / sq.seqs);
     } else {
-        s = seq_of_item(sq, p.items - 1 - unit, p.group, kRows, 1, place);
+        s = seq_of_item(sq, p.items - 1 - unit, p.group, kRows, 1, place, p.err);
     }
     const SeqRange r = seq_range(sq, s, c.page, p.err);
     const int rows_all = r.n * p.group, first = (int)min(place * kRows, (int64_t)0x7fffffff);

@@ -55,6 +55,7 @@ __device__ __forceinline__ float2 e4m3_to_f32x2(uint16_t c) {
 struct SeqRange {
     int row0, n;  // its rows
     int len;      // its tokens in the cache
+    bool ok;      // neither had to be brought into bounds
     __device__ __forceinline__ int position(int row) const { return len - n + (row - row0); }
 };
 
@@ -63,20 +64,37 @@ __device__ __forceinline__ int seq_start(const Seqs &q, uint32_t s) {
     return min(max(q.starts[s], 0), (int)q.tokens);
 }
 
-// The rows of a sequence, its starts checked.
-__device__ __forceinline__ int seq_rows(const Seqs &q, uint32_t s, int &row0, int32_t *err) {
+// The rows of a sequence, its starts checked (ok: not changed where they are in order).
+__device__ __forceinline__ int seq_rows(const Seqs &q, uint32_t s, int &row0, int32_t *err, bool &ok) {
     row0 = seq_start(q, s);
     const int end = seq_start(q, s + 1);
-    if (q.starts && (end < row0 || q.starts[s] != row0 || q.starts[s + 1] != end)) record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
+    if (q.starts && (end < row0 || q.starts[s] != row0 || q.starts[s + 1] != end)) {
+        record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
+        ok = false;
+    }
     return max(end - row0, 0);
+}
+__device__ __forceinline__ int seq_rows(const Seqs &q, uint32_t s, int &row0, int32_t *err) {
+    bool ok = true;
+    return seq_rows(q, s, row0, err, ok);
+}
+// Whether the starts around a sequence's own leave its rows to it alone: where starts descend, the
+// sequences on both sides may claim the same rows, and which of them is wrong is not known.
+__device__ __forceinline__ bool seq_apart(const Seqs &q, uint32_t s) {
+    if (!q.starts) return true;
+    return (s == 0 || q.starts[s - 1] <= q.starts[s]) && (s + 2 > q.seqs || q.starts[s + 1] <= q.starts[s + 2]);
 }
 
 __device__ __forceinline__ SeqRange seq_range(const Seqs &q, uint32_t s, int page, int32_t *err) {
     SeqRange r;
+    r.ok = true;
     const int most = (int)min((uint64_t)q.width * page, (uint64_t)0x7fffff00u), len = q.lens[s];
-    r.n = seq_rows(q, s, r.row0, err);
+    r.n = seq_rows(q, s, r.row0, err, r.ok);
     r.len = min(max(len, 0), most);
-    if (len != r.len) record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
+    if (len != r.len) {
+        record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
+        r.ok = false;
+    }
     return r;
 }
 
@@ -88,8 +106,14 @@ __host__ __device__ inline size_t seq_items(size_t tokens, size_t seqs, int per,
     return tokens * per / size + extra * seqs;
 }
 // The sequence of item w and its place there (below 0: of no sequence); a whole warp calls.
-__device__ __forceinline__ uint32_t seq_of_item(const Seqs &q, int64_t w, int per, int size, int extra, int64_t &place) {
+// Where starts descend the search may come to some sequences by no item, so the items look through
+// all starts as well, each at its share, a lane each.
+__device__ __forceinline__ uint32_t seq_of_item(const Seqs &q, int64_t w, int per, int size, int extra, int64_t &place, int32_t *err) {
     const int lane = threadIdx.x & 31;
+    for (int64_t i = w * 32 + lane; i < q.seqs; i += extra ? q.seqs : (int64_t)q.tokens * 32) {
+        int row0;
+        seq_rows(q, (uint32_t)i, row0, err);
+    }
     auto first = [&](uint32_t s) { return (int64_t)seq_start(q, s) * per / size + (int64_t)extra * s; };
     uint32_t lo = 0, count = q.seqs;
     while (count > 1) {  // the last of 32 evenly spaced ones that does not start behind w
@@ -103,12 +127,17 @@ __device__ __forceinline__ uint32_t seq_of_item(const Seqs &q, int64_t w, int pe
     return lo;
 }
 
-// The page of a sequence's token `t`, in bounds in any case.
-__device__ __forceinline__ uint32_t seq_page(const Seqs &q, const KvCache &c, uint32_t s, uint32_t index, int32_t *err) {
+// A sequence's page `index` (its tokens from index * page on); c.pages where the table names none.
+__device__ __forceinline__ uint32_t seq_page_or_none(const Seqs &q, const KvCache &c, uint32_t s, uint32_t index, int32_t *err) {
     const uint32_t id = (uint32_t)q.table[(size_t)s * q.width + index];
     if (id < c.pages) return id;
     record_error(err, DW_DEV_BAD_ARG, 62, (int)s);
-    return 0;
+    return c.pages;
+}
+// The same to read from, in bounds in any case.
+__device__ __forceinline__ uint32_t seq_page(const Seqs &q, const KvCache &c, uint32_t s, uint32_t index, int32_t *err) {
+    const uint32_t id = seq_page_or_none(q, c, s, index, err);
+    return id < c.pages ? id : 0;
 }
 
 }  // namespace dw

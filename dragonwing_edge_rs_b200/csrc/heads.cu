@@ -388,8 +388,9 @@ __device__ __forceinline__ void rescale_codes(uint8_t *p, float f) {
 }
 
 // The place of item w of rows whose sequences have as many each.
-__device__ __forceinline__ uint32_t seq_and_place(const Seqs &q, uint32_t w, uint32_t each, int per, int size, int extra, int64_t &place) {
-    if (q.starts) return seq_of_item(q, w, per, size, extra, place);
+__device__ __forceinline__ uint32_t seq_and_place(const Seqs &q, uint32_t w, uint32_t each, int per, int size, int extra, int64_t &place,
+                                                  int32_t *err) {
+    if (q.starts) return seq_of_item(q, w, per, size, extra, place, err);
     place = w % each;
     return w / each;
 }
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(512)
         const size_t row = unit / p.chunks;
         if (row >= p.tokens) return;
         int64_t place;
-        const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place);
+        const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place, err);
         const SeqRange r = seq_range(q, s, c.page, err);
         if (place < 0 || place >= r.n) return;
         HeadParams pq = p;
@@ -422,17 +423,21 @@ __global__ void __launch_bounds__(512)
     }
     const int head = (int)(blockIdx.x % p.hk);
     int64_t place;
-    const uint32_t s = seq_and_place(q, blockIdx.x / p.hk, each_pages, 1, c.page, 2, place);
+    const uint32_t s = seq_and_place(q, blockIdx.x / p.hk, each_pages, 1, c.page, 2, place, err);
     const SeqRange r = seq_range(q, s, c.page, err);
     const int shift = 31 - __clz(c.page);   // pages hold a power of two of tokens
     const int first = max(r.len - r.n, 0);  // the sequence's first new token
     const int64_t begin = ((first >> shift) + place) << shift;
     if (place < 0 || first >= r.len || begin >= r.len) return;
+    // Nothing is written for a sequence whose length, starts or page lie outside: what they were
+    // brought to belongs to other sequences, or to other tokens of this one.  (The same for all
+    // threads of the block, and before its first barrier.)
+    const uint32_t page = seq_page_or_none(q, c, s, (uint32_t)(begin >> shift), err);
+    if (!r.ok || !seq_apart(q, s) || page >= c.pages) return;
     const int t0 = max(first, (int)begin), t1 = (int)min((int64_t)r.len, begin + c.page);
     const int w0 = (int)begin + warp * kWarpTokens;  // the warp's first token
     const Slot<E> slot(lane, p.rot, p.neighbours);
     const T *const kp = (const T *)p.k + (size_t)head * p.d, *const vp = (const T *)p.v + (size_t)head * p.d;
-    const uint32_t page = seq_page(q, c, s, (uint32_t)(begin >> shift), err);
     uint8_t *const scale = c.s + kv_block(c, page, head) * 2;
     const bool has_old = t0 > begin;
     const int k_old = has_old ? kv_exponent(scale[0]) : kKvMinExp, v_old = has_old ? kv_exponent(scale[1]) : kKvMinExp;
@@ -603,7 +608,7 @@ __global__ void __launch_bounds__(kThreads)
     T *out = values ? v_out : k_out;
     if (row >= q.tokens || !out) return;
     int64_t place;
-    const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place);
+    const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place, err);
     const SeqRange r = seq_range(q, s, c.page, err);
     if (place < 0 || place >= r.n) return;
     out += row * (values ? v_pitch : k_pitch);

@@ -656,7 +656,9 @@ DW_API size_t dw_kv_scale_bytes(size_t pages, size_t kv_heads);
  * are neither read nor written, nor are table entries behind a sequence's last page.
  * Positions below 0 (n > lens[s]) are no tokens of the cache.  Lengths, starts and pages that
  * lie outside are not followed: dw_synchronize reports DW_ERR_DEVICE, and the call's
- * results are not to be used. */
+ * results are not to be used.  An append leaves the cache alone for a sequence whose length
+ * or starts lie outside or whose starts descend, or a neighbour's do, and where a page lies outside;
+ * the other sequences' tokens are appended as ever. */
 typedef struct dw_sequences {
     const dw_buf *table;  /* int32 [seqs, width] */
     const dw_buf *lens;   /* int32 [seqs] */
