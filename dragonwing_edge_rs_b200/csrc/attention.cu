@@ -77,7 +77,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2
     if (p.per_seq) {
         s = item / (uint32_t)p.per_seq, place = item % (uint32_t)p.per_seq;
     } else {
-        s = seq_of_item(sq, item, p.group, R, 1, place, p.err);
+        s = seq_of_item(sq, item, p.group, R, 1, place);
+        if (head == 0 && warp == 0 && bad_start(sq, (int64_t)item * 32 + lane)) record_error(p.err, DW_DEV_BAD_ARG, 61, (int)s);
     }
     // (without a window the first tiles' pages are looked up before the length is known)
     const bool two = c.page < kTile;
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2
             }
         }
     }
-    const SeqRange r = seq_range(sq, s, c.page, p.err);
+    const SeqRange r = seq_range(sq, s, c.page, p.err, -1);
     const int token_a = first / p.group, token_b = (first + rows - 1) / p.group;
     const int lo = row_bounds(p, r, token_a).lo, hi = row_bounds(p, r, token_b).hi;
     // tokens that every row sees: tiles inside need no mask

@@ -177,9 +177,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (p.per_seq) {
         s = unit % sq.seqs, place = p.per_seq - 1 - (int)(unit / sq.seqs);
     } else {
-        s = seq_of_item(sq, p.items - 1 - unit, p.group, kRows, 1, place, p.err);
+        s = seq_of_item(sq, p.items - 1 - unit, p.group, kRows, 1, place);
     }
-    const SeqRange r = seq_range(sq, s, c.page, p.err);
+    const SeqRange r = seq_range(sq, s, c.page, p.err, p.items - 1 - unit);
     const int rows_all = r.n * p.group, first = (int)min(place * kRows, (int64_t)0x7fffffff);
     if (place < 0 || first >= rows_all) {
         pdl_trigger();

@@ -85,16 +85,24 @@ __device__ __forceinline__ bool seq_apart(const Seqs &q, uint32_t s) {
     return (s == 0 || q.starts[s - 1] <= q.starts[s]) && (s + 2 > q.seqs || q.starts[s + 1] <= q.starts[s + 2]);
 }
 
-__device__ __forceinline__ SeqRange seq_range(const Seqs &q, uint32_t s, int page, int32_t *err) {
+__device__ __forceinline__ bool bad_start(const Seqs &q, int64_t s) {
+    if (!q.starts || s >= q.seqs) return false;
+    const int a = q.starts[s], b = q.starts[s + 1];
+    return a < 0 || a > b || (uint32_t)b > q.tokens;
+}
+
+// Where starts descend, the search for an item's sequence comes to some sequences by no item, so the
+// items look through all starts as well: the lanes of item w at the 32 of its share (items are as
+// many as sequences at least; below 0: no share).
+__device__ __forceinline__ SeqRange seq_range(const Seqs &q, uint32_t s, int page, int32_t *err, int64_t w) {
     SeqRange r;
     r.ok = true;
     const int most = (int)min((uint64_t)q.width * page, (uint64_t)0x7fffff00u), len = q.lens[s];
+    const bool bad = w >= 0 && bad_start(q, w * 32 + (threadIdx.x & 31));
     r.n = seq_rows(q, s, r.row0, err, r.ok);
     r.len = min(max(len, 0), most);
-    if (len != r.len) {
-        record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
-        r.ok = false;
-    }
+    r.ok = r.ok && len == r.len;
+    if (len != r.len || bad) record_error(err, DW_DEV_BAD_ARG, 61, (int)s);
     return r;
 }
 
@@ -106,14 +114,8 @@ __host__ __device__ inline size_t seq_items(size_t tokens, size_t seqs, int per,
     return tokens * per / size + extra * seqs;
 }
 // The sequence of item w and its place there (below 0: of no sequence); a whole warp calls.
-// Where starts descend the search may come to some sequences by no item, so the items look through
-// all starts as well, each at its share, a lane each.
-__device__ __forceinline__ uint32_t seq_of_item(const Seqs &q, int64_t w, int per, int size, int extra, int64_t &place, int32_t *err) {
+__device__ __forceinline__ uint32_t seq_of_item(const Seqs &q, int64_t w, int per, int size, int extra, int64_t &place) {
     const int lane = threadIdx.x & 31;
-    for (int64_t i = w * 32 + lane; i < q.seqs; i += extra ? q.seqs : (int64_t)q.tokens * 32) {
-        int row0;
-        seq_rows(q, (uint32_t)i, row0, err);
-    }
     auto first = [&](uint32_t s) { return (int64_t)seq_start(q, s) * per / size + (int64_t)extra * s; };
     uint32_t lo = 0, count = q.seqs;
     while (count > 1) {  // the last of 32 evenly spaced ones that does not start behind w
@@ -127,17 +129,12 @@ __device__ __forceinline__ uint32_t seq_of_item(const Seqs &q, int64_t w, int pe
     return lo;
 }
 
-// A sequence's page `index` (its tokens from index * page on); c.pages where the table names none.
-__device__ __forceinline__ uint32_t seq_page_or_none(const Seqs &q, const KvCache &c, uint32_t s, uint32_t index, int32_t *err) {
+// A sequence's page `index` (its tokens from index * page on) to read from, in bounds in any case.
+__device__ __forceinline__ uint32_t seq_page(const Seqs &q, const KvCache &c, uint32_t s, uint32_t index, int32_t *err) {
     const uint32_t id = (uint32_t)q.table[(size_t)s * q.width + index];
     if (id < c.pages) return id;
     record_error(err, DW_DEV_BAD_ARG, 62, (int)s);
-    return c.pages;
-}
-// The same to read from, in bounds in any case.
-__device__ __forceinline__ uint32_t seq_page(const Seqs &q, const KvCache &c, uint32_t s, uint32_t index, int32_t *err) {
-    const uint32_t id = seq_page_or_none(q, c, s, index, err);
-    return id < c.pages ? id : 0;
+    return 0;
 }
 
 }  // namespace dw

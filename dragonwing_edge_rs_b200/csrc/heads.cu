@@ -388,9 +388,8 @@ __device__ __forceinline__ void rescale_codes(uint8_t *p, float f) {
 }
 
 // The place of item w of rows whose sequences have as many each.
-__device__ __forceinline__ uint32_t seq_and_place(const Seqs &q, uint32_t w, uint32_t each, int per, int size, int extra, int64_t &place,
-                                                  int32_t *err) {
-    if (q.starts) return seq_of_item(q, w, per, size, extra, place, err);
+__device__ __forceinline__ uint32_t seq_and_place(const Seqs &q, uint32_t w, uint32_t each, int per, int size, int extra, int64_t &place) {
+    if (q.starts) return seq_of_item(q, w, per, size, extra, place);
     place = w % each;
     return w / each;
 }
@@ -409,8 +408,8 @@ __global__ void __launch_bounds__(512)
         const size_t row = unit / p.chunks;
         if (row >= p.tokens) return;
         int64_t place;
-        const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place, err);
-        const SeqRange r = seq_range(q, s, c.page, err);
+        const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place);
+        const SeqRange r = seq_range(q, s, c.page, err, -1);
         if (place < 0 || place >= r.n) return;
         HeadParams pq = p;
         pq.hk = 0;
@@ -423,17 +422,18 @@ __global__ void __launch_bounds__(512)
     }
     const int head = (int)(blockIdx.x % p.hk);
     int64_t place;
-    const uint32_t s = seq_and_place(q, blockIdx.x / p.hk, each_pages, 1, c.page, 2, place, err);
-    const SeqRange r = seq_range(q, s, c.page, err);
+    const uint32_t s = seq_and_place(q, blockIdx.x / p.hk, each_pages, 1, c.page, 2, place);
+    const SeqRange r = seq_range(q, s, c.page, err, blockIdx.x / p.hk);
     const int shift = 31 - __clz(c.page);   // pages hold a power of two of tokens
     const int first = max(r.len - r.n, 0);  // the sequence's first new token
     const int64_t begin = ((first >> shift) + place) << shift;
     if (place < 0 || first >= r.len || begin >= r.len) return;
+    const uint32_t named = (uint32_t)q.table[(size_t)s * q.width + (uint32_t)(begin >> shift)], page = min(named, c.pages - 1);
     // Nothing is written for a sequence whose length, starts or page lie outside: what they were
     // brought to belongs to other sequences, or to other tokens of this one.  (The same for all
-    // threads of the block, and before its first barrier.)
-    const uint32_t page = seq_page_or_none(q, c, s, (uint32_t)(begin >> shift), err);
-    if (!r.ok || !seq_apart(q, s) || page >= c.pages) return;
+    // threads of the block.)
+    if (named >= c.pages) record_error(err, DW_DEV_BAD_ARG, 62, (int)s);
+    if (named >= c.pages || !r.ok || !seq_apart(q, s)) return;
     const int t0 = max(first, (int)begin), t1 = (int)min((int64_t)r.len, begin + c.page);
     const int w0 = (int)begin + warp * kWarpTokens;  // the warp's first token
     const Slot<E> slot(lane, p.rot, p.neighbours);
@@ -608,8 +608,10 @@ __global__ void __launch_bounds__(kThreads)
     T *out = values ? v_out : k_out;
     if (row >= q.tokens || !out) return;
     int64_t place;
-    const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place, err);
-    const SeqRange r = seq_range(q, s, c.page, err);
+    const uint32_t s = seq_and_place(q, (uint32_t)row, each_rows, 1, 1, 0, place);
+    const SeqRange r = seq_range(q, s, c.page, err, -1);
+    for (size_t i = row * 32 + lane; q.starts && i < q.seqs; i += (size_t)q.tokens * 32)
+        if (bad_start(q, (int64_t)i)) record_error(err, DW_DEV_BAD_ARG, 61, (int)i);
     if (place < 0 || place >= r.n) return;
     out += row * (values ? v_pitch : k_pitch);
     const int t = r.position((int)row), shift = 31 - __clz(c.page), d_shift = 31 - __clz(c.d);  // powers of two
