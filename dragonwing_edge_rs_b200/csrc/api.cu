@@ -353,6 +353,8 @@ DW_API dw_status dw_graph_launch(dw_backend *be, dw_graph *g) {
     return dw_cuda_check(be, cudaGraphLaunch(g->exec, be->stream), "graph launch");
 }
 
+DW_API uint64_t dw_graph_kernels(const dw_graph *g) { return g ? g->kernels : 0; }
+
 DW_API void dw_graph_destroy(dw_graph *g) {
     if (!g) return;
     if (g->exec) cudaGraphExecDestroy(g->exec);

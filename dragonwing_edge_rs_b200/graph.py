@@ -1525,13 +1525,13 @@ class CudaGraphRuntime:
         return g
 
     def capture(self) -> int:
-        """Records the op list once as a CUDA graph; returns its kernel count."""
-        before = self.be.launch_count()
-        self._cgraph = self._record(self._dispatch)
-        # a launch records its kernels; count them by replaying once
-        self.run()
-        self.be.synchronize(60000)
-        return self.be.launch_count() - before
+        """Records the op list as a CUDA graph, which run() replays from then on; returns its kernel count.
+        Nothing runs here: inputs need not be set yet, and state that ops change (a cache) stays as it is."""
+        graph = self._record(self._dispatch)
+        if self._cgraph is not None:
+            L.load().dw_graph_destroy(self._cgraph)
+        self._cgraph = graph
+        return int(L.load().dw_graph_kernels(graph))
 
     def capture_slots(self, depth: int) -> list:
         """Records `depth` CUDA graphs of the op list for a serving loop.  Graph d

@@ -162,6 +162,8 @@ DW_API dw_status dw_capture_begin(dw_backend *be);
 DW_API dw_status dw_capture_end(dw_backend *be, dw_graph **out);
 DW_API dw_status dw_graph_launch(dw_backend *be, dw_graph *g);
 DW_API void dw_graph_destroy(dw_graph *g);
+/* Kernel launches that a replay makes (what dw_launch_count grows by). */
+DW_API uint64_t dw_graph_kernels(const dw_graph *g);
 /* Test hook: runs one bounded device-side wait on a flag that nothing sets,
  * with a cap of cap_us microseconds; the kernel gives up and records the
  * failure, and the next dw_synchronize reports DW_ERR_KERNEL_WAIT_EXPIRED. */
