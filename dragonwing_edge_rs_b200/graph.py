@@ -1237,6 +1237,9 @@ class CudaGraphRuntime:
         """buffers: CudaBuffers of other owners for tensors, by name (a cache that several graphs share)."""
         if fuse:
             graph = lower_for_device(graph, residual_i8=residual_i8)
+        unknown = sorted(set(buffers or {}) - set(graph.tensors))
+        if unknown:
+            raise BackendError(L.DW_ERR_INVALID_ARG, f"buffers given for no tensor of the graph: {', '.join(unknown)}")
         self.graph = graph
         self.be = backend
         self.bufs: dict[str, CudaBuffer] = {}
