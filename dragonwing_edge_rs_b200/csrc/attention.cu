@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2
     }
     // (without a window the first tiles' pages are looked up before the length is known)
     const bool two = c.page < kTile;
+    constexpr uint32_t kGone = ~0u;
     const int shift = 31 - __clz(c.page);  // pages hold a power of two of tokens
     const int step = (int)S * kWarps, gid = (int)rank * kWarps + warp;
     uint32_t guess[2];
@@ -137,9 +138,12 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2
     auto fetch_pages = [&](Pages &b, int base) {
         const int i = base + lane, t = (tile0 + gid + i * step) * kTile;
         if (i >= mine) return;
-        b.page[0] = seq_page(sq, c, s, (uint32_t)t >> shift, p.err);
-        b.page[1] = two && t + 16 < r.len ? seq_page(sq, c, s, (uint32_t)(t + 16) >> shift, p.err) : b.page[0];
+        // (a page whose tokens lie before the window may have been given away: zeros in its place)
+        const bool gone = two && t + 16 <= lo;
+        b.page[0] = seq_page(sq, c, s, (uint32_t)(gone ? t + 16 : t) >> shift, p.err);
+        b.page[1] = two && !gone && t + 16 < r.len ? seq_page(sq, c, s, (uint32_t)(t + 16) >> shift, p.err) : b.page[0];
         places(b, t);
+        if (gone) b.row[0] = kGone;
     };
     auto fetch_scales = [&](Pages &b, int base) {
         if (base + lane >= mine) return;
@@ -163,14 +167,16 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 1 : NT == 1 ? 3 : 2
             const uint32_t stage = (uint32_t)(i % kStages) * 2 * kBytes;
             if ((i & 31) == 0 && i) now = next;
             const uint32_t at0 = __shfl_sync(0xffffffffu, now.row[0], i & 31), at1 = __shfl_sync(0xffffffffu, now.row[1], i & 31);
-            const size_t from[2] = {(size_t)at0 * D + lane * 16, (size_t)at1 * D + lane * 16};
+            const size_t from[2] = {(size_t)(at0 == kGone ? at1 : at0) * D + lane * 16, (size_t)at1 * D + lane * 16};
+            const uint32_t bytes[2] = {at0 == kGone ? 0u : 16u, 16u};  // read; the rest of 16 is zeros
 #pragma unroll
             for (int k = 0; k < kTile / kLines; k++) {
                 constexpr int kHalfCopies = kTile / kLines / 2;
                 const size_t at = from[k / kHalfCopies] + (k % kHalfCopies) * 512;
                 const uint32_t to = c_to[k & 1] + stage + (k & ~1) * 512;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(c.k + at) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + kBytes), "l"(c.v + at) : "memory");
+                const uint32_t n = bytes[k / kHalfCopies];
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(c.k + at), "r"(n) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + kBytes), "l"(c.v + at), "r"(n) : "memory");
             }
             if (lane == (i & 31)) scales[warp][i % kStages] = now.scale;
             if ((i & 31) == 8) fetch_pages(next, (i & ~31) + 32);

@@ -245,8 +245,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t scales;  // of group tid
         } x0, x1;
         bool bad = false;
+        const int begin = lo & -c.page;  // pages that end before the window may have been given away
         auto lookup = [&](int t) {  // the page of token t, in bounds in any case
-            if (t >= r.len) return 0u;
+            if (t >= r.len || t < begin) return 0u;
             const uint32_t id = (uint32_t)sq.table[(size_t)s * sq.width + (uint32_t)(t >> shift)];
             bad |= id >= c.pages;
             return id;
@@ -264,8 +265,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t row = ((min(pg.row[g], c.pages - 1) * (uint32_t)c.heads + (uint32_t)head) << shift) + (uint32_t)(t & (c.page - 1));
                 const uint4 *from = reinterpret_cast<const uint4 *>(codes + (size_t)row * D) + part;
 #pragma unroll
-                for (int h = 0; h < kHalves; h++)  // no token: zeros, whatever the page holds there
-                    x[g * kHalves + h] = t < r.len ? from[4 * h] : make_uint4(0, 0, 0, 0);
+                for (int h = 0; h < kHalves; h++)  // no token, or none that a row sees: zeros, whatever the page holds there
+                    x[g * kHalves + h] = t < r.len && t >= begin ? from[4 * h] : make_uint4(0, 0, 0, 0);
             }
         };
         auto load_scales = [&](Codes &x, const Pages &pg) {

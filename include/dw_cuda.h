@@ -655,7 +655,10 @@ DW_API size_t dw_kv_scale_bytes(size_t pages, size_t kv_heads);
  * page t / page_tokens of them.  Its rows are starts[s] .. starts[s + 1] - 1 (ascending,
  * within `tokens`; none is allowed), or without starts tokens / seqs rows each; they are
  * its last tokens: the i-th of its n rows is position lens[s] - n + i.  Rows of no sequence
- * are neither read nor written, nor are table entries behind a sequence's last page.
+ * are neither read nor written, nor are table entries behind a sequence's last page
+ * followed; an append follows those of the pages that it writes to, a read those of its rows, and
+ * attention in a window those of the pages that hold a token which some row sees: pages before
+ * these may be given to other sequences and their entries be anything.
  * Positions below 0 (n > lens[s]) are no tokens of the cache.  Lengths, starts and pages that
  * lie outside are not followed: dw_synchronize reports DW_ERR_DEVICE, and the call's
  * results are not to be used.  An append leaves the cache alone for a sequence whose length
