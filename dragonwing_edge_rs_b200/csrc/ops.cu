@@ -1229,7 +1229,7 @@ DW_API dw_status dw_prepare_rope(dw_backend *be, const double *freqs, size_t pai
     for (size_t i = 0; i < pairs; i++) {
         if (!std::isfinite(freqs[i])) return dw_fail(be, DW_ERR_INVALID_ARG, "%s: freqs[%zu] is not finite", op, i);
         long double t = (long double)freqs[i] / two_pi;
-        t = (t - floorl(t)) * 18446744073709551616.0L;  // [0, 1) of a turn, in 2^-64; 1 (by rounding) is 0
+        t = rintl((t - floorl(t)) * 18446744073709551616.0L);  // [0, 1) of a turn, to the nearest 2^-64; 1 is 0
         turns[i] = t >= 18446744073709551616.0L ? 0 : (uint64_t)t;
         const double c = (double)cosl((long double)freqs[i]), s = (double)sinl((long double)freqs[i]);
         memcpy(&turns[pairs + i], &c, 8), memcpy(&turns[2 * pairs + i], &s, 8);

@@ -619,8 +619,10 @@ typedef struct dw_head_desc {
 } dw_head_desc;
 
 /* Builds what the rotations read: freqs[pairs] in radians a position (host memory,
- * finite), held as 64-bit fractions of a turn, so that an angle is exact to 2^-53 of
- * its freq at every int32 position, with cosine and sine of one position's step.  *out is a new buffer owned by the caller. */
+ * finite), held as 64-bit fractions of a turn, with cosine and sine of one position's step.
+ * An angle is off by at most |position| * 2^-64 of a turn where freqs are up to 1 (2^-33 of a
+ * turn at the farthest int32 position), by |position| * 2^-62 of its freq more where they are
+ * above.  *out is a new buffer owned by the caller. */
 DW_API dw_status dw_prepare_rope(dw_backend *be, const double *freqs, size_t pairs, dw_buf **out);
 
 /* Query and key heads of `tokens` rows, normed and turned by their positions
