@@ -123,6 +123,7 @@ SIGNATURES = {
     "dw_launch_count": ([vp], ctypes.c_uint64),
     "dw_scratch_bytes": ([vp], ctypes.c_size_t),
     "dw_debug_expire_wait": ([vp, u32], i32),
+    "dw_debug_seq_items": ([vp, sz, sz, i32, i32, i32, vp, vp], sz),
     "dw_capture_begin": ([vp], i32),
     "dw_capture_end": ([vp, PVP], i32),
     "dw_graph_launch": ([vp, vp], i32),

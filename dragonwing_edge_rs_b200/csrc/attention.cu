@@ -447,7 +447,7 @@ template <typename T, int D, int NT>
 dw_status attend_rows(dw_backend *be, AttendParams p, const KvCache &c, const Seqs &s) {
     constexpr int R = 8 * NT;
     const size_t n = s.tokens / s.seqs, sms = (size_t)be->sm_count;
-    p.per_seq = s.starts ? 0 : (int)((n * p.group + R - 1) / R);
+    p.per_seq = s.starts ? 0 : (int)seq_items_each(n, p.group, R, 1);
     const size_t items = s.starts ? seq_items(s.tokens, s.seqs, p.group, R, 1) : (size_t)p.per_seq * s.seqs, units = items * c.heads;
     if (units * kMaxShare > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "attention_kv8: too many rows");
     p.items = (uint32_t)items;

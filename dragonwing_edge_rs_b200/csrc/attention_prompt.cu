@@ -609,7 +609,7 @@ dw_status attend_prompt(dw_backend *be, AttendParams p, const KvCache &c, const 
     auto kernel = k_attend_prompt<T, D>;
     constexpr size_t smem = 1024 + (size_t)(2 * 128 + 2 * kStages * kTile) * D * 2;
     const size_t n = s.tokens / s.seqs;
-    p.per_seq = s.starts ? 0 : (int)((n * p.group + kRows - 1) / kRows);
+    p.per_seq = s.starts ? 0 : (int)seq_items_each(n, p.group, kRows, 1);
     const size_t items = s.starts ? seq_items(s.tokens, s.seqs, p.group, kRows, 1) : (size_t)p.per_seq * s.seqs;
     if (items * c.heads > 0x7fffffffu) return dw_fail(be, DW_ERR_UNSUPPORTED, "attention_kv8: too many rows");
     p.items = (uint32_t)items;

@@ -113,20 +113,39 @@ __device__ __forceinline__ SeqRange seq_range(const Seqs &q, uint32_t s, int pag
 __host__ __device__ inline size_t seq_items(size_t tokens, size_t seqs, int per, int size, int extra) {
     return tokens * per / size + extra * seqs;
 }
-// The sequence of item w and its place there (below 0: of no sequence); a whole warp calls.
-__device__ __forceinline__ uint32_t seq_of_item(const Seqs &q, int64_t w, int per, int size, int extra, int64_t &place) {
-    const int lane = threadIdx.x & 31;
-    auto first = [&](uint32_t s) { return (int64_t)seq_start(q, s) * per / size + (int64_t)extra * s; };
-    uint32_t lo = 0, count = q.seqs;
+__host__ __device__ inline int64_t seq_first_item(int64_t start, uint32_t s, int per, int size, int extra) {
+    return start * per / size + (int64_t)extra * s;
+}
+// Those of each sequence where all have n rows: blocks of `size` of n * per rows, or with extra = 2 the
+// pages of `size` tokens that n rows can lie in, from anywhere in the first.
+__host__ __device__ inline size_t seq_items_each(size_t n, int per, int size, int extra) {
+    return extra == 2 ? (n + size - 2) / size + 1 : (n * per + size - 1) / size;
+}
+// The sequence of item w, by the items that sequences begin with, and its place there (below 0: of no
+// sequence).  vote(f): the bits of f(0) .. f(31).
+template <typename First, typename Vote>
+__host__ __device__ __forceinline__ uint32_t find_item(uint32_t seqs, int64_t w, First first, Vote vote, int64_t &place) {
+    uint32_t lo = 0, count = seqs;
     while (count > 1) {  // the last of 32 evenly spaced ones that does not start behind w
-        const uint32_t step = (count + 31) / 32, at = (uint32_t)lane * step;
-        const uint32_t mask = __ballot_sync(0xffffffffu, at < count && first(lo + at) <= w) | 1u;
+        const uint32_t step = (count + 31) / 32;
+        const uint32_t mask = vote([&](uint32_t i) { return i * step < count && first(lo + i * step) <= w; }) | 1u;
+#ifdef __CUDA_ARCH__
         const uint32_t k = 31 - __clz(mask);
+#else
+        const uint32_t k = 31 - __builtin_clz(mask);
+#endif
         lo += k * step;
-        count = min(step, count - k * step);
+        count = count - k * step < step ? count - k * step : step;
     }
     place = w - first(lo);
     return lo;
+}
+// The same of a call's sequences; a whole warp calls.
+__device__ __forceinline__ uint32_t seq_of_item(const Seqs &q, int64_t w, int per, int size, int extra, int64_t &place) {
+    const uint32_t lane = threadIdx.x & 31;
+    return find_item(
+        q.seqs, w, [&](uint32_t s) { return seq_first_item(seq_start(q, s), s, per, size, extra); },
+        [&](auto f) { return __ballot_sync(0xffffffffu, f(lane)); }, place);
 }
 
 // A sequence's page `index` (its tokens from index * page on) to read from, in bounds in any case.

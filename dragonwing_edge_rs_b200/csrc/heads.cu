@@ -713,8 +713,7 @@ template <typename T, int E>
 dw_status append(dw_backend *be, HeadParams p, const KvCache &c, const Seqs &s, const HeadArgs &a) {
     const bool vec = aligned(a.k, sizeof(T), E * sizeof(T)) && aligned(a.v, sizeof(T), 2 * E * sizeof(T));
     const unsigned threads = (unsigned)(c.page / kWarpTokens * 32);
-    // pages that n rows can lie in, from anywhere in the first
-    const size_t n = s.tokens / s.seqs, each = (n + c.page - 2) / c.page + 1;
+    const size_t n = s.tokens / s.seqs, each = seq_items_each(n, 1, c.page, 2);
     const size_t pages = (s.starts ? seq_items(s.tokens, s.seqs, 1, c.page, 2) : each * s.seqs) * p.hk;
     auto go = [&](auto kernel, int QE, int QJ) {
         size_t blocks = pages;
@@ -775,3 +774,26 @@ dw_status launch_read_kv(dw_backend *be, const KvCache &c, const Seqs &s, int dt
 }
 
 }  // namespace dw
+
+// What the kernels of sequences are launched over, on the host.
+extern "C" DW_API size_t dw_debug_seq_items(const int32_t *starts, size_t seqs, size_t tokens, int per, int size, int extra, uint32_t *seq,
+                                            int64_t *place) {
+    if (!seqs || per <= 0 || size <= 0 || extra < 0) return 0;
+    const size_t each = dw::seq_items_each(tokens / seqs, per, size, extra);
+    const size_t n = starts ? dw::seq_items(tokens, seqs, per, size, extra) : each * seqs;
+    for (size_t w = 0; seq && place && w < n; w++) {
+        if (!starts) {
+            seq[w] = (uint32_t)(w / each), place[w] = (int64_t)(w % each);
+            continue;
+        }
+        seq[w] = dw::find_item(
+            (uint32_t)seqs, (int64_t)w, [&](uint32_t s) { return dw::seq_first_item(starts[s], s, per, size, extra); },
+            [](auto f) {
+                uint32_t m = 0;
+                for (uint32_t i = 0; i < 32; i++) m |= (uint32_t)f(i) << i;
+                return m;
+            },
+            place[w]);
+    }
+    return n;
+}

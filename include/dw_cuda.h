@@ -168,6 +168,11 @@ DW_API uint64_t dw_graph_kernels(const dw_graph *g);
  * with a cap of cap_us microseconds; the kernel gives up and records the
  * failure, and the next dw_synchronize reports DW_ERR_KERNEL_WAIT_EXPIRED. */
 DW_API dw_status dw_debug_expire_wait(dw_backend *be, uint32_t cap_us);
+/* Test hook: the items of work that a call over sequences is cut into (blocks of `size` of
+ * each sequence's rows times `per`, with extra = 2 pages of `size` tokens), by the kernels' own
+ * rule on the host: their number, and in seq and place (NULL: not wanted) whose each is. */
+DW_API size_t dw_debug_seq_items(const int32_t *starts, size_t seqs, size_t tokens, int per, int size, int extra, uint32_t *seq,
+                                 int64_t *place);
 
 /* ---------------------------------------------------------------------- */
 /* Fused INT8 convolution (the hot path)                                   */
