@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import enum
+import weakref
 
 import numpy as np
 
@@ -34,12 +35,22 @@ class BufferKind(enum.Enum):
 class CudaBuffer:
     """Device byte buffer (``impl BackendBuffer``)."""
 
-    __slots__ = ("_backend", "handle", "_len", "__weakref__")
+    __slots__ = ("_backend", "handle", "_len", "_held", "__weakref__")
 
     def __init__(self, backend: "CudaBackend", handle: ctypes.c_void_p, length: int):
         self._backend = backend
         self.handle = handle
         self._len = length
+        self._held = None
+
+    def held_by(self, struct, field: str):
+        """The handle, for a descriptor's `field`: freeing the buffer sets that to null, which calls refuse."""
+        if self._held is None:
+            self._held = []
+        elif len(self._held) % 64 == 0:
+            self._held = [h for h in self._held if h[0]() is not None]
+        self._held.append((weakref.ref(struct), field))
+        return self.handle
 
     def len_bytes(self) -> int:
         return self._len
@@ -52,6 +63,10 @@ class CudaBuffer:
         if self.handle:
             self._backend._check(L.load().dw_free(self._backend.handle, self.handle))
             self.handle = None
+            for struct, field in self._held or ():
+                if struct() is not None:
+                    setattr(struct(), field, None)
+            self._held = None
 
     def __del__(self):
         try:

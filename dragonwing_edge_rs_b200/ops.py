@@ -444,7 +444,7 @@ class Heads(L.DwHeads):
     `pitch` elements apart (0: the heads' own width)."""
 
     def __init__(self, buf: CudaBuffer, offset: int = 0, pitch: int = 0):
-        super().__init__(buf and buf.handle, offset, pitch)
+        super().__init__(buf and buf.held_by(self, "buf"), offset, pitch)
         self.keep = buf
         self.ref = ctypes.addressof(self)
 
@@ -463,7 +463,8 @@ class KvCache(L.DwKvCache):
 
     def __init__(self, k: CudaBuffer, v: CudaBuffer, scales: CudaBuffer, pages: int, kv_heads: int, page_tokens: int,
                  head_dim: int):
-        super().__init__(k and k.handle, v and v.handle, scales and scales.handle, pages, kv_heads, page_tokens, head_dim)
+        super().__init__(*(b and b.held_by(self, n) for b, n in ((k, "k"), (v, "v"), (scales, "scales"))), pages, kv_heads,
+                         page_tokens, head_dim)
         self.keep = (k, v, scales)
         self.ref = ctypes.addressof(self)
 
@@ -472,7 +473,9 @@ class Sequences(L.DwSequences):
     """The sequences that a call's rows belong to: their pages, lengths and rows (dw_sequences)."""
 
     def __init__(self, table: CudaBuffer, lens: CudaBuffer, starts, seqs: int, tokens: int, width: int):
-        super().__init__(table and table.handle, lens and lens.handle, starts and starts.handle, seqs, tokens, width)
+        # (no starts are even rows: it is the table that goes with freed ones)
+        super().__init__(*(b and b.held_by(self, n) for b, n in ((table, "table"), (lens, "lens"), (starts, "table"))), seqs,
+                         tokens, width)
         self.keep = (table, lens, starts)
         self.ref = ctypes.addressof(self)
 
