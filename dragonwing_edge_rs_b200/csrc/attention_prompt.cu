@@ -62,11 +62,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t *barrier, uint32_t parity, co
     return __all_sync(0xffffffffu, wait_phase(barrier, parity, p, abort_flag, site));
 }
 
-__device__ __forceinline__ uint32_t elect_one() {
-    uint32_t e;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-    return e;
-}
 // One product of 128 x N x 16, by an elected lane: both operands in shared memory, or the first
 // in tensor memory.
 __device__ __forceinline__ void mma_ss(uint32_t elected, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {

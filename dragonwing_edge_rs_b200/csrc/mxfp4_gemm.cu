@@ -101,11 +101,6 @@ __device__ __forceinline__ void drain_phase(uint32_t bar, uint32_t parity, uint6
 __device__ __forceinline__ void prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-__device__ __forceinline__ uint32_t elect_one() {
-    uint32_t e;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-    return e;
-}
 
 // 512 bytes (32 rows of 16) -> 4 columns of all four lane quarters of tensor memory
 // (of both CTAs of a pair).
