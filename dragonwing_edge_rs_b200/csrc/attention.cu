@@ -482,6 +482,9 @@ dw_status attend(dw_backend *be, const AttendParams &p, const KvCache &c, const 
     // gains only where CTAs are few and share the tokens (40 rows of 16 sequences of 4000 72 and
     // 83; 48 rows of 64 of 1000 87 and 92, of one of 8000 36 and 22).
     if (rows > 48 || (rows > 24 && s.seqs * c.heads * 2 <= (size_t)be->sm_count)) return attend_prompt<T, D>(be, p, c, s);
+    // (The average: a call's starts are known on the device alone.  Sequences of very different rows
+    // lose by it: 1024 rows behind 3000 tokens beside 63 single tokens 375 us, in calls of their own 85 and
+    // 95; a prompt of 512 beside 255 single tokens 161, of their own 20 and 90.)
     // (fewer rows than it has places cost a warp products and registers: one row of 64 sequences of up
     // to 8192 tokens 94 us by 8 places, 129 by 16, 182 by 24; 8 rows over 8000 tokens 11.1, 13.9, 18.2)
     if (rows <= 8) return attend_rows<T, D, 1>(be, p, c, s);

@@ -43,6 +43,9 @@ __device__ __forceinline__ float carry(float x, float y) { return x == y ? 1.0f 
 // weights far below f16's range that count in the sum of weights).  Both sums take these, so only
 // what the cuts differ by between a row's tokens is an error, as much as of a rounding to nearest, and
 // a row of one token is exact; with the uncut ones in the sum of weights it was half as much again.
+// (f16 itself, for the products: weights times their block's scale, 2^ev, keep the 11 bits down to 2^-20
+// of a row's largest, fewer down to 2^-31 and are 0 below, where they still count in the sum of weights.
+// A block of so much larger values that has zeros in a channel therefore hides the others there.)
 __device__ __forceinline__ float2 eleven_bits(float x, float y) {
     return make_float2(__uint_as_float(__float_as_uint(x) & ~0x1FFFu), __uint_as_float(__float_as_uint(y) & ~0x1FFFu));
 }

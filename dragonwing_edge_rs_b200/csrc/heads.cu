@@ -93,8 +93,8 @@ __device__ __forceinline__ void norm_rope_row(const HeadParams &p, size_t row, i
         live[j] = 2 * E * c < p.d;
         a[j] = slot.a, b[j] = slot.b, turns[j] = slot.turns && live[j];
     }
-    // Two groups' values are on their way while one is computed (8192 x 40 heads of 128 bf16 49.3 us,
-    // 49.6 with one: the instructions are the bound).
+    // Two groups' values are on their way while one is computed (8192 x 40 heads of 128, 64 of them
+    // turned: bf16 50.9 us, f32 71.4; 16-bit rows are bound by the instructions).
     struct Group {
         Raw<T, E> a[J], b[J];
     } g0, g1;
@@ -196,7 +196,7 @@ constexpr int kAhead = 4;
 // The same for heads that turn whole and fill their lanes (d = 2 E * 32 / kPer; kPer heads a
 // group): a lane keeps the products of weights and angles, so that a value is
 // rstd * (a * (w_a cos) - b * (w_b sin)), and finds one in kPer of its angles, the others by
-// XX
+// exchange with the lanes that have the same pairs of the group's other heads.
 template <typename T, int E, int kPer>
 __device__ __forceinline__ void rope_row(const HeadParams &p, size_t row, int64_t position, int first) {
     constexpr int kGroup = 32 / kPer, kMine = E > kPer ? E / kPer : 1, kD = 2 * E * kGroup;
@@ -341,7 +341,8 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ 
 // bound has to hold for the pair, and one token in five had a value too small beside its
 // partner.)  A warp's tokens follow each other, so the angles after the first come by one
 // complex product each.  The blocks behind those of the pages norm and turn query rows.  (4096
-// tokens, 8 heads of 128 bf16: 17.5 us, 25 MB; with 32 query heads 29.3, 92 MB.)
+// tokens, 8 heads of 128 bf16, three sets of inputs in turn: 18.4 us, 25 MB; with 32 query heads
+// 31.9, 92 MB.)
 constexpr int kWarpTokens = 8;
 
 __device__ __forceinline__ float round_to_odd(double v) {
@@ -594,7 +595,7 @@ __global__ void __launch_bounds__(512)
 
 // ---- read --------------------------------------------------------------------------
 // A warp has a row's keys or values, a lane 16 of them at a time (4096 rows of 8 heads of 128 bf16
-// 7.5 us, 25 MB).
+// 7.2 us, 25 MB: a row's lookups and its loads, one after the other).
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     k_read(const __grid_constant__ KvCache c, const __grid_constant__ Seqs q, const uint32_t each_rows, T *k_out, T *v_out, size_t k_pitch,

@@ -699,7 +699,10 @@ DW_API dw_status dw_read_kv(dw_backend *be, const dw_kv_cache *cache, const dw_s
  * causal) the last `window` of these.  Query head h reads cache head h / (q_heads /
  * kv_heads).  A row that sees nothing gives 0.  q and out: DW_F16 or DW_BF16; products
  * and sums are f32, the softmax's weights are cut to 11 bits, in numerator and
- * denominator.  The sums' order depends on the sizes and lengths alone.  out may be q itself. */
+ * denominator; in the numerator a weight times its block's X below 2^-20 of the row's largest
+ * has fewer bits, and none below 2^-31.  The sums' order depends on the sizes and lengths alone.  out may be q itself.
+ * Which kernel a call runs on goes by the rows of a sequence on average: prompts beside single
+ * tokens are right in one call, but faster as one call of each kind, each on its rows of q and out. */
 typedef struct dw_attention_desc {
     int32_t q_heads; /* a multiple of the cache's kv_heads */
     int32_t dtype;
