@@ -669,7 +669,7 @@ DW_API size_t dw_kv_scale_bytes(size_t pages, size_t kv_heads);
  * Positions below 0 (n > lens[s]) are no tokens of the cache.  Lengths, starts and pages that
  * lie outside are not followed: dw_synchronize reports DW_ERR_DEVICE, and the call's
  * results are not to be used.  An append leaves the cache alone for a sequence whose length
- * or starts lie outside or whose starts descend, or a neighbour's do, and where a page lies outside;
+ * or starts lie outside, or whose starts or a neighbour's descend, and where a page lies outside;
  * the other sequences' tokens are appended as ever. */
 typedef struct dw_sequences {
     const dw_buf *table;  /* int32 [seqs, width] */
@@ -683,7 +683,7 @@ typedef struct dw_sequences {
  * q).  rope is NULL where rot_dim is 0.  A block that tokens are added to keeps its X or
  * takes a larger one, and the codes that it holds are then rounded again; the first token of a
  * page makes the block anew.  Keys are computed in f64, so their codes are the
- * definition's; queries in f32.  Two sequences may share pages that the call
+ * definition's (by angles as dw_prepare_rope holds them); queries in f32.  Two sequences may share pages that the call
  * does not write. */
 DW_API dw_status dw_append_kv(dw_backend *be, const dw_head_desc *d, const dw_kv_cache *cache, const dw_sequences *seqs,
                               const dw_heads *k, const dw_heads *v, const dw_buf *w_k, const dw_buf *rope,
